@@ -192,6 +192,28 @@ int oxide_add_rms_norm_bf16(const oxide_bf16* x, const oxide_bf16* r, const oxid
                             oxide_bf16* h, oxide_bf16* y, uint64_t rows, uint64_t cols,
                             float eps, oxide_stream_t stream);
 
+/* ---- normalisation with an int8 output -----------------------------------------
+ * rms_norm, and residual add + rms_norm, whose rows leave as int8 codes with
+ * one f32 scale a row, for a caller whose next product reads int8:
+ *     scale[r] = max_j |y_j| / 127,  out[r, j] = nearest(y_j / scale[r])
+ * (ties to even), y = (h / rms) * w unrounded, so out * scale stands for y.
+ * The codes are decided exactly (nearest(127 p_j / max|p|) with p = h * w:
+ * the rms cancels); the scale is correct to a few f32 ulp.  An all-zero row
+ * has scale 0 and codes 0 (eps > 0); a row that holds a NaN or an infinity,
+ * or meets one in w, has scale NaN and codes 0, so that it reads as NaN.  The
+ * add form stores h = x + r rounded to the I/O type, as oxide_add_rms_norm_*
+ * does, and normalises the stored value; h may alias x or r, out must not
+ * alias x, r or h.  API addition: the reference has no 8-bit path. */
+int oxide_rms_norm_q8_f32(const float* x, const float* w, int8_t* out, float* scale, uint64_t rows,
+                          uint64_t cols, float eps, oxide_stream_t stream);
+int oxide_rms_norm_q8_bf16(const oxide_bf16* x, const oxide_bf16* w, int8_t* out, float* scale,
+                           uint64_t rows, uint64_t cols, float eps, oxide_stream_t stream);
+int oxide_add_rms_norm_q8_f32(const float* x, const float* r, const float* w, float* h, int8_t* out,
+                              float* scale, uint64_t rows, uint64_t cols, float eps, oxide_stream_t stream);
+int oxide_add_rms_norm_q8_bf16(const oxide_bf16* x, const oxide_bf16* r, const oxide_bf16* w, oxide_bf16* h,
+                               int8_t* out, float* scale, uint64_t rows, uint64_t cols, float eps,
+                               oxide_stream_t stream);
+
 /* Per row of x[rows, cols]: mean = sum(x) / cols; var = sum((x - mean)^2) / cols;
  * out = (x - mean) / sqrt(var + eps) * w + b.  Replaces ops::layer_norm
  * (src/ops/norm.rs:53-117) and KernelManager::launch_layer_norm
@@ -302,6 +324,52 @@ int oxide_kv_cache_append_bf16(oxide_bf16* k_cache, oxide_bf16* v_cache, const o
                                const oxide_bf16* v, uint64_t batch, uint64_t kv_heads, uint64_t max_seq,
                                uint64_t head_dim, uint64_t cur_len, uint64_t new_len, oxide_stream_t stream);
 
+/* ---- int8 KV cache -----------------------------------------------------------------
+ * Caches [batch, kv_heads, max_seq, head_dim] of int8 codes with f32 scales
+ * [batch, kv_heads, nblk], nblk = ceil(max_seq / block): one scale for each
+ * `block` consecutive positions of a head (block a power of two in [1, 128]);
+ * a code c stands for c * scale.  API addition: the reference's cache is f32.
+ *
+ * Append: k, v [batch, kv_heads, new_len, head_dim] are quantised into
+ * positions [cur, cur + n) of each sequence, both in one launch.  cur is
+ * cur_lens[b] (device int32, where cur_lens != NULL) else cur_len; n is
+ * new_lens[b] held to [0, new_len] (where new_lens != NULL: tokens behind it
+ * are padding and are not read) else new_len.  For each block that receives
+ * tokens, need = max|x| / 127 over them (one f32 division); the scale becomes
+ * need if the block starts at or behind cur, else max(its scale, need), and
+ * where that grows the codes of the positions before cur are restated,
+ * nearest(c * old / new).  New codes are nearest(x / scale), ties to even,
+ * decided exactly, 0 under a zero scale.  A block that receives a NaN or an
+ * infinity gets the scale NaN and codes 0: all of it reads as NaN.  Nothing
+ * else is written: not the positions at or behind cur + n, not other blocks'
+ * scales.  cur_len + new_len > max_seq (without cur_lens) is
+ * OXIDE_ERR_INVALID_ARG ("KV cache overflow"), nothing written; a sequence
+ * whose cur_lens[b] is negative or whose tokens do not fit is left as it is.
+ * k and v must not overlap the caches.  Calls on one cache must be ordered. */
+int oxide_kv_cache_append_q8_f32(int8_t* k_cache, int8_t* v_cache, float* k_scale, float* v_scale,
+                                 const float* k, const float* v, uint64_t batch, uint64_t kv_heads,
+                                 uint64_t max_seq, uint64_t head_dim, uint64_t block, uint64_t cur_len,
+                                 const int32_t* cur_lens, uint64_t new_len, const int32_t* new_lens,
+                                 oxide_stream_t stream);
+int oxide_kv_cache_append_q8_bf16(int8_t* k_cache, int8_t* v_cache, float* k_scale, float* v_scale,
+                                  const oxide_bf16* k, const oxide_bf16* v, uint64_t batch, uint64_t kv_heads,
+                                  uint64_t max_seq, uint64_t head_dim, uint64_t block, uint64_t cur_len,
+                                  const int32_t* cur_lens, uint64_t new_len, const int32_t* new_lens,
+                                  oxide_stream_t stream);
+/* Read back: positions [start, start + n) of every head as k, v [batch,
+ * kv_heads, n, head_dim], code * scale (one f32 product, rounded to the output
+ * type); positions at or behind lens[b] (device int32, may be NULL) are not
+ * read and are written as zeros.  start + n > max_seq is
+ * OXIDE_ERR_INVALID_ARG. */
+int oxide_kv_cache_read_q8_f32(const int8_t* k_cache, const int8_t* v_cache, const float* k_scale,
+                               const float* v_scale, float* k, float* v, uint64_t batch, uint64_t kv_heads,
+                               uint64_t max_seq, uint64_t head_dim, uint64_t block, uint64_t start, uint64_t n,
+                               const int32_t* lens, oxide_stream_t stream);
+int oxide_kv_cache_read_q8_bf16(const int8_t* k_cache, const int8_t* v_cache, const float* k_scale,
+                                const float* v_scale, oxide_bf16* k, oxide_bf16* v, uint64_t batch,
+                                uint64_t kv_heads, uint64_t max_seq, uint64_t head_dim, uint64_t block,
+                                uint64_t start, uint64_t n, const int32_t* lens, oxide_stream_t stream);
+
 /* ---- decode attention ---------------------------------------------------------
  * One query token per (batch, head) against KV caches [batch, kv_heads,
  * max_seq, head_dim]: the inline attention of scaled_dot_product_attention
@@ -344,6 +412,33 @@ int oxide_decode_attention_bf16(const oxide_bf16* q, const oxide_bf16* k_cache, 
                                 const int32_t* lens, oxide_bf16* out, uint64_t batch, uint64_t q_heads,
                                 uint64_t kv_heads, uint64_t max_seq, uint64_t head_dim, float scale,
                                 void* workspace, uint64_t workspace_bytes, oxide_stream_t stream);
+
+/* decode_attention over int8 caches (the caches and scales of
+ * oxide_kv_cache_append_q8_*): s_j = (q . k_j) * scale over the values the
+ * codes stand for, softmax over j < lens[b] (lens NULL: every position; held
+ * to [0, max_seq]), out = sum_j p_j v_j; query head h reads kv head
+ * h / (q_heads / kv_heads).  q, out [batch, q_heads, head_dim], f32 or bf16,
+ * head_dim <= 256, batch <= 4096.  Sums, scores and softmax statistics are
+ * f32 (the tensor-core products are exact integer sums of q and p written in
+ * 23 bits).  A sequence of length 0 gives zeros; a key whose block has the
+ * scale NaN, or a query head that holds a NaN or an infinity, gives NaN;
+ * positions at or behind lens[b] and their scales may hold anything.  out must
+ * not alias q.  `workspace` is device memory of at least
+ * oxide_decode_attention_q8_workspace_bytes(...) bytes, 16-byte aligned, that
+ * no other call which may run at the same time uses; it needs no
+ * initialisation. */
+uint64_t oxide_decode_attention_q8_workspace_bytes(uint64_t batch, uint64_t q_heads, uint64_t kv_heads,
+                                                   uint64_t head_dim);
+int oxide_decode_attention_q8_f32(const float* q, const int8_t* k_cache, const int8_t* v_cache,
+                                  const float* k_scale, const float* v_scale, const int32_t* lens, float* out,
+                                  uint64_t batch, uint64_t q_heads, uint64_t kv_heads, uint64_t max_seq,
+                                  uint64_t head_dim, uint64_t block, float scale, void* workspace,
+                                  uint64_t workspace_bytes, oxide_stream_t stream);
+int oxide_decode_attention_q8_bf16(const oxide_bf16* q, const int8_t* k_cache, const int8_t* v_cache,
+                                   const float* k_scale, const float* v_scale, const int32_t* lens,
+                                   oxide_bf16* out, uint64_t batch, uint64_t q_heads, uint64_t kv_heads,
+                                   uint64_t max_seq, uint64_t head_dim, uint64_t block, float scale,
+                                   void* workspace, uint64_t workspace_bytes, oxide_stream_t stream);
 
 /* ---- token sampling ----------------------------------------------------------
  * sample_next_token (src/pipeline.rs:181-205) for each row of logits

@@ -1,0 +1,390 @@
+// k_attention_q8.cu -- one-token (decode) attention over int8 KV caches with a
+// scale for each block of tokens and head (the caches of k_kvcache_q8.cu).
+//
+// Reference: the attention of src/ops/attention.rs:41-87 for q_len = 1, with
+// the head map of repeat_kv (:161-201); the 8-bit cache is an addition.
+// With codes c, d and scales ks, vs of key j's block:
+//     s_j = (q . c_j) ks scale,  p = softmax(s),  out = sum_j p_j vs d_j:
+// the scales factor out of both products, so codes enter them as they are.
+//
+// Two kernels write partial results in one form (oxide_attn_q8.cuh) and
+// decode_attn_q8_combine_kernel merges them:
+//   k_attention_q8_tc.cu   head_dim 128 and 1, 2, 4 or 8 query heads a kv
+//                          head: both products in int8 on tcgen05;
+//   here, any other shape  (head_dim up to 256, any group): a warp is a
+//                          worker and streams 32-key tiles.  Scores: lane =
+//                          key, its row read in 16-byte (4-byte, 1-byte)
+//                          pieces against the group's query heads in shared
+//                          memory; P V: lane = four dims (one, for odd
+//                          sizes), each key's weights broadcast by shuffles.
+//                          f32 throughout.
+// Bound by HBM bytes, 2 head_dim a key and kv head.
+#include "oxide_attn_q8.cuh"
+
+namespace oxide {
+
+constexpr int QW_WARPS = 8;
+constexpr uint32_t QW_TK = 32;  // keys a tile
+
+// Dims a lane owns: D4: four of every 128 (NG groups); else one of every 32.
+template <int NR, int NG, bool D4>
+__global__ void __launch_bounds__(QW_WARPS * 32, 2) decode_attn_q8_warp_kernel(Q8AttnArgs p) {
+    pdl_begin();
+    extern __shared__ __align__(16) unsigned char smem[];
+    constexpr int W = D4 ? 4 : 1;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const uint32_t D = p.head_dim, DP = (D + 3) & ~3u;
+    float* qs = reinterpret_cast<float*>(smem) + (size_t)warp * NR * DP;  // this warp's query heads [NR][DP]
+    uint32_t* pre = reinterpret_cast<uint32_t*>(smem + (size_t)QW_WARPS * NR * DP * 4);
+    if (warp == 0) q8a_prefix(p, QW_TK, pre, blockIdx.x == 0);
+    if (blockIdx.x == 0 && threadIdx.x == 0) *p.err = 0u;
+    __syncthreads();
+    const uint32_t heads = p.kv_heads * p.chunks;
+    const uint32_t T = pre[p.batch] * heads, G = p.workers;
+    const uint32_t c = blockIdx.x * QW_WARPS + warp;
+    if (c >= G) return;
+    const uint32_t t0 = (uint32_t)((uint64_t)c * T / G), t1 = (uint32_t)((uint64_t)(c + 1) * T / G);
+    if (t0 >= t1) return;
+    TileWalk w{pre, p.batch, heads, 0, 0, 0, 0};
+    w.seek(t0);
+    float m[NR], l[NR], acc[NR][NG * W];
+    uint32_t nh = 0, len = 0;
+    const int8_t *kh = nullptr, *vh = nullptr;
+    const float *ksh = nullptr, *vsh = nullptr;
+    for (uint32_t t = t0; t < t1; ++t, w.next()) {
+        if (t == t0 || w.lt == 0) {  // a new pair: its query heads and caches
+            const uint32_t kvh = w.kvh / p.chunks, h0 = (w.kvh % p.chunks) * NR;
+            nh = min(p.rep - h0, (uint32_t)NR);
+            len = q8a_len(p, w.b);
+            const uint64_t bh = (uint64_t)w.b * p.kv_heads + kvh, row = (uint64_t)w.b * p.q_heads + kvh * p.rep + h0;
+            kh = p.kc + bh * p.max_seq * D;
+            vh = p.vc + bh * p.max_seq * D;
+            ksh = p.ks + bh * p.nblk;
+            vsh = p.vs + bh * p.nblk;
+            __syncwarp();
+            for (uint32_t i = lane; i < NR * DP; i += 32) {
+                const uint32_t h = i / DP, d = i - h * DP;
+                float v = 0.0f;
+                if (h < nh && d < D) {
+                    const uint64_t at = (row + h) * D + d;
+                    v = p.q_bf16 ? Vec<bf16_t>::load1(static_cast<const bf16_t*>(p.q) + at)
+                                 : Vec<float>::load1(static_cast<const float*>(p.q) + at);
+                }
+                qs[i] = v;
+            }
+            __syncwarp();
+#pragma unroll
+            for (int h = 0; h < NR; ++h) {
+                m[h] = -INFINITY;
+                l[h] = 0.0f;
+#pragma unroll
+                for (int e = 0; e < NG * W; ++e) acc[h][e] = 0.0f;
+            }
+        }
+        const uint32_t key0 = w.lt * QW_TK, nk = min(len - key0, QW_TK);
+        const bool on = (uint32_t)lane < nk;
+        float dot[NR], ks = 0.0f, vs = 0.0f;
+#pragma unroll
+        for (int h = 0; h < NR; ++h) dot[h] = 0.0f;
+        if (on) {
+            const uint32_t key = key0 + lane;
+            ks = __ldg(ksh + (key >> p.shift));
+            vs = __ldg(vsh + (key >> p.shift));
+            const int8_t* row = kh + (uint64_t)key * D;
+            if (D4 && D % 16 == 0) {
+#pragma unroll 4
+                for (uint32_t i = 0; i < D; i += 16) {
+                    const uint4 v = __ldg(reinterpret_cast<const uint4*>(row + i));
+                    const uint32_t wd[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        float f[4];
+                        q8_unpack4(wd[e], f);
+#pragma unroll
+                        for (int h = 0; h < NR; ++h) {
+                            const float4 qv = *reinterpret_cast<const float4*>(qs + h * DP + i + 4 * e);
+                            dot[h] = __fmaf_rn(f[0], qv.x, dot[h]);
+                            dot[h] = __fmaf_rn(f[1], qv.y, dot[h]);
+                            dot[h] = __fmaf_rn(f[2], qv.z, dot[h]);
+                            dot[h] = __fmaf_rn(f[3], qv.w, dot[h]);
+                        }
+                    }
+                }
+            } else if (D4) {
+#pragma unroll 4
+                for (uint32_t i = 0; i < D; i += 4) {
+                    float f[4];
+                    q8_unpack4(__ldg(reinterpret_cast<const unsigned int*>(row + i)), f);
+#pragma unroll
+                    for (int h = 0; h < NR; ++h)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) dot[h] = __fmaf_rn(f[e], qs[h * DP + i + e], dot[h]);
+                }
+            } else {
+#pragma unroll 4
+                for (uint32_t i = 0; i < D; ++i) {
+                    const float f = (float)__ldg(reinterpret_cast<const signed char*>(row + i));
+#pragma unroll
+                    for (int h = 0; h < NR; ++h) dot[h] = __fmaf_rn(f, qs[h * DP + i], dot[h]);
+                }
+            }
+        }
+        float pv[NR];
+        const float kf = fmul(ks, p.c1);
+#pragma unroll
+        for (int h = 0; h < NR; ++h) {
+            const float s = on ? fmul(dot[h], kf) : -INFINITY;
+            const float mn = fmaxf(m[h], warp_fmax(s));
+            const float cr = m[h] == -INFINITY ? 0.0f : ex2_approx(fsub(m[h], mn));
+            const float pr = s == -INFINITY ? 0.0f : ex2_approx(fsub(s, mn));  // a NaN score stays NaN
+            m[h] = mn;
+            l[h] = __fmaf_rn(l[h], cr, pr);
+            pv[h] = on ? fmul(pr, vs) : 0.0f;
+#pragma unroll
+            for (int e = 0; e < NG * W; ++e) acc[h][e] = fmul(acc[h][e], cr);
+        }
+        const int8_t* vrow = vh + (uint64_t)key0 * D;
+#pragma unroll 8
+        for (uint32_t j = 0; j < nk; ++j) {
+            float f[NG][W];
+#pragma unroll
+            for (int g = 0; g < NG; ++g) {
+                const uint32_t d = W * (lane + 32 * g);
+                if constexpr (D4) {
+                    const uint32_t x = d < D ? __ldg(reinterpret_cast<const unsigned int*>(vrow + (uint64_t)j * D + d)) : 0u;
+                    q8_unpack4(x, f[g]);
+                } else {
+                    f[g][0] = d < D ? (float)__ldg(reinterpret_cast<const signed char*>(vrow + (uint64_t)j * D + d)) : 0.0f;
+                }
+            }
+#pragma unroll
+            for (int h = 0; h < NR; ++h) {
+                const float x = __shfl_sync(0xffffffffu, pv[h], j);
+#pragma unroll
+                for (int g = 0; g < NG; ++g)
+#pragma unroll
+                    for (int e = 0; e < W; ++e) acc[h][g * W + e] = __fmaf_rn(x, f[g][e], acc[h][g * W + e]);
+            }
+        }
+        if (t + 1 == t1 || w.lt + 1 == w.tb) {  // this worker's last tile of the pair
+            const uint64_t part = (uint64_t)c + (uint64_t)w.b * heads + w.kvh;
+#pragma unroll
+            for (int h = 0; h < NR; ++h) {
+                const float ls = warp_sum(l[h]);
+                if ((uint32_t)h >= nh) continue;
+                const uint64_t slot = part * NR + h;
+                if (lane == 0) {
+                    p.part_ml[slot * 2] = m[h];
+                    p.part_ml[slot * 2 + 1] = ls;
+                }
+#pragma unroll
+                for (int g = 0; g < NG; ++g)
+#pragma unroll
+                    for (int e = 0; e < W; ++e) {
+                        const uint32_t d = W * (lane + 32 * g) + e;
+                        if (d < D) p.part_o[slot * D + d] = acc[h][g * W + e];
+                    }
+            }
+        }
+    }
+}
+
+// Merge the parts of one (batch, query head): warp w takes every eighth part
+// of the pair, lane = dim, and the eight states are joined through shared
+// memory.  A part without keys has sum 0; a pair without keys gives zeros; NaN
+// if a wait of the main kernel ran out.
+template <typename T>
+__global__ void __launch_bounds__(256) decode_attn_q8_combine_kernel(T* out, Q8AttnArgs p) {
+    pdl_begin();
+    constexpr int NW = 8, DPL = Q8A_MAX_D / 32;
+    __shared__ float wm[NW], wl[NW], wo[NW][Q8A_MAX_D];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const uint32_t bh = blockIdx.x, b = bh / p.q_heads, qh = bh - b * p.q_heads;
+    const uint32_t kvh = qh / p.rep, r = qh - kvh * p.rep, chunk = r / p.nr, h = r - chunk * p.nr;
+    const uint32_t heads = p.kv_heads * p.chunks, D = p.head_dim;
+    const uint32_t before = p.pre_out[b], tb = p.pre_out[b + 1] - before, T_ = p.pre_out[p.batch] * heads;
+    const uint32_t failed = *p.err;
+    float M = -INFINITY, L = 0.0f, acc[DPL];
+#pragma unroll
+    for (int i = 0; i < DPL; ++i) acc[i] = 0.0f;
+    if (tb) {
+        const uint32_t pair = b * heads + kvh * p.chunks + chunk, tfirst = before * heads + (pair - b * heads) * tb,
+                       tlast = tfirst + tb - 1;
+        const uint32_t c0 = tc_owner(tfirst, T_, p.workers), c1 = tc_owner(tlast, T_, p.workers);
+        for (uint32_t i = warp; i < (c1 - c0 + 1) * p.halves; i += NW) {
+            const uint32_t c = c0 + i / p.halves, half = i % p.halves;
+            const uint32_t f0 = (uint32_t)((uint64_t)c * T_ / p.workers), f1 = (uint32_t)((uint64_t)(c + 1) * T_ / p.workers);
+            const uint32_t a = max(f0, tfirst), e = min(f1, tlast + 1);
+            if (a >= e || (e - a < p.halves && ((a - f0) ^ half) & 1)) continue;  // no tile, or the other half's one tile
+            const uint64_t slot = (((uint64_t)c + pair) * p.halves + half) * p.nr + h;
+            const float ms = p.part_ml[slot * 2], ls = p.part_ml[slot * 2 + 1];
+            float o[DPL];
+#pragma unroll
+            for (int k = 0; k < DPL; ++k) {
+                const uint32_t d = lane + 32 * k;
+                o[k] = d < D ? p.part_o[slot * D + d] : 0.0f;
+            }
+            if (ls == 0.0f) continue;
+            const float mn = fmaxf(M, ms);
+            const float cr = M == -INFINITY ? 0.0f : ex2_approx(fsub(M, mn)), x = ex2_approx(fsub(ms, mn));
+            L = __fmaf_rn(ls, x, fmul(L, cr));
+#pragma unroll
+            for (int k = 0; k < DPL; ++k) acc[k] = __fmaf_rn(o[k], x, fmul(acc[k], cr));
+            M = mn;
+        }
+    }
+    if (lane == 0) {
+        wm[warp] = M;
+        wl[warp] = L;
+    }
+#pragma unroll
+    for (int k = 0; k < DPL; ++k) wo[warp][lane + 32 * k] = acc[k];
+    __syncthreads();
+    for (uint32_t d = threadIdx.x; d < D; d += 256) {
+        float mx = -INFINITY, ls = 0.0f, o = 0.0f;
+#pragma unroll
+        for (int i = 0; i < NW; ++i) mx = fmaxf(mx, wm[i]);
+#pragma unroll
+        for (int i = 0; i < NW; ++i) {
+            if (wl[i] == 0.0f) continue;
+            const float x = ex2_approx(fsub(wm[i], mx));
+            ls = __fmaf_rn(wl[i], x, ls);
+            o = __fmaf_rn(wo[i][d], x, o);
+        }
+        float y = ls == 0.0f ? 0.0f : fdiv(o, ls);
+        if (failed) y = q8_nan();
+        Vec<T>::store1(out + (uint64_t)bh * D + d, y);
+    }
+}
+
+int q8_block_shift(uint64_t block);
+int q8_cache_check(const char* name, uint64_t batch, uint64_t kv_heads, uint64_t max_seq, uint64_t head_dim,
+                   uint64_t block);
+
+template <int NR, int NG, bool D4>
+static cudaError_t launch_warp(Q8AttnArgs& a, cudaStream_t st) {
+    auto kern = decode_attn_q8_warp_kernel<NR, NG, D4>;
+    const size_t smem = (size_t)QW_WARPS * NR * ((a.head_dim + 3) & ~3u) * 4 + (a.batch + 1) * 4;
+    if (!ensure_dyn_smem(reinterpret_cast<const void*>(kern), smem)) return cudaErrorInvalidConfiguration;
+    // one worker a resident warp, as many as the workspace has parts for
+    uint64_t ctas = (uint64_t)resident_blocks(reinterpret_cast<const void*>(kern), QW_WARPS * 32, smem);
+    if (ctas > Q8A_PARTS / QW_WARPS) ctas = Q8A_PARTS / QW_WARPS;
+    const uint64_t tiles = (uint64_t)a.batch * a.kv_heads * a.chunks * ((a.max_seq + QW_TK - 1) / QW_TK);
+    if (ctas > (tiles + QW_WARPS - 1) / QW_WARPS) ctas = (tiles + QW_WARPS - 1) / QW_WARPS;
+    a.workers = (uint32_t)ctas * QW_WARPS;
+    return launch_k(kern, (unsigned)ctas, QW_WARPS * 32, smem, st, a);
+}
+template <int NR>
+static cudaError_t launch_warp_d(Q8AttnArgs& a, bool d4, cudaStream_t st) {
+    if (!d4) return launch_warp<NR, 8, false>(a, st);
+    return a.head_dim <= 128 ? launch_warp<NR, 1, true>(a, st) : launch_warp<NR, 2, true>(a, st);
+}
+
+static uint64_t attn_q8_parts(uint64_t batch, uint64_t q_heads, uint64_t kv_heads) {
+    // pairs: pieces of up to 8 query heads of each kv head; workers * halves <= Q8A_PARTS
+    const uint64_t rep = kv_heads ? q_heads / kv_heads : 0, chunks = (rep + 7) / 8;
+    return 2 * batch * kv_heads * chunks + Q8A_PARTS;
+}
+static uint64_t attn_q8_nr(uint64_t q_heads, uint64_t kv_heads) {
+    const uint64_t rep = kv_heads ? q_heads / kv_heads : 0;
+    return rep <= 1 ? 1 : (rep <= 2 ? 2 : (rep <= 4 ? 4 : 8));
+}
+
+template <typename T>
+static int attn_q8_entry(const char* name, const T* q, const int8_t* kc, const int8_t* vc, const float* ks,
+                         const float* vs, const int32_t* lens, T* out, uint64_t batch, uint64_t q_heads,
+                         uint64_t kv_heads, uint64_t max_seq, uint64_t head_dim, uint64_t block, float scale, void* ws,
+                         uint64_t ws_bytes, cudaStream_t st) {
+    OXIDE_INJECT(name);
+    if (int rc = q8_cache_check(name, batch, kv_heads, max_seq, head_dim, block)) return rc;
+    if (batch == 0 || q_heads == 0) return OXIDE_OK;
+    OXIDE_REQUIRE(q && kc && vc && ks && vs && out, name, "null pointer");
+    OXIDE_REQUIRE(kv_heads >= 1 && q_heads % kv_heads == 0, name, "q_heads must be a multiple of kv_heads");
+    OXIDE_REQUIRE(head_dim >= 1 && head_dim <= Q8A_MAX_D, name, "head_dim must be in [1, 256]");
+    OXIDE_REQUIRE(q_heads < (1u << 20) && max_seq >= 1, name, "q_heads must be < 2^20 and max_seq >= 1");
+    OXIDE_REQUIRE(batch <= Q8A_MAX_BATCH && batch * q_heads < (1ull << 31), name,
+                  "batch must be <= 4096 and batch * q_heads < 2^31");
+    OXIDE_REQUIRE(out != q, name, "out must not alias q");
+    const uint64_t rep = q_heads / kv_heads, nr = attn_q8_nr(q_heads, kv_heads), chunks = (rep + 7) / 8;
+    // the flattened tile index is 32 bits wide (tiles of at least 32 keys)
+    OXIDE_REQUIRE(batch * kv_heads * chunks * ((max_seq + QW_TK - 1) / QW_TK) < (1ull << 31), name,
+                  "too many keys for one call: batch * kv_heads * max_seq must be < 2^36 (for up to 8 query heads a kv head)");
+    const uint64_t need = oxide_decode_attention_q8_workspace_bytes(batch, q_heads, kv_heads, head_dim);
+    if (!ws || ws_bytes < need || !aligned16(ws))
+        return set_error(OXIDE_ERR_WORKSPACE, "%s: workspace must be 16-byte aligned and >= %llu bytes", name,
+                         (unsigned long long)need);
+    const uint64_t parts = attn_q8_parts(batch, q_heads, kv_heads);
+    Q8AttnArgs a{};
+    a.kc = kc;
+    a.vc = vc;
+    a.ks = ks;
+    a.vs = vs;
+    a.q = q;
+    a.lens = lens;
+    a.part_o = static_cast<float*>(ws);
+    a.part_ml = a.part_o + parts * nr * head_dim;
+    a.err = reinterpret_cast<uint32_t*>(a.part_ml + parts * nr * 2);
+    a.pre_out = a.err + 4;
+    a.max_seq = max_seq;
+    a.batch = (uint32_t)batch;
+    a.q_heads = (uint32_t)q_heads;
+    a.kv_heads = (uint32_t)kv_heads;
+    a.head_dim = (uint32_t)head_dim;
+    a.rep = (uint32_t)rep;
+    a.chunks = (uint32_t)chunks;
+    a.nr = (uint32_t)nr;
+    a.shift = (uint32_t)q8_block_shift(block);
+    a.nblk = (uint32_t)((max_seq + block - 1) / block);
+    a.halves = 1;
+    a.q_bf16 = sizeof(T) == 2;
+    a.c1 = scale * 1.4426950408889634f;
+    cudaError_t e = cudaSuccess;
+    const uint64_t word = head_dim % 16 == 0 ? 16 : 4;
+    const bool d4 = head_dim % 4 == 0 && (reinterpret_cast<uintptr_t>(kc) & (word - 1)) == 0 &&
+                    (reinterpret_cast<uintptr_t>(vc) & 3) == 0;
+    switch (nr) {
+        case 1: e = launch_warp_d<1>(a, d4, st); break;
+        case 2: e = launch_warp_d<2>(a, d4, st); break;
+        case 4: e = launch_warp_d<4>(a, d4, st); break;
+        default: e = launch_warp_d<8>(a, d4, st); break;
+    }
+    if (e == cudaSuccess)
+        e = launch_k(decode_attn_q8_combine_kernel<T>, (unsigned)(batch * q_heads), 256, 0, st, out, a);
+    if (e != cudaSuccess) {
+        cudaGetLastError();
+        return set_error(OXIDE_ERR_LAUNCH, "%s: launch failed: %s", name, cudaGetErrorString(e));
+    }
+    return check_launch(name);
+}
+
+}  // namespace oxide
+
+using oxide::bf16_t;
+
+extern "C" {
+
+uint64_t oxide_decode_attention_q8_workspace_bytes(uint64_t batch, uint64_t q_heads, uint64_t kv_heads,
+                                                   uint64_t head_dim) {
+    const uint64_t parts = oxide::attn_q8_parts(batch, q_heads, kv_heads);
+    return parts * oxide::attn_q8_nr(q_heads, kv_heads) * (head_dim + 2) * 4 + 16 + (batch + 4) / 4 * 16;
+}
+int oxide_decode_attention_q8_f32(const float* q, const int8_t* k_cache, const int8_t* v_cache, const float* k_scale,
+                                  const float* v_scale, const int32_t* lens, float* out, uint64_t batch,
+                                  uint64_t q_heads, uint64_t kv_heads, uint64_t max_seq, uint64_t head_dim,
+                                  uint64_t block, float scale, void* workspace, uint64_t workspace_bytes,
+                                  oxide_stream_t stream) {
+    return oxide::attn_q8_entry<float>("oxide_decode_attention_q8_f32", q, k_cache, v_cache, k_scale, v_scale, lens,
+                                       out, batch, q_heads, kv_heads, max_seq, head_dim, block, scale, workspace,
+                                       workspace_bytes, stream);
+}
+int oxide_decode_attention_q8_bf16(const oxide_bf16* q, const int8_t* k_cache, const int8_t* v_cache,
+                                   const float* k_scale, const float* v_scale, const int32_t* lens, oxide_bf16* out,
+                                   uint64_t batch, uint64_t q_heads, uint64_t kv_heads, uint64_t max_seq,
+                                   uint64_t head_dim, uint64_t block, float scale, void* workspace,
+                                   uint64_t workspace_bytes, oxide_stream_t stream) {
+    return oxide::attn_q8_entry<bf16_t>("oxide_decode_attention_q8_bf16", q, k_cache, v_cache, k_scale, v_scale,
+                                        lens, out, batch, q_heads, kv_heads, max_seq, head_dim, block, scale,
+                                        workspace, workspace_bytes, stream);
+}
+
+}  // extern "C"

@@ -1,0 +1,458 @@
+// k_kvcache_q8.cu -- KV cache held as int8 codes: quantised as it is written,
+// and read back.
+//
+// Caches [batch, kv_heads, max_seq, head_dim] int8 with f32 scales [batch,
+// kv_heads, nblk], one for each block of `block` consecutive positions of a
+// head (nblk = ceil(max_seq / block)); a code c stands for c * scale.  The
+// unquantised append is KVCache::update (src/cache/kv_cache.rs:55-85); the
+// 8-bit form has no counterpart in the reference.
+//
+// Append.  A block that receives tokens needs the scale need = max|x| / 127
+// over the tokens it receives.  If it holds no token of its sequence yet (it
+// starts at or behind the sequence's cached length) its scale becomes need;
+// otherwise max(old, need), and where that is larger than the old scale the
+// codes of the tokens it holds are restated, c' = nearest(c old / new) -- at
+// most one more rounding of half a step each time the scale grows, and none
+// for blocks written whole.  c' depends on |c| only, so the 128 quotients are
+// computed once into a table and the codes looked up.
+//
+// Layout.  An item is one touched block of one head of k or v: its new tokens
+// are one contiguous run in the source and in the cache, so a warp (runs of
+// at most 128 16-byte vectors) or a CTA loads the run once into registers,
+// reduces, and writes the codes: each byte crosses HBM once.  Bound by HBM
+// bytes for prompts, by launch latency for single tokens.
+//
+// Read back is one pass, x = c * scale rounded to the output type.
+#include "oxide_q8.cuh"
+
+namespace oxide {
+
+struct AppendQ8Args {
+    uint64_t max_seq, cur_len, new_len;
+    const int32_t* cur_lens;   // per sequence; NULL: cur_len
+    const int32_t* new_lens;   // per sequence; NULL: new_len
+    uint32_t heads, kv_heads;  // batch * kv_heads, kv_heads
+    uint32_t head_dim, nblk, shift, wide;  // block = 1 << shift; wide: blocks an append can touch
+    uint32_t items;            // 2 * heads * wide
+};
+
+// One item: the block, the positions [lo, hi) it receives, where they come
+// from and go to.
+struct AppendItem {
+    bool is_v;
+    uint32_t bh, blk;
+    uint64_t lo, hi, start;  // new positions; the block's first position
+    uint64_t src;            // first new row in k / v, counted in rows
+    bool holds;              // tokens of this sequence before lo are in the block
+};
+__device__ __forceinline__ bool append_item(const AppendQ8Args& p, uint32_t i, AppendItem& it) {
+    const uint32_t half = p.heads * p.wide;
+    it.is_v = i >= half;
+    const uint32_t r = it.is_v ? i - half : i;
+    it.bh = r / p.wide;
+    const uint32_t j = r - it.bh * p.wide, b = it.bh / p.kv_heads;
+    uint64_t cur = p.cur_len, n = p.new_len;
+    if (p.cur_lens) {
+        const int32_t c = p.cur_lens[b];
+        if (c < 0 || (uint64_t)c > p.max_seq) return false;
+        cur = (uint64_t)c;
+    }
+    if (p.new_lens) {
+        const int32_t c = p.new_lens[b];
+        n = c <= 0 ? 0 : ((uint64_t)c < n ? (uint64_t)c : n);
+    }
+    if (n == 0 || n > p.max_seq - cur) return false;  // nothing to write, or it does not fit: the sequence is left as it is
+    const uint64_t blk = (cur >> p.shift) + j;
+    it.start = blk << p.shift;
+    const uint64_t end = cur + n, stop = it.start + (1ull << p.shift);
+    if (it.start >= end) return false;
+    it.blk = (uint32_t)blk;
+    it.lo = it.start > cur ? it.start : cur;
+    it.hi = stop < end ? stop : end;
+    it.src = (uint64_t)it.bh * p.new_len + (it.lo - cur);
+    it.holds = it.start < cur;
+    return true;
+}
+
+// The block's scale after this append, and whether its codes are restated.
+// Scales are compared as bits, which carries a NaN along.
+__device__ __forceinline__ float append_scale(const AppendItem& it, float had, uint32_t amax, bool& grown) {
+    const float need = q8_scale_of(amax);
+    grown = false;
+    if (!it.holds) return need;
+    const uint32_t a = q8_abs_bits(had), b = q8_abs_bits(need);
+    if (b <= a) return __uint_as_float(a);
+    grown = b < Q8_INF;
+    return need;
+}
+
+// Restate the codes of positions [start, lo) from scale `had` to scale `s`.
+// `lut` (128 bytes of shared memory) is this group's own; TPI threads take part.
+template <int TPI>
+__device__ __forceinline__ void append_restate(int8_t* head, const AppendQ8Args& p, const AppendItem& it, float had,
+                                               float s, uint8_t* lut, uint32_t t) {
+    const Q8Coder coder((double)had, (double)s);
+    for (uint32_t i = t; i < 128; i += TPI) lut[i] = (uint8_t)coder.exact((double)i);
+    if (TPI == 32) __syncwarp();
+    else __syncthreads();
+    int8_t* c = head + it.start * p.head_dim;
+    const uint64_t n = (it.lo - it.start) * p.head_dim;
+    auto restate = [&](int v) -> uint32_t {
+        const int a = v < 0 ? (v < -127 ? 127 : -v) : v;
+        const int q = lut[a];
+        return (uint32_t)(v < 0 ? -q : q) & 0xffu;
+    };
+    if (p.head_dim % 4 == 0 && (reinterpret_cast<uintptr_t>(c) & 3) == 0) {
+        uint32_t* w = reinterpret_cast<uint32_t*>(c);
+#pragma unroll 4
+        for (uint64_t i = t; i < n / 4; i += TPI) {
+            const uint32_t v = w[i];
+            w[i] = restate((int8_t)v) | restate((int8_t)(v >> 8)) << 8 | restate((int8_t)(v >> 16)) << 16 |
+                   restate((int8_t)(v >> 24)) << 24;
+        }
+    } else {
+        for (uint64_t i = t; i < n; i += TPI) c[i] = (int8_t)restate(c[i]);
+    }
+}
+
+// Largest |x| bits over the group's threads (contains __syncthreads() for a CTA).
+template <int TPI>
+__device__ __forceinline__ uint32_t append_max(uint32_t a) {
+    a = q8_warp_max(a);
+    if (TPI == 32) return a;
+    __shared__ uint32_t red[32];
+    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = a;
+    __syncthreads();
+    a = red[0];
+#pragma unroll
+    for (int i = 1; i < TPI / 32; ++i) a = max(a, red[i]);
+    __syncthreads();
+    return a;
+}
+
+// TPI threads an item (32: eight items per CTA), VPT vectors a thread.
+template <typename T, int TPI, int VPT>
+__global__ void __launch_bounds__(TPI == 32 ? 256 : TPI)
+    kv_append_q8_vec_kernel(int8_t* kc, int8_t* vc, float* ks, float* vs, const T* k, const T* v, AppendQ8Args p) {
+    pdl_begin();
+    constexpr int V = Vec<T>::N, IPC = TPI == 32 ? 8 : 1;
+    __shared__ uint8_t luts[IPC][128];
+    const uint32_t t = TPI == 32 ? threadIdx.x & 31 : threadIdx.x, g = TPI == 32 ? threadIdx.x >> 5 : 0;
+    for (uint64_t i = (uint64_t)blockIdx.x * IPC + g; i < p.items; i += (uint64_t)gridDim.x * IPC) {
+        AppendItem it;
+        if (!append_item(p, (uint32_t)i, it)) continue;  // the same for the whole group
+        const T* src = (it.is_v ? v : k) + it.src * p.head_dim;
+        int8_t* head = (it.is_v ? vc : kc) + (uint64_t)it.bh * p.max_seq * p.head_dim;
+        float* sp = (it.is_v ? vs : ks) + (uint64_t)it.bh * p.nblk + it.blk;
+        const uint32_t nvec = (uint32_t)((it.hi - it.lo) * p.head_dim / V);
+        uint4 raw[VPT];
+#pragma unroll
+        for (int u = 0; u < VPT; ++u)
+            if (t + u * TPI < nvec) raw[u] = ld_stream(src + (uint64_t)(t + u * TPI) * V);
+        const float had = it.holds ? *reinterpret_cast<volatile float*>(sp) : 0.0f;
+        uint32_t a = 0;
+#pragma unroll
+        for (int u = 0; u < VPT; ++u)
+            if (t + u * TPI < nvec) a = q8_vec_amax(raw[u], a, T());
+        a = append_max<TPI>(q8_amax_join(a, T()));  // also: every thread has read the old scale
+        bool grown;
+        const float s = append_scale(it, had, a, grown);
+        if (t == 0) *sp = s;
+        const Q8Coder coder(s);
+        int8_t* dst = head + it.lo * p.head_dim;
+#pragma unroll
+        for (int u = 0; u < VPT; ++u)
+            if (t + u * TPI < nvec) {
+                float x[V];
+                uint32_t c[V / 4];
+                Vec<T>::unpack(raw[u], x);
+                q8_codes<V>(coder, x, c);
+                q8_store(dst + (uint64_t)(t + u * TPI) * V, c);
+            }
+        if (grown) {
+            append_restate<TPI>(head, p, it, had, s, luts[g], t);
+            if (TPI == 32) __syncwarp();  // the table is written again for the next item
+            else __syncthreads();
+        }
+    }
+}
+
+// Any head size and alignment: the run is read twice.
+template <typename T, int TPI>
+__global__ void __launch_bounds__(256)
+    kv_append_q8_scalar_kernel(int8_t* kc, int8_t* vc, float* ks, float* vs, const T* k, const T* v, AppendQ8Args p) {
+    pdl_begin();
+    constexpr int IPC = 256 / TPI;
+    __shared__ uint8_t luts[IPC][128];
+    const uint32_t t = threadIdx.x % TPI, g = threadIdx.x / TPI;
+    for (uint64_t i = (uint64_t)blockIdx.x * IPC + g; i < p.items; i += (uint64_t)gridDim.x * IPC) {
+        AppendItem it;
+        if (!append_item(p, (uint32_t)i, it)) continue;
+        const T* src = (it.is_v ? v : k) + it.src * p.head_dim;
+        int8_t* head = (it.is_v ? vc : kc) + (uint64_t)it.bh * p.max_seq * p.head_dim;
+        float* sp = (it.is_v ? vs : ks) + (uint64_t)it.bh * p.nblk + it.blk;
+        const uint32_t n = (uint32_t)((it.hi - it.lo) * p.head_dim);
+        const float had = it.holds ? *reinterpret_cast<volatile float*>(sp) : 0.0f;
+        uint32_t a = 0;
+        for (uint32_t e = t; e < n; e += TPI) a = max(a, q8_abs_bits(Vec<T>::load1(src + e)));
+        a = append_max<TPI>(a);
+        bool grown;
+        const float s = append_scale(it, had, a, grown);
+        if (t == 0) *sp = s;
+        const Q8Coder coder(s);
+        int8_t* dst = head + it.lo * p.head_dim;
+        for (uint32_t e = t; e < n; e += TPI) {
+            const float x = Vec<T>::load1(src + e);
+            float near = 0.0f;
+            const float2 q = coder.fast2(f2(x, x), near);
+            int c = (int)(int8_t)(__float_as_uint(q.x) & 0xffu);
+            if (coder.slow || near > Q8_NEAR) c = coder.exact((double)x);
+            dst[e] = (int8_t)c;
+        }
+        if (grown) {
+            append_restate<TPI>(head, p, it, had, s, luts[g], t);
+            if (TPI == 32) __syncwarp();
+            else __syncthreads();
+        }
+    }
+}
+
+struct ReadQ8Args {
+    uint64_t max_seq, start, n;  // positions [start, start + n) of every head
+    const int32_t* lens;         // per sequence; NULL: all positions
+    uint32_t heads, kv_heads, head_dim, nblk, shift;
+};
+
+// How many of the n positions of this sequence hold a token.
+__device__ __forceinline__ uint64_t read_live(const ReadQ8Args& p, uint32_t bh) {
+    if (!p.lens) return p.n;
+    const int32_t l = p.lens[bh / p.kv_heads];
+    if (l <= 0 || (uint64_t)l <= p.start) return 0;
+    return (uint64_t)l - p.start < p.n ? (uint64_t)l - p.start : p.n;
+}
+
+// One 16-byte output vector (V codes) a step, RQ_UNROLL steps in flight.
+constexpr int RQ_UNROLL = 4;
+template <typename T>
+__global__ void __launch_bounds__(256)
+    kv_read_q8_vec_kernel(const int8_t* kc, const int8_t* vc, const float* ks, const float* vs, T* k, T* v,
+                          ReadQ8Args p, uint64_t half, FastDiv rdiv, FastDiv ndiv, bool narrow) {
+    pdl_begin();
+    constexpr int V = Vec<T>::N;
+    const uint32_t per_row = p.head_dim / V;
+    const uint64_t stride = (uint64_t)gridDim.x * 256;
+    for (uint64_t i0 = (uint64_t)blockIdx.x * 256 + threadIdx.x; i0 < 2 * half; i0 += stride * RQ_UNROLL) {
+        uint32_t c[RQ_UNROLL][V / 4];
+        float s[RQ_UNROLL];
+#pragma unroll
+        for (int u = 0; u < RQ_UNROLL; ++u) {
+            const uint64_t i = i0 + u * stride;
+            s[u] = 0.0f;
+#pragma unroll
+            for (int e = 0; e < V / 4; ++e) c[u][e] = 0;
+            if (i >= 2 * half) continue;
+            const bool is_v = i >= half;
+            const uint64_t r = is_v ? i - half : i;
+            uint64_t row, bh;
+            if (narrow) {
+                row = rdiv.div((uint32_t)r);
+                bh = ndiv.div((uint32_t)row);
+            } else {
+                row = r / per_row;
+                bh = row / p.n;
+            }
+            const uint64_t at = row - bh * p.n;
+            if (at >= read_live(p, (uint32_t)bh)) continue;
+            const uint64_t pos = p.start + at;
+            const int8_t* src = (is_v ? vc : kc) + (bh * p.max_seq + pos) * p.head_dim + (r - row * per_row) * V;
+            if (V == 8) {
+                const uint2 w = __ldcs(reinterpret_cast<const uint2*>(src));
+                c[u][0] = w.x;
+                c[u][V / 4 - 1] = w.y;
+            } else {
+                c[u][0] = __ldcs(reinterpret_cast<const unsigned int*>(src));
+            }
+            s[u] = __ldg((is_v ? vs : ks) + bh * p.nblk + (pos >> p.shift));
+        }
+#pragma unroll
+        for (int u = 0; u < RQ_UNROLL; ++u) {
+            const uint64_t i = i0 + u * stride;
+            if (i >= 2 * half) break;
+            float x[V];
+#pragma unroll
+            for (int e = 0; e < V; e += 4) {
+                float f[4];
+                q8_unpack4(c[u][e / 4], f);
+#pragma unroll
+                for (int d = 0; d < 4; ++d) x[e + d] = fmul(f[d], s[u]);
+            }
+            st_stream((i >= half ? v + (i - half) * V : k + i * V), Vec<T>::pack(x));
+        }
+    }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(256)
+    kv_read_q8_scalar_kernel(const int8_t* kc, const int8_t* vc, const float* ks, const float* vs, T* k, T* v,
+                             ReadQ8Args p, uint64_t half) {
+    pdl_begin();
+    for (uint64_t i = (uint64_t)blockIdx.x * 256 + threadIdx.x; i < 2 * half; i += (uint64_t)gridDim.x * 256) {
+        const bool is_v = i >= half;
+        const uint64_t r = is_v ? i - half : i, row = r / p.head_dim, bh = row / p.n, at = row - bh * p.n;
+        float x = 0.0f;
+        if (at < read_live(p, (uint32_t)bh)) {
+            const uint64_t pos = p.start + at;
+            x = fmul((float)(is_v ? vc : kc)[(bh * p.max_seq + pos) * p.head_dim + (r - row * p.head_dim)],
+                     __ldg((is_v ? vs : ks) + bh * p.nblk + (pos >> p.shift)));
+        }
+        Vec<T>::store1((is_v ? v : k) + r, x);
+    }
+}
+
+// log2 of a block size the caches can have, or -1.
+int q8_block_shift(uint64_t block) {
+    for (int s = 0; s <= 7; ++s)
+        if (block == (1ull << s)) return s;
+    return -1;
+}
+
+// Checks shared by the entry points of the int8 cache; OXIDE_OK or an error.
+int q8_cache_check(const char* name, uint64_t batch, uint64_t kv_heads, uint64_t max_seq, uint64_t head_dim,
+                   uint64_t block) {
+    OXIDE_REQUIRE(q8_block_shift(block) >= 0, name, "block must be a power of two in [1, 128]");
+    OXIDE_REQUIRE(head_dim < (1u << 16), name, "head_dim must be < 65536");
+    OXIDE_REQUIRE(max_seq < (1ull << 31), name, "max_seq must be < 2^31");
+    OXIDE_REQUIRE(batch < (1ull << 31) && kv_heads < (1ull << 31) && batch * kv_heads < (1ull << 31), name,
+                  "batch * kv_heads must be < 2^31");
+    // heads < 2^31, max_seq < 2^31: their product and the row bytes stay below 2^62 x 2^16
+    OXIDE_REQUIRE(batch == 0 || kv_heads == 0 || head_dim == 0 ||
+                      max_seq <= (UINT64_MAX >> 3) / head_dim / (batch * kv_heads), name, "cache size overflows");
+    return OXIDE_OK;
+}
+
+static bool aligned_to(const void* p, uint64_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
+
+template <typename T>
+static int append_q8_entry(const char* name, int8_t* kc, int8_t* vc, float* ks, float* vs, const T* k, const T* v,
+                           uint64_t batch, uint64_t kv_heads, uint64_t max_seq, uint64_t head_dim, uint64_t block,
+                           uint64_t cur_len, const int32_t* cur_lens, uint64_t new_len, const int32_t* new_lens,
+                           cudaStream_t st) {
+    OXIDE_INJECT(name);
+    if (int rc = q8_cache_check(name, batch, kv_heads, max_seq, head_dim, block)) return rc;
+    OXIDE_REQUIRE(new_len <= max_seq && (cur_lens || cur_len <= max_seq - new_len), name,
+                  "KV cache overflow: cur_len + new_len > max_seq");
+    if (batch == 0 || kv_heads == 0 || new_len == 0 || head_dim == 0) return OXIDE_OK;
+    OXIDE_REQUIRE(kc && vc && ks && vs && k && v, name, "null pointer");
+    OXIDE_REQUIRE(kc != vc && ks != vs, name, "the key and value caches must not alias");
+    constexpr uint64_t V = Vec<T>::N;
+    AppendQ8Args p{};
+    p.max_seq = max_seq;
+    p.cur_len = cur_len;
+    p.new_len = new_len;
+    p.cur_lens = cur_lens;
+    p.new_lens = new_lens;
+    p.heads = (uint32_t)(batch * kv_heads);
+    p.kv_heads = (uint32_t)kv_heads;
+    p.head_dim = (uint32_t)head_dim;
+    p.shift = (uint32_t)q8_block_shift(block);
+    p.nblk = (uint32_t)((max_seq + block - 1) / block);
+    const uint64_t wide = (new_len + block - 2) / block + 1;  // a run of new_len positions meets at most so many blocks
+    p.wide = (uint32_t)(wide < p.nblk ? wide : p.nblk);
+    const uint64_t items = 2ull * p.heads * p.wide;
+    OXIDE_REQUIRE(items < (1ull << 32), name, "too many blocks for one call (2^32): append fewer tokens at a time");
+    p.items = (uint32_t)items;
+    const uint64_t run = (block < new_len ? block : new_len) * head_dim;  // elements of the longest item
+    const uint64_t cap = 1ull << 30, warps = (items + 7) / 8 < cap ? (items + 7) / 8 : cap,
+                   ctas = items < cap ? items : cap;
+    const bool vec = head_dim % V == 0 && aligned16(k) && aligned16(v) && aligned_to(kc, V) && aligned_to(vc, V) &&
+                     run / V <= 4096;
+    if (!vec) {
+        if (run <= 1024) launch_k(kv_append_q8_scalar_kernel<T, 32>, (unsigned)warps, 256, 0, st, kc, vc, ks, vs, k, v, p);
+        else launch_k(kv_append_q8_scalar_kernel<T, 256>, (unsigned)ctas, 256, 0, st, kc, vc, ks, vs, k, v, p);
+    } else if (run / V <= 128) {
+        launch_k(kv_append_q8_vec_kernel<T, 32, 4>, (unsigned)warps, 256, 0, st, kc, vc, ks, vs, k, v, p);
+    } else if (run / V <= 1024) {
+        launch_k(kv_append_q8_vec_kernel<T, 256, 4>, (unsigned)ctas, 256, 0, st, kc, vc, ks, vs, k, v, p);
+    } else {
+        launch_k(kv_append_q8_vec_kernel<T, 1024, 4>, (unsigned)ctas, 1024, 0, st, kc, vc, ks, vs, k, v, p);
+    }
+    return check_launch(name);
+}
+
+template <typename T>
+static int read_q8_entry(const char* name, const int8_t* kc, const int8_t* vc, const float* ks, const float* vs, T* k,
+                         T* v, uint64_t batch, uint64_t kv_heads, uint64_t max_seq, uint64_t head_dim, uint64_t block,
+                         uint64_t start, uint64_t n, const int32_t* lens, cudaStream_t st) {
+    OXIDE_INJECT(name);
+    if (int rc = q8_cache_check(name, batch, kv_heads, max_seq, head_dim, block)) return rc;
+    OXIDE_REQUIRE(n <= max_seq && start <= max_seq - n, name, "positions out of range: start + n > max_seq");
+    if (batch == 0 || kv_heads == 0 || n == 0 || head_dim == 0) return OXIDE_OK;
+    OXIDE_REQUIRE(kc && vc && ks && vs && k && v, name, "null pointer");
+    OXIDE_REQUIRE(k != v, name, "the key and value outputs must not alias");
+    constexpr uint64_t V = Vec<T>::N;
+    ReadQ8Args p{};
+    p.max_seq = max_seq;
+    p.start = start;
+    p.n = n;
+    p.lens = lens;
+    p.heads = (uint32_t)(batch * kv_heads);
+    p.kv_heads = (uint32_t)kv_heads;
+    p.head_dim = (uint32_t)head_dim;
+    p.shift = (uint32_t)q8_block_shift(block);
+    p.nblk = (uint32_t)((max_seq + block - 1) / block);
+    const uint64_t elems = (uint64_t)p.heads * n * head_dim;
+    const bool vec = head_dim % V == 0 && aligned16(k) && aligned16(v) && aligned_to(kc, V) && aligned_to(vc, V);
+    const uint64_t half = vec ? elems / V : elems;
+    const void* kern = vec ? reinterpret_cast<const void*>(kv_read_q8_vec_kernel<T>)
+                           : reinterpret_cast<const void*>(kv_read_q8_scalar_kernel<T>);
+    const uint64_t want = (2 * half + 255) / 256, cap = (uint64_t)resident_blocks(kern, 256, 0);
+    const unsigned grid = (unsigned)(want < cap ? want : cap);
+    if (vec) {
+        const bool narrow = half < (1ull << 32);
+        launch_k(kv_read_q8_vec_kernel<T>, grid, 256, 0, st, kc, vc, ks, vs, k, v, p, half,
+                 FastDiv((uint32_t)(head_dim / V)), FastDiv((uint32_t)n), narrow);
+    } else {
+        launch_k(kv_read_q8_scalar_kernel<T>, grid, 256, 0, st, kc, vc, ks, vs, k, v, p, half);
+    }
+    return check_launch(name);
+}
+
+}  // namespace oxide
+
+using oxide::bf16_t;
+
+extern "C" {
+
+int oxide_kv_cache_append_q8_f32(int8_t* k_cache, int8_t* v_cache, float* k_scale, float* v_scale, const float* k,
+                                 const float* v, uint64_t batch, uint64_t kv_heads, uint64_t max_seq,
+                                 uint64_t head_dim, uint64_t block, uint64_t cur_len, const int32_t* cur_lens,
+                                 uint64_t new_len, const int32_t* new_lens, oxide_stream_t stream) {
+    return oxide::append_q8_entry<float>("oxide_kv_cache_append_q8_f32", k_cache, v_cache, k_scale, v_scale, k, v,
+                                         batch, kv_heads, max_seq, head_dim, block, cur_len, cur_lens, new_len,
+                                         new_lens, stream);
+}
+int oxide_kv_cache_append_q8_bf16(int8_t* k_cache, int8_t* v_cache, float* k_scale, float* v_scale,
+                                  const oxide_bf16* k, const oxide_bf16* v, uint64_t batch, uint64_t kv_heads,
+                                  uint64_t max_seq, uint64_t head_dim, uint64_t block, uint64_t cur_len,
+                                  const int32_t* cur_lens, uint64_t new_len, const int32_t* new_lens,
+                                  oxide_stream_t stream) {
+    return oxide::append_q8_entry<bf16_t>("oxide_kv_cache_append_q8_bf16", k_cache, v_cache, k_scale, v_scale, k, v,
+                                          batch, kv_heads, max_seq, head_dim, block, cur_len, cur_lens, new_len,
+                                          new_lens, stream);
+}
+int oxide_kv_cache_read_q8_f32(const int8_t* k_cache, const int8_t* v_cache, const float* k_scale,
+                               const float* v_scale, float* k, float* v, uint64_t batch, uint64_t kv_heads,
+                               uint64_t max_seq, uint64_t head_dim, uint64_t block, uint64_t start, uint64_t n,
+                               const int32_t* lens, oxide_stream_t stream) {
+    return oxide::read_q8_entry<float>("oxide_kv_cache_read_q8_f32", k_cache, v_cache, k_scale, v_scale, k, v, batch,
+                                       kv_heads, max_seq, head_dim, block, start, n, lens, stream);
+}
+int oxide_kv_cache_read_q8_bf16(const int8_t* k_cache, const int8_t* v_cache, const float* k_scale,
+                                const float* v_scale, oxide_bf16* k, oxide_bf16* v, uint64_t batch,
+                                uint64_t kv_heads, uint64_t max_seq, uint64_t head_dim, uint64_t block,
+                                uint64_t start, uint64_t n, const int32_t* lens, oxide_stream_t stream) {
+    return oxide::read_q8_entry<bf16_t>("oxide_kv_cache_read_q8_bf16", k_cache, v_cache, k_scale, v_scale, k, v,
+                                        batch, kv_heads, max_seq, head_dim, block, start, n, lens, stream);
+}
+
+}  // extern "C"

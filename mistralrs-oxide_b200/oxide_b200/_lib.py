@@ -43,6 +43,10 @@ SIGNATURES: dict[str, tuple] = {
     "oxide_rms_norm_bf16": (i32, [vp, vp, vp, u64, u64, f32, vp]),
     "oxide_add_rms_norm_f32": (i32, [vp, vp, vp, vp, vp, u64, u64, f32, vp]),
     "oxide_add_rms_norm_bf16": (i32, [vp, vp, vp, vp, vp, u64, u64, f32, vp]),
+    "oxide_rms_norm_q8_f32": (i32, [vp, vp, vp, vp, u64, u64, f32, vp]),
+    "oxide_rms_norm_q8_bf16": (i32, [vp, vp, vp, vp, u64, u64, f32, vp]),
+    "oxide_add_rms_norm_q8_f32": (i32, [vp, vp, vp, vp, vp, vp, u64, u64, f32, vp]),
+    "oxide_add_rms_norm_q8_bf16": (i32, [vp, vp, vp, vp, vp, vp, u64, u64, f32, vp]),
     "oxide_softmax_f32": (i32, [vp, vp, u64, u64, u64, vp]),
     "oxide_softmax_bf16": (i32, [vp, vp, u64, u64, u64, vp]),
     "oxide_scale_mask_softmax_f32": (i32, [vp, vp, u64, u64, f32, vp, u64, vp, u64, u64, vp]),
@@ -73,6 +77,13 @@ SIGNATURES: dict[str, tuple] = {
     "oxide_device_status": (i32, [i32, C.POINTER(C.c_uint32)]),
     "oxide_decode_attention_f32": (i32, [vp, vp, vp, vp, vp, u64, u64, u64, u64, u64, f32, vp, u64, vp]),
     "oxide_decode_attention_bf16": (i32, [vp, vp, vp, vp, vp, u64, u64, u64, u64, u64, f32, vp, u64, vp]),
+    "oxide_kv_cache_append_q8_f32": (i32, [vp] * 6 + [u64] * 6 + [vp, u64, vp, vp]),
+    "oxide_kv_cache_append_q8_bf16": (i32, [vp] * 6 + [u64] * 6 + [vp, u64, vp, vp]),
+    "oxide_kv_cache_read_q8_f32": (i32, [vp] * 6 + [u64] * 7 + [vp, vp]),
+    "oxide_kv_cache_read_q8_bf16": (i32, [vp] * 6 + [u64] * 7 + [vp, vp]),
+    "oxide_decode_attention_q8_workspace_bytes": (u64, [u64, u64, u64, u64]),
+    "oxide_decode_attention_q8_f32": (i32, [vp] * 7 + [u64] * 6 + [f32, vp, u64, vp]),
+    "oxide_decode_attention_q8_bf16": (i32, [vp] * 7 + [u64] * 6 + [f32, vp, u64, vp]),
     "oxide_sample_f32": (i32, [vp, u64, u64, f32, u64, f32, vp, vp, vp, vp]),
     "oxide_sample_bf16": (i32, [vp, u64, u64, f32, u64, f32, vp, vp, vp, vp]),
     "oxide_softmax_with_temperature_f32": (i32, [vp, vp, u64, u64, f32, vp]),

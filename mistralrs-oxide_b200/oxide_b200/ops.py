@@ -13,6 +13,7 @@ from __future__ import annotations
 import math
 from typing import Optional, Sequence
 
+import numpy as np
 import torch
 
 from . import _lib
@@ -64,6 +65,22 @@ def _p(t: Optional[torch.Tensor]):
 
 def _stream() -> int:
     return torch.cuda.current_stream().cuda_stream
+
+
+def _one_device(op: str, ref: torch.Tensor, **named: Optional[torch.Tensor]) -> None:
+    """Every named tensor lives where ref does."""
+    for name, t in named.items():
+        if t is not None:
+            _need(t.device == ref.device, op, f"{name} is on {t.device}, not on {ref.device}")
+
+
+def _call_on(ref: torch.Tensor, name: str, *args) -> None:
+    """Call an entry point on ref's device, on that device's current stream."""
+    if ref.device.index == torch.cuda.current_device():
+        call(name, *args, _stream())
+    else:
+        with torch.cuda.device(ref.device):
+            call(name, *args, _stream())
 
 
 def broadcast_shape(a: Sequence[int], b: Sequence[int]) -> list[int]:
@@ -303,6 +320,50 @@ def add_rms_norm(x: torch.Tensor, r: torch.Tensor, w: torch.Tensor, eps: float,
     call(f"oxide_add_rms_norm_{_sfx(x)}", _p(x), _p(r), _p(w), _p(h), _p(y), x.numel() // cols, cols,
          float(eps), _stream())
     return h, y
+
+
+def _norm_q8_out(op: str, x: torch.Tensor, out: Optional[torch.Tensor], scale: Optional[torch.Tensor]) -> None:
+    _need(out is None or (out.dtype == torch.int8 and out.numel() == x.numel()), op,
+          f"out must be int8 with {x.numel()} elements")
+    _need(scale is None or (scale.dtype == torch.float32 and scale.numel() == math.prod(x.shape[:-1])), op,
+          f"scale must be float32 with one value per row ({math.prod(x.shape[:-1])})")
+
+
+def rms_norm_q8(x: torch.Tensor, w: torch.Tensor, eps: float, out: Optional[torch.Tensor] = None,
+                scale: Optional[torch.Tensor] = None):
+    """(codes, scale): rms_norm (src/ops/norm.rs:4-51) whose rows leave as int8
+    codes with one f32 scale a row, scale = max|y| / 127, code = the integer
+    nearest to y / scale.  codes has x's shape, scale x.shape[:-1]."""
+    cols = _norm_check(x, w)
+    _need(cols >= 1, "rms_norm_q8", "rows must not be empty")
+    _norm_q8_out("rms_norm_q8", x, out, scale)
+    _check(x, w, out, scale)
+    _one_device("rms_norm_q8", x, weight=w, out=out, scale=scale)
+    out = torch.empty_like(x, dtype=torch.int8) if out is None else out
+    scale = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device) if scale is None else scale
+    _call_on(x, f"oxide_rms_norm_q8_{_sfx(x)}", _p(x), _p(w), _p(out), _p(scale), x.numel() // cols, cols, float(eps))
+    return out, scale
+
+
+def add_rms_norm_q8(x: torch.Tensor, r: torch.Tensor, w: torch.Tensor, eps: float,
+                    h: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None,
+                    scale: Optional[torch.Tensor] = None):
+    """(h, codes, scale): h = x + r (src/layers/transformer.rs:64-67), then
+    rms_norm_q8(h).  h may be x or r (in place)."""
+    cols = _norm_check(x, w)
+    _need(cols >= 1, "add_rms_norm_q8", "rows must not be empty")
+    _need(r.shape == x.shape and r.dtype == x.dtype, "add_rms_norm_q8",
+          "residual must match the input's shape and dtype")
+    _out_like("add_rms_norm_q8", x, h=h)
+    _norm_q8_out("add_rms_norm_q8", x, out, scale)
+    _check(x, r, w, h, out, scale)
+    _one_device("add_rms_norm_q8", x, residual=r, weight=w, h=h, out=out, scale=scale)
+    h = torch.empty_like(x) if h is None else h
+    out = torch.empty_like(x, dtype=torch.int8) if out is None else out
+    scale = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device) if scale is None else scale
+    _call_on(x, f"oxide_add_rms_norm_q8_{_sfx(x)}", _p(x), _p(r), _p(w), _p(h), _p(out), _p(scale),
+             x.numel() // cols, cols, float(eps))
+    return h, out, scale
 
 
 def softmax(x: torch.Tensor, dim: int) -> torch.Tensor:
@@ -578,6 +639,171 @@ def decode_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
     call(f"oxide_decode_attention_{_sfx(q)}", _p(q), _p(k_cache), _p(v_cache), _p(lens), _p(out), b, hq, hkv,
          m, d, float(scale), _p(workspace), workspace.numel() * workspace.element_size(), _stream())
     return out
+
+
+# ---- the int8 KV cache ----
+def _q8_cache_check(op: str, k_cache, v_cache, k_scale, v_scale, block: int) -> None:
+    _need(k_cache.dim() == 4 and k_cache.dtype == torch.int8 and v_cache.dtype == torch.int8 and
+          v_cache.shape == k_cache.shape, op,
+          f"caches must be int8 [batch, kv_heads, max_seq, head_dim] alike, got {k_cache.dtype} "
+          f"{list(k_cache.shape)} and {v_cache.dtype} {list(v_cache.shape)}")
+    _need(block in (1, 2, 4, 8, 16, 32, 64, 128), op, "block must be a power of two in [1, 128]")
+    want = [k_cache.shape[0], k_cache.shape[1], -(-k_cache.shape[2] // block)]
+    for name, t in (("k_scale", k_scale), ("v_scale", v_scale)):
+        _need(t.dtype == torch.float32 and list(t.shape) == want, op,
+              f"{name} must be float32 {want}, got {t.dtype} {list(t.shape)}")
+
+
+def _q8_lens(op: str, name: str, t: Optional[torch.Tensor], batch: int) -> None:
+    _need(t is None or (t.dtype == torch.int32 and t.numel() == batch), op, f"{name} must be int32 with {batch} entries")
+
+
+def kv_cache_append_q8(k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor,
+                       k: torch.Tensor, v: torch.Tensor, cur_len, block: int,
+                       new_lens: Optional[torch.Tensor] = None) -> None:
+    """Quantise k, v [batch, kv_heads, new_len, head_dim] (f32 or bf16) into int8
+    caches [batch, kv_heads, max_seq, head_dim] at positions cur_len.. of each
+    sequence (KVCache::update, src/cache/kv_cache.rs:55-85, for an 8-bit cache).
+    k_scale, v_scale [batch, kv_heads, ceil(max_seq / block)] hold one f32 scale
+    per block of positions and head, max|x| / 127; a block that already holds
+    tokens keeps the larger scale, and its codes are restated when it grows.
+    cur_len: an int, or an int32 device tensor with one length a sequence (a
+    sequence whose length is negative or whose tokens do not fit is left as it
+    is).  new_lens (int32 device tensor): tokens of a padded batch that count."""
+    op = "kv_cache_append_q8"
+    _q8_cache_check(op, k_cache, v_cache, k_scale, v_scale, block)
+    b, hkv, m, d = k_cache.shape
+    _need(k.dim() == 4 and k.shape == v.shape and k.shape[0] == b and k.shape[1] == hkv and k.shape[3] == d and
+          k.dtype == v.dtype, op,
+          f"key/value {list(k.shape)}, {list(v.shape)} do not match the cache {list(k_cache.shape)}")
+    each = cur_len if isinstance(cur_len, torch.Tensor) else None
+    _q8_lens(op, "cur_len", each, b)
+    _q8_lens(op, "new_lens", new_lens, b)
+    cur = 0 if each is not None else int(cur_len)
+    _need(cur >= 0, op, "cur_len must be >= 0")
+    _need(cur + k.shape[2] <= m, op, f"KV cache overflow: {cur + k.shape[2]} > {m}")
+    _check(k_cache, v_cache, k_scale, v_scale, k, v, each, new_lens)
+    _one_device(op, k_cache, v_cache=v_cache, k_scale=k_scale, v_scale=v_scale, key=k, value=v, cur_len=each,
+                new_lens=new_lens)
+    _call_on(k_cache, f"oxide_kv_cache_append_q8_{_sfx(k)}", _p(k_cache), _p(v_cache), _p(k_scale), _p(v_scale),
+             _p(k), _p(v), b, hkv, m, d, block, cur, _p(each), k.shape[2], _p(new_lens))
+
+
+def kv_cache_read_q8(k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor,
+                     block: int, start: int = 0, n: Optional[int] = None, lens: Optional[torch.Tensor] = None,
+                     dtype=torch.bfloat16, k: Optional[torch.Tensor] = None, v: Optional[torch.Tensor] = None):
+    """(k, v) [batch, kv_heads, n, head_dim] of positions [start, start + n) of
+    int8 caches (default: to the end), code * scale in dtype (f32 or bf16);
+    positions at or behind lens[b] (int32 device tensor) are zeros."""
+    op = "kv_cache_read_q8"
+    _q8_cache_check(op, k_cache, v_cache, k_scale, v_scale, block)
+    b, hkv, m, d = k_cache.shape
+    start, n = int(start), m - int(start) if n is None else int(n)
+    _need(0 <= start and 0 <= n and start + n <= m, op, f"positions [{start}, {start + n}) out of range for {m}")
+    _q8_lens(op, "lens", lens, b)
+    dtype = k.dtype if k is not None else v.dtype if v is not None else dtype
+    if dtype not in _SFX:
+        raise OxideError(_lib.ERR_UNSUPPORTED, op, f"dtype {dtype} is not float32/bfloat16")
+    for name, t in (("k", k), ("v", v)):
+        _need(t is None or (t.dtype == dtype and list(t.shape) == [b, hkv, n, d]), op,
+              f"{name} must be {dtype} {[b, hkv, n, d]}")
+    _check(k_cache, v_cache, k_scale, v_scale, lens, k, v)
+    _one_device(op, k_cache, v_cache=v_cache, k_scale=k_scale, v_scale=v_scale, lens=lens, k=k, v=v)
+    k = torch.empty((b, hkv, n, d), dtype=dtype, device=k_cache.device) if k is None else k
+    v = torch.empty((b, hkv, n, d), dtype=dtype, device=k_cache.device) if v is None else v
+    _call_on(k_cache, f"oxide_kv_cache_read_q8_{_SFX[dtype]}", _p(k_cache), _p(v_cache), _p(k_scale), _p(v_scale),
+             _p(k), _p(v), b, hkv, m, d, block, start, n, _p(lens))
+    return k, v
+
+
+def decode_attention_q8(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor,
+                        v_scale: torch.Tensor, block: int, lens: Optional[torch.Tensor] = None,
+                        scale: Optional[float] = None, workspace: Optional[torch.Tensor] = None,
+                        out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """decode_attention over int8 caches: q [batch, q_heads, head_dim] (f32 or
+    bf16, head_dim <= 256) against caches [batch, kv_heads, max_seq, head_dim]
+    with the block scales of kv_cache_append_q8, keys j < lens[b] (int32; None:
+    every position).  An empty sequence gives zeros.  A workspace given must not
+    be in use by another call that may run at the same time."""
+    op = "decode_attention_q8"
+    _q8_cache_check(op, k_cache, v_cache, k_scale, v_scale, block)
+    _need(q.dim() == 3 and q.shape[0] == k_cache.shape[0] and q.shape[2] == k_cache.shape[3], op,
+          f"q {list(q.shape)} and caches {list(k_cache.shape)} do not match")
+    b, hq, d = q.shape
+    hkv, m = k_cache.shape[1], k_cache.shape[2]
+    _need(hkv >= 1 and hq % hkv == 0, op, f"{hq} query heads are not a multiple of {hkv} kv heads")
+    _q8_lens(op, "lens", lens, b)
+    _out_like(op, q, out=out)
+    need = int(_lib.lib().oxide_decode_attention_q8_workspace_bytes(b, hq, hkv, d))
+    _need(workspace is None or workspace.numel() * workspace.element_size() >= need, op,
+          f"workspace must hold {need} bytes")
+    _check(q, k_cache, v_cache, k_scale, v_scale, lens, workspace, out)
+    _one_device(op, q, k_cache=k_cache, v_cache=v_cache, k_scale=k_scale, v_scale=v_scale, lens=lens,
+                workspace=workspace, out=out)
+    if scale is None:
+        scale = float(np.float32(1) / np.sqrt(np.float32(d)))
+    if workspace is None:
+        workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
+    out = torch.empty_like(q) if out is None else out
+    _call_on(q, f"oxide_decode_attention_q8_{_sfx(q)}", _p(q), _p(k_cache), _p(v_cache), _p(k_scale), _p(v_scale),
+             _p(lens), _p(out), b, hq, hkv, m, d, block, float(scale), _p(workspace),
+             workspace.numel() * workspace.element_size())
+    return out
+
+
+class KvCacheQ8(KvCache):
+    """KvCache held as int8 codes with one f32 scale per block of `block`
+    positions and head: about half the memory of bf16 caches and, in a decode
+    step, half the bytes read.  update() quantises as it writes
+    (kv_cache_append_q8), get() reads values back (kv_cache_read_q8, in
+    `dtype`), attend() is one decode step of attention over a layer."""
+
+    def __init__(self, num_layers: int, batch_size: int, num_kv_heads: int, head_dim: int,
+                 max_seq_len: int, block: int = 64, dtype=torch.bfloat16, device="cuda"):
+        super().__init__(0, batch_size, num_kv_heads, head_dim, max_seq_len, dtype, device)
+        _need(block in (1, 2, 4, 8, 16, 32, 64, 128), "KvCacheQ8", "block must be a power of two in [1, 128]")
+        shape = (batch_size, num_kv_heads, max_seq_len, head_dim)
+        scales = (batch_size, num_kv_heads, -(-max_seq_len // block))
+        self.block, self.dtype, self.num_layers = block, dtype, num_layers
+        for codes, scale in (("k_cache", "k_scale"), ("v_cache", "v_scale")):
+            setattr(self, codes, [torch.zeros(shape, dtype=torch.int8, device=device) for _ in range(num_layers)])
+            setattr(self, scale, [torch.zeros(scales, dtype=torch.float32, device=device) for _ in range(num_layers)])
+        self._len = [0] * num_layers
+
+    def _caches(self, layer_idx: int):
+        return (self.k_cache[layer_idx], self.v_cache[layer_idx], self.k_scale[layer_idx], self.v_scale[layer_idx])
+
+    def update(self, layer_idx: int, key: torch.Tensor, value: torch.Tensor) -> None:
+        """Append key/value [batch, kv_heads, new_len, head_dim] (f32 or bf16)."""
+        self._layer(layer_idx)
+        cur = self._len[layer_idx]
+        kv_cache_append_q8(*self._caches(layer_idx), key, value, cur, self.block)
+        self._len[layer_idx] = cur + key.shape[2]
+
+    def get(self, layer_idx: int, seq_len: Optional[int] = None):
+        """(k, v) [batch, kv_heads, seq_len, head_dim] of the first seq_len
+        positions (default: the layer's length) as values, None if 0."""
+        self._layer(layer_idx)
+        n = self._len[layer_idx] if seq_len is None else seq_len
+        if n == 0:
+            return None
+        return kv_cache_read_q8(*self._caches(layer_idx), self.block, 0, n, dtype=self.dtype)
+
+    def attend(self, layer_idx: int, q: torch.Tensor, lens: Optional[torch.Tensor] = None,
+               scale: Optional[float] = None, workspace: Optional[torch.Tensor] = None,
+               out: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """Attention of q [batch, q_heads, head_dim] over the layer's positions
+        (lens, int32: fewer for some sequences)."""
+        self._layer(layer_idx)
+        if lens is None:
+            lens = torch.full((self.batch_size,), self._len[layer_idx], dtype=torch.int32,
+                              device=self.k_cache[layer_idx].device)
+        return decode_attention_q8(q, *self._caches(layer_idx), self.block, lens, scale, workspace, out)
+
+    def get_cache_size(self) -> int:
+        """Bytes held by all layers' codes and scales."""
+        return sum(t.numel() * t.element_size() for ts in (self.k_cache, self.v_cache, self.k_scale, self.v_scale)
+                   for t in ts)
 
 
 # ---- token sampling (src/tokenizer.rs:166-232, src/pipeline.rs:181-205) ----

@@ -1,0 +1,270 @@
+"""decode_attention_q8 against the attention over the values the codes stand
+for, in 64 bits, element by element within what f32 arithmetic allows
+(_q8.attend_tolerance), bf16 outputs with their own rounding on top."""
+import pytest
+import torch
+
+import _q8
+from oxide_b200 import _lib, ops
+
+pytestmark = pytest.mark.gpu
+DT = {"f32": torch.float32, "bf16": torch.bfloat16}
+
+
+def _case(dev, b, hq, hkv, d, m, block, dtype, seed=0, sharp=1.0):
+    g = torch.Generator(device=dev).manual_seed(seed + b * 7 + hq * 31 + d * 1009 + m)
+    c = [torch.randn((b, hkv, m, d), generator=g, device=dev).mul_(40).round_().clamp_(-127, 127).to(torch.int8)
+         for _ in range(2)]
+    s = [(torch.rand((b, hkv, -(-m // block)), generator=g, device=dev) + 0.5) / 40 for _ in range(2)]
+    q = (torch.randn((b, hq, d), generator=g, device=dev) * sharp).to(DT[dtype])
+    return q, c[0], c[1], s[0], s[1]
+
+
+def _lens(dev, v):
+    return torch.tensor(v, dtype=torch.int32, device=dev)
+
+
+def _close(got, want, mag, size, d):
+    tol = _q8.attend_tolerance(mag, size, d)
+    if got.dtype == torch.bfloat16:
+        tol = tol + want.abs() * 2.0 ** -8 + 2.0 ** -134
+    err = (got.double() - want).abs()
+    assert bool(torch.isfinite(got).all())
+    assert bool((err <= tol + 2.0 ** -149).all()), float((err / (tol + 2.0 ** -149)).max())
+
+
+def _run(case, block, lens, **kw):
+    q = case[0]
+    got = ops.decode_attention_q8(*case, block, lens, **kw)
+    scale = kw.get("scale") or q.shape[2] ** -0.5
+    want, mag, size = _q8.attend(*case, lens, block, scale)
+    _close(got, want, mag, size, q.shape[2])
+    return got, want
+
+
+# every group size (and pieces of more than eight), head size and kernel
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("hq,hkv,d", [(2, 2, 128), (4, 2, 128), (8, 2, 128), (16, 2, 128), (6, 2, 128), (24, 2, 128),
+                                      (4, 4, 64), (6, 2, 80), (8, 1, 96), (3, 1, 256), (8, 1, 256), (5, 5, 37),
+                                      (12, 4, 20), (34, 2, 36), (2, 1, 1)])
+@pytest.mark.parametrize("block", [1, 64])
+def test_shapes(cuda, dtype, hq, hkv, d, block):
+    case = _case(cuda, 5, hq, hkv, d, 517, block, dtype)
+    _run(case, block, _lens(cuda, [517, 0, 1, 129, 300]))
+
+
+EDGES = [0, 1, 2, 31, 32, 33, 63, 64, 65, 127, 128, 129, 255, 256, 257, 383, 384, 385, 511, 512]
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("hq,hkv,d", [(8, 2, 128), (2, 2, 128), (6, 2, 64)])
+@pytest.mark.parametrize("block", [1, 2, 4, 8, 16, 32, 128])
+def test_lengths(cuda, dtype, hq, hkv, d, block):
+    case = _case(cuda, len(EDGES), hq, hkv, d, 512, block, dtype)
+    _run(case, block, _lens(cuda, EDGES))
+
+
+@pytest.mark.parametrize("d", [128, 80])
+def test_lengths_out_of_range_and_all_positions(cuda, d):
+    """Lengths are held to [0, max_seq].  The work is divided over all sequences'
+    tiles, so another sequence's length changes the order of the sums, not more:
+    both calls are within the tolerance of the same definition."""
+    case = _case(cuda, 3, 4, 2, d, 300, 16, "f32")
+    _run(case, 16, None)
+    odd, want = _run(case, 16, _lens(cuda, [-1, 301, 2 ** 31 - 1]))
+    assert bool((odd[0] == 0).all()) and bool((want[1:] != 0).all())
+
+
+@pytest.mark.parametrize("hq,hkv,d,b,m", [(8, 2, 128, 1, 1), (8, 2, 128, 1, 40000), (32, 8, 128, 2, 9000),
+                                          (4, 4, 128, 300, 130), (4, 1, 64, 1, 30000), (2, 2, 48, 700, 40)])
+def test_work_division(cuda, hq, hkv, d, b, m):
+    """One sequence over every worker, and many sequences to a worker."""
+    case = _case(cuda, b, hq, hkv, d, m, 32, "bf16")
+    lens = [m - (i * 37) % m for i in range(b)]
+    _run(case, 32, _lens(cuda, lens))
+
+
+@pytest.mark.parametrize("hq,hkv,d", [(8, 2, 128), (2, 2, 128), (16, 2, 128), (6, 2, 80), (3, 3, 33)])
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_anything_behind_the_length(cuda, hq, hkv, d, dtype):
+    """Codes and scales behind a sequence's end may hold anything, -128 and NaN
+    among them."""
+    block, lens = 8, [200, 8, 0, 131]
+    case = _case(cuda, 4, hq, hkv, d, 260, block, dtype)
+    clean = ops.decode_attention_q8(*case, block, _lens(cuda, lens))
+    for i, n in enumerate(lens):
+        for codes, scales in ((case[1], case[3]), (case[2], case[4])):
+            codes[i, :, n:] = -128
+            scales[i, :, -(-n // block):] = float("nan") if i % 2 else float("inf")
+    assert torch.equal(ops.decode_attention_q8(*case, block, _lens(cuda, lens)), clean)
+    _run([*case[:3], *[torch.nan_to_num(s, nan=0.0, posinf=0.0) for s in case[3:]]], block, _lens(cuda, lens))
+
+
+@pytest.mark.parametrize("hq,hkv,d", [(8, 2, 128), (2, 2, 128), (6, 2, 80)])
+def test_not_finite_inside(cuda, hq, hkv, d):
+    """A block with the scale NaN among a sequence's keys, in k or in v, and a
+    query head with a NaN or an infinity make exactly their heads NaN."""
+    block, lens = 16, _lens(cuda, [200, 200, 200])
+    case = _case(cuda, 3, hq, hkv, d, 256, block, "f32")
+    clean = ops.decode_attention_q8(*case, block, lens)
+    case[3][0, 0, 5] = float("nan")
+    case[4][1, 1, 12] = float("nan")
+    case[0][2, 0, 3] = float("nan")
+    case[0][2, hq - 1, 0] = float("inf")
+    got = ops.decode_attention_q8(*case, block, lens)
+    rep = hq // hkv
+    bad = torch.zeros(3, hq, dtype=torch.bool, device=cuda)
+    bad[0, :rep] = True
+    bad[1, rep:] = True
+    bad[2, 0] = bad[2, hq - 1] = True
+    assert torch.equal(torch.isnan(got).all(-1), bad) and torch.equal(torch.isnan(got).any(-1), bad)
+    assert torch.equal(got[~bad], clean[~bad])
+
+
+@pytest.mark.parametrize("hq,hkv,d", [(8, 2, 128), (2, 2, 128), (6, 2, 80)])
+def test_zero_and_uneven_scales(cuda, hq, hkv, d):
+    """Blocks of zeros, scales 60 orders of magnitude apart, and a cache of
+    zeros only (the weights are even then, the values zero)."""
+    block = 4
+    case = _case(cuda, 2, hq, hkv, d, 300, block, "f32")
+    case[4][0, :, ::3] = 0.0
+    case[3][0, :, 1::3] = 0.0
+    e = torch.arange(case[4].shape[2], device=cuda) % 7
+    case[4][1] = torch.pow(10.0, e.double() * 10 - 30).float()
+    _run(case, block, _lens(cuda, [300, 290]))
+    case[4].zero_()
+    assert bool((ops.decode_attention_q8(*case, block) == 0).all())
+
+
+@pytest.mark.parametrize("hq,hkv,d", [(8, 2, 128), (16, 2, 128), (6, 2, 80)])
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_one_key_takes_all(cuda, hq, hkv, d, dtype):
+    """Scores of some hundred: one key holds the weight, wherever its tile is."""
+    case = _case(cuda, 4, hq, hkv, d, 1030, 64, dtype, sharp=20.0)
+    _run(case, 64, _lens(cuda, [1030, 700, 129, 128]))
+
+
+@pytest.mark.parametrize("hq,hkv,d", [(8, 2, 128), (4, 4, 64)])
+def test_faint_keys_add_up(cuda, hq, hkv, d):
+    """One key far above a long even rest whose weights are 2^-24 to 2^-20 of it:
+    the rest still counts."""
+    m, block = 20000, 64
+    case = _case(cuda, 1, hq, hkv, d, m, block, "f32")
+    q, kc, vc, ks, vs = case
+    q.fill_(1.0)
+    kc.zero_()
+    kc[:, :, 777] = 100
+    vc[:, :, :, :] = 100
+    vc[:, :, 777] = -100
+    ks.fill_(15.0 / 100 / d ** 0.5)  # the key's score is 15: the others' weights are e^-15
+    vs.fill_(0.01)
+    _run(case, block, None)
+
+
+@pytest.mark.parametrize("scale", [0.0, -0.5, 3.0])
+def test_scale(cuda, scale):
+    for d, hq in ((128, 8), (64, 8)):
+        case = _case(cuda, 2, hq, 2, d, 200, 16, "f32")
+        got = ops.decode_attention_q8(*case, 16, scale=scale)
+        want, mag, size = _q8.attend(*case, None, 16, scale)
+        _close(got, want, mag, size, d)
+
+
+def test_repeats_and_own_outputs(cuda):
+    """The same call twice gives the same bits; given outputs and workspaces are
+    used; a workspace may hold anything before."""
+    for d, hq in ((128, 8), (96, 6)):
+        case = _case(cuda, 3, hq, 2, d, 3000, 32, "bf16")
+        lens = _lens(cuda, [3000, 17, 1999])
+        a = ops.decode_attention_q8(*case, 32, lens)
+        n = int(_lib.lib().oxide_decode_attention_q8_workspace_bytes(3, hq, 2, d))
+        ws = torch.full((n,), 255, dtype=torch.uint8, device=cuda)
+        out = torch.empty_like(case[0])
+        assert ops.decode_attention_q8(*case, 32, lens, workspace=ws, out=out) is out
+        assert torch.equal(out, a)
+
+
+def test_nothing_behind_the_workspace(cuda):
+    for b, hq, hkv, d in ((3, 8, 2, 128), (2, 24, 2, 64)):
+        case = _case(cuda, b, hq, hkv, d, 700, 32, "bf16")
+        n = int(_lib.lib().oxide_decode_attention_q8_workspace_bytes(b, hq, hkv, d))
+        buf = torch.full((n + 4096,), 171, dtype=torch.uint8, device=cuda)
+        ops.decode_attention_q8(*case, 32, workspace=buf[:n])
+        assert bool((buf[n:] == 171).all())
+
+
+def test_two_streams(cuda):
+    """Two calls at once, each with a workspace of its own."""
+    cases = [_case(cuda, 4, 8, 2, 128, 5000, 64, "bf16", seed=s) for s in (1, 2)]
+    want = [ops.decode_attention_q8(*c, 64) for c in cases]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in cases]
+    for _ in range(10):
+        got = []
+        for s, c in zip(streams, cases):
+            with torch.cuda.stream(s):
+                got.append(ops.decode_attention_q8(*c, 64))
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_graph_replay_with_growing_lengths(cuda):
+    case = _case(cuda, 3, 8, 2, 128, 900, 64, "bf16")
+    lens = _lens(cuda, [1, 400, 890])
+    out = ops.decode_attention_q8(*case, 64, lens)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        ops.decode_attention_q8(*case, 64, lens, out=out)
+    for add in (0, 1, 9):
+        lens += add
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, ops.decode_attention_q8(*case, 64, lens))
+
+
+def test_matches_bf16_attention_of_the_values(cuda):
+    """Against the unquantised operator over the values read back (exact in bf16
+    when the scales are powers of two)."""
+    case = _case(cuda, 2, 8, 2, 128, 640, 16, "bf16")
+    for s in case[3:]:
+        s.copy_(torch.exp2(torch.round(torch.log2(s))))
+    lens = _lens(cuda, [640, 333])
+    k, v = ops.kv_cache_read_q8(*case[1:], 16)
+    a = ops.decode_attention_q8(*case, 16, lens).double()
+    b = ops.decode_attention(case[0], k, v, lens).double()
+    want, mag, size = _q8.attend(*case, lens, 16, 128 ** -0.5)
+    # both round to bf16 once; the bf16 kernel holds its weights in 16 bits
+    assert bool(((a - b).abs() <= want.abs() * 2.0 ** -7 + mag * 2.0 ** -13).all())
+
+
+def test_a_decode_loop(cuda):
+    """The operators as they are used together: the layer's normalisation hands
+    int8 rows to a product, keys and values go into the int8 cache, attention
+    reads it; several steps, against the same steps in 64 bits."""
+    b, hq, hkv, d, hidden, block = 3, 8, 2, 128, 256, 16
+    g = torch.Generator(device=cuda).manual_seed(0)
+    wq, wk, wv = (torch.randn((n * d, hidden), generator=g, device=cuda) / 16 for n in (hq, hkv, hkv))
+    w = (torch.rand(hidden, generator=g, device=cuda) + 0.5).bfloat16()
+    cache = ops.KvCacheQ8(1, b, hkv, d, 96, block=block)
+    mine = [torch.zeros((b, hkv, 96, d), dtype=torch.int8), torch.zeros((b, hkv, 96, d), dtype=torch.int8),
+            torch.zeros((b, hkv, 6)), torch.zeros((b, hkv, 6))]
+    x = torch.randn((b, 33, hidden), generator=g, device=cuda).bfloat16()
+    at = 0
+    for step in range(6):
+        r = torch.randn(x.shape, generator=g, device=cuda).bfloat16()
+        h, codes, scale = ops.add_rms_norm_q8(x, r, w, 1e-5)
+        ref = _q8.norm_q8(x, r, w, 1e-5)
+        assert torch.equal(h, ref[0]) and torch.equal(codes, ref[1])
+        y = codes.float() * scale[..., None]
+        n = y.shape[1]
+        q, k, v = ((y @ m.T).view(b, n, -1, d).transpose(1, 2).contiguous().bfloat16() for m in (wq, wk, wv))
+        cache.update(0, k, v)
+        _q8.append(*mine, k.cpu(), v.cpu(), [at] * b, [n] * b, block)
+        at += n
+        assert torch.equal(cache.k_cache[0].cpu(), mine[0]) and torch.equal(cache.v_scale[0].cpu(), mine[3])
+        last = q[:, :, -1].contiguous()
+        got = cache.attend(0, last)
+        want, mag, size = _q8.attend(last, *[t.to(cuda) for t in mine], [at] * b, block, d ** -0.5)
+        _close(got, want, mag, size, d)
+        x = torch.randn((b, 1, hidden), generator=g, device=cuda).bfloat16()
