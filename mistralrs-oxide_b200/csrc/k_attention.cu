@@ -592,6 +592,7 @@ int device_status(int reset, uint32_t* flags);
 // the split-K (mma.sync) kernel; 2: the tcgen05 kernel with its loads
 // withheld (oxide_debug_decode_attention_path).
 static std::atomic<int> g_decode_path{0};
+int decode_path() { return g_decode_path.load(std::memory_order_relaxed); }
 
 template <typename T>
 static int decode_entry(const char* name, const T* q, const T* kc, const T* vc, const int32_t* lens, T* out,
@@ -624,7 +625,7 @@ static int decode_entry(const char* name, const T* q, const T* kc, const T* vc, 
     cudaError_t e = cudaSuccess;
     bool done = false;  // the tcgen05 kernel ran
     if constexpr (std::is_same<T, bf16_t>::value) {
-        const int path = g_decode_path.load(std::memory_order_relaxed);
+        const int path = decode_path();
         if (fast && path != 1)
             e = decode_attention_tc_bf16(q, kc, vc, lens, out, batch, q_heads, kv_heads, max_seq, scale, ws, ws_bytes,
                                          st, path == 2, &done);

@@ -9,8 +9,9 @@
 //
 // Two kernels write partial results in one form (oxide_attn_q8.cuh) and
 // decode_attn_q8_combine_kernel merges them:
-//   k_attention_q8_tc.cu   head_dim 128 and 1, 2, 4 or 8 query heads a kv
-//                          head: both products in int8 on tcgen05;
+//   k_attention_q8_tc.cu   head_dim a multiple of 16 up to 128, caches of at
+//                          least 128 positions: both products in int8 on
+//                          tcgen05;
 //   here, any other shape  (head_dim up to 256, any group): a warp is a
 //                          worker and streams 32-key tiles.  Scores: lane =
 //                          key, its row read in 16-byte (4-byte, 1-byte)
@@ -338,11 +339,13 @@ static int attn_q8_entry(const char* name, const T* q, const int8_t* kc, const i
     a.halves = 1;
     a.q_bf16 = sizeof(T) == 2;
     a.c1 = scale * 1.4426950408889634f;
-    cudaError_t e = cudaSuccess;
+    const int path = decode_path();
+    bool done = false;  // the tcgen05 kernel ran
+    cudaError_t e = path == 1 ? cudaSuccess : decode_attention_q8_tc(a, path == 2, st, &done);
     const uint64_t word = head_dim % 16 == 0 ? 16 : 4;
     const bool d4 = head_dim % 4 == 0 && (reinterpret_cast<uintptr_t>(kc) & (word - 1)) == 0 &&
                     (reinterpret_cast<uintptr_t>(vc) & 3) == 0;
-    switch (nr) {
+    if (e == cudaSuccess && !done) switch (nr) {
         case 1: e = launch_warp_d<1>(a, d4, st); break;
         case 2: e = launch_warp_d<2>(a, d4, st); break;
         case 4: e = launch_warp_d<4>(a, d4, st); break;

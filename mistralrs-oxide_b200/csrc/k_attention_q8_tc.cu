@@ -1,0 +1,556 @@
+// k_attention_q8_tc.cu -- decode attention over int8 KV caches with both
+// products in int8 on the 5th-generation tensor cores.
+//
+// Mathematics.  The cache's codes c, d are int8 as they lie in memory, so the
+// other operand of each product is written in int8 digits as well and the
+// products are exact integer sums:
+//   q of a head = (x) amax / Q_UNIT with |x| <= Q_UNIT = 8e6 integers, and
+//   x = x0 + 256 x1 + 65536 x2 in balanced digits (-128 .. 127), so
+//   q . c = (x0 . c + 256 x1 . c + 65536 x2 . c) amax / Q_UNIT: the three digit
+//   rows are three columns of one product (each sum below 2^22, exact in f32),
+//   and q is held to 2^-23 of its largest element, as good as f32 sums;
+//   p_j vs_j (the softmax weight times the value block's scale) likewise, as
+//   integers against the largest of the tile, found in the log2 domain
+//   (t_j + log2 vs_j), so neither a far maximum in another tile nor blocks
+//   with very different scales cost a weight its digits.
+// The padding of the N side, which a group of at most eight query heads leaves
+// anyway, carries the digits: the tensor cores read the cache once.
+//
+// Work division as in k_attention_tc.cu (tiles of 128 keys laid end to end,
+// one CTA per SM, equal ranges); partials as in oxide_attn_q8.cuh, two halves
+// a CTA.  head_dim a multiple of 16 up to 128: the tile is 128 bytes wide and
+// TMA fills what lies past head_dim with zeros.
+//
+// CTA of 12 warps:
+//   warp 0      (one lane) TMA producer: K and V tiles [128 keys x 128 bytes],
+//               128-byte swizzle, 6-stage ring (32 KB a stage: the bytes of
+//               half as many bf16 keys);
+//   warp 1      TMEM owner and (one lane) MMA issuer:
+//                 S[128 keys x N] = K . X^T   (A = K, K-major; B = digits of q)
+//                 O[128 dims x N] = V^T . Y^T (A = V read MN-major; B = digits
+//                                              of the weights)
+//               N = 16 for up to 4 heads, 32 for 8 (M = 128 takes N in steps
+//               of 16);
+//   warp 2      the query heads' digits, one pair ahead;
+//   warp 3      the tile prefix at the start;
+//   warps 4-7 and 8-11  two softmax groups that take the tiles in turn, each
+//               with its own S and O in TMEM, weights buffer and online state:
+//               one group's barriers and latencies hide behind the other's
+//               work.  Thread i = key i of S and dim i of O.
+// A group's buffers need few barriers: its O of tile k is read before its
+// weights of tile k + 1 are handed over, so that hand-over also says that O and
+// the weights buffer are free.
+// Every wait is bounded, as in k_attention_tc.cu: a wait that runs out raises
+// the CTA's abort flag, all roles stop at points their barriers agree on,
+// copies and products in flight are waited for, TMEM is freed, and the error
+// word makes the combine kernel write NaN.
+#include <stdlib.h>
+
+#include "oxide_attn_q8.cuh"
+#include "oxide_tc.cuh"
+
+namespace oxide {
+
+constexpr uint32_t QT_TK = 128, QT_DB = 128;  // keys a tile, bytes a row in shared memory
+constexpr int QT_STAGES = 6;
+constexpr int QT_THREADS = 384;
+constexpr uint32_t QT_MAX_BATCH = 1024;
+constexpr float Q_UNIT = 8.0e6f;  // below 0x7f7f7f = 8355711, the largest three balanced digits hold
+constexpr uint32_t QT_TMEM_COLS = 128, QT_TMEM_O = 64;  // S at 32 g, O at 64 + 32 g for group g
+constexpr uint32_t QT_TILE = QT_TK * QT_DB;       // 16 KB
+constexpr uint32_t QT_STAGE_BYTES = 2 * QT_TILE;  // K, V
+constexpr uint32_t QT_BBYTES = 32 * 128;          // a B operand: up to 32 rows of 128 bytes
+// shared memory map (offsets from a 1024-byte aligned base)
+constexpr uint32_t QT_OFF_Q = QT_STAGES * QT_STAGE_BYTES;                // 2 slots
+constexpr uint32_t QT_OFF_P = QT_OFF_Q + 2 * QT_BBYTES;                  // 2 groups
+constexpr uint32_t QT_OFF_PRE = QT_OFF_P + 2 * QT_BBYTES;
+constexpr uint32_t QT_OFF_SQ = QT_OFF_PRE + (QT_MAX_BATCH + 8) * 4;      // [2][8] factors of the scores
+constexpr uint32_t QT_OFF_RED = QT_OFF_SQ + 2 * 8 * 4;                   // [2][4][16] tile maxima
+constexpr uint32_t QT_OFF_SUM = QT_OFF_RED + 2 * 4 * 16 * 4;             // [2][4][8] sums
+constexpr uint32_t QT_OFF_BAR = QT_OFF_SUM + 2 * 4 * 8 * 4;
+enum : int {
+    QB_FULL = 0,                      // [6] stage loaded (TMA bytes)
+    QB_EMPTY = QB_FULL + QT_STAGES,   // [6] stage consumed (MMA commit)
+    QB_QFULL = QB_EMPTY + QT_STAGES,  // [2] digits of a pair's query heads written (warp 2)
+    QB_QEMPTY = QB_QFULL + 2,         // [2] read: MMA commit and the eight softmax warps
+    QB_SFULL = QB_QEMPTY + 2,         // [2] scores in TMEM (MMA commit)
+    QB_SEMPTY = QB_SFULL + 2,         // [2] scores read (4 warps)
+    QB_PFULL = QB_SEMPTY + 2,         // [2] weights written, O free (1 thread)
+    QB_OFULL = QB_PFULL + 2,          // [2] tile output in TMEM, weights read (MMA commit)
+    QB_DONE = QB_OFULL + 2,           // every product issued has completed
+    QB_COUNT = QB_DONE + 1
+};
+constexpr uint32_t QT_OFF_MISC = QT_OFF_BAR + ((QB_COUNT + 1) & ~1) * 8;
+constexpr size_t QT_SMEM = QT_OFF_MISC + 32 + 1024;  // + alignment slack
+static_assert(QT_SMEM <= 227 * 1024, "shared memory of one CTA");
+static_assert(2 * 1024 <= Q8A_PARTS, "two parts a CTA fit the workspace");
+
+__device__ unsigned int g_device_status_q8;  // sticky failure flags, read by oxide_device_status
+
+// Columns of a product, and how many of them are read back (three digits a head).
+template <int NR>
+constexpr uint32_t qt_n() { return (3 * NR + 15) / 16 * 16; }
+template <int NR>
+constexpr uint32_t qt_cols() { return (3 * NR + 7) / 8 * 8; }
+
+template <int NR>
+__device__ __forceinline__ void qt_load(uint32_t taddr, uint32_t (&v)[qt_cols<NR>()]) {
+#pragma unroll
+    for (int i = 0; i < (int)qt_cols<NR>(); i += 8) tmem_ld8(taddr + i, v + i);
+    tmem_wait_ld();
+}
+// Three digit sums as the number they spell.
+__device__ __forceinline__ float qt_spell(uint32_t d0, uint32_t d1, uint32_t d2) {
+    return __fmaf_rn((float)(int)d2, 65536.0f, __fmaf_rn((float)(int)d1, 256.0f, (float)(int)d0));
+}
+// Balanced digits of |x| <= Q_UNIT in bytes 0, 1, 2.
+__device__ __forceinline__ uint32_t qt_digits(float x) {
+    return ((uint32_t)__float2int_rn(x) + 0x808080u) ^ 0x808080u;
+}
+
+struct QtScales {
+    float k, v;
+};
+
+template <int NR>
+__global__ void __launch_bounds__(QT_THREADS, 1)
+    decode_attn_q8_tc_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_constant__ CUtensorMap tmv,
+                             Q8AttnArgs p, uint32_t withhold) {
+    pdl_trigger();
+    constexpr uint32_t N = qt_n<NR>();
+    extern __shared__ __align__(1024) unsigned char smem_raw[];
+    unsigned char* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+    const uint32_t sbase = smem_u32(smem);
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    uint32_t* pre = reinterpret_cast<uint32_t*>(smem + QT_OFF_PRE);
+    float* sq = reinterpret_cast<float*>(smem + QT_OFF_SQ);
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + QT_OFF_MISC);
+    volatile int* abort = reinterpret_cast<volatile int*>(smem + QT_OFF_MISC + 4);
+    volatile int* consumed = reinterpret_cast<volatile int*>(smem + QT_OFF_MISC + 8);  // stages the MMA warp waited for
+    auto bar = [&](int i) { return sbase + QT_OFF_BAR + 8u * (uint32_t)i; };
+
+    if (tid == 0) {
+        *abort = 0;
+        *consumed = 0;
+        for (int i = 0; i < QT_STAGES; ++i) {
+            mbar_init(bar(QB_FULL + i), 1);
+            mbar_init(bar(QB_EMPTY + i), 1);
+        }
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(bar(QB_QFULL + i), 1);
+            mbar_init(bar(QB_QEMPTY + i), 9);
+            mbar_init(bar(QB_SFULL + i), 1);
+            mbar_init(bar(QB_SEMPTY + i), 4);
+            mbar_init(bar(QB_PFULL + i), 1);
+            mbar_init(bar(QB_OFULL + i), 1);
+        }
+        mbar_init(bar(QB_DONE), 1);
+        mbar_init_fence();
+        tma_prefetch_map(&tmk);
+        tma_prefetch_map(&tmv);
+    }
+    if (warp == 1) {
+        tmem_alloc(smem_u32(tmem_slot), QT_TMEM_COLS);
+        tmem_relinquish();
+    }
+    pdl_wait();  // the previous kernel's writes (lengths, caches, queries) are visible
+    if (warp == 3) q8a_prefix(p, QT_TK, pre, blockIdx.x == 0);
+    if (tid == 0 && blockIdx.x == 0) *p.err = 0u;
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *tmem_slot;
+    const uint32_t heads = p.kv_heads * p.chunks, T = pre[p.batch] * heads, G = p.workers;
+    const uint32_t t0 = (uint32_t)((uint64_t)blockIdx.x * T / G);
+    const uint32_t nt = (uint32_t)((uint64_t)(blockIdx.x + 1) * T / G) - t0;  // this CTA's tiles, n = 0 .. nt - 1
+    TileWalk w{pre, p.batch, heads, 0, 0, 0, 0};
+
+    if (warp == 0) {
+        // ---------------- TMA producer ----------------
+        uint32_t n = 0;
+        if (lane == 0 && nt && !withhold) {
+            w.seek(t0);
+            for (; n < nt && !*abort; w.next()) {
+                const uint32_t s = n % QT_STAGES;
+                if (!tc_wait(bar(QB_EMPTY + s), ((n / QT_STAGES) & 1u) ^ 1u, abort)) break;
+                mbar_arrive_expect_tx(bar(QB_FULL + s), QT_STAGE_BYTES);
+                const int z = (int)(w.b * p.kv_heads + w.kvh / p.chunks), y = (int)(w.lt * QT_TK);
+                const uint32_t sd = sbase + s * QT_STAGE_BYTES;
+                tma_load_3d(sd, &tmk, bar(QB_FULL + s), 0, y, z);
+                tma_load_3d(sd + QT_TILE, &tmv, bar(QB_FULL + s), 0, y, z);
+                ++n;
+            }
+        }
+        // Drain (after an abort): copies issued but never waited for by the
+        // MMA warp land before the CTA exits.
+        if (lane == 0 && *abort) {
+            for (uint32_t i = (uint32_t)*consumed; i < n; ++i)
+                tc_wait_drain(bar(QB_FULL + i % QT_STAGES), (i / QT_STAGES) & 1u);
+        }
+        __syncwarp();
+    } else if (warp == 1) {
+        // ---------------- MMA issuer ----------------
+        if (lane == 0 && nt) {
+            constexpr uint32_t IDESC_S = umma_idesc_s8(128, N, false, false);
+            constexpr uint32_t IDESC_O = umma_idesc_s8(128, N, true, false);
+            w.seek(t0);  // of the next S product
+            uint32_t q = 0, ns = 0;
+            auto issue_s = [&]() -> bool {
+                const uint32_t n = ns, s = n % QT_STAGES, g = n & 1u;
+                if (n == 0 || w.lt == 0) {
+                    if (!tc_wait(bar(QB_QFULL + (q & 1u)), (q >> 1) & 1u, abort)) return false;
+                }
+                if (!tc_wait(bar(QB_FULL + s), (n / QT_STAGES) & 1u, abort)) return false;
+                *consumed = (int)n + 1;
+                if (!tc_wait(bar(QB_SEMPTY + g), ((n >> 1) & 1u) ^ 1u, abort)) return false;
+                tc_fence_after();
+                const uint32_t ka = sbase + s * QT_STAGE_BYTES, qa = sbase + QT_OFF_Q + (q & 1u) * QT_BBYTES;
+#pragma unroll
+                for (uint32_t kk = 0; kk < 4; ++kk)  // 32 dims a product
+                    umma_s8(tmem + g * 32, umma_desc(ka + kk * 32, 16, 1024, UMMA_SWIZZLE_128B),
+                            umma_desc(qa + kk * 32, 16, 1024, UMMA_SWIZZLE_128B), IDESC_S, kk > 0);
+                umma_commit(bar(QB_SFULL + g));
+                if (n + 1 == nt || w.lt + 1 == w.tb) {  // this pair's last product that reads its digits
+                    umma_commit(bar(QB_QEMPTY + (q & 1u)));
+                    ++q;
+                }
+                ++ns;
+                w.next();
+                return true;
+            };
+            bool ok = issue_s() && (nt < 2 || issue_s());
+            for (uint32_t n = 0; ok && n < nt; ++n) {
+                // The scores of tile n + 2 go first if its keys are here, else
+                // this tile's output does.
+                const uint32_t g = n & 1u, s = n % QT_STAGES, s2 = (n + 2) % QT_STAGES;
+                const bool more = n + 2 < nt;
+                const bool early = more && mbar_test_wait(bar(QB_FULL + s2), ((n + 2) / QT_STAGES) & 1u);
+                if (early && !issue_s()) break;
+                if (!tc_wait(bar(QB_PFULL + g), (n >> 1) & 1u, abort)) break;
+                tc_fence_after();
+                const uint32_t va = sbase + s * QT_STAGE_BYTES + QT_TILE, pa = sbase + QT_OFF_P + g * QT_BBYTES;
+#pragma unroll
+                for (uint32_t kk = 0; kk < 4; ++kk)  // 32 keys a product
+                    umma_s8(tmem + QT_TMEM_O + g * 32, umma_desc(va + kk * 4096, 16, 1024, UMMA_SWIZZLE_128B),
+                            umma_desc(pa + kk * 256, 128, 1024, UMMA_SWIZZLE_NONE), IDESC_O, kk > 0);
+                umma_commit(bar(QB_OFULL + g));
+                umma_commit(bar(QB_EMPTY + s));
+                if (more && !early) ok = issue_s();
+            }
+        }
+        if (lane == 0) {  // every product issued above has completed before TMEM is freed
+            umma_commit(bar(QB_DONE));
+            if (!tc_wait_drain(bar(QB_DONE), 0)) *abort = 1;
+        }
+        __syncwarp();
+    } else if (warp == 2) {
+        // ---------------- digits of the query heads ----------------
+        if (nt) w.seek(t0);
+        for (uint32_t n = 0, q = 0; n < nt; ++q) {
+            const uint32_t slot = q & 1u, h0 = (w.kvh % p.chunks) * NR, nh = min(p.rep - h0, (uint32_t)NR);
+            const uint64_t row = (uint64_t)w.b * p.q_heads + (w.kvh / p.chunks) * p.rep + h0;
+            float x[NR][4];
+#pragma unroll
+            for (int h = 0; h < NR; ++h) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) x[h][e] = 0.0f;
+                if ((uint32_t)h < nh && 4u * lane < p.head_dim) {
+                    const uint64_t at = (row + h) * p.head_dim + 4u * lane;
+                    if (p.q_bf16) {
+                        const uint2 v = __ldg(reinterpret_cast<const uint2*>(static_cast<const bf16_t*>(p.q) + at));
+                        x[h][0] = bf16_lo(v.x);
+                        x[h][1] = bf16_hi(v.x);
+                        x[h][2] = bf16_lo(v.y);
+                        x[h][3] = bf16_hi(v.y);
+                    } else {
+                        const float4 v = __ldg(reinterpret_cast<const float4*>(static_cast<const float*>(p.q) + at));
+                        x[h][0] = v.x;
+                        x[h][1] = v.y;
+                        x[h][2] = v.z;
+                        x[h][3] = v.w;
+                    }
+                }
+            }
+            if (!warp_wait(bar(QB_QEMPTY + slot), ((q >> 1) & 1u) ^ 1u, abort)) break;
+#pragma unroll
+            for (int h = 0; h < NR; ++h) {
+                uint32_t a = 0;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) a = max(a, q8_abs_bits(x[h][e]));
+                a = q8_warp_max(a);
+                const bool bad = a >= Q8_INF, tiny = a < 0x21800000u;  // not finite; below 2^-60
+                const float up = tiny ? 0x1p80f : 1.0f, amax = fmul(__uint_as_float(a), up);
+                const float inv = bad || a == 0 ? 0.0f : fdiv(Q_UNIT, amax);
+                uint32_t d[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) d[e] = qt_digits(bad ? 0.0f : fmul(fmul(x[h][e], up), inv));
+#pragma unroll
+                for (int g = 0; g < 3; ++g) {
+                    const uint32_t r = g * NR + h;
+                    *reinterpret_cast<uint32_t*>(smem + QT_OFF_Q + slot * QT_BBYTES + r * 128 +
+                                                 (((lane >> 2) ^ (r & 7)) << 4) + ((lane & 3) << 2)) =
+                        q8_pack4(d[0] >> (8 * g), d[1] >> (8 * g), d[2] >> (8 * g), d[3] >> (8 * g));
+                }
+                if (lane == 0)
+                    sq[slot * 8 + h] = bad ? q8_nan() : fmul(fmul(fdiv(amax, Q_UNIT), p.c1), tiny ? 0x1p-80f : 1.0f);
+            }
+            fence_async_smem();  // the digits are visible to the tensor core
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bar(QB_QFULL + slot));
+            const uint32_t cnt = min(w.tb - w.lt, nt - n);
+            n += cnt;
+            w.lt += cnt - 1;
+            w.next();
+        }
+    } else if (warp >= 4) {
+        // ---------------- softmax and epilogue: group g takes tiles n = g mod 2 ----------------
+        const uint32_t g = (uint32_t)(warp >> 2) - 1, q4 = (uint32_t)(warp & 3);
+        const uint32_t L = q4 * 32 + (uint32_t)lane;  // key of the S tile, dim of the O tile
+        const uint32_t s_tmem = tmem + ((q4 * 32u) << 16) + g * 32, o_tmem = s_tmem + QT_TMEM_O;
+        const int nbar = 1 + (int)g;
+        float* red = reinterpret_cast<float*>(smem + QT_OFF_RED) + g * 64;   // [4][16]
+        float* lsum = reinterpret_cast<float*>(smem + QT_OFF_SUM) + g * 32;  // [4][8]
+        unsigned char* pt = smem + QT_OFF_P + g * QT_BBYTES;
+        // m, l: online softmax of the scores; wm, acc: the same for the
+        // weights times scales; corr, tf: factors of the output not yet read
+        float m[NR], l[NR], wm[NR], acc[NR], corr[NR], tf[NR];
+        bool fail = false, pending = false;
+
+        // scales of this group's tiles, loaded two of them ahead
+        TileWalk ahead = w;
+        auto fetch = [&]() -> QtScales {  // of key L of the tile `ahead` is at
+            const uint64_t bh = (uint64_t)ahead.b * p.kv_heads + ahead.kvh / p.chunks;
+            const uint32_t key = ahead.lt * QT_TK + L;
+            QtScales s{0.0f, 1.0f};
+            if (key < q8a_len(p, ahead.b)) {
+                s.k = __ldg(p.ks + bh * p.nblk + (key >> p.shift));
+                s.v = __ldg(p.vs + bh * p.nblk + (key >> p.shift));
+            }
+            return s;
+        };
+        QtScales cur{0.0f, 1.0f}, next{0.0f, 1.0f};
+        uint32_t na = g;  // the tile `ahead` is at
+        auto step_ahead = [&](QtScales& s) {
+            if (na >= nt) return;
+            s = fetch();
+            na += 2;
+            if (na < nt) {
+                ahead.next();
+                ahead.next();
+            }
+        };
+        if (g < nt) {
+            w.seek(t0);
+            ahead = w;
+            if (g) ahead.next();
+            step_ahead(cur);
+            step_ahead(next);
+        } else if (nt) {
+            w.seek(t0);
+        }
+        auto epilogue = [&](uint32_t k) {  // add the output of this group's tile k
+            const bool ok = warp_wait(bar(QB_OFULL + g), k & 1u, abort);
+            fail |= !ok;
+            if (!ok) return;
+            tc_fence_after();
+            uint32_t o[qt_cols<NR>()];
+            qt_load<NR>(o_tmem, o);
+            tc_fence_before();
+#pragma unroll
+            for (int h = 0; h < NR; ++h)
+                acc[h] = __fmaf_rn(acc[h], corr[h], fmul(qt_spell(o[h], o[NR + h], o[2 * NR + h]), tf[h]));
+        };
+
+        bool dead = false;
+        for (uint32_t n = 0, q = 0; n < nt && !dead; ++q) {
+            const uint32_t cnt = min(w.tb - w.lt, nt - n), j0 = (n ^ g) & 1u, len = q8a_len(p, w.b);
+            // every warp waits for the digits, also of a pair without a tile
+            // for it: its arrival below then belongs to this use of the slot
+            fail |= !warp_wait(bar(QB_QFULL + (q & 1u)), (q >> 1) & 1u, abort);
+            __syncwarp();  // lane 0's wait covers the other lanes' reads of the factors
+            float f[NR];
+#pragma unroll
+            for (int h = 0; h < NR; ++h) {
+                f[h] = sq[(q & 1u) * 8 + h];
+                m[h] = wm[h] = -INFINITY;
+                l[h] = acc[h] = 0.0f;
+            }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bar(QB_QEMPTY + (q & 1u)));
+            pending = false;
+            for (uint32_t j = j0; j < cnt; j += 2) {
+                const uint32_t k = (n + j) >> 1, key0 = (w.lt + j) * QT_TK;
+                const bool on = key0 + L < len;
+                float t[NR], tv[NR];
+                const QtScales sc = cur;
+                cur = next;
+                const bool ok = warp_wait(bar(QB_SFULL + g), k & 1u, abort);
+                fail |= !ok;
+                if (ok) {
+                    tc_fence_after();
+                    uint32_t v[qt_cols<NR>()];
+                    qt_load<NR>(s_tmem, v);
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(bar(QB_SEMPTY + g));
+                    // a scale that is NaN, infinite or negative makes its keys' scores NaN
+                    const float sound = sc.v >= 0.0f && sc.v < INFINITY ? 0.0f : q8_nan(), lv = lg2_approx(sc.v);
+#pragma unroll
+                    for (int h = 0; h < NR; ++h) {
+                        t[h] = on ? fadd(fmul(qt_spell(v[h], v[NR + h], v[2 * NR + h]), fmul(sc.k, f[h])), sound) : -INFINITY;
+                        tv[h] = on ? fadd(t[h], lv) : -INFINITY;
+                    }
+                } else {
+#pragma unroll
+                    for (int h = 0; h < NR; ++h) t[h] = tv[h] = -INFINITY;
+                }
+                step_ahead(next);
+#pragma unroll
+                for (int h = 0; h < NR; ++h) {
+                    const float a = warp_fmax(t[h]), b = warp_fmax(tv[h]);
+                    if (lane == 0) {
+                        red[q4 * 16 + h] = a;
+                        red[q4 * 16 + 8 + h] = b;
+                    }
+                }
+                if (pending) epilogue(k - 1);  // its product has run meanwhile; the weights buffer and O are free after it
+                nbar_sync128(nbar);            // the four warps' maxima are in red
+#pragma unroll
+                for (int h = 0; h < NR; ++h) {
+                    const float* r = red + h;
+                    const float mt = fmaxf(fmaxf(r[0], r[16]), fmaxf(r[32], r[48]));
+                    const float wt = fmaxf(fmaxf(r[8], r[24]), fmaxf(r[40], r[56]));
+                    const float mn = fmaxf(m[h], mt), wn = fmaxf(wm[h], wt);
+                    const float cr = m[h] == -INFINITY ? 0.0f : ex2_approx(fsub(m[h], mn));
+                    l[h] = __fmaf_rn(l[h], cr, t[h] == -INFINITY ? 0.0f : ex2_approx(fsub(t[h], mn)));
+                    m[h] = mn;
+                    corr[h] = wm[h] == -INFINITY ? 0.0f : ex2_approx(fsub(wm[h], wn));
+                    tf[h] = wt == -INFINITY ? 0.0f : fmul(ex2_approx(fsub(wt, wn)), 1.0f / Q_UNIT);
+                    wm[h] = wn;
+                    const uint32_t d = qt_digits(tv[h] == -INFINITY ? 0.0f : fmul(ex2_approx(fsub(tv[h], wt)), Q_UNIT));
+#pragma unroll
+                    for (int i = 0; i < 3; ++i) {  // row r of the B operand, byte L: K-major cores of 8 rows x 16 bytes
+                        const uint32_t r8 = i * NR + h;
+                        pt[(r8 >> 3) * 1024 + (L >> 4) * 128 + (r8 & 7) * 16 + (L & 15)] = (unsigned char)(d >> (8 * i));
+                    }
+                }
+                fence_async_smem();  // the weights are visible to the tensor core
+                tc_fence_before();
+                if (nbar_or128(fail, nbar)) {
+                    dead = true;
+                    break;
+                }
+                if ((tid & 127) == 0) mbar_arrive(bar(QB_PFULL + g));  // every thread has written its weights and read O
+                pending = true;
+            }
+            if (dead) break;
+            if (j0 < cnt) {  // the pair is complete here: its partial
+                epilogue((n + cnt - 1 - ((n + cnt - 1 - g) & 1u)) >> 1);
+#pragma unroll
+                for (int h = 0; h < NR; ++h) {
+                    const float x = warp_sum(l[h]);
+                    if (lane == 0) lsum[q4 * 8 + h] = x;
+                }
+                if (nbar_or128(fail, nbar)) {
+                    dead = true;
+                    break;
+                }
+                const uint64_t part = ((uint64_t)blockIdx.x + (uint64_t)w.b * heads + w.kvh) * 2 + g;
+                const uint32_t nh = min(p.rep - (w.kvh % p.chunks) * NR, (uint32_t)NR);
+#pragma unroll
+                for (int h = 0; h < NR; ++h) {
+                    if ((uint32_t)h >= nh) continue;
+                    const uint64_t slot = part * NR + h;
+                    if (L < p.head_dim)
+                        p.part_o[slot * p.head_dim + L] =
+                            wm[h] == -INFINITY ? 0.0f : fmul(acc[h], ex2_approx(fsub(wm[h], m[h])));
+                    if (L == 0) {
+                        p.part_ml[slot * 2] = m[h];
+                        p.part_ml[slot * 2 + 1] = fadd(fadd(lsum[h], lsum[8 + h]), fadd(lsum[16 + h], lsum[24 + h]));
+                    }
+                }
+                // lsum is written again behind the next tile's barriers
+            }
+            n += cnt;
+            w.lt += cnt - 1;
+            w.next();
+        }
+        if (fail || dead) *abort = 1;
+    }
+    // ---------------- teardown ----------------
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    if (warp == 1) tmem_dealloc(tmem, QT_TMEM_COLS);
+    if (tid == 0 && *abort) {
+        atomicOr(p.err, 1u);
+        atomicOr(&g_device_status_q8, OXIDE_DEVICE_WAIT_TIMEOUT);
+    }
+}
+
+typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
+                                  const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
+                                  CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+// A cache [heads, max_seq, head_dim] of bytes as a TMA map with boxes of 128
+// positions by 128 bytes, 128-byte swizzle; bytes past head_dim and positions
+// past max_seq are filled with zeros.  False if the driver refuses it.
+static bool qt_map(CUtensorMap* m, const void* base, uint64_t heads, uint64_t max_seq, uint64_t head_dim) {
+    static EncodeTiledFn enc = reinterpret_cast<EncodeTiledFn>(driver_fn("cuTensorMapEncodeTiled"));
+    if (!enc) return false;
+    const cuuint64_t dims[3] = {head_dim, max_seq, heads};
+    const cuuint64_t strides[2] = {head_dim, max_seq * head_dim};
+    const cuuint32_t box[3] = {QT_DB, QT_TK, 1};
+    const cuuint32_t es[3] = {1, 1, 1};
+    return enc(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<void*>(base), dims, strides, box, es,
+               CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+bool tc_enabled();  // an sm_100 device, and not switched off (k_attention_tc.cu)
+
+template <int NR>
+static cudaError_t qt_launch(const CUtensorMap& mk, const CUtensorMap& mv, const Q8AttnArgs& a, bool withhold,
+                             cudaStream_t st) {
+    auto kern = decode_attn_q8_tc_kernel<NR>;
+    if (!ensure_dyn_smem(reinterpret_cast<const void*>(kern), QT_SMEM)) return cudaErrorInvalidConfiguration;
+    return launch_k(kern, a.workers, QT_THREADS, QT_SMEM, st, mk, mv, a, withhold ? 1u : 0u);
+}
+
+cudaError_t decode_attention_q8_tc(Q8AttnArgs& a, bool withhold, cudaStream_t st, bool* used) {
+    *used = false;
+    // head_dim: rows of whole 16-byte units (TMA strides), at most one 128-byte row.
+    if (!tc_enabled() || a.head_dim % 16 != 0 || a.head_dim > QT_DB || a.batch > QT_MAX_BATCH || a.max_seq < QT_TK ||
+        !aligned16(a.kc) || !aligned16(a.vc) || !aligned16(a.q))
+        return cudaSuccess;
+    const uint64_t pairs = (uint64_t)a.batch * a.kv_heads, tiles = pairs * a.chunks * ((a.max_seq + QT_TK - 1) / QT_TK);
+    uint64_t G = (uint64_t)sm_count();
+    if (G > tiles) G = tiles;
+    if (2 * G > Q8A_PARTS) return cudaSuccess;
+    CUtensorMap mk, mv;
+    if (!qt_map(&mk, a.kc, pairs, a.max_seq, a.head_dim) || !qt_map(&mv, a.vc, pairs, a.max_seq, a.head_dim))
+        return cudaSuccess;
+    a.workers = (uint32_t)G;
+    a.halves = 2;
+    *used = true;
+    switch (a.nr) {
+        case 1: return qt_launch<1>(mk, mv, a, withhold, st);
+        case 2: return qt_launch<2>(mk, mv, a, withhold, st);
+        case 4: return qt_launch<4>(mk, mv, a, withhold, st);
+        default: return qt_launch<8>(mk, mv, a, withhold, st);
+    }
+}
+
+int device_status_q8(int reset, uint32_t* flags) {
+    unsigned int v = 0;
+    cudaError_t e = cudaMemcpyFromSymbol(&v, g_device_status_q8, sizeof(v));
+    if (e == cudaSuccess && reset) {
+        const unsigned int zero = 0;
+        e = cudaMemcpyToSymbol(g_device_status_q8, &zero, sizeof(zero));
+    }
+    if (e != cudaSuccess) return set_error(OXIDE_ERR_CUDA, "oxide_device_status: %s", cudaGetErrorString(e));
+    *flags |= v;
+    return OXIDE_OK;
+}
+
+}  // namespace oxide

@@ -571,7 +571,7 @@ static bool tc_map(CUtensorMap* m, const void* base, uint64_t rows, uint32_t box
                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-static bool tc_enabled() {
+bool tc_enabled() {
     static const bool on = [] {
         const char* v = getenv("OXIDE_NO_TCGEN05");
         if (v && v[0] == '1') return false;
@@ -641,6 +641,8 @@ cudaError_t decode_attention_tc_bf16(const bf16_t* q, const bf16_t* kc, const bf
     }
 }
 
+int device_status_q8(int reset, uint32_t* flags);  // adds the int8-cache kernel's flags
+
 int device_status(int reset, uint32_t* flags) {
     unsigned int v = 0;
     cudaError_t e = cudaDeviceSynchronize();
@@ -652,7 +654,7 @@ int device_status(int reset, uint32_t* flags) {
     if (e != cudaSuccess)
         return set_error(OXIDE_ERR_CUDA, "oxide_device_status: %s", cudaGetErrorString(e));
     *flags = v;
-    return OXIDE_OK;
+    return device_status_q8(reset, flags);
 }
 
 }  // namespace oxide

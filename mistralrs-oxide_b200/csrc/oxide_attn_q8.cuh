@@ -69,9 +69,9 @@ __device__ __forceinline__ float warp_fmax(float v) {
     return r;
 }
 
-// The tcgen05 kernel; *used is false where shapes or device do not allow it.
-cudaError_t decode_attention_q8_tc(Q8AttnArgs a, bool withhold, cudaStream_t st, bool* used);
-int device_status_q8(int reset, uint32_t* flags);
+// The tcgen05 kernel (sets a.workers and a.halves); *used is false where
+// shapes or device do not allow it.
+cudaError_t decode_attention_q8_tc(Q8AttnArgs& a, bool withhold, cudaStream_t st, bool* used);
 int decode_path();  // oxide_debug_decode_attention_path's choice
 
 }  // namespace oxide

@@ -68,14 +68,28 @@ def values(codes, scales, block):
     return codes.to(F64) * per
 
 
+GRID = 0.5 / 8.0e6  # half a step of the tensor-core kernel's integers
+
+
 def attend(q, kc, vc, ks, vs, lens, block, scale):
-    """(out, sum p |v|, largest sum |q k| scale) of the decode attention, f64."""
+    """(out, sum p |v|, tolerance) of the decode attention in f64.  The tolerance
+    is how far f32 arithmetic may be from the definition, element by element:
+    u = 2^-24 a rounding.
+    Scores sum head_dim products and take eight more roundings (the factors, the
+    log2(e) factor, the difference from the maximum), each at most u of
+    sum |q k| scale.  The tensor-core kernel writes q in integers of 1 / 8e6 of
+    the head's largest element, so a score is off by GRID max|q| sum |k| scale
+    more.  Both act on numerator and denominator: twice, relative to sum p |v|.
+    Weights: three base-2 functions (2^-22 each) and 16 roundings in the sums of
+    the parts and the quotient, again twice.  And the kernel writes p vs of a
+    tile of 128 keys in integers of 1 / 8e6 of the tile's largest: an output is
+    off by GRID max(p vs) sum |code| of each tile, whatever its own size."""
     b, hq, d = q.shape
     hkv, m = kc.shape[1], kc.shape[2]
     rep = hq // hkv
+    u = 2.0 ** -24
     out = torch.zeros((b, hq, d), dtype=F64, device=q.device)
-    mag = torch.zeros_like(out)
-    size = torch.zeros((b, hq, 1), dtype=F64, device=q.device)
+    mag, tol = torch.zeros_like(out), torch.zeros_like(out)
     for i in range(b):
         n = m if lens is None else max(0, min(int(lens[i]), m))
         if n == 0:
@@ -84,21 +98,14 @@ def attend(q, kc, vc, ks, vs, lens, block, scale):
         k = values(kc[i:i + 1, :, :n], ks[i:i + 1, :, :nb], block)[0]
         v = values(vc[i:i + 1, :, :n], vs[i:i + 1, :, :nb], block)[0]
         qi = q[i].to(F64).view(hkv, rep, d)
-        s = qi @ k.transpose(1, 2) * scale
-        p = torch.softmax(s, -1)
-        out[i] = (p @ v).view(hq, d)
-        mag[i] = (p @ v.abs()).view(hq, d)
-        size[i] = (qi.abs() @ k.abs().transpose(1, 2) * abs(scale)).amax(-1).view(hq, 1)
-    return out, mag, size
-
-
-def attend_tolerance(mag, size, head_dim):
-    """How far f32 arithmetic may be from the definition, element by element:
-    u = 2^-24 a rounding.  A score sums head_dim products and takes four more
-    roundings (two factors, the log2(e) factor and the difference from the
-    maximum), each at most u of sum |q k| scale = `size`: off by at most
-    (head_dim + 8) u size, twice (numerator and denominator).  Weights: two
-    base-2 exponentials (2^-22 each) and the digits' 2^-22, the sums of the
-    parts and the final quotient 16 u, again twice.  All relative to sum p |v|."""
-    u = 2.0 ** -24
-    return mag * (2 * (head_dim + 8) * u * size + 2 * (3 * 2.0 ** -22 + 16 * u))
+        p = torch.softmax(qi @ k.transpose(1, 2) * scale, -1)
+        one = p @ v.abs()
+        size = (qi.abs() @ k.abs().transpose(1, 2)).amax(-1, keepdim=True) * abs(scale)
+        wide = qi.abs().amax(-1, keepdim=True) * k.abs().sum(-1).amax(-1)[:, None, None] * abs(scale)
+        t = one * (2 * ((d + 8) * u * size + GRID * wide) + 2 * (3 * 2.0 ** -22 + 16 * u))
+        pv = p * vs[i, :, :nb].to(F64).repeat_interleave(block, 1)[:, None, :n]
+        for j in range(0, n, 128):
+            top = pv[:, :, j:j + 128].amax(-1, keepdim=True)
+            t += GRID * top * vc[i, :, None, j:j + 128].to(F64).abs().sum(2)
+        out[i], mag[i], tol[i] = (p @ v).view(hq, d), one.view(hq, d), t.view(hq, d)
+    return out, mag, tol

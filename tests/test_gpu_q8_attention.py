@@ -1,6 +1,6 @@
 """decode_attention_q8 against the attention over the values the codes stand
 for, in 64 bits, element by element within what f32 arithmetic allows
-(_q8.attend_tolerance), bf16 outputs with their own rounding on top."""
+(_q8.attend's tolerance), bf16 outputs with their own rounding on top."""
 import pytest
 import torch
 
@@ -24,8 +24,7 @@ def _lens(dev, v):
     return torch.tensor(v, dtype=torch.int32, device=dev)
 
 
-def _close(got, want, mag, size, d):
-    tol = _q8.attend_tolerance(mag, size, d)
+def _close(got, want, tol):
     if got.dtype == torch.bfloat16:
         tol = tol + want.abs() * 2.0 ** -8 + 2.0 ** -134
     err = (got.double() - want).abs()
@@ -37,8 +36,8 @@ def _run(case, block, lens, **kw):
     q = case[0]
     got = ops.decode_attention_q8(*case, block, lens, **kw)
     scale = kw.get("scale") or q.shape[2] ** -0.5
-    want, mag, size = _q8.attend(*case, lens, block, scale)
-    _close(got, want, mag, size, q.shape[2])
+    want, mag, tol = _q8.attend(*case, lens, block, scale)
+    _close(got, want, tol)
     return got, want
 
 
@@ -166,8 +165,8 @@ def test_scale(cuda, scale):
     for d, hq in ((128, 8), (64, 8)):
         case = _case(cuda, 2, hq, 2, d, 200, 16, "f32")
         got = ops.decode_attention_q8(*case, 16, scale=scale)
-        want, mag, size = _q8.attend(*case, None, 16, scale)
-        _close(got, want, mag, size, d)
+        want, mag, tol = _q8.attend(*case, None, 16, scale)
+        _close(got, want, tol)
 
 
 def test_repeats_and_own_outputs(cuda):
@@ -233,7 +232,7 @@ def test_matches_bf16_attention_of_the_values(cuda):
     k, v = ops.kv_cache_read_q8(*case[1:], 16)
     a = ops.decode_attention_q8(*case, 16, lens).double()
     b = ops.decode_attention(case[0], k, v, lens).double()
-    want, mag, size = _q8.attend(*case, lens, 16, 128 ** -0.5)
+    want, mag, tol = _q8.attend(*case, lens, 16, 128 ** -0.5)
     # both round to bf16 once; the bf16 kernel holds its weights in 16 bits
     assert bool(((a - b).abs() <= want.abs() * 2.0 ** -7 + mag * 2.0 ** -13).all())
 
@@ -265,6 +264,57 @@ def test_a_decode_loop(cuda):
         assert torch.equal(cache.k_cache[0].cpu(), mine[0]) and torch.equal(cache.v_scale[0].cpu(), mine[3])
         last = q[:, :, -1].contiguous()
         got = cache.attend(0, last)
-        want, mag, size = _q8.attend(last, *[t.to(cuda) for t in mine], [at] * b, block, d ** -0.5)
-        _close(got, want, mag, size, d)
+        want, mag, tol = _q8.attend(last, *[t.to(cuda) for t in mine], [at] * b, block, d ** -0.5)
+        _close(got, want, tol)
         x = torch.randn((b, 1, hidden), generator=g, device=cuda).bfloat16()
+
+
+def _on_path(path, case, block, lens):
+    _lib.lib().oxide_debug_decode_attention_path(path)
+    try:
+        out = ops.decode_attention_q8(*case, block, lens)
+        torch.cuda.synchronize()
+    finally:
+        _lib.lib().oxide_debug_decode_attention_path(0)
+    return out
+
+
+@pytest.mark.parametrize("hq,hkv,d", [(1, 1, 128), (4, 2, 128), (8, 2, 128), (16, 2, 128), (6, 2, 128), (24, 2, 128),
+                                      (8, 2, 64), (8, 2, 16), (4, 4, 112)])
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_both_kernels(cuda, hq, hkv, d, dtype):
+    """Shapes that the tensor-core kernel takes, on it and on the other one."""
+    case = _case(cuda, 4, hq, hkv, d, 1000, 32, dtype)
+    lens = _lens(cuda, [1000, 999, 3, 514])
+    want, mag, tol = _q8.attend(*case, lens, 32, d ** -0.5)
+    for path in (0, 1):
+        _close(_on_path(path, case, 32, lens), want, tol)
+
+
+def test_query_magnitudes(cuda):
+    """Queries of every magnitude: the digits follow the head's largest element,
+    subnormal ones included; a head of zeros weighs its keys evenly."""
+    case = _case(cuda, 1, 8, 1, 128, 400, 16, "f32")
+    for h, s in enumerate((1e-44, 1e-38, 1e-25, 1e-18, 1.0, 1e3, 0.0, 1e-30)):
+        case[0][0, h] = (case[0][0, h].double() * s).float()
+    _run(case, 16, None)
+    big = case[0].clone()
+    big[0, 0] = 3e38 * torch.sign(big[0, 1])
+    got = ops.decode_attention_q8(big, *case[1:], 16, scale=1e-38)
+    want, mag, tol = _q8.attend(big, *case[1:], None, 16, 1e-38)
+    _close(got, want, tol)
+
+
+def test_a_wait_that_runs_out(cuda):
+    """With its copies withheld every wait of the tensor-core kernel runs out:
+    NaN outputs and the sticky flag, then the context works on."""
+    case = _case(cuda, 2, 8, 2, 128, 1024, 64, "bf16")
+    flags = _lib.C.c_uint32()
+    _lib.call("oxide_device_status", 1, _lib.C.byref(flags))
+    out = _on_path(2, case, 64, None)
+    assert bool(torch.isnan(out).all())
+    _lib.call("oxide_device_status", 1, _lib.C.byref(flags))
+    assert flags.value == _lib.DEVICE_WAIT_TIMEOUT
+    _run(case, 64, None)
+    _lib.call("oxide_device_status", 0, _lib.C.byref(flags))
+    assert flags.value == 0

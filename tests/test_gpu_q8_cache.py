@@ -213,22 +213,21 @@ def test_offsets_past_32_bits(cuda):
     assert torch.equal(v, _q8.values(vc[:, :, -384:], vs[:, :, -3:], block)[:, :, 84:].float())
     # and the attention over it: two heads of the second sequence's last keys
     q = torch.randn((2, 2, d), generator=g, device=cuda)
-    # all other keys are zero codes: score 0, value 0 -- the definition in closed form
+    # all other keys are zero codes: score 0, value 0 -- the definition over the
+    # last 512 keys with the others' mass added
     out = ops.decode_attention_q8(q, kc, vc, ks, vs, block, torch.tensor([m, m - 7], dtype=torch.int32, device=cuda))
     for i, n in enumerate((m, m - 7)):
         lo = m - 512
-        kk = _q8.values(kc[i:i + 1, :, lo:n], ks[i:i + 1, :, lo // block:], block)[0, 0]
-        vv = _q8.values(vc[i:i + 1, :, lo:n], vs[i:i + 1, :, lo // block:], block)[0, 0]
-        s = q[i].double() @ kk.T / d ** 0.5
-        top = s.amax(-1, keepdim=True).clamp(min=0.0)
-        p = torch.exp(s - top)
-        total = p.sum(-1, keepdim=True) + lo * torch.exp(-top)
-        want = p @ vv / total
-        mag = p @ vv.abs() / total
-        size = (q[i].double().abs() @ kk.abs().T / d ** 0.5).amax()
-        # f32 sums over 2^25 equal weights: each worker adds its keys' weights
-        # one after another, at most 2^25 / 128 a lane before they are joined
-        assert bool(((out[i].double() - want).abs() <= _q8.attend_tolerance(mag, size, d) + mag * 2.0 ** -24 * 2 ** 12).all())
+        tail = (q[i:i + 1], *[t[i:i + 1, :, lo:n] for t in (kc, vc)], *[t[i:i + 1, :, lo // block:] for t in (ks, vs)])
+        want, mag, tol = _q8.attend(*tail, None, block, d ** -0.5)
+        k = _q8.values(tail[1], tail[3], block)[0, 0]
+        s = q[i].double() @ k.T * d ** -0.5
+        share = torch.exp(torch.logsumexp(s, -1) - torch.logaddexp(torch.logsumexp(s, -1),
+                                                                    torch.tensor(float(lo), device=cuda).double().log()))
+        # the tail's tolerance, and the mass of the others: each worker adds up
+        # to 2^25 / 128 equal weights one after another, half a rounding each
+        tol = (tol + mag * 2.0 ** -24 * 2 ** 18) * share[:, None]
+        assert bool(((out[i].double() - want[0] * share[:, None]).abs() <= tol[0]).all())
 
 
 def test_class_round_trip(cuda):
