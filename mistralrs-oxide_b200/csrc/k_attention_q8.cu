@@ -183,55 +183,82 @@ __global__ void __launch_bounds__(QW_WARPS * 32, 2) decode_attn_q8_warp_kernel(Q
 #pragma unroll
                     for (int e = 0; e < W; ++e) {
                         const uint32_t d = W * (lane + 32 * g) + e;
-                        if (d < D) p.part_o[slot * D + d] = acc[h][g * W + e];
+                        if (d < D) p.part_o[slot * DP + d] = acc[h][g * W + e];
                     }
             }
         }
     }
 }
 
-// Merge the parts of one (batch, query head): warp w takes every eighth part
-// of the pair, lane = dim, and the eight states are joined through shared
-// memory.  A part without keys has sum 0; a pair without keys gives zeros; NaN
-// if a wait of the main kernel ran out.
-template <typename T>
-__global__ void __launch_bounds__(256) decode_attn_q8_combine_kernel(T* out, Q8AttnArgs p) {
+// Merge the parts of one (batch, query head): warp w of NW takes every NW-th
+// part of the pair, the loads of QC_UNROLL of them in flight at once (the
+// parts' places follow from the tile division alone), lane = four dims (DV of
+// them 128 apart), and the NW states are joined through shared memory.  A part
+// without keys has sum 0; a pair without keys gives zeros; NaN if a wait of the
+// main kernel ran out.
+// NW: 8 warps while there are fewer CTAs than SMs -- a CTA then merges many
+// parts (one sequence of 131072 keys, 37 parts a head: the whole call 51.0 us
+// against 53.0 with 4) -- else 4, so that more CTAs are resident at once (8
+// sequences of 1024 to 32768, 256 CTAs: 54.7 us against 55.9 with 8).
+constexpr int QC_UNROLL = 5;
+template <typename T, int DV, int NW>
+__global__ void __launch_bounds__(NW * 32) decode_attn_q8_combine_kernel(T* out, Q8AttnArgs p) {
     pdl_begin();
-    constexpr int NW = 8, DPL = Q8A_MAX_D / 32;
-    __shared__ float wm[NW], wl[NW], wo[NW][Q8A_MAX_D];
+    __shared__ float wm[NW], wl[NW];
+    __shared__ float4 wo[NW][32 * DV];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const uint32_t bh = blockIdx.x, b = bh / p.q_heads, qh = bh - b * p.q_heads;
     const uint32_t kvh = qh / p.rep, r = qh - kvh * p.rep, chunk = r / p.nr, h = r - chunk * p.nr;
-    const uint32_t heads = p.kv_heads * p.chunks, D = p.head_dim;
-    const uint32_t before = p.pre_out[b], tb = p.pre_out[b + 1] - before, T_ = p.pre_out[p.batch] * heads;
+    const uint32_t heads = p.kv_heads * p.chunks, D = p.head_dim, DP = q8a_dims(D), W = p.workers;
+    const uint32_t before = p.pre_out[b], tb = p.pre_out[b + 1] - before, all = p.pre_out[p.batch] * heads;
     const uint32_t failed = *p.err;
-    float M = -INFINITY, L = 0.0f, acc[DPL];
+    float M = -INFINITY, L = 0.0f;
+    float4 acc[DV];
 #pragma unroll
-    for (int i = 0; i < DPL; ++i) acc[i] = 0.0f;
+    for (int k = 0; k < DV; ++k) acc[k] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
     if (tb) {
         const uint32_t pair = b * heads + kvh * p.chunks + chunk, tfirst = before * heads + (pair - b * heads) * tb,
-                       tlast = tfirst + tb - 1;
-        const uint32_t c0 = tc_owner(tfirst, T_, p.workers), c1 = tc_owner(tlast, T_, p.workers);
-        for (uint32_t i = warp; i < (c1 - c0 + 1) * p.halves; i += NW) {
-            const uint32_t c = c0 + i / p.halves, half = i % p.halves;
-            const uint32_t f0 = (uint32_t)((uint64_t)c * T_ / p.workers), f1 = (uint32_t)((uint64_t)(c + 1) * T_ / p.workers);
-            const uint32_t a = max(f0, tfirst), e = min(f1, tlast + 1);
-            if (a >= e || (e - a < p.halves && ((a - f0) ^ half) & 1)) continue;  // no tile, or the other half's one tile
-            const uint64_t slot = (((uint64_t)c + pair) * p.halves + half) * p.nr + h;
-            const float ms = p.part_ml[slot * 2], ls = p.part_ml[slot * 2 + 1];
-            float o[DPL];
+                       tend = tfirst + tb;
+        const uint32_t c0 = tc_owner(tfirst, all, W), c1 = tc_owner(tend - 1, all, W);
+        const uint32_t n = (c1 - c0 + 1) * p.halves;
+        for (uint32_t i0 = warp; i0 < n; i0 += NW * QC_UNROLL) {
+            float ms[QC_UNROLL], ls[QC_UNROLL];
+            float4 o[QC_UNROLL][DV];
 #pragma unroll
-            for (int k = 0; k < DPL; ++k) {
-                const uint32_t d = lane + 32 * k;
-                o[k] = d < D ? p.part_o[slot * D + d] : 0.0f;
+            for (int u = 0; u < QC_UNROLL; ++u) {
+                const uint32_t i = i0 + u * NW, c = c0 + i / p.halves, half = i % p.halves;
+                ms[u] = -INFINITY;
+                ls[u] = 0.0f;
+#pragma unroll
+                for (int k = 0; k < DV; ++k) o[u][k] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                if (i >= n) continue;
+                const uint32_t f0 = (uint32_t)((uint64_t)c * all / W), f1 = (uint32_t)((uint64_t)(c + 1) * all / W);
+                const uint32_t a = max(f0, tfirst), e = min(f1, tend);
+                if (a >= e || (e - a < p.halves && ((a - f0) ^ half) & 1)) continue;  // no tile, or the other half's one tile
+                const uint64_t slot = (((uint64_t)c + pair) * p.halves + half) * p.nr + h;
+                ms[u] = p.part_ml[slot * 2];
+                ls[u] = p.part_ml[slot * 2 + 1];
+#pragma unroll
+                for (int k = 0; k < DV; ++k) {
+                    const uint32_t d = 4 * (lane + 32 * k);
+                    if (d < DP) o[u][k] = *reinterpret_cast<const float4*>(p.part_o + slot * DP + d);
+                }
             }
-            if (ls == 0.0f) continue;
-            const float mn = fmaxf(M, ms);
-            const float cr = M == -INFINITY ? 0.0f : ex2_approx(fsub(M, mn)), x = ex2_approx(fsub(ms, mn));
-            L = __fmaf_rn(ls, x, fmul(L, cr));
 #pragma unroll
-            for (int k = 0; k < DPL; ++k) acc[k] = __fmaf_rn(o[k], x, fmul(acc[k], cr));
-            M = mn;
+            for (int u = 0; u < QC_UNROLL; ++u) {
+                if (ls[u] == 0.0f) continue;
+                const float mn = fmaxf(M, ms[u]);
+                const float cr = M == -INFINITY ? 0.0f : ex2_approx(fsub(M, mn)), x = ex2_approx(fsub(ms[u], mn));
+                L = __fmaf_rn(ls[u], x, fmul(L, cr));
+#pragma unroll
+                for (int k = 0; k < DV; ++k) {
+                    acc[k].x = __fmaf_rn(o[u][k].x, x, fmul(acc[k].x, cr));
+                    acc[k].y = __fmaf_rn(o[u][k].y, x, fmul(acc[k].y, cr));
+                    acc[k].z = __fmaf_rn(o[u][k].z, x, fmul(acc[k].z, cr));
+                    acc[k].w = __fmaf_rn(o[u][k].w, x, fmul(acc[k].w, cr));
+                }
+                M = mn;
+            }
         }
     }
     if (lane == 0) {
@@ -239,9 +266,9 @@ __global__ void __launch_bounds__(256) decode_attn_q8_combine_kernel(T* out, Q8A
         wl[warp] = L;
     }
 #pragma unroll
-    for (int k = 0; k < DPL; ++k) wo[warp][lane + 32 * k] = acc[k];
+    for (int k = 0; k < DV; ++k) wo[warp][lane + 32 * k] = acc[k];
     __syncthreads();
-    for (uint32_t d = threadIdx.x; d < D; d += 256) {
+    for (uint32_t d = threadIdx.x; d < D; d += NW * 32) {
         float mx = -INFINITY, ls = 0.0f, o = 0.0f;
 #pragma unroll
         for (int i = 0; i < NW; ++i) mx = fmaxf(mx, wm[i]);
@@ -250,7 +277,7 @@ __global__ void __launch_bounds__(256) decode_attn_q8_combine_kernel(T* out, Q8A
             if (wl[i] == 0.0f) continue;
             const float x = ex2_approx(fsub(wm[i], mx));
             ls = __fmaf_rn(wl[i], x, ls);
-            o = __fmaf_rn(wo[i][d], x, o);
+            o = __fmaf_rn(reinterpret_cast<const float*>(wo[i])[d], x, o);
         }
         float y = ls == 0.0f ? 0.0f : fdiv(o, ls);
         if (failed) y = q8_nan();
@@ -279,6 +306,13 @@ template <int NR>
 static cudaError_t launch_warp_d(Q8AttnArgs& a, bool d4, cudaStream_t st) {
     if (!d4) return launch_warp<NR, 8, false>(a, st);
     return a.head_dim <= 128 ? launch_warp<NR, 1, true>(a, st) : launch_warp<NR, 2, true>(a, st);
+}
+
+template <typename T, int DV>
+static cudaError_t launch_combine(T* out, const Q8AttnArgs& a, cudaStream_t st) {
+    const unsigned grid = a.batch * a.q_heads;
+    return grid < (unsigned)sm_count() ? launch_k(decode_attn_q8_combine_kernel<T, DV, 8>, grid, 256, 0, st, out, a)
+                                       : launch_k(decode_attn_q8_combine_kernel<T, DV, 4>, grid, 128, 0, st, out, a);
 }
 
 static uint64_t attn_q8_parts(uint64_t batch, uint64_t q_heads, uint64_t kv_heads) {
@@ -323,7 +357,7 @@ static int attn_q8_entry(const char* name, const T* q, const int8_t* kc, const i
     a.q = q;
     a.lens = lens;
     a.part_o = static_cast<float*>(ws);
-    a.part_ml = a.part_o + parts * nr * head_dim;
+    a.part_ml = a.part_o + parts * nr * q8a_dims((uint32_t)head_dim);
     a.err = reinterpret_cast<uint32_t*>(a.part_ml + parts * nr * 2);
     a.pre_out = a.err + 4;
     a.max_seq = max_seq;
@@ -351,8 +385,7 @@ static int attn_q8_entry(const char* name, const T* q, const int8_t* kc, const i
         case 4: e = launch_warp_d<4>(a, d4, st); break;
         default: e = launch_warp_d<8>(a, d4, st); break;
     }
-    if (e == cudaSuccess)
-        e = launch_k(decode_attn_q8_combine_kernel<T>, (unsigned)(batch * q_heads), 256, 0, st, out, a);
+    if (e == cudaSuccess) e = head_dim <= 128 ? launch_combine<T, 1>(out, a, st) : launch_combine<T, 2>(out, a, st);
     if (e != cudaSuccess) {
         cudaGetLastError();
         return set_error(OXIDE_ERR_LAUNCH, "%s: launch failed: %s", name, cudaGetErrorString(e));
@@ -369,7 +402,7 @@ extern "C" {
 uint64_t oxide_decode_attention_q8_workspace_bytes(uint64_t batch, uint64_t q_heads, uint64_t kv_heads,
                                                    uint64_t head_dim) {
     const uint64_t parts = oxide::attn_q8_parts(batch, q_heads, kv_heads);
-    return parts * oxide::attn_q8_nr(q_heads, kv_heads) * (head_dim + 2) * 4 + 16 + (batch + 4) / 4 * 16;
+    return parts * oxide::attn_q8_nr(q_heads, kv_heads) * ((head_dim + 3) / 4 * 4 + 2) * 4 + 16 + (batch + 4) / 4 * 16;
 }
 int oxide_decode_attention_q8_f32(const float* q, const int8_t* k_cache, const int8_t* v_cache, const float* k_scale,
                                   const float* v_scale, const int32_t* lens, float* out, uint64_t batch,

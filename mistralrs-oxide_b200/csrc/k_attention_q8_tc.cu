@@ -21,18 +21,24 @@
 // a CTA.  head_dim a multiple of 16 up to 128: the tile is 128 bytes wide and
 // TMA fills what lies past head_dim with zeros.
 //
-// CTA of 12 warps:
-//   warp 0      (one lane) TMA producer: K and V tiles [128 keys x 128 bytes],
+// CTA of 13 warps:
+//   warp 0      TMA producer: K and V tiles [128 keys x 128 bytes],
 //               128-byte swizzle, 6-stage ring (32 KB a stage: the bytes of
 //               half as many bf16 keys);
-//   warp 1      TMEM owner and (one lane) MMA issuer:
-//                 S[128 keys x N] = K . X^T   (A = K, K-major; B = digits of q)
+//   warp 1      TMEM owner and issuer of the scores' products,
+//                 S[128 keys x N] = K . X^T   (A = K, K-major; B = digits of q);
+//   warp 12     issuer of the outputs' products,
 //                 O[128 dims x N] = V^T . Y^T (A = V read MN-major; B = digits
-//                                              of the weights)
+//                                              of the weights),
 //               N = 16 for up to 4 heads, 32 for 8 (M = 128 takes N in steps
-//               of 16);
+//               of 16).  One thread issuing both spent 2100 cycles a tile on
+//               waits and issue, twice what the loads allow;
 //   warp 2      the query heads' digits, one pair ahead;
-//   warp 3      the tile prefix at the start;
+//   warp 3      the tile prefix; then each tile's scales, ready for the softmax
+//               threads (the key scale, log2 of the value scale, masks), loaded
+//               two tiles ahead.  One scale for a lane's four keys wherever
+//               blocks allow it: with one for every key this warp alone took
+//               1400 cycles a tile, 200 more than the loads;
 //   warps 4-7 and 8-11  two softmax groups that take the tiles in turn, each
 //               with its own S and O in TMEM, weights buffer and online state:
 //               one group's barriers and latencies hide behind the other's
@@ -53,8 +59,11 @@ namespace oxide {
 
 constexpr uint32_t QT_TK = 128, QT_DB = 128;  // keys a tile, bytes a row in shared memory
 constexpr int QT_STAGES = 6;
-constexpr int QT_THREADS = 384;
+constexpr int QT_THREADS = 416;
 constexpr uint32_t QT_MAX_BATCH = 1024;
+// Maxima start here, not at -infinity: differences stay numbers, and a masked
+// score (-infinity) is a zero weight without being asked about.
+constexpr float QT_LOW = -3.0e38f;
 constexpr float Q_UNIT = 8.0e6f;  // below 0x7f7f7f = 8355711, the largest three balanced digits hold
 constexpr uint32_t QT_TMEM_COLS = 128, QT_TMEM_O = 64;  // S at 32 g, O at 64 + 32 g for group g
 constexpr uint32_t QT_TILE = QT_TK * QT_DB;       // 16 KB
@@ -64,14 +73,16 @@ constexpr uint32_t QT_BBYTES = 32 * 128;          // a B operand: up to 32 rows 
 constexpr uint32_t QT_OFF_Q = QT_STAGES * QT_STAGE_BYTES;                // 2 slots
 constexpr uint32_t QT_OFF_P = QT_OFF_Q + 2 * QT_BBYTES;                  // 2 groups
 constexpr uint32_t QT_OFF_PRE = QT_OFF_P + 2 * QT_BBYTES;
-constexpr uint32_t QT_OFF_SQ = QT_OFF_PRE + (QT_MAX_BATCH + 8) * 4;      // [2][8] factors of the scores
-constexpr uint32_t QT_OFF_RED = QT_OFF_SQ + 2 * 8 * 4;                   // [2][4][16] tile maxima
+constexpr uint32_t QT_OFF_SC = QT_OFF_PRE + (QT_MAX_BATCH + 8) * 4;      // a stage's keys: float2 [128]
+constexpr uint32_t QT_OFF_SQ = QT_OFF_SC + QT_STAGES * QT_TK * 8;        // [2][8] factors of the scores
+constexpr uint32_t QT_OFF_RED = QT_OFF_SQ + 2 * 8 * 4;                   // [2][4][16] each warp's tile maxima
 constexpr uint32_t QT_OFF_SUM = QT_OFF_RED + 2 * 4 * 16 * 4;             // [2][4][8] sums
 constexpr uint32_t QT_OFF_BAR = QT_OFF_SUM + 2 * 4 * 8 * 4;
 enum : int {
     QB_FULL = 0,                      // [6] stage loaded (TMA bytes)
     QB_EMPTY = QB_FULL + QT_STAGES,   // [6] stage consumed (MMA commit)
-    QB_QFULL = QB_EMPTY + QT_STAGES,  // [2] digits of a pair's query heads written (warp 2)
+    QB_CFULL = QB_EMPTY + QT_STAGES,  // [6] the stage's scales written (warp 3)
+    QB_QFULL = QB_CFULL + QT_STAGES,  // [2] digits of a pair's query heads written (warp 2)
     QB_QEMPTY = QB_QFULL + 2,         // [2] read: MMA commit and the eight softmax warps
     QB_SFULL = QB_QEMPTY + 2,         // [2] scores in TMEM (MMA commit)
     QB_SEMPTY = QB_SFULL + 2,         // [2] scores read (4 warps)
@@ -81,8 +92,11 @@ enum : int {
     QB_COUNT = QB_DONE + 1
 };
 constexpr uint32_t QT_OFF_MISC = QT_OFF_BAR + ((QB_COUNT + 1) & ~1) * 8;
-constexpr size_t QT_SMEM = QT_OFF_MISC + 32 + 1024;  // + alignment slack
-static_assert(QT_SMEM <= 227 * 1024, "shared memory of one CTA");
+constexpr size_t QT_SMEM = QT_OFF_MISC + 48 + 1024;  // + alignment slack
+static_assert(QT_STAGES % 2 == 0, "a softmax group's stages repeat after half a ring");
+// Leaves room beside it for a CTA of the combine kernel (4.1 KB), which is
+// launched early and waits there.
+static_assert(QT_SMEM <= 221 * 1024, "shared memory of one CTA");
 static_assert(2 * 1024 <= Q8A_PARTS, "two parts a CTA fit the workspace");
 
 __device__ unsigned int g_device_status_q8;  // sticky failure flags, read by oxide_device_status
@@ -99,18 +113,26 @@ __device__ __forceinline__ void qt_load(uint32_t taddr, uint32_t (&v)[qt_cols<NR
     for (int i = 0; i < (int)qt_cols<NR>(); i += 8) tmem_ld8(taddr + i, v + i);
     tmem_wait_ld();
 }
-// Three digit sums as the number they spell.
+// Three digit sums as the number they spell (each sum is below 2^21 in
+// magnitude, so the lower two join in 32 bits).
 __device__ __forceinline__ float qt_spell(uint32_t d0, uint32_t d1, uint32_t d2) {
-    return __fmaf_rn((float)(int)d2, 65536.0f, __fmaf_rn((float)(int)d1, 256.0f, (float)(int)d0));
+    return __fmaf_rn((float)(int)d2, 65536.0f, (float)((int)d1 * 256 + (int)d0));
 }
 // Balanced digits of |x| <= Q_UNIT in bytes 0, 1, 2.
 __device__ __forceinline__ uint32_t qt_digits(float x) {
     return ((uint32_t)__float2int_rn(x) + 0x808080u) ^ 0x808080u;
 }
 
-struct QtScales {
-    float k, v;
-};
+__device__ __forceinline__ void prefetch_l2(const void* p) {
+    asm volatile("prefetch.global.L2 [%0];" ::"l"(p) : "memory");
+}
+
+// Weights and rescaling factors: results below 2^-126 are zero.
+__device__ __forceinline__ float qt_ex2(float t) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(t));
+    return y;
+}
 
 template <int NR>
 __global__ void __launch_bounds__(QT_THREADS, 1)
@@ -126,7 +148,8 @@ __global__ void __launch_bounds__(QT_THREADS, 1)
     float* sq = reinterpret_cast<float*>(smem + QT_OFF_SQ);
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + QT_OFF_MISC);
     volatile int* abort = reinterpret_cast<volatile int*>(smem + QT_OFF_MISC + 4);
-    volatile int* consumed = reinterpret_cast<volatile int*>(smem + QT_OFF_MISC + 8);  // stages the MMA warp waited for
+    volatile int* consumed = reinterpret_cast<volatile int*>(smem + QT_OFF_MISC + 8);  // stages warp 1 waited for
+    uint32_t* begin = reinterpret_cast<uint32_t*>(smem + QT_OFF_MISC + 16);  // where this CTA's tiles begin: b, kvh, lt, tb
     auto bar = [&](int i) { return sbase + QT_OFF_BAR + 8u * (uint32_t)i; };
 
     if (tid == 0) {
@@ -135,6 +158,7 @@ __global__ void __launch_bounds__(QT_THREADS, 1)
         for (int i = 0; i < QT_STAGES; ++i) {
             mbar_init(bar(QB_FULL + i), 1);
             mbar_init(bar(QB_EMPTY + i), 1);
+            mbar_init(bar(QB_CFULL + i), 1);
         }
         for (int i = 0; i < 2; ++i) {
             mbar_init(bar(QB_QFULL + i), 1);
@@ -144,7 +168,7 @@ __global__ void __launch_bounds__(QT_THREADS, 1)
             mbar_init(bar(QB_PFULL + i), 1);
             mbar_init(bar(QB_OFULL + i), 1);
         }
-        mbar_init(bar(QB_DONE), 1);
+        mbar_init(bar(QB_DONE), 2);
         mbar_init_fence();
         tma_prefetch_map(&tmk);
         tma_prefetch_map(&tmv);
@@ -154,98 +178,136 @@ __global__ void __launch_bounds__(QT_THREADS, 1)
         tmem_relinquish();
     }
     pdl_wait();  // the previous kernel's writes (lengths, caches, queries) are visible
-    if (warp == 3) q8a_prefix(p, QT_TK, pre, blockIdx.x == 0);
+    const uint32_t heads = p.kv_heads * p.chunks, G = p.workers;
+    if (warp == 3) {  // the tile prefix and this CTA's first tile
+        q8a_prefix(p, QT_TK, pre, blockIdx.x == 0);
+        const uint32_t all = pre[p.batch] * heads;
+        if (all) {
+            TileWalk at{pre, p.batch, heads, 0, 0, 0, 0};
+            at.seek((uint32_t)((uint64_t)blockIdx.x * all / G));
+            if (lane == 0) {
+                begin[0] = at.b;
+                begin[1] = at.kvh;
+                begin[2] = at.lt;
+                begin[3] = at.tb;
+            }
+            // The first pair's query heads and scales go ahead of the ring's 192 KB
+            // a CTA: asked for behind them they came 3 us later.
+            const uint32_t kvh = at.kvh / p.chunks, h0 = (at.kvh % p.chunks) * NR;
+            const uint32_t es = p.q_bf16 ? 2 : 4, bytes = min(p.rep - h0, (uint32_t)NR) * p.head_dim * es;
+            if (lane * 128u < bytes)
+                prefetch_l2(static_cast<const char*>(p.q) +
+                            ((uint64_t)at.b * p.q_heads + kvh * p.rep + h0) * p.head_dim * es + lane * 128u);
+            const uint64_t sc = ((uint64_t)at.b * p.kv_heads + kvh) * p.nblk + ((at.lt * QT_TK) >> p.shift);
+            if (lane < 2) prefetch_l2((lane ? p.vs : p.ks) + sc);
+        }
+    }
     if (tid == 0 && blockIdx.x == 0) *p.err = 0u;
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
-    const uint32_t heads = p.kv_heads * p.chunks, T = pre[p.batch] * heads, G = p.workers;
+    const uint32_t T = pre[p.batch] * heads;
     const uint32_t t0 = (uint32_t)((uint64_t)blockIdx.x * T / G);
     const uint32_t nt = (uint32_t)((uint64_t)(blockIdx.x + 1) * T / G) - t0;  // this CTA's tiles, n = 0 .. nt - 1
-    TileWalk w{pre, p.batch, heads, 0, 0, 0, 0};
+    TileWalk w{pre, p.batch, heads, begin[0], begin[1], begin[2], begin[3]};  // (unset, and unused, without tiles)
 
     if (warp == 0) {
         // ---------------- TMA producer ----------------
-        uint32_t n = 0;
-        if (lane == 0 && nt && !withhold) {
-            w.seek(t0);
-            for (; n < nt && !*abort; w.next()) {
-                const uint32_t s = n % QT_STAGES;
-                if (!tc_wait(bar(QB_EMPTY + s), ((n / QT_STAGES) & 1u) ^ 1u, abort)) break;
-                mbar_arrive_expect_tx(bar(QB_FULL + s), QT_STAGE_BYTES);
-                const int z = (int)(w.b * p.kv_heads + w.kvh / p.chunks), y = (int)(w.lt * QT_TK);
+        const bool leader = elect_one();
+        uint32_t n = 0, s = 0, ph = 1;  // the stage and its phase
+        if (!withhold) {
+            for (; n < nt && !*abort; ++n) {
+                if (!warp_wait_all(bar(QB_EMPTY + s), ph, abort)) break;
+                const int z = (int)(w.b * p.kv_heads + (p.chunks == 1 ? w.kvh : w.kvh / p.chunks));
+                const int y = (int)(w.lt * QT_TK);
                 const uint32_t sd = sbase + s * QT_STAGE_BYTES;
-                tma_load_3d(sd, &tmk, bar(QB_FULL + s), 0, y, z);
-                tma_load_3d(sd + QT_TILE, &tmv, bar(QB_FULL + s), 0, y, z);
-                ++n;
+                if (leader) {
+                    mbar_arrive_expect_tx(bar(QB_FULL + s), QT_STAGE_BYTES);
+                    tma_load_3d(sd, &tmk, bar(QB_FULL + s), 0, y, z);
+                    tma_load_3d(sd + QT_TILE, &tmv, bar(QB_FULL + s), 0, y, z);
+                }
+                __syncwarp();
+                w.next();
+                if (++s == QT_STAGES) {
+                    s = 0;
+                    ph ^= 1u;
+                }
             }
         }
-        // Drain (after an abort): copies issued but never waited for by the
-        // MMA warp land before the CTA exits.
-        if (lane == 0 && *abort) {
+        // Drain (after an abort): copies issued but never waited for by warp 1
+        // land before the CTA exits.
+        if (leader && *abort) {
             for (uint32_t i = (uint32_t)*consumed; i < n; ++i)
                 tc_wait_drain(bar(QB_FULL + i % QT_STAGES), (i / QT_STAGES) & 1u);
         }
         __syncwarp();
     } else if (warp == 1) {
-        // ---------------- MMA issuer ----------------
-        if (lane == 0 && nt) {
-            constexpr uint32_t IDESC_S = umma_idesc_s8(128, N, false, false);
-            constexpr uint32_t IDESC_O = umma_idesc_s8(128, N, true, false);
-            w.seek(t0);  // of the next S product
-            uint32_t q = 0, ns = 0;
-            auto issue_s = [&]() -> bool {
-                const uint32_t n = ns, s = n % QT_STAGES, g = n & 1u;
-                if (n == 0 || w.lt == 0) {
-                    if (!tc_wait(bar(QB_QFULL + (q & 1u)), (q >> 1) & 1u, abort)) return false;
-                }
-                if (!tc_wait(bar(QB_FULL + s), (n / QT_STAGES) & 1u, abort)) return false;
-                *consumed = (int)n + 1;
-                if (!tc_wait(bar(QB_SEMPTY + g), ((n >> 1) & 1u) ^ 1u, abort)) return false;
-                tc_fence_after();
-                const uint32_t ka = sbase + s * QT_STAGE_BYTES, qa = sbase + QT_OFF_Q + (q & 1u) * QT_BBYTES;
-#pragma unroll
-                for (uint32_t kk = 0; kk < 4; ++kk)  // 32 dims a product
-                    umma_s8(tmem + g * 32, umma_desc(ka + kk * 32, 16, 1024, UMMA_SWIZZLE_128B),
-                            umma_desc(qa + kk * 32, 16, 1024, UMMA_SWIZZLE_128B), IDESC_S, kk > 0);
-                umma_commit(bar(QB_SFULL + g));
-                if (n + 1 == nt || w.lt + 1 == w.tb) {  // this pair's last product that reads its digits
-                    umma_commit(bar(QB_QEMPTY + (q & 1u)));
-                    ++q;
-                }
-                ++ns;
+        // ---------------- issuer of the scores ----------------
+        constexpr uint32_t IDESC_S = umma_idesc_s8(128, N, false, false);
+        const bool leader = elect_one();
+        const uint64_t kd = umma_desc(sbase, 16, 1024, UMMA_SWIZZLE_128B);
+        const uint64_t qd = umma_desc(sbase + QT_OFF_Q, 16, 1024, UMMA_SWIZZLE_128B);
+        uint32_t left = 0, q = 0, s = 0, ph = 0;  // tiles left of the pair, its number, the stage and its phase
+        for (uint32_t n = 0; n < nt; ++n) {
+            const uint32_t g = n & 1u;
+            if (left == 0) {
+                left = min(w.tb - w.lt, nt - n);
+                w.lt += left - 1;
                 w.next();
-                return true;
-            };
-            bool ok = issue_s() && (nt < 2 || issue_s());
-            for (uint32_t n = 0; ok && n < nt; ++n) {
-                // The scores of tile n + 2 go first if its keys are here, else
-                // this tile's output does.
-                const uint32_t g = n & 1u, s = n % QT_STAGES, s2 = (n + 2) % QT_STAGES;
-                const bool more = n + 2 < nt;
-                const bool early = more && mbar_test_wait(bar(QB_FULL + s2), ((n + 2) / QT_STAGES) & 1u);
-                if (early && !issue_s()) break;
-                if (!tc_wait(bar(QB_PFULL + g), (n >> 1) & 1u, abort)) break;
-                tc_fence_after();
-                const uint32_t va = sbase + s * QT_STAGE_BYTES + QT_TILE, pa = sbase + QT_OFF_P + g * QT_BBYTES;
+                if (!warp_wait_all(bar(QB_QFULL + (q & 1u)), (q >> 1) & 1u, abort)) break;
+            }
+            if (!warp_wait_all(bar(QB_FULL + s), ph, abort)) break;
+            if (leader) *consumed = (int)n + 1;
+            if (!warp_wait_all(bar(QB_SEMPTY + g), ((n >> 1) & 1u) ^ 1u, abort)) break;
+            tc_fence_after();
+            const uint64_t ka = kd + s * (QT_STAGE_BYTES >> 4), qa = qd + (q & 1u) * (QT_BBYTES >> 4);
+            --left;
+            if (leader) {
 #pragma unroll
-                for (uint32_t kk = 0; kk < 4; ++kk)  // 32 keys a product
-                    umma_s8(tmem + QT_TMEM_O + g * 32, umma_desc(va + kk * 4096, 16, 1024, UMMA_SWIZZLE_128B),
-                            umma_desc(pa + kk * 256, 128, 1024, UMMA_SWIZZLE_NONE), IDESC_O, kk > 0);
-                umma_commit(bar(QB_OFULL + g));
-                umma_commit(bar(QB_EMPTY + s));
-                if (more && !early) ok = issue_s();
+                for (uint32_t kk = 0; kk < 4; ++kk)  // 32 dims (32 bytes) a product
+                    umma_s8(tmem + g * 32, ka + kk * 2, qa + kk * 2, IDESC_S, kk > 0);
+                umma_commit(bar(QB_SFULL + g));
+                if (left == 0) umma_commit(bar(QB_QEMPTY + (q & 1u)));  // the pair's last product that reads its digits
+            }
+            __syncwarp();
+            if (left == 0) ++q;
+            if (++s == QT_STAGES) {
+                s = 0;
+                ph ^= 1u;
             }
         }
-        if (lane == 0) {  // every product issued above has completed before TMEM is freed
+        if (leader) umma_commit(bar(QB_DONE));
+        __syncwarp();
+    } else if (warp == 12) {
+        // ---------------- issuer of the outputs ----------------
+        constexpr uint32_t IDESC_O = umma_idesc_s8(128, N, true, false);
+        const bool leader = elect_one();
+        const uint64_t vd = umma_desc(sbase + QT_TILE, 16, 1024, UMMA_SWIZZLE_128B);
+        const uint64_t pd = umma_desc(sbase + QT_OFF_P, 128, 1024, UMMA_SWIZZLE_NONE);
+        uint32_t s = 0;
+        for (uint32_t n = 0; n < nt; ++n) {
+            const uint32_t g = n & 1u;
+            if (!warp_wait_all(bar(QB_PFULL + g), (n >> 1) & 1u, abort)) break;
+            tc_fence_after();
+            const uint64_t va = vd + s * (QT_STAGE_BYTES >> 4), pa = pd + g * (QT_BBYTES >> 4);
+            if (leader) {
+#pragma unroll
+                for (uint32_t kk = 0; kk < 4; ++kk)  // 32 keys a product: 4096 bytes of V, 256 of the weights
+                    umma_s8(tmem + QT_TMEM_O + g * 32, va + kk * 256, pa + kk * 16, IDESC_O, kk > 0);
+                umma_commit(bar(QB_OFULL + g));
+                umma_commit(bar(QB_EMPTY + s));
+            }
+            __syncwarp();
+            if (++s == QT_STAGES) s = 0;
+        }
+        if (leader) {  // every product issued has completed before TMEM is freed
             umma_commit(bar(QB_DONE));
             if (!tc_wait_drain(bar(QB_DONE), 0)) *abort = 1;
         }
         __syncwarp();
     } else if (warp == 2) {
         // ---------------- digits of the query heads ----------------
-        if (nt) w.seek(t0);
         for (uint32_t n = 0, q = 0; n < nt; ++q) {
             const uint32_t slot = q & 1u, h0 = (w.kvh % p.chunks) * NR, nh = min(p.rep - h0, (uint32_t)NR);
             const uint64_t row = (uint64_t)w.b * p.q_heads + (w.kvh / p.chunks) * p.rep + h0;
@@ -302,6 +364,87 @@ __global__ void __launch_bounds__(QT_THREADS, 1)
             w.lt += cnt - 1;
             w.next();
         }
+    } else if (warp == 3) {
+        // ---------------- scales of the tiles: keys 4 lane .. 4 lane + 3 ----------------
+        struct Keys {
+            float k[4], v[4];
+            uint32_t live;  // how many of the tile's keys the sequence has
+        };
+        const bool shared = p.shift >= 2;  // the lane's four keys share a scale
+        uint32_t len = 0, ahead = 0, s = 0, ph = 1;  // ahead: the tile loaded next; the stage and its phase
+        const float *ks = p.ks, *vs = p.vs;          // the head's scales
+        auto load = [&](Keys& x) {
+            if (ahead >= nt) return;
+            if (ahead == 0 || w.lt == 0) {  // a new pair
+                len = q8a_len(p, w.b);
+                const uint64_t bh = (uint64_t)w.b * p.kv_heads + (p.chunks == 1 ? w.kvh : w.kvh / p.chunks);
+                ks = p.ks + bh * p.nblk;
+                vs = p.vs + bh * p.nblk;
+            }
+            const uint32_t key0 = w.lt * QT_TK, key = key0 + 4 * lane;
+            x.live = len - key0;
+            if (shared) {
+                x.k[0] = x.v[0] = 1.0f;
+                if (key < len) {
+                    x.k[0] = __ldg(ks + (key >> p.shift));
+                    x.v[0] = __ldg(vs + (key >> p.shift));
+                }
+            } else {
+#pragma unroll
+                for (uint32_t i = 0; i < 4; ++i) {
+                    x.k[i] = x.v[i] = 1.0f;
+                    if (key + i < len) {
+                        x.k[i] = __ldg(ks + ((key + i) >> p.shift));
+                        x.v[i] = __ldg(vs + ((key + i) >> p.shift));
+                    }
+                }
+            }
+            ++ahead;
+            w.next();
+        };
+        // What a softmax thread needs of its key: the key scale and log2 of the
+        // value scale.  A value scale that is NaN, infinite or negative makes
+        // the key's scores NaN; +infinity as the log2 marks a masked key.
+        auto ready = [&](float k, float v) -> float2 {
+            const bool sound = v >= 0.0f && v < INFINITY;
+            return make_float2(sound ? k : q8_nan(), sound ? lg2_approx(v) : 0.0f);
+        };
+        auto put = [&](const Keys& x) -> bool {
+            float2 r[4];
+            r[0] = ready(x.k[0], x.v[0]);
+            if (shared) {
+                r[1] = r[2] = r[3] = r[0];
+            } else {
+#pragma unroll
+                for (int i = 1; i < 4; ++i) r[i] = ready(x.k[i], x.v[i]);
+            }
+            if (x.live < QT_TK) {
+#pragma unroll
+                for (uint32_t i = 0; i < 4; ++i)
+                    if (4 * lane + i >= x.live) r[i] = make_float2(0.0f, INFINITY);
+            }
+            // the output product of the stage's last tile came after its scales were read
+            if (!warp_wait_all(bar(QB_EMPTY + s), ph, abort)) return false;
+            float4* out = reinterpret_cast<float4*>(smem + QT_OFF_SC) + (s * QT_TK + 4 * lane) / 2;
+            out[0] = make_float4(r[0].x, r[0].y, r[1].x, r[1].y);
+            out[1] = make_float4(r[2].x, r[2].y, r[3].x, r[3].y);
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bar(QB_CFULL + s));
+            if (++s == QT_STAGES) {
+                s = 0;
+                ph ^= 1u;
+            }
+            return true;
+        };
+        Keys a, b;  // tiles n and n + 1 in turn
+        load(a);
+        load(b);
+        for (uint32_t n = 0; n < nt; n += 2) {
+            if (!put(a)) break;
+            load(a);
+            if (n + 1 >= nt || !put(b)) break;
+            load(b);
+        }
     } else if (warp >= 4) {
         // ---------------- softmax and epilogue: group g takes tiles n = g mod 2 ----------------
         const uint32_t g = (uint32_t)(warp >> 2) - 1, q4 = (uint32_t)(warp & 3);
@@ -316,40 +459,10 @@ __global__ void __launch_bounds__(QT_THREADS, 1)
         float m[NR], l[NR], wm[NR], acc[NR], corr[NR], tf[NR];
         bool fail = false, pending = false;
 
-        // scales of this group's tiles, loaded two of them ahead
-        TileWalk ahead = w;
-        auto fetch = [&]() -> QtScales {  // of key L of the tile `ahead` is at
-            const uint64_t bh = (uint64_t)ahead.b * p.kv_heads + ahead.kvh / p.chunks;
-            const uint32_t key = ahead.lt * QT_TK + L;
-            QtScales s{0.0f, 1.0f};
-            if (key < q8a_len(p, ahead.b)) {
-                s.k = __ldg(p.ks + bh * p.nblk + (key >> p.shift));
-                s.v = __ldg(p.vs + bh * p.nblk + (key >> p.shift));
-            }
-            return s;
-        };
-        QtScales cur{0.0f, 1.0f}, next{0.0f, 1.0f};
-        uint32_t na = g;  // the tile `ahead` is at
-        auto step_ahead = [&](QtScales& s) {
-            if (na >= nt) return;
-            s = fetch();
-            na += 2;
-            if (na < nt) {
-                ahead.next();
-                ahead.next();
-            }
-        };
-        if (g < nt) {
-            w.seek(t0);
-            ahead = w;
-            if (g) ahead.next();
-            step_ahead(cur);
-            step_ahead(next);
-        } else if (nt) {
-            w.seek(t0);
-        }
+        const float2* scales = reinterpret_cast<const float2*>(smem + QT_OFF_SC) + L;
+        uint32_t st = g, ph = 0, k = 0;  // the stage and its phase, and the number, of this group's next tile
         auto epilogue = [&](uint32_t k) {  // add the output of this group's tile k
-            const bool ok = warp_wait(bar(QB_OFULL + g), k & 1u, abort);
+            const bool ok = warp_wait_all(bar(QB_OFULL + g), k & 1u, abort);
             fail |= !ok;
             if (!ok) return;
             tc_fence_after();
@@ -363,28 +476,26 @@ __global__ void __launch_bounds__(QT_THREADS, 1)
 
         bool dead = false;
         for (uint32_t n = 0, q = 0; n < nt && !dead; ++q) {
-            const uint32_t cnt = min(w.tb - w.lt, nt - n), j0 = (n ^ g) & 1u, len = q8a_len(p, w.b);
+            const uint32_t cnt = min(w.tb - w.lt, nt - n), j0 = (n ^ g) & 1u;
             // every warp waits for the digits, also of a pair without a tile
             // for it: its arrival below then belongs to this use of the slot
-            fail |= !warp_wait(bar(QB_QFULL + (q & 1u)), (q >> 1) & 1u, abort);
-            __syncwarp();  // lane 0's wait covers the other lanes' reads of the factors
+            fail |= !warp_wait_all(bar(QB_QFULL + (q & 1u)), (q >> 1) & 1u, abort);
             float f[NR];
 #pragma unroll
             for (int h = 0; h < NR; ++h) {
                 f[h] = sq[(q & 1u) * 8 + h];
-                m[h] = wm[h] = -INFINITY;
+                m[h] = wm[h] = QT_LOW;
                 l[h] = acc[h] = 0.0f;
             }
             __syncwarp();
             if (lane == 0) mbar_arrive(bar(QB_QEMPTY + (q & 1u)));
             pending = false;
             for (uint32_t j = j0; j < cnt; j += 2) {
-                const uint32_t k = (n + j) >> 1, key0 = (w.lt + j) * QT_TK;
-                const bool on = key0 + L < len;
                 float t[NR], tv[NR];
-                const QtScales sc = cur;
-                cur = next;
-                const bool ok = warp_wait(bar(QB_SFULL + g), k & 1u, abort);
+                bool ok = warp_wait_all(bar(QB_CFULL + st), ph, abort);
+                const float2 sc = scales[st * QT_TK];  // key scale; log2 of the value scale, or the mark of a masked key
+                const float mask = sc.y == INFINITY ? -INFINITY : 0.0f, lv = sc.y == INFINITY ? 0.0f : sc.y;
+                ok = warp_wait_all(bar(QB_SFULL + g), k & 1u, abort) && ok;
                 fail |= !ok;
                 if (ok) {
                     tc_fence_after();
@@ -393,18 +504,15 @@ __global__ void __launch_bounds__(QT_THREADS, 1)
                     tc_fence_before();
                     __syncwarp();
                     if (lane == 0) mbar_arrive(bar(QB_SEMPTY + g));
-                    // a scale that is NaN, infinite or negative makes its keys' scores NaN
-                    const float sound = sc.v >= 0.0f && sc.v < INFINITY ? 0.0f : q8_nan(), lv = lg2_approx(sc.v);
 #pragma unroll
                     for (int h = 0; h < NR; ++h) {
-                        t[h] = on ? fadd(fmul(qt_spell(v[h], v[NR + h], v[2 * NR + h]), fmul(sc.k, f[h])), sound) : -INFINITY;
-                        tv[h] = on ? fadd(t[h], lv) : -INFINITY;
+                        t[h] = __fmaf_rn(qt_spell(v[h], v[NR + h], v[2 * NR + h]), fmul(sc.x, f[h]), mask);
+                        tv[h] = fadd(t[h], lv);
                     }
                 } else {
 #pragma unroll
                     for (int h = 0; h < NR; ++h) t[h] = tv[h] = -INFINITY;
                 }
-                step_ahead(next);
 #pragma unroll
                 for (int h = 0; h < NR; ++h) {
                     const float a = warp_fmax(t[h]), b = warp_fmax(tv[h]);
@@ -415,19 +523,31 @@ __global__ void __launch_bounds__(QT_THREADS, 1)
                 }
                 if (pending) epilogue(k - 1);  // its product has run meanwhile; the weights buffer and O are free after it
                 nbar_sync128(nbar);            // the four warps' maxima are in red
+                float mn[NR], wt[NR], wn[NR];
+                bool moved = false;
 #pragma unroll
                 for (int h = 0; h < NR; ++h) {
                     const float* r = red + h;
-                    const float mt = fmaxf(fmaxf(r[0], r[16]), fmaxf(r[32], r[48]));
-                    const float wt = fmaxf(fmaxf(r[8], r[24]), fmaxf(r[40], r[56]));
-                    const float mn = fmaxf(m[h], mt), wn = fmaxf(wm[h], wt);
-                    const float cr = m[h] == -INFINITY ? 0.0f : ex2_approx(fsub(m[h], mn));
-                    l[h] = __fmaf_rn(l[h], cr, t[h] == -INFINITY ? 0.0f : ex2_approx(fsub(t[h], mn)));
-                    m[h] = mn;
-                    corr[h] = wm[h] == -INFINITY ? 0.0f : ex2_approx(fsub(wm[h], wn));
-                    tf[h] = wt == -INFINITY ? 0.0f : fmul(ex2_approx(fsub(wt, wn)), 1.0f / Q_UNIT);
-                    wm[h] = wn;
-                    const uint32_t d = qt_digits(tv[h] == -INFINITY ? 0.0f : fmul(ex2_approx(fsub(tv[h], wt)), Q_UNIT));
+                    mn[h] = fmaxf(fmaxf(fmaxf(r[0], r[16]), fmaxf(r[32], r[48])), m[h]);
+                    wt[h] = fmaxf(fmaxf(fmaxf(r[8], r[24]), fmaxf(r[40], r[56])), QT_LOW);
+                    wn[h] = fmaxf(wt[h], wm[h]);
+                    moved |= mn[h] != m[h] || wn[h] != wm[h];
+                    corr[h] = 1.0f;
+                }
+                if (moved) {  // the same for every thread of the group
+#pragma unroll
+                    for (int h = 0; h < NR; ++h) {
+                        l[h] = fmul(l[h], qt_ex2(fsub(m[h], mn[h])));
+                        corr[h] = qt_ex2(fsub(wm[h], wn[h]));
+                        m[h] = mn[h];
+                        wm[h] = wn[h];
+                    }
+                }
+#pragma unroll
+                for (int h = 0; h < NR; ++h) {
+                    l[h] = fadd(l[h], qt_ex2(fsub(t[h], m[h])));
+                    tf[h] = fmul(qt_ex2(fsub(wt[h], wm[h])), 1.0f / Q_UNIT);
+                    const uint32_t d = qt_digits(fmul(qt_ex2(fsub(tv[h], wt[h])), Q_UNIT));
 #pragma unroll
                     for (int i = 0; i < 3; ++i) {  // row r of the B operand, byte L: K-major cores of 8 rows x 16 bytes
                         const uint32_t r8 = i * NR + h;
@@ -442,10 +562,16 @@ __global__ void __launch_bounds__(QT_THREADS, 1)
                 }
                 if ((tid & 127) == 0) mbar_arrive(bar(QB_PFULL + g));  // every thread has written its weights and read O
                 pending = true;
+                ++k;
+                st += 2;
+                if (st >= QT_STAGES) {
+                    st -= QT_STAGES;
+                    ph ^= 1u;
+                }
             }
             if (dead) break;
             if (j0 < cnt) {  // the pair is complete here: its partial
-                epilogue((n + cnt - 1 - ((n + cnt - 1 - g) & 1u)) >> 1);
+                epilogue(k - 1);
 #pragma unroll
                 for (int h = 0; h < NR; ++h) {
                     const float x = warp_sum(l[h]);
@@ -463,7 +589,7 @@ __global__ void __launch_bounds__(QT_THREADS, 1)
                     const uint64_t slot = part * NR + h;
                     if (L < p.head_dim)
                         p.part_o[slot * p.head_dim + L] =
-                            wm[h] == -INFINITY ? 0.0f : fmul(acc[h], ex2_approx(fsub(wm[h], m[h])));
+                            fmul(acc[h], qt_ex2(fsub(wm[h], m[h])));
                     if (L == 0) {
                         p.part_ml[slot * 2] = m[h];
                         p.part_ml[slot * 2 + 1] = fadd(fadd(lsum[h], lsum[8 + h]), fadd(lsum[16 + h], lsum[24 + h]));

@@ -23,7 +23,7 @@ struct Q8AttnArgs {
     const void* q;             // f32 or bf16 (q_bf16)
     const int32_t* lens;       // NULL: max_seq
     float* part_ml;            // [part][nr][2]: base-2 maximum, sum
-    float* part_o;             // [part][nr][head_dim], relative to the maximum
+    float* part_o;             // [part][nr][q8a_dims(head_dim)], relative to the maximum
     uint32_t* err;             // set when a bounded wait ran out
     uint32_t* pre_out;         // [batch + 1] tile prefix, for the combine kernel
     uint64_t max_seq;
@@ -34,6 +34,9 @@ struct Q8AttnArgs {
     uint32_t q_bf16;
     float c1;                  // scale * log2(e)
 };
+
+// Floats a row of part_o has: whole 16-byte vectors.
+__host__ __device__ __forceinline__ uint32_t q8a_dims(uint32_t head_dim) { return (head_dim + 3) & ~3u; }
 
 __device__ __forceinline__ uint32_t q8a_len(const Q8AttnArgs& p, uint32_t b) {
     if (!p.lens) return (uint32_t)p.max_seq;

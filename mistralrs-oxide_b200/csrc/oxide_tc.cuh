@@ -98,6 +98,13 @@ __device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatil
     if ((threadIdx.x & 31) == 0) ok = tc_wait(bar, parity, abort) ? 1 : 0;
     return __shfl_sync(0xffffffffu, ok, 0) != 0;
 }
+// The same with every lane asking first: the usual case costs one vote, and
+// orders every lane behind the phase.
+__device__ __forceinline__ bool warp_wait_all(uint32_t bar, uint32_t parity, volatile int* abort) {
+    if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
+    const bool ok = warp_wait(bar, parity, abort);
+    return __all_sync(0xffffffffu, ok && mbar_try_wait(bar, parity));
+}
 // Named barrier 1 over 128 threads (four warps), and the same barrier
 // returning the OR of every participant's flag (a uniform decision).
 __device__ __forceinline__ void nbar_sync128() {
@@ -245,6 +252,19 @@ __device__ __forceinline__ void umma_s8(uint32_t d_tmem, uint64_t adesc, uint64_
         "tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
         "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
         : "memory");
+}
+// One lane of a converged warp.  Roles whose instructions are issued by a
+// single thread keep the whole warp on their loop and issue under this: the
+// addresses then stay in uniform registers (the int8 decode attention's S
+// issuer: 1000 cycles a tile in a lane-0 branch, 600 so).
+__device__ __forceinline__ bool elect_one() {
+    uint32_t r;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "elect.sync _|p, 0xffffffff;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(r));
+    return r != 0;
 }
 // The mbarrier arrives once every tcgen05 operation this thread issued
 // before it has completed.
