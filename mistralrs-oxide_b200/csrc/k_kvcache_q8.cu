@@ -91,8 +91,7 @@ __device__ __forceinline__ float append_scale(const AppendItem& it, float had, u
 template <int TPI>
 __device__ __forceinline__ void append_restate(int8_t* head, const AppendQ8Args& p, const AppendItem& it, float had,
                                                float s, uint8_t* lut, uint32_t t) {
-    const Q8Coder coder((double)had, (double)s);
-    for (uint32_t i = t; i < 128; i += TPI) lut[i] = (uint8_t)coder.exact((double)i);
+    for (uint32_t i = t; i < 128; i += TPI) lut[i] = (uint8_t)q8_exact((double)i, (double)had, (double)s);
     if (TPI == 32) __syncwarp();
     else __syncthreads();
     int8_t* c = head + it.start * p.head_dim;
@@ -166,7 +165,7 @@ __global__ void __launch_bounds__(TPI == 32 ? 256 : TPI)
                 float x[V];
                 uint32_t c[V / 4];
                 Vec<T>::unpack(raw[u], x);
-                q8_codes<V>(coder, x, c);
+                if (q8_codes<V>(coder, x, c)) q8_take(c, q8_decide<T>(raw[u], s));
                 q8_store(dst + (uint64_t)(t + u * TPI) * V, c);
             }
         if (grown) {
@@ -203,11 +202,7 @@ __global__ void __launch_bounds__(256)
         int8_t* dst = head + it.lo * p.head_dim;
         for (uint32_t e = t; e < n; e += TPI) {
             const float x = Vec<T>::load1(src + e);
-            float near = 0.0f;
-            const float2 q = coder.fast2(f2(x, x), near);
-            int c = (int)(int8_t)(__float_as_uint(q.x) & 0xffu);
-            if (coder.slow || near > Q8_NEAR) c = coder.exact((double)x);
-            dst[e] = (int8_t)c;
+            dst[e] = (int8_t)q8_code(coder, x, [&] { return coder.exact(x); });
         }
         if (grown) {
             append_restate<TPI>(head, p, it, had, s, luts[g], t);
@@ -231,63 +226,52 @@ __device__ __forceinline__ uint64_t read_live(const ReadQ8Args& p, uint32_t bh) 
     return (uint64_t)l - p.start < p.n ? (uint64_t)l - p.start : p.n;
 }
 
-// One 16-byte output vector (V codes) a step, RQ_UNROLL steps in flight.
-constexpr int RQ_UNROLL = 4;
-template <typename T>
+// A CTA reads a run of one head's rows of k or of v, NC codes a thread: thread t
+// keeps its place in the row (t mod head_dim / NC) and steps over the rows, so
+// the places in memory take a few additions a vector; dividing a flat index for
+// every vector instead took longer than HBM does (100 us for 8 sequences of
+// 8192 x 8 heads x 128 against 51 us of bytes).  UNROLL rows are in flight.
+template <typename T, int NC, int UNROLL>
 __global__ void __launch_bounds__(256)
     kv_read_q8_vec_kernel(const int8_t* kc, const int8_t* vc, const float* ks, const float* vs, T* k, T* v,
-                          ReadQ8Args p, uint64_t half, FastDiv rdiv, FastDiv ndiv, bool narrow) {
+                          ReadQ8Args p, uint32_t per_row, uint32_t rows, uint32_t runs) {
     pdl_begin();
-    constexpr int V = Vec<T>::N;
-    const uint32_t per_row = p.head_dim / V;
-    const uint64_t stride = (uint64_t)gridDim.x * 256;
-    for (uint64_t i0 = (uint64_t)blockIdx.x * 256 + threadIdx.x; i0 < 2 * half; i0 += stride * RQ_UNROLL) {
-        uint32_t c[RQ_UNROLL][V / 4];
-        float s[RQ_UNROLL];
+    const uint32_t r0 = threadIdx.x / per_row, col = (threadIdx.x - r0 * per_row) * NC;
+    if (r0 >= rows) return;  // threads beyond the last whole row of a step
+    const uint32_t run = blockIdx.x % runs, hv = blockIdx.x / runs;  // run of rows; head of k or (behind them) v
+    const bool is_v = hv >= p.heads;
+    const uint32_t bh = is_v ? hv - p.heads : hv;
+    const uint64_t live = read_live(p, bh);
+    const int8_t* codes = (is_v ? vc : kc) + ((uint64_t)bh * p.max_seq + p.start) * p.head_dim + col;
+    const float* scales = (is_v ? vs : ks) + (uint64_t)bh * p.nblk;
+    T* out = (is_v ? v : k) + (uint64_t)bh * p.n * p.head_dim + col;
+    const uint64_t at0 = (uint64_t)run * rows * UNROLL + r0;
+    uint32_t c[UNROLL][NC / 4];
+    float s[UNROLL];
 #pragma unroll
-        for (int u = 0; u < RQ_UNROLL; ++u) {
-            const uint64_t i = i0 + u * stride;
-            s[u] = 0.0f;
+    for (int u = 0; u < UNROLL; ++u) {
+        const uint64_t at = at0 + (uint64_t)u * rows;
+        s[u] = 0.0f;
 #pragma unroll
-            for (int e = 0; e < V / 4; ++e) c[u][e] = 0;
-            if (i >= 2 * half) continue;
-            const bool is_v = i >= half;
-            const uint64_t r = is_v ? i - half : i;
-            uint64_t row, bh;
-            if (narrow) {
-                row = rdiv.div((uint32_t)r);
-                bh = ndiv.div((uint32_t)row);
-            } else {
-                row = r / per_row;
-                bh = row / p.n;
-            }
-            const uint64_t at = row - bh * p.n;
-            if (at >= read_live(p, (uint32_t)bh)) continue;
-            const uint64_t pos = p.start + at;
-            const int8_t* src = (is_v ? vc : kc) + (bh * p.max_seq + pos) * p.head_dim + (r - row * per_row) * V;
-            if (V == 8) {
-                const uint2 w = __ldcs(reinterpret_cast<const uint2*>(src));
-                c[u][0] = w.x;
-                c[u][V / 4 - 1] = w.y;
-            } else {
-                c[u][0] = __ldcs(reinterpret_cast<const unsigned int*>(src));
-            }
-            s[u] = __ldg((is_v ? vs : ks) + bh * p.nblk + (pos >> p.shift));
+        for (int e = 0; e < NC / 4; ++e) c[u][e] = 0;
+        if (at < live) {
+            q8_load(codes + at * p.head_dim, c[u]);
+            s[u] = __ldg(scales + ((p.start + at) >> p.shift));
         }
+    }
 #pragma unroll
-        for (int u = 0; u < RQ_UNROLL; ++u) {
-            const uint64_t i = i0 + u * stride;
-            if (i >= 2 * half) break;
-            float x[V];
+    for (int u = 0; u < UNROLL; ++u) {
+        const uint64_t at = at0 + (uint64_t)u * rows;
+        if (at >= p.n) break;
+        float x[NC];
 #pragma unroll
-            for (int e = 0; e < V; e += 4) {
-                float f[4];
-                q8_unpack4(c[u][e / 4], f);
+        for (int e = 0; e < NC; e += 4) {
+            float f[4];
+            q8_unpack4(c[u][e / 4], f);
 #pragma unroll
-                for (int d = 0; d < 4; ++d) x[e + d] = fmul(f[d], s[u]);
-            }
-            st_stream((i >= half ? v + (i - half) * V : k + i * V), Vec<T>::pack(x));
+            for (int d = 0; d < 4; ++d) x[e + d] = fmul(f[d], s[u]);
         }
+        q8_store_values(out + at * p.head_dim, x);
     }
 }
 
@@ -400,19 +384,31 @@ static int read_q8_entry(const char* name, const int8_t* kc, const int8_t* vc, c
     p.head_dim = (uint32_t)head_dim;
     p.shift = (uint32_t)q8_block_shift(block);
     p.nblk = (uint32_t)((max_seq + block - 1) / block);
-    const uint64_t elems = (uint64_t)p.heads * n * head_dim;
-    const bool vec = head_dim % V == 0 && aligned16(k) && aligned16(v) && aligned_to(kc, V) && aligned_to(vc, V);
-    const uint64_t half = vec ? elems / V : elems;
-    const void* kern = vec ? reinterpret_cast<const void*>(kv_read_q8_vec_kernel<T>)
-                           : reinterpret_cast<const void*>(kv_read_q8_scalar_kernel<T>);
-    const uint64_t want = (2 * half + 255) / 256, cap = (uint64_t)resident_blocks(kern, 256, 0);
-    const unsigned grid = (unsigned)(want < cap ? want : cap);
-    if (vec) {
-        const bool narrow = half < (1ull << 32);
-        launch_k(kv_read_q8_vec_kernel<T>, grid, 256, 0, st, kc, vc, ks, vs, k, v, p, half,
-                 FastDiv((uint32_t)(head_dim / V)), FastDiv((uint32_t)n), narrow);
-    } else {
-        launch_k(kv_read_q8_scalar_kernel<T>, grid, 256, 0, st, kc, vc, ks, vs, k, v, p, half);
+    const uint64_t cap = 1ull << 30;
+    auto launch = [&](auto kern, uint64_t nc, uint64_t unroll) {
+        const uint64_t per_row = head_dim / nc, rows = 256 / per_row;
+        const uint64_t runs = (n + rows * unroll - 1) / (rows * unroll), ctas = 2ull * p.heads * runs;
+        if (ctas >= (1ull << 31)) return false;
+        launch_k(kern, (unsigned)ctas, 256, 0, st, kc, vc, ks, vs, k, v, p, (uint32_t)per_row, (uint32_t)rows, (uint32_t)runs);
+        return true;
+    };
+    // Rows in flight a thread: 8 for long reads (8192 x 64 heads x 128 bf16: 62.7
+    // us); 2 where eight would leave SMs without a CTA (1001 x 15 heads x 64 f32:
+    // 4.3 us against 6.4).
+    auto vec = [&](auto many, auto few, uint64_t nc) {
+        const uint64_t steps = n * (head_dim / nc) / 256;  // per head
+        return 2ull * p.heads * (steps / 8 + 1) >= 2ull * (uint64_t)sm_count() ? launch(many, nc, 8) : launch(few, nc, 2);
+    };
+    // 32 output bytes a thread, else 16 (odd multiples, other alignments).
+    auto fits = [&](uint64_t nc) {
+        return head_dim % nc == 0 && head_dim / nc <= 256 && aligned_to(k, nc * sizeof(T)) &&
+               aligned_to(v, nc * sizeof(T)) && aligned_to(kc, nc) && aligned_to(vc, nc);
+    };
+    const bool done = (fits(2 * V) && vec(kv_read_q8_vec_kernel<T, 2 * V, 8>, kv_read_q8_vec_kernel<T, 2 * V, 2>, 2 * V)) ||
+                      (fits(V) && vec(kv_read_q8_vec_kernel<T, V, 8>, kv_read_q8_vec_kernel<T, V, 2>, V));
+    if (!done) {
+        const uint64_t half = (uint64_t)p.heads * n * head_dim, want = (2 * half + 255) / 256;
+        launch_k(kv_read_q8_scalar_kernel<T>, (unsigned)(want < cap ? want : cap), 256, 0, st, kc, vc, ks, vs, k, v, p, half);
     }
     return check_launch(name);
 }

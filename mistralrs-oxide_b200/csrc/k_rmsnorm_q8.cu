@@ -13,16 +13,20 @@
 // a stored y would take a second one behind the first.
 //
 // bf16: p is exact in f32 (two 8-bit significands).  f32: p in f32 decides
-// almost every code; max|p| is found in f64 (the products of two floats are
-// exact there), and a code next to a half-integer is decided from the f64
+// almost every code; the products of two floats are exact in f64, max|p| there
+// is the largest of the elements whose f32 product is the f32 maximum (rounding
+// is monotonic), and a code next to a half-integer is decided from the f64
 // product (oxide_q8.cuh).
 //
 // Layout.  A warp (rows of at most 128 vectors of 16 bytes) or a CTA owns a
 // row and keeps it packed in registers, four vectors a thread, so each row
-// crosses HBM once; w comes from L1 both times it is needed.  Bound by HBM
-// bytes: x, r and h in their type, one byte out.  Odd or unaligned rows and
-// rows over 4096 vectors take a two-pass kernel whose second read is served
-// by L1 / L2.
+// crosses HBM once.  A thread meets the same columns in every row: its part of
+// w stays in registers too, and CTAs take rows in turn (reading w twice a row
+// through L1 instead left L1 the bound: 118 us at [16384, 4096] bf16 against
+// 72 us of bytes).  Bound by HBM bytes: x, r and h in their type, one byte out.
+// Rows that do not divide into aligned vectors are held element by element in
+// the same way (up to 16 a thread); longer ones are read twice, the second
+// time through L1 / L2.
 #include "oxide_q8.cuh"
 
 namespace oxide {
@@ -33,93 +37,120 @@ struct NormQ8Args {
     float eps;
 };
 
+// The larger of two magnitudes, NaN if one is.
+__device__ __forceinline__ float norm_larger(float a, float b) {
+    asm("max.NaN.f32 %0, %0, %1;" : "+f"(a) : "f"(b));
+    return a;
+}
+// |p| in f64 as an ordered number that carries NaN and infinities.
+__device__ __forceinline__ unsigned long long norm_top_bits(float h, float w) {
+    return (unsigned long long)__double_as_longlong((double)h * (double)w) & 0x7fffffffffffffffull;
+}
+// The f32 products neither overflowed nor lost bits below the normal range.
+__device__ __forceinline__ bool norm_sure(float top) { return top >= 0x1p-90f && top <= 0x1p90f; }
+
+// Where a CTA's threads meet: two sets, alternating from row to row (`turn`), so
+// that a row's writes never meet the reads of the row before it.
+struct NormShared {
+    float2 red[2][32];
+    unsigned long long top[2];
+};
+__device__ __forceinline__ NormShared& norm_shared() {
+    __shared__ NormShared s;
+    return s;
+}
+
 // Sum of squares and the largest |p| over a row's threads: a warp, or the
-// whole CTA (then through shared memory; contains __syncthreads()).
-template <bool WARP, typename M>
-__device__ __forceinline__ void norm_q8_reduce(float& ss, M& top) {
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-        ss = fadd(ss, __shfl_xor_sync(0xffffffffu, ss, o));
-        const M t = __shfl_xor_sync(0xffffffffu, top, o);
-        top = t > top ? t : top;
-    }
-    if (WARP) return;
-    __shared__ float rs[32];
-    __shared__ M rt[32];
-    const int warp = threadIdx.x >> 5, nw = blockDim.x >> 5;
-    if ((threadIdx.x & 31) == 0) {
-        rs[warp] = ss;
-        rt[warp] = top;
-    }
-    __syncthreads();
-    ss = rs[0];
-    top = rt[0];
-    for (int i = 1; i < nw; ++i) {
-        ss = fadd(ss, rs[i]);
-        top = rt[i] > top ? rt[i] : top;
-    }
-    __syncthreads();  // the arrays are written again for the next row
-}
+// whole CTA (one barrier).
 template <bool WARP>
-__device__ __forceinline__ double norm_q8_sum(double v) {
-    v = warp_sum_d(v);
-    if (WARP) return v;
-    __shared__ double rd[32];
+__device__ __forceinline__ void norm_q8_reduce(float& ss, float& top, int turn) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) ss = fadd(ss, __shfl_xor_sync(0xffffffffu, ss, o));
+    top = __uint_as_float(q8_warp_max(__float_as_uint(top)));  // magnitudes: ordered as their bits, NaN last
+    if (WARP) return;
+    NormShared& sh = norm_shared();
     const int warp = threadIdx.x >> 5, nw = blockDim.x >> 5;
-    if ((threadIdx.x & 31) == 0) rd[warp] = v;
+    if ((threadIdx.x & 31) == 0) sh.red[turn][warp] = make_float2(ss, top);
+    if (threadIdx.x == 0) sh.top[turn] = 0;  // for norm_q8_refine
     __syncthreads();
-    v = rd[0];
-    for (int i = 1; i < nw; ++i) v += rd[i];
+    float2 v = sh.red[turn][0];
+    ss = v.x;
+    top = v.y;
+    for (int i = 1; i < nw; ++i) {
+        v = sh.red[turn][i];
+        ss = fadd(ss, v.x);
+        top = norm_larger(top, v.y);
+    }
+}
+// Rare: a f64 sum and maximum over the row's threads (two barriers).
+template <bool WARP>
+__device__ __noinline__ double2 norm_q8_again(double ss, unsigned long long top) {
+    ss = warp_sum_d(ss);
+    top = warp_max_u64(top);
+    if (!WARP) {
+        __shared__ double rs[32];
+        __shared__ unsigned long long rt[32];
+        const int warp = threadIdx.x >> 5, nw = blockDim.x >> 5;
+        if ((threadIdx.x & 31) == 0) {
+            rs[warp] = ss;
+            rt[warp] = top;
+        }
+        __syncthreads();
+        ss = rs[0];
+        top = rt[0];
+        for (int i = 1; i < nw; ++i) {
+            ss += rs[i];
+            top = rt[i] > top ? rt[i] : top;
+        }
+        __syncthreads();
+    }
+    return make_double2(ss, __longlong_as_double((long long)top));
+}
+// f32 rows: max|p| in f64 from the elements whose f32 product is the largest
+// (one barrier).
+template <bool WARP, typename VISIT>
+__device__ __forceinline__ double norm_q8_refine(float top, int turn, VISIT visit) {
+    unsigned long long t = 0;
+    visit([&](float h, float w) {
+        if (fabsf(fmul(h, w)) == top) {
+            const unsigned long long b = norm_top_bits(h, w);
+            t = b > t ? b : t;
+        }
+    });
+    if (WARP) return __longlong_as_double((long long)warp_max_u64(t));
+    NormShared& sh = norm_shared();
+    if (t) atomicMax(&sh.top[turn], t);
     __syncthreads();
-    return v;
+    return __longlong_as_double((long long)sh.top[turn]);
 }
 
-// |p| of one product as an ordered number that carries NaN and infinities:
-// bf16 products in f32 (exact), f32 products in f64 (exact).
-template <typename T>
-struct NormTop;
-template <>
-struct NormTop<bf16_t> {
-    typedef uint32_t M;
-    __device__ __forceinline__ static M of(float h, float w) { return q8_abs_bits(fmul(h, w)); }
-    __device__ __forceinline__ static double value(M m) { return (double)__uint_as_float(m); }
-    // the f32 products neither overflowed nor lost bits below the normal range
-    __device__ __forceinline__ static bool sure(M m) { return m >= 0x0d800000u && m < 0x72000000u; }
-};
-template <>
-struct NormTop<float> {
-    typedef unsigned long long M;
-    __device__ __forceinline__ static M of(float h, float w) {
-        return (M)__double_as_longlong((double)h * (double)w) & 0x7fffffffffffffffull;
-    }
-    __device__ __forceinline__ static double value(M m) { return __longlong_as_double((long long)m); }
-    __device__ __forceinline__ static bool sure(M m) {
-        const double v = value(m);
-        return v >= 0x1p-100 && v <= 0x1p100;
-    }
-};
-
-// What a row's codes are decided by, and its scale.  `again(what)` recomputes
-// a row statistic in f64 (every thread of the row calls it together): the f32
-// sum of squares has left its range (values near 1e19, or all below 1e-18),
-// or the bf16 products have.
+// What a row's codes are decided by, and its scale.  visit(f) calls f(h, w) for
+// each of the thread's elements, all threads of the row together.  Where the
+// f32 sum of squares has left its range (values near 1e19, or all below 1e-18)
+// or the f32 products have, both are taken in f64.
 struct NormRow {
     double top;   // max|p|
     float scale;
 };
-template <typename T, typename SS, typename TT>
-__device__ __forceinline__ NormRow norm_q8_row(float ss, typename NormTop<T>::M m, const NormQ8Args& p, SS again_ss,
-                                               TT again_top) {
+template <typename T, bool WARP, typename VISIT>
+__device__ __forceinline__ NormRow norm_q8_row(float ss, float top, int turn, const NormQ8Args& p, VISIT visit) {
     NormRow r;
-    if (NormTop<T>::sure(m) && ss >= 0x1p-80f && ss <= 0x1p100f) {
-        r.top = NormTop<T>::value(m);
+    if (norm_sure(top) && ss >= 0x1p-80f && ss <= 0x1p100f) {
+        r.top = sizeof(T) == 4 ? norm_q8_refine<WARP>(top, turn, visit) : (double)top;
         const float rms = fsqrt(fadd(fdiv(ss, (float)p.cols), p.eps));
-        r.scale = fdiv((float)r.top, fmul(127.0f, rms));
+        r.scale = fdiv(top, fmul(127.0f, rms));
         return r;
     }
-    const double s = again_ss();
-    r.top = again_top();
-    const double rms = sqrt(s / (double)p.cols + (double)p.eps);
+    double d = 0.0;
+    unsigned long long t = 0;
+    visit([&](float h, float w) {
+        d = __fma_rn((double)h, (double)h, d);
+        const unsigned long long b = norm_top_bits(h, w);
+        t = b > t ? b : t;
+    });
+    const double2 again = norm_q8_again<WARP>(d, t);
+    r.top = again.y;
+    const double rms = sqrt(again.x / (double)p.cols + (double)p.eps);
     r.scale = (float)(r.top / (127.0 * rms));
     if (!(r.top <= 1.7976931348623157e308)) {  // a NaN or an infinity in the row (or in w): the whole row is NaN
         r.scale = q8_nan();
@@ -128,41 +159,65 @@ __device__ __forceinline__ NormRow norm_q8_row(float ss, typename NormTop<T>::M 
     return r;
 }
 
-// Codes of N products h w, in f32 where that is certain, else in f64.
-template <int N>
-__device__ __forceinline__ void norm_q8_codes(const Q8Coder& c, const float (&h)[N], const float (&w)[N],
-                                              uint32_t (&out)[N / 4]) {
-    float near = 0.0f;
-#pragma unroll
-    for (int e = 0; e < N; e += 4) {
-        const float2 a = c.fast2(fmul2(f2(h[e], h[e + 1]), f2(w[e], w[e + 1])), near);
-        const float2 b = c.fast2(fmul2(f2(h[e + 2], h[e + 3]), f2(w[e + 2], w[e + 3])), near);
-        out[e / 4] = q8_pack4(__float_as_uint(a.x), __float_as_uint(a.y), __float_as_uint(b.x), __float_as_uint(b.y));
+// Codes nearest(127 p / top).
+template <typename T>
+struct NormCoder {
+    double top;
+    float ftop, inv;
+    bool slow;
+    Q8Bracket br;
+    __device__ __forceinline__ explicit NormCoder(double t)
+        : top(t),
+          ftop((float)t),
+          inv(norm_sure(ftop) ? fdiv(127.0f, ftop) : 0.0f),
+          slow(!norm_sure(ftop)),
+          br(inv) {}
+    __device__ __forceinline__ int exact(float h, float w) const {
+        if (sizeof(T) == 4 || slow) return q8_exact((double)h * (double)w, 127.0, top);
+        const float p = fmul(h, w);  // 16 bits; 254 |p| and (2 n + 1) top are exact
+        return q8_beside(p, 254.0f * fabsf(p), inv, ftop);
     }
-    if (c.slow || near > Q8_NEAR) {
-#pragma unroll 1
-        for (int e = 0; e < N; e += 4) {
-            uint32_t q[4];
+};
+// The codes of a packed vector by the definition.
+template <typename T>
+__device__ __noinline__ uint2 norm_decide(uint4 h, uint4 w, double top) {
+    constexpr int V = Vec<T>::N;
+    const NormCoder<T> c(top);
+    float hv[V], wv[V];
+    uint32_t q[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+    Vec<T>::unpack(h, hv);
+    Vec<T>::unpack(w, wv);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) q[i] = (uint32_t)c.exact((double)h[e + i] * (double)w[e + i]);
-            out[e / 4] = q8_pack4(q[0], q[1], q[2], q[3]);
-        }
-    }
+    for (int e = 0; e < V; ++e) q[e] = (uint32_t)c.exact(hv[e], wv[e]);
+    return make_uint2(q8_pack4(q[0], q[1], q[2], q[3]), q8_pack4(q[4], q[5], q[6], q[7]));
 }
 
 constexpr int NQ_VPT = 4;  // 16-byte vectors a thread holds
 
-// WARP: eight rows per 256-thread CTA; else one row per CTA.
-template <typename T, bool ADD, bool WARP>
-__global__ void __launch_bounds__(WARP ? 256 : 1024)
+// WARP: eight rows per 256-thread CTA; else one row per CTA of up to MAXT threads.
+// The register budget of 85 (three CTAs of 256) holds x, r and w of a thread.
+template <typename T, bool ADD, bool WARP, int MAXT>
+__global__ void __launch_bounds__(MAXT, MAXT == 256 ? 3 : 1)
     rmsnorm_q8_vec_kernel(const T* x, const T* r, const T* w, T* h, int8_t* y, float* scale, NormQ8Args p) {
     pdl_begin();
     constexpr int V = Vec<T>::N;
-    typedef NormTop<T> Top;
+    constexpr bool KEEP = MAXT == 256;  // w in registers
     const uint32_t t = WARP ? threadIdx.x & 31 : threadIdx.x, tpr = WARP ? 32 : blockDim.x;
     const uint32_t nvec = p.cols / V;
     const uint64_t per = WARP ? 8 : 1;
-    for (uint64_t row = blockIdx.x * per + (WARP ? threadIdx.x >> 5 : 0); row < p.rows; row += gridDim.x * per) {
+    uint4 wraw[KEEP ? NQ_VPT : 1] = {};
+    auto weight = [&](int k) -> uint4 {
+        if (KEEP) return wraw[KEEP ? k : 0];
+        return ld_keep(w + (uint64_t)(t + k * tpr) * V);
+    };
+    if (KEEP) {
+#pragma unroll
+        for (int k = 0; k < NQ_VPT; ++k)
+            if (t + k * tpr < nvec) wraw[KEEP ? k : 0] = ld_keep(w + (uint64_t)(t + k * tpr) * V);
+    }
+    int turn = 0;
+    for (uint64_t row = blockIdx.x * per + (WARP ? threadIdx.x >> 5 : 0); row < p.rows;
+         row += gridDim.x * per, turn ^= 1) {
         const uint64_t off = row * p.cols;
         uint4 raw[NQ_VPT], rawr[ADD ? NQ_VPT : 1];
 #pragma unroll
@@ -174,78 +229,67 @@ __global__ void __launch_bounds__(WARP ? 256 : 1024)
             }
         }
         float2 acc = f2(0.0f, 0.0f);
-        typename Top::M top = 0;
+        float top = 0.0f;
 #pragma unroll
         for (int k = 0; k < NQ_VPT; ++k) {
             const uint32_t j = t + k * tpr;
             if (j < nvec) {
                 float v[V], wv[V];
                 Vec<T>::unpack(raw[k], v);
-                Vec<T>::unpack(ld_keep(w + (uint64_t)j * V), wv);
                 if (ADD) {
-                    float rv[V];
+                    float rv[V], sv[V];
                     Vec<T>::unpack(rawr[ADD ? k : 0], rv);
 #pragma unroll
-                    for (int e = 0; e < V; ++e) v[e] = Vec<T>::rnd(fadd(v[e], rv[e]));
-                    raw[k] = Vec<T>::pack(v);  // exact: v already holds T values
+                    for (int e = 0; e < V; e += 2) {
+                        const float2 u = fadd2(f2(v[e], v[e + 1]), f2(rv[e], rv[e + 1]));
+                        sv[e] = u.x;
+                        sv[e + 1] = u.y;
+                    }
+                    raw[k] = Vec<T>::pack(sv);  // h as stored
+                    Vec<T>::unpack(raw[k], v);
                     st_stream(h + off + (uint64_t)j * V, raw[k]);
                 }
+                Vec<T>::unpack(weight(k), wv);
 #pragma unroll
                 for (int e = 0; e < V; e += 2) {
                     const float2 u = f2(v[e], v[e + 1]);
                     acc = __ffma2_rn(u, u, acc);
-                    const typename Top::M a = Top::of(v[e], wv[e]), b = Top::of(v[e + 1], wv[e + 1]);
-                    const typename Top::M ab = a > b ? a : b;
-                    top = ab > top ? ab : top;
+                    const float2 pr = fmul2(u, f2(wv[e], wv[e + 1]));
+                    top = norm_larger(top, fabsf(pr.x));
+                    top = norm_larger(top, fabsf(pr.y));
                 }
             }
         }
         float ss = fadd(acc.x, acc.y);
-        norm_q8_reduce<WARP>(ss, top);
-        auto again_ss = [&]() {
-            double d = 0.0;
+        norm_q8_reduce<WARP>(ss, top, turn);
+        const NormRow nr = norm_q8_row<T, WARP>(ss, top, turn, p, [&](auto f) {
 #pragma unroll
             for (int k = 0; k < NQ_VPT; ++k) {
                 if (t + k * tpr < nvec) {
-                    float v[V];
-                    Vec<T>::unpack(raw[k], v);
-#pragma unroll
-                    for (int e = 0; e < V; ++e) d = __fma_rn((double)v[e], (double)v[e], d);
-                }
-            }
-            return norm_q8_sum<WARP>(d);
-        };
-        auto again_top = [&]() {
-            unsigned long long m = 0;
-#pragma unroll
-            for (int k = 0; k < NQ_VPT; ++k) {
-                const uint32_t j = t + k * tpr;
-                if (j < nvec) {
                     float v[V], wv[V];
                     Vec<T>::unpack(raw[k], v);
-                    Vec<T>::unpack(ld_keep(w + (uint64_t)j * V), wv);
+                    Vec<T>::unpack(weight(k), wv);
 #pragma unroll
-                    for (int e = 0; e < V; ++e) {
-                        const unsigned long long a = NormTop<float>::of(v[e], wv[e]);
-                        m = a > m ? a : m;
-                    }
+                    for (int e = 0; e < V; ++e) f(v[e], wv[e]);
                 }
             }
-            float none = 0.0f;
-            norm_q8_reduce<WARP>(none, m);
-            return NormTop<float>::value(m);
-        };
-        const NormRow nr = norm_q8_row<T>(ss, top, p, again_ss, again_top);
-        const Q8Coder coder(127.0, nr.top);
+        });
+        const NormCoder<T> coder(nr.top);
 #pragma unroll
         for (int k = 0; k < NQ_VPT; ++k) {
             const uint32_t j = t + k * tpr;
             if (j < nvec) {
-                float v[V], wv[V];
+                float v[V], wv[V], pr[V];
                 uint32_t c[V / 4];
                 Vec<T>::unpack(raw[k], v);
-                Vec<T>::unpack(ld_keep(w + (uint64_t)j * V), wv);
-                norm_q8_codes<V>(coder, v, wv, c);
+                Vec<T>::unpack(weight(k), wv);
+#pragma unroll
+                for (int e = 0; e < V; e += 2) {
+                    const float2 u = fmul2(f2(v[e], v[e + 1]), f2(wv[e], wv[e + 1]));
+                    pr[e] = u.x;
+                    pr[e + 1] = u.y;
+                }
+                if (q8_codes<V>(coder, pr, c)) q8_take(c, norm_decide<T>(raw[k], weight(k), nr.top));
                 q8_store(y + off + (uint64_t)j * V, c);
             }
         }
@@ -253,14 +297,64 @@ __global__ void __launch_bounds__(WARP ? 256 : 1024)
     }
 }
 
-// Any row length and alignment: one CTA per row, the row read twice (pass 2
-// re-reads x, or the stored h, with coherent loads, so x or r may be h).
-template <typename T, bool ADD>
-__global__ void __launch_bounds__(256)
-    rmsnorm_q8_scalar_kernel(const T* x, const T* r, const T* w, T* h, int8_t* y, float* scale, NormQ8Args p) {
+// Rows that are no whole aligned vectors, element by element in registers:
+// thread t holds columns t + k blockDim.x, EPT of them, and its part of w.
+template <typename T, bool ADD, int EPT>
+__global__ void __launch_bounds__(1024)
+    rmsnorm_q8_odd_kernel(const T* x, const T* r, const T* w, T* h, int8_t* y, float* scale, NormQ8Args p) {
     pdl_begin();
-    typedef NormTop<T> Top;
-    for (uint64_t row = blockIdx.x; row < p.rows; row += gridDim.x) {
+    float wv[EPT];
+#pragma unroll
+    for (int k = 0; k < EPT; ++k) {
+        const uint32_t i = threadIdx.x + k * blockDim.x;
+        wv[k] = i < p.cols ? Vec<T>::load1(w + i) : 0.0f;
+    }
+    int turn = 0;
+    for (uint64_t row = blockIdx.x; row < p.rows; row += gridDim.x, turn ^= 1) {
+        const uint64_t off = row * p.cols;
+        float v[EPT], rv[ADD ? EPT : 1];
+#pragma unroll
+        for (int k = 0; k < EPT; ++k) {
+            const uint32_t i = threadIdx.x + k * blockDim.x;
+            v[k] = i < p.cols ? Vec<T>::load1(x + off + i) : 0.0f;
+            if (ADD) rv[ADD ? k : 0] = i < p.cols ? Vec<T>::load1(r + off + i) : 0.0f;
+        }
+        float ss = 0.0f, top = 0.0f;
+#pragma unroll
+        for (int k = 0; k < EPT; ++k) {
+            const uint32_t i = threadIdx.x + k * blockDim.x;
+            if (ADD) {
+                v[k] = Vec<T>::rnd(fadd(v[k], rv[ADD ? k : 0]));
+                if (i < p.cols) Vec<T>::store1(h + off + i, v[k]);
+            }
+            // places behind the row are zeros (0 + 0): they add nothing
+            ss = __fmaf_rn(v[k], v[k], ss);
+            top = norm_larger(top, fabsf(fmul(v[k], wv[k])));
+        }
+        norm_q8_reduce<false>(ss, top, turn);
+        const NormRow nr = norm_q8_row<T, false>(ss, top, turn, p, [&](auto f) {
+#pragma unroll
+            for (int k = 0; k < EPT; ++k) f(v[k], wv[k]);
+        });
+        const NormCoder<T> coder(nr.top);
+#pragma unroll
+        for (int k = 0; k < EPT; ++k) {
+            const uint32_t i = threadIdx.x + k * blockDim.x;
+            const float hv = v[k], wk = wv[k];
+            if (i < p.cols) y[off + i] = (int8_t)q8_code(coder, fmul(hv, wk), [&] { return coder.exact(hv, wk); });
+        }
+        if (threadIdx.x == 0) scale[row] = nr.scale;
+    }
+}
+
+// Any row length: one CTA per row, the row read twice (pass 2 re-reads x, or
+// the stored h, with coherent loads, so x or r may be h).
+template <typename T, bool ADD>
+__global__ void __launch_bounds__(1024)
+    rmsnorm_q8_long_kernel(const T* x, const T* r, const T* w, T* h, int8_t* y, float* scale, NormQ8Args p) {
+    pdl_begin();
+    int turn = 0;
+    for (uint64_t row = blockIdx.x; row < p.rows; row += gridDim.x, turn ^= 1) {
         const uint64_t off = row * p.cols;
         const T* src = (ADD ? h : x) + off;
         auto held = [&](uint32_t i) -> float {
@@ -268,7 +362,8 @@ __global__ void __launch_bounds__(256)
             return bf16_to_f32(*reinterpret_cast<const volatile uint16_t*>(src + i));
         };
         float ss = 0.0f;
-        typename Top::M top = 0;
+        float top = 0.0f;
+#pragma unroll 4
         for (uint32_t i = threadIdx.x; i < p.cols; i += blockDim.x) {
             float v = Vec<T>::load1(x + off + i);
             if (ADD) {
@@ -276,34 +371,17 @@ __global__ void __launch_bounds__(256)
                 Vec<T>::store1(h + off + i, v);
             }
             ss = __fmaf_rn(v, v, ss);
-            const typename Top::M a = Top::of(v, Vec<T>::load1(w + i));
-            top = a > top ? a : top;
+            top = norm_larger(top, fabsf(fmul(v, Vec<T>::load1(w + i))));
         }
-        norm_q8_reduce<false>(ss, top);
-        auto again_ss = [&]() {
-            double d = 0.0;
-            for (uint32_t i = threadIdx.x; i < p.cols; i += blockDim.x) d = __fma_rn((double)held(i), (double)held(i), d);
-            return norm_q8_sum<false>(d);
-        };
-        auto again_top = [&]() {
-            unsigned long long m = 0;
-            for (uint32_t i = threadIdx.x; i < p.cols; i += blockDim.x) {
-                const unsigned long long a = NormTop<float>::of(held(i), Vec<T>::load1(w + i));
-                m = a > m ? a : m;
-            }
-            float none = 0.0f;
-            norm_q8_reduce<false>(none, m);
-            return NormTop<float>::value(m);
-        };
-        const NormRow nr = norm_q8_row<T>(ss, top, p, again_ss, again_top);
-        const Q8Coder coder(127.0, nr.top);
+        norm_q8_reduce<false>(ss, top, turn);
+        const NormRow nr = norm_q8_row<T, false>(ss, top, turn, p, [&](auto f) {
+            for (uint32_t i = threadIdx.x; i < p.cols; i += blockDim.x) f(held(i), Vec<T>::load1(w + i));
+        });
+        const NormCoder<T> coder(nr.top);
+#pragma unroll 4
         for (uint32_t i = threadIdx.x; i < p.cols; i += blockDim.x) {
-            const float v = held(i), wv = Vec<T>::load1(w + i);
-            float near = 0.0f;
-            const float2 q = coder.fast2(fmul2(f2(v, v), f2(wv, wv)), near);
-            int c = (int)(int8_t)(__float_as_uint(q.x) & 0xffu);
-            if (coder.slow || near > Q8_NEAR) c = coder.exact((double)v * (double)wv);
-            y[off + i] = (int8_t)c;
+            const float hv = held(i), wv = Vec<T>::load1(w + i);
+            y[off + i] = (int8_t)q8_code(coder, fmul(hv, wv), [&] { return coder.exact(hv, wv); });
         }
         if (threadIdx.x == 0) scale[row] = nr.scale;
     }
@@ -324,17 +402,24 @@ static int norm_q8_entry(const char* name, const T* x, const T* r, const T* w, T
     const bool vec = cols % V == 0 && aligned16(x) && aligned16(w) && (!ADD || (aligned16(r) && aligned16(h))) &&
                      (reinterpret_cast<uintptr_t>(y) & (V - 1)) == 0;
     const uint64_t nvec = cols / V, cap = 1ull << 30;
+    // CTAs take rows in turn, one wave of them
+    auto go = [&](auto kern, int threads, uint64_t per) {
+        const uint64_t want = (rows + per - 1) / per;
+        const uint64_t wave = (uint64_t)resident_blocks(reinterpret_cast<const void*>(kern), threads, 0);
+        launch_k(kern, (unsigned)(want < wave ? want : wave), threads, 0, st, x, r, w, h, y, scale, p);
+    };
     if (vec && nvec <= 32ull * NQ_VPT) {
-        const uint64_t want = (rows + 7) / 8;
-        launch_k(rmsnorm_q8_vec_kernel<T, ADD, true>, (unsigned)(want < cap ? want : cap), 256, 0, st, x, r, w, h, y,
-                 scale, p);
+        go(rmsnorm_q8_vec_kernel<T, ADD, true, 256>, 256, 8);
     } else if (vec && nvec <= 1024ull * NQ_VPT) {
         const int threads = (int)(((nvec + NQ_VPT - 1) / NQ_VPT + 31) / 32 * 32);
-        launch_k(rmsnorm_q8_vec_kernel<T, ADD, false>, (unsigned)(rows < cap ? rows : cap), threads, 0, st, x, r, w, h,
-                 y, scale, p);
+        if (threads <= 256) go(rmsnorm_q8_vec_kernel<T, ADD, false, 256>, threads, 1);
+        else go(rmsnorm_q8_vec_kernel<T, ADD, false, 1024>, threads, 1);
+    } else if (cols <= 1024ull * 16) {
+        auto threads = [&](uint64_t ept) { return (int)(((cols + ept - 1) / ept + 31) / 32 * 32); };
+        if (cols <= 1024ull * 8) go(rmsnorm_q8_odd_kernel<T, ADD, 8>, threads(8), 1);
+        else go(rmsnorm_q8_odd_kernel<T, ADD, 16>, threads(16), 1);
     } else {
-        launch_k(rmsnorm_q8_scalar_kernel<T, ADD>, (unsigned)(rows < cap ? rows : cap), 256, 0, st, x, r, w, h, y,
-                 scale, p);
+        launch_k(rmsnorm_q8_long_kernel<T, ADD>, (unsigned)(rows < cap ? rows : cap), 1024, 0, st, x, r, w, h, y, scale, p);
     }
     return check_launch(name);
 }

@@ -1,15 +1,17 @@
 // oxide_q8.cuh -- symmetric int8 codes: a code c stands for c * s, s the f32
 // scale of its group (a row, or a block of tokens of one head), s = amax / 127.
 //
-// A code is the integer nearest to the real quotient x / s, ties to even,
-// decided exactly: the fast path multiplies by a rounded reciprocal and is
-// certain unless the product lies within its error of a half-integer; such a
-// vector (about 1 element in 10^4) is redone with the f64 quotient.  That is
-// enough: x and s have 24-bit significands, so near a half-integer
-// x - (n + 1/2) s is a multiple of ulp(s) / 4, and a quotient that is not a
-// half-integer is at least 2^-26 away from it, far above f64's 2^-47.
-// So codes do not depend on the order of any sum or on the rounding of a
-// reciprocal, and a 64-bit evaluation of the definition gives the same ones.
+// A code is the integer nearest to the real quotient x / s, ties to even, and
+// is decided exactly.  The fast path brackets the quotient: x times a
+// reciprocal made a little smaller and a little larger than 1 / s, each rounded
+// to an integer in one fused step.  Rounding is monotonic, so where both agree
+// the quotient's integer is theirs; where they differ (about 1 element in 10^5)
+// the quotient lies next to a half-integer and is compared with it: the sign
+// of x - (n + 1/2) s from one fused step is exact.  So codes do not depend on
+// the order of any sum or on the rounding of a reciprocal, and a 64-bit
+// evaluation of the definition gives the same ones (near a half-integer
+// x - (n + 1/2) s is a multiple of ulp(s) / 4, so another quotient is at least
+// 2^-26 away from it, far above f64's 2^-47).
 #pragma once
 
 #include "oxide_common.cuh"
@@ -18,10 +20,10 @@ namespace oxide {
 
 constexpr uint32_t Q8_INF = 0x7f800000u;  // bits of +inf: |x| bits above or at it are not finite
 constexpr float Q8_MAGIC = 12582912.0f;   // 1.5 * 2^23: adding it rounds to an integer in the low bits
-// |t - round(t)| above this may be on either side of the half-integer.  t is
-// off by at most 127.5 * 3 * 2^-24 = 2.3e-5 (three roundings: the reciprocal,
-// and -- the norm's f32 products -- x and its maximum).
-constexpr float Q8_NEAR = 0.49996f;
+// Relative half-width of the bracket around a quotient: 8 units of 2^-24, where
+// the reciprocal, its two copies and -- the norm's f32 products -- x and the
+// divisor are off by at most 5.
+constexpr float Q8_WIDTH = 0x1p-21f;
 
 __device__ __forceinline__ float q8_nan() { return __uint_as_float(0x7fffffffu); }
 
@@ -53,40 +55,54 @@ __device__ __forceinline__ uint32_t q8_vec_amax(uint4 v, uint32_t a, bf16_t) {
 __device__ __forceinline__ uint32_t q8_amax_join(uint32_t a, float) { return a; }
 __device__ __forceinline__ uint32_t q8_amax_join(uint32_t a, bf16_t) { return max(a << 16, a & 0xffff0000u); }
 
-// Codes of values x against a divisor: code = nearest(x * num / den).
-//   num = 1, den = s: a group's f32 scale;  num = 127, den = amax: a row's codes
-//   from its largest value, without the rounding of a scale.
+// The definition in f64 for every divisor: nearest(x num / den), 0 where the
+// divisor is zero or not finite.  The quotient passes 127 only against a
+// subnormal scale, whose own rounding is coarse: it is held to 127.
+static __device__ __noinline__ int q8_exact(double x, double num, double den) {
+    if (!(den > 0.0 && den <= 1.7976931348623157e308)) return 0;
+    const double q = rint(x * num / den);
+    return (int)(q > 127.0 ? 127.0 : (q < -127.0 ? -127.0 : q));
+}
+
+// The bracket of x times a factor.
+struct Q8Bracket {
+    float lo, hi;
+    __device__ __forceinline__ explicit Q8Bracket(float inv)
+        : lo(fmul(inv, 1.0f - Q8_WIDTH)), hi(fmul(inv, 1.0f + Q8_WIDTH)) {}
+    // Two codes, in the low bytes of the result's bits; `diff` stays zero
+    // while both ends of every bracket agree.
+    __device__ __forceinline__ uint2 two(float2 x, uint32_t& diff) const {
+        const float2 m = f2(Q8_MAGIC, Q8_MAGIC);
+        const float2 a = __ffma2_rn(x, f2(lo, lo), m), b = __ffma2_rn(x, f2(hi, hi), m);
+        diff |= __float_as_uint(a.x) ^ __float_as_uint(b.x);
+        diff |= __float_as_uint(a.y) ^ __float_as_uint(b.y);
+        return make_uint2(__float_as_uint(a.x), __float_as_uint(a.y));
+    }
+};
+
+// A code next to a half-integer: |x| against (n - 1/2) s and (n + 1/2) s for an
+// n within one of |x| / s.  a = 2 |x| u and s = d u, both exact, for any unit u.
+__device__ __forceinline__ int q8_beside(float x, float twice, float inv, float d) {
+    const float n = rintf(fmul(fabsf(x), inv));
+    const float up = __fmaf_rn(-(2.0f * n + 1.0f), d, twice), down = __fmaf_rn(-(2.0f * n - 1.0f), d, twice);
+    int c = (int)n;
+    if (up > 0.0f || (up == 0.0f && (c & 1))) ++c;
+    else if (down < 0.0f || (down == 0.0f && (c & 1))) --c;
+    return x < 0.0f ? -c : c;
+}
+
+// Codes under a group's f32 scale.
 struct Q8Coder {
-    double num, den;
-    float inv;    // RN(num / den)
-    bool slow;    // den zero, not finite, or so small or large that the fast path leaves the normal range
-    __device__ __forceinline__ Q8Coder(double n, double d) : num(n), den(d) {
-        const float df = (float)d;
-        slow = !(df >= 0x1p-100f && df <= 0x1p100f);
-        inv = slow ? 0.0f : (float)(n / d);
-    }
-    // A group's f32 scale as the divisor: one f32 reciprocal.
-    __device__ __forceinline__ explicit Q8Coder(float s) : num(1.0), den((double)s) {
-        slow = !(s >= 0x1p-100f && s <= 0x1p100f);
-        inv = slow ? 0.0f : __frcp_rn(s);
-    }
-    // The definition itself; 0 where the divisor is zero or not finite.  The
-    // quotient passes 127 only against a subnormal scale, whose own rounding
-    // is coarse: it is held to 127.
-    __device__ __forceinline__ int exact(double x) const {
-        if (!(den > 0.0 && den <= 1.7976931348623157e308)) return 0;
-        const double q = rint(x * num / den);
-        return (int)(q > 127.0 ? 127.0 : (q < -127.0 ? -127.0 : q));
-    }
-    // Two codes, in the low bytes of the results' bits; `near` collects the
-    // largest distance from an integer.
-    __device__ __forceinline__ float2 fast2(float2 x, float& near) const {
-        const float2 i2 = f2(inv, inv);
-        const float2 r = __ffma2_rn(x, i2, f2(Q8_MAGIC, Q8_MAGIC));
-        const float2 q = fadd2(r, f2(-Q8_MAGIC, -Q8_MAGIC));
-        const float2 d = __ffma2_rn(x, i2, make_float2(-q.x, -q.y));
-        near = fmaxf(near, fmaxf(fabsf(d.x), fabsf(d.y)));
-        return r;
+    float s, inv;
+    bool slow;  // zero, not finite, or so small or large that the fast path leaves the normal range
+    Q8Bracket br;
+    __device__ __forceinline__ explicit Q8Coder(float scale)
+        : s(scale),
+          inv(scale >= 0x1p-100f && scale <= 0x1p100f ? fdiv(1.0f, scale) : 0.0f),
+          slow(!(scale >= 0x1p-100f && scale <= 0x1p100f)),
+          br(inv) {}
+    __device__ __forceinline__ int exact(float x) const {
+        return slow ? q8_exact((double)x, 1.0, (double)s) : q8_beside(x, 2.0f * fabsf(x), inv, s);
     }
 };
 
@@ -95,21 +111,42 @@ __device__ __forceinline__ uint32_t q8_pack4(uint32_t a, uint32_t b, uint32_t c,
     return __byte_perm(__byte_perm(a, b, 0x0040), __byte_perm(c, d, 0x0040), 0x5410);
 }
 
-// N codes of N values (N = 4 or 8) as N / 4 words.
-template <int N>
-__device__ __forceinline__ void q8_codes(const Q8Coder& c, const float (&x)[N], uint32_t (&out)[N / 4]) {
-    float near = 0.0f;
+// N codes of N values (N = 4 or 8) as N / 4 words; true if some of them have to
+// be decided by the definition (the caller does that from its packed vector, in
+// a call of its own: kept inline, the rare path's registers halved the CTAs).
+template <int N, typename C>
+__device__ __forceinline__ bool q8_codes(const C& c, const float (&x)[N], uint32_t (&out)[N / 4]) {
+    uint32_t diff = 0;
 #pragma unroll
     for (int e = 0; e < N; e += 4) {
-        const float2 a = c.fast2(f2(x[e], x[e + 1]), near), b = c.fast2(f2(x[e + 2], x[e + 3]), near);
-        out[e / 4] = q8_pack4(__float_as_uint(a.x), __float_as_uint(a.y), __float_as_uint(b.x), __float_as_uint(b.y));
+        const uint2 a = c.br.two(f2(x[e], x[e + 1]), diff), b = c.br.two(f2(x[e + 2], x[e + 3]), diff);
+        out[e / 4] = q8_pack4(a.x, a.y, b.x, b.y);
     }
-    if (c.slow || near > Q8_NEAR) {
-#pragma unroll 1
-        for (int e = 0; e < N; e += 4)
-            out[e / 4] = q8_pack4((uint32_t)c.exact(x[e]), (uint32_t)c.exact(x[e + 1]), (uint32_t)c.exact(x[e + 2]),
-                                  (uint32_t)c.exact(x[e + 3]));
-    }
+    return c.slow || diff != 0;
+}
+// The codes of a packed vector by the definition.
+template <typename T>
+__device__ __noinline__ uint2 q8_decide(uint4 raw, float scale) {
+    constexpr int V = Vec<T>::N;
+    const Q8Coder c(scale);
+    float x[V];
+    uint32_t q[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+    Vec<T>::unpack(raw, x);
+#pragma unroll
+    for (int e = 0; e < V; ++e) q[e] = (uint32_t)c.exact(x[e]);
+    return make_uint2(q8_pack4(q[0], q[1], q[2], q[3]), q8_pack4(q[4], q[5], q[6], q[7]));
+}
+__device__ __forceinline__ void q8_take(uint32_t (&c)[1], uint2 v) { c[0] = v.x; }
+__device__ __forceinline__ void q8_take(uint32_t (&c)[2], uint2 v) {
+    c[0] = v.x;
+    c[1] = v.y;
+}
+// One code.
+template <typename C, typename X>
+__device__ __forceinline__ int q8_code(const C& c, float x, X exact) {
+    uint32_t diff = 0;
+    const int q = (int)(int8_t)(c.br.two(f2(x, x), diff).x & 0xffu);
+    return c.slow || diff != 0 ? exact() : q;
 }
 
 // Four codes as floats: the biased byte becomes the low significand bits of
@@ -127,6 +164,36 @@ __device__ __forceinline__ void q8_store(int8_t* p, const uint32_t (&c)[1]) {
 }
 __device__ __forceinline__ void q8_store(int8_t* p, const uint32_t (&c)[2]) {
     asm volatile("st.global.cs.v2.u32 [%0], {%1, %2};" ::"l"(p), "r"(c[0]), "r"(c[1]) : "memory");
+}
+
+// Loads of 4, 8 or 16 codes, used once.
+__device__ __forceinline__ void q8_load(const int8_t* p, uint32_t (&c)[1]) {
+    c[0] = __ldcs(reinterpret_cast<const unsigned int*>(p));
+}
+__device__ __forceinline__ void q8_load(const int8_t* p, uint32_t (&c)[2]) {
+    const uint2 v = __ldcs(reinterpret_cast<const uint2*>(p));
+    c[0] = v.x;
+    c[1] = v.y;
+}
+__device__ __forceinline__ void q8_load(const int8_t* p, uint32_t (&c)[4]) {
+    const uint4 v = __ldcs(reinterpret_cast<const uint4*>(p));
+    c[0] = v.x;
+    c[1] = v.y;
+    c[2] = v.z;
+    c[3] = v.w;
+}
+// Stores of 16 or 32 bytes of values.
+__device__ __forceinline__ void st_stream32(void* p, uint4 a, uint4 b) {
+    asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w),
+                 "r"(b.x), "r"(b.y), "r"(b.z), "r"(b.w)
+                 : "memory");
+}
+template <typename T, int N>
+__device__ __forceinline__ void q8_store_values(T* p, const float (&x)[N]) {
+    constexpr int V = Vec<T>::N;
+    static_assert(N == V || N == 2 * V, "one or two 16-byte vectors");
+    if constexpr (N == V) st_stream(p, Vec<T>::pack(x));
+    else st_stream32(p, Vec<T>::pack(x), Vec<T>::pack(x + V));
 }
 
 // Largest value over the warp (one instruction for unsigned numbers).
