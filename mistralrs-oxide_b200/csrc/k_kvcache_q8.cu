@@ -28,62 +28,65 @@
 namespace oxide {
 
 struct AppendQ8Args {
-    uint64_t max_seq, cur_len, new_len;
     const int32_t* cur_lens;   // per sequence; NULL: cur_len
     const int32_t* new_lens;   // per sequence; NULL: new_len
-    uint32_t heads, kv_heads;  // batch * kv_heads, kv_heads
-    uint32_t head_dim, nblk, shift, wide;  // block = 1 << shift; wide: blocks an append can touch
-    uint32_t items;            // 2 * heads * wide
+    uint32_t max_seq, cur_len, new_len;
+    uint32_t head_dim, nblk, shift;  // block = 1 << shift
+    uint32_t half;             // heads * wide: items of k; as many of v follow
+    uint32_t items;            // 2 * half
+    FastDiv wide, kv_heads;    // wide: blocks an append can touch
 };
 
 // One item: the block, the positions [lo, hi) it receives, where they come
-// from and go to.
+// from and go to (positions are below 2^31).
 struct AppendItem {
     bool is_v;
+    bool holds;               // tokens of this sequence before lo are in the block
     uint32_t bh, blk;
-    uint64_t lo, hi, start;  // new positions; the block's first position
-    uint64_t src;            // first new row in k / v, counted in rows
-    bool holds;              // tokens of this sequence before lo are in the block
+    uint32_t lo, hi, start;   // new positions; the block's first position
+    uint64_t src;             // first new row in k / v, counted in rows
 };
 __device__ __forceinline__ bool append_item(const AppendQ8Args& p, uint32_t i, AppendItem& it) {
-    const uint32_t half = p.heads * p.wide;
-    it.is_v = i >= half;
-    const uint32_t r = it.is_v ? i - half : i;
-    it.bh = r / p.wide;
-    const uint32_t j = r - it.bh * p.wide, b = it.bh / p.kv_heads;
-    uint64_t cur = p.cur_len, n = p.new_len;
-    if (p.cur_lens) {
-        const int32_t c = p.cur_lens[b];
-        if (c < 0 || (uint64_t)c > p.max_seq) return false;
-        cur = (uint64_t)c;
-    }
-    if (p.new_lens) {
-        const int32_t c = p.new_lens[b];
-        n = c <= 0 ? 0 : ((uint64_t)c < n ? (uint64_t)c : n);
+    it.is_v = i >= p.half;
+    const uint32_t r = it.is_v ? i - p.half : i;
+    it.bh = p.wide.div(r);
+    const uint32_t j = r - it.bh * p.wide.d;
+    uint32_t cur = p.cur_len, n = p.new_len;
+    if (p.cur_lens || p.new_lens) {
+        const uint32_t b = p.kv_heads.div(it.bh);
+        if (p.cur_lens) {
+            cur = (uint32_t)__ldg(p.cur_lens + b);
+            if (cur > p.max_seq) return false;  // negative ones too
+        }
+        if (p.new_lens) {
+            const int32_t c = __ldg(p.new_lens + b);
+            n = c <= 0 ? 0u : min((uint32_t)c, n);
+        }
     }
     if (n == 0 || n > p.max_seq - cur) return false;  // nothing to write, or it does not fit: the sequence is left as it is
-    const uint64_t blk = (cur >> p.shift) + j;
-    it.start = blk << p.shift;
-    const uint64_t end = cur + n, stop = it.start + (1ull << p.shift);
+    it.blk = (cur >> p.shift) + j;
+    it.start = it.blk << p.shift;  // an untouched block's may pass 2^31, not 2^32
+    const uint32_t end = cur + n;
     if (it.start >= end) return false;
-    it.blk = (uint32_t)blk;
-    it.lo = it.start > cur ? it.start : cur;
-    it.hi = stop < end ? stop : end;
+    it.lo = max(it.start, cur);
+    it.hi = min(it.start + (1u << p.shift), end);
     it.src = (uint64_t)it.bh * p.new_len + (it.lo - cur);
     it.holds = it.start < cur;
     return true;
 }
 
-// The block's scale after this append, and whether its codes are restated.
+// The block's scale after this append, whether it is the new tokens' own, and
+// whether the codes the block holds are restated.
 // Scales are compared as bits, which carries a NaN along.
-__device__ __forceinline__ float append_scale(const AppendItem& it, float had, uint32_t amax, bool& grown) {
+__device__ __forceinline__ float append_scale(const AppendItem& it, float had, uint32_t amax, bool& fresh, bool& grown) {
     const float need = q8_scale_of(amax);
+    fresh = true;
     grown = false;
     if (!it.holds) return need;
     const uint32_t a = q8_abs_bits(had), b = q8_abs_bits(need);
-    if (b <= a) return __uint_as_float(a);
-    grown = b < Q8_INF;
-    return need;
+    fresh = b > a;
+    grown = fresh && b < Q8_INF;
+    return fresh ? need : __uint_as_float(a);
 }
 
 // Restate the codes of positions [start, lo) from scale `had` to scale `s`.
@@ -91,11 +94,11 @@ __device__ __forceinline__ float append_scale(const AppendItem& it, float had, u
 template <int TPI>
 __device__ __forceinline__ void append_restate(int8_t* head, const AppendQ8Args& p, const AppendItem& it, float had,
                                                float s, uint8_t* lut, uint32_t t) {
-    for (uint32_t i = t; i < 128; i += TPI) lut[i] = (uint8_t)q8_exact((double)i, (double)had, (double)s);
+    for (uint32_t i = t; i < 128; i += TPI) lut[i] = (uint8_t)q8_restated((int)i, had, s);
     if (TPI == 32) __syncwarp();
     else __syncthreads();
-    int8_t* c = head + it.start * p.head_dim;
-    const uint64_t n = (it.lo - it.start) * p.head_dim;
+    int8_t* c = head + (uint64_t)it.start * p.head_dim;
+    const uint32_t n = (it.lo - it.start) * p.head_dim;
     auto restate = [&](int v) -> uint32_t {
         const int a = v < 0 ? (v < -127 ? 127 : -v) : v;
         const int q = lut[a];
@@ -104,13 +107,13 @@ __device__ __forceinline__ void append_restate(int8_t* head, const AppendQ8Args&
     if (p.head_dim % 4 == 0 && (reinterpret_cast<uintptr_t>(c) & 3) == 0) {
         uint32_t* w = reinterpret_cast<uint32_t*>(c);
 #pragma unroll 4
-        for (uint64_t i = t; i < n / 4; i += TPI) {
+        for (uint32_t i = t; i < n / 4; i += TPI) {
             const uint32_t v = w[i];
             w[i] = restate((int8_t)v) | restate((int8_t)(v >> 8)) << 8 | restate((int8_t)(v >> 16)) << 16 |
                    restate((int8_t)(v >> 24)) << 24;
         }
     } else {
-        for (uint64_t i = t; i < n; i += TPI) c[i] = (int8_t)restate(c[i]);
+        for (uint32_t i = t; i < n; i += TPI) c[i] = (int8_t)restate(c[i]);
     }
 }
 
@@ -131,7 +134,7 @@ __device__ __forceinline__ uint32_t append_max(uint32_t a) {
 
 // TPI threads an item (32: eight items per CTA), VPT vectors a thread.
 template <typename T, int TPI, int VPT>
-__global__ void __launch_bounds__(TPI == 32 ? 256 : TPI)
+__global__ void __launch_bounds__(TPI == 32 ? 256 : TPI, TPI == 256 ? 4 : 1)
     kv_append_q8_vec_kernel(int8_t* kc, int8_t* vc, float* ks, float* vs, const T* k, const T* v, AppendQ8Args p) {
     pdl_begin();
     constexpr int V = Vec<T>::N, IPC = TPI == 32 ? 8 : 1;
@@ -143,7 +146,7 @@ __global__ void __launch_bounds__(TPI == 32 ? 256 : TPI)
         const T* src = (it.is_v ? v : k) + it.src * p.head_dim;
         int8_t* head = (it.is_v ? vc : kc) + (uint64_t)it.bh * p.max_seq * p.head_dim;
         float* sp = (it.is_v ? vs : ks) + (uint64_t)it.bh * p.nblk + it.blk;
-        const uint32_t nvec = (uint32_t)((it.hi - it.lo) * p.head_dim / V);
+        const uint32_t nvec = (it.hi - it.lo) * p.head_dim / V;
         uint4 raw[VPT];
 #pragma unroll
         for (int u = 0; u < VPT; ++u)
@@ -154,20 +157,30 @@ __global__ void __launch_bounds__(TPI == 32 ? 256 : TPI)
         for (int u = 0; u < VPT; ++u)
             if (t + u * TPI < nvec) a = q8_vec_amax(raw[u], a, T());
         a = append_max<TPI>(q8_amax_join(a, T()));  // also: every thread has read the old scale
-        bool grown;
-        const float s = append_scale(it, had, a, grown);
+        bool fresh, grown;
+        const float s = append_scale(it, had, a, fresh, grown);
         if (t == 0) *sp = s;
-        const Q8Coder coder(s);
-        int8_t* dst = head + it.lo * p.head_dim;
+        const Q8Coder<T> coder(s, fresh ? __uint_as_float(a) : -1.0f);
+        int8_t* dst = head + (uint64_t)it.lo * p.head_dim;
+        uint32_t open = 0;  // vectors with codes that the definition has to decide
 #pragma unroll
         for (int u = 0; u < VPT; ++u)
             if (t + u * TPI < nvec) {
                 float x[V];
                 uint32_t c[V / 4];
                 Vec<T>::unpack(raw[u], x);
-                if (q8_codes<V>(coder, x, c)) q8_take(c, q8_decide<T>(raw[u], s));
-                q8_store(dst + (uint64_t)(t + u * TPI) * V, c);
+                open |= (q8_codes<V>(coder, x, c) ? 1u : 0u) << u;
+                q8_store(dst + (t + u * TPI) * V, c);
             }
+        if (open) {  // once more, behind the other stores: a branch at every vector kept them from overlapping
+#pragma unroll
+            for (int u = 0; u < VPT; ++u)
+                if (open >> u & 1u) {
+                    uint32_t c[V / 4];
+                    q8_take(c, q8_decide<T>(raw[u], s));
+                    q8_store(dst + (t + u * TPI) * V, c);
+                }
+        }
         if (grown) {
             append_restate<TPI>(head, p, it, had, s, luts[g], t);
             if (TPI == 32) __syncwarp();  // the table is written again for the next item
@@ -190,19 +203,19 @@ __global__ void __launch_bounds__(256)
         const T* src = (it.is_v ? v : k) + it.src * p.head_dim;
         int8_t* head = (it.is_v ? vc : kc) + (uint64_t)it.bh * p.max_seq * p.head_dim;
         float* sp = (it.is_v ? vs : ks) + (uint64_t)it.bh * p.nblk + it.blk;
-        const uint32_t n = (uint32_t)((it.hi - it.lo) * p.head_dim);
+        const uint32_t n = (it.hi - it.lo) * p.head_dim;
         const float had = it.holds ? *reinterpret_cast<volatile float*>(sp) : 0.0f;
         uint32_t a = 0;
         for (uint32_t e = t; e < n; e += TPI) a = max(a, q8_abs_bits(Vec<T>::load1(src + e)));
         a = append_max<TPI>(a);
-        bool grown;
-        const float s = append_scale(it, had, a, grown);
+        bool fresh, grown;
+        const float s = append_scale(it, had, a, fresh, grown);
         if (t == 0) *sp = s;
-        const Q8Coder coder(s);
-        int8_t* dst = head + it.lo * p.head_dim;
+        const Q8Coder<T> coder(s, fresh ? __uint_as_float(a) : -1.0f);
+        int8_t* dst = head + (uint64_t)it.lo * p.head_dim;
         for (uint32_t e = t; e < n; e += TPI) {
             const float x = Vec<T>::load1(src + e);
-            dst[e] = (int8_t)q8_code(coder, x, [&] { return coder.exact(x); });
+            dst[e] = (int8_t)q8_code(coder, x, [&] { return q8_definition(x, s); });
         }
         if (grown) {
             append_restate<TPI>(head, p, it, had, s, luts[g], t);
@@ -330,21 +343,23 @@ static int append_q8_entry(const char* name, int8_t* kc, int8_t* vc, float* ks, 
     OXIDE_REQUIRE(kc != vc && ks != vs, name, "the key and value caches must not alias");
     constexpr uint64_t V = Vec<T>::N;
     AppendQ8Args p{};
-    p.max_seq = max_seq;
-    p.cur_len = cur_len;
-    p.new_len = new_len;
+    p.max_seq = (uint32_t)max_seq;
+    p.cur_len = cur_lens ? 0u : (uint32_t)cur_len;
+    p.new_len = (uint32_t)new_len;
     p.cur_lens = cur_lens;
     p.new_lens = new_lens;
-    p.heads = (uint32_t)(batch * kv_heads);
-    p.kv_heads = (uint32_t)kv_heads;
     p.head_dim = (uint32_t)head_dim;
     p.shift = (uint32_t)q8_block_shift(block);
     p.nblk = (uint32_t)((max_seq + block - 1) / block);
-    const uint64_t wide = (new_len + block - 2) / block + 1;  // a run of new_len positions meets at most so many blocks
-    p.wide = (uint32_t)(wide < p.nblk ? wide : p.nblk);
-    const uint64_t items = 2ull * p.heads * p.wide;
+    const uint64_t heads = batch * kv_heads;
+    uint64_t wide = (new_len + block - 2) / block + 1;  // a run of new_len positions meets at most so many blocks
+    if (wide > p.nblk) wide = p.nblk;
+    const uint64_t items = 2 * heads * wide;
     OXIDE_REQUIRE(items < (1ull << 32), name, "too many blocks for one call (2^32): append fewer tokens at a time");
+    p.half = (uint32_t)(heads * wide);
     p.items = (uint32_t)items;
+    p.wide = FastDiv((uint32_t)wide);
+    p.kv_heads = FastDiv((uint32_t)kv_heads);
     const uint64_t run = (block < new_len ? block : new_len) * head_dim;  // elements of the longest item
     const uint64_t cap = 1ull << 30, warps = (items + 7) / 8 < cap ? (items + 7) / 8 : cap,
                    ctas = items < cap ? items : cap;

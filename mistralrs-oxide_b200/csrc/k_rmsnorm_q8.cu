@@ -111,12 +111,14 @@ __device__ __noinline__ double2 norm_q8_again(double ss, unsigned long long top)
 template <bool WARP, typename VISIT>
 __device__ __forceinline__ double norm_q8_refine(float top, int turn, VISIT visit) {
     unsigned long long t = 0;
-    visit([&](float h, float w) {
-        if (fabsf(fmul(h, w)) == top) {
+    bool here = false;  // one branch for the few threads that hold the maximum
+    visit([&](float h, float w) { here |= fabsf(fmul(h, w)) == top; });
+    if (here) {
+        visit([&](float h, float w) {
             const unsigned long long b = norm_top_bits(h, w);
             t = b > t ? b : t;
-        }
-    });
+        });
+    }
     if (WARP) return __longlong_as_double((long long)warp_max_u64(t));
     NormShared& sh = norm_shared();
     if (t) atomicMax(&sh.top[turn], t);
@@ -275,6 +277,7 @@ __global__ void __launch_bounds__(MAXT, MAXT == 256 ? 3 : 1)
             }
         });
         const NormCoder<T> coder(nr.top);
+        uint32_t open = 0;  // vectors with codes that the definition has to decide
 #pragma unroll
         for (int k = 0; k < NQ_VPT; ++k) {
             const uint32_t j = t + k * tpr;
@@ -289,9 +292,18 @@ __global__ void __launch_bounds__(MAXT, MAXT == 256 ? 3 : 1)
                     pr[e] = u.x;
                     pr[e + 1] = u.y;
                 }
-                if (q8_codes<V>(coder, pr, c)) q8_take(c, norm_decide<T>(raw[k], weight(k), nr.top));
+                open |= (q8_codes<V>(coder, pr, c) ? 1u : 0u) << k;
                 q8_store(y + off + (uint64_t)j * V, c);
             }
+        }
+        if (open) {  // once more, behind the other stores
+#pragma unroll
+            for (int k = 0; k < NQ_VPT; ++k)
+                if (open >> k & 1u) {
+                    uint32_t c[V / 4];
+                    q8_take(c, norm_decide<T>(raw[k], weight(k), nr.top));
+                    q8_store(y + off + (uint64_t)(t + k * tpr) * V, c);
+                }
         }
         if (t == 0) scale[row] = nr.scale;
     }
@@ -299,8 +311,8 @@ __global__ void __launch_bounds__(MAXT, MAXT == 256 ? 3 : 1)
 
 // Rows that are no whole aligned vectors, element by element in registers:
 // thread t holds columns t + k blockDim.x, EPT of them, and its part of w.
-template <typename T, bool ADD, int EPT>
-__global__ void __launch_bounds__(1024)
+template <typename T, bool ADD, int EPT, int MAXT>
+__global__ void __launch_bounds__(MAXT, MAXT == 320 ? 3 : 1)
     rmsnorm_q8_odd_kernel(const T* x, const T* r, const T* w, T* h, int8_t* y, float* scale, NormQ8Args p) {
     pdl_begin();
     float wv[EPT];
@@ -337,11 +349,21 @@ __global__ void __launch_bounds__(1024)
             for (int k = 0; k < EPT; ++k) f(v[k], wv[k]);
         });
         const NormCoder<T> coder(nr.top);
+        uint32_t c[EPT], diff = 0;
+#pragma unroll
+        for (int k = 0; k < EPT; k += 2) {
+            const uint2 q = coder.br.two(fmul2(f2(v[k], v[k + 1]), f2(wv[k], wv[k + 1])), diff);
+            c[k] = q.x;
+            c[k + 1] = q.y;
+        }
+        if (coder.slow || diff != 0) {
+#pragma unroll
+            for (int k = 0; k < EPT; ++k) c[k] = (uint32_t)coder.exact(v[k], wv[k]);
+        }
 #pragma unroll
         for (int k = 0; k < EPT; ++k) {
             const uint32_t i = threadIdx.x + k * blockDim.x;
-            const float hv = v[k], wk = wv[k];
-            if (i < p.cols) y[off + i] = (int8_t)q8_code(coder, fmul(hv, wk), [&] { return coder.exact(hv, wk); });
+            if (i < p.cols) y[off + i] = (int8_t)(c[k] & 0xffu);
         }
         if (threadIdx.x == 0) scale[row] = nr.scale;
     }
@@ -415,9 +437,9 @@ static int norm_q8_entry(const char* name, const T* x, const T* r, const T* w, T
         if (threads <= 256) go(rmsnorm_q8_vec_kernel<T, ADD, false, 256>, threads, 1);
         else go(rmsnorm_q8_vec_kernel<T, ADD, false, 1024>, threads, 1);
     } else if (cols <= 1024ull * 16) {
-        auto threads = [&](uint64_t ept) { return (int)(((cols + ept - 1) / ept + 31) / 32 * 32); };
-        if (cols <= 1024ull * 8) go(rmsnorm_q8_odd_kernel<T, ADD, 8>, threads(8), 1);
-        else go(rmsnorm_q8_odd_kernel<T, ADD, 16>, threads(16), 1);
+        const int threads = (int)(((cols + 15) / 16 + 31) / 32 * 32);
+        if (threads <= 320) go(rmsnorm_q8_odd_kernel<T, ADD, 16, 320>, threads, 1);
+        else go(rmsnorm_q8_odd_kernel<T, ADD, 16, 1024>, threads, 1);
     } else {
         launch_k(rmsnorm_q8_long_kernel<T, ADD>, (unsigned)(rows < cap ? rows : cap), 1024, 0, st, x, r, w, h, y, scale, p);
     }

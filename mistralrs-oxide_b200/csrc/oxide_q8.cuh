@@ -91,20 +91,63 @@ __device__ __forceinline__ int q8_beside(float x, float twice, float inv, float 
     return x < 0.0f ? -c : c;
 }
 
-// Codes under a group's f32 scale.
+// Codes of values of type T under a group's f32 scale.
+//
+// bf16 values under a bf16 maximum's scale meet half-integers all the time (half
+// the maximum is 63.5 steps), so they get a factor that needs no bracket.  Let a
+// be the bf16 value with s = RN(a / 127), X and A the 8-bit significands of x
+// and a.  127 x / a is a half-integer or at least a 254 X-th part of itself away
+// from one (its distance is a fraction over 2 A 2^k): more than 2^-16.  x / s is
+// (1 + d) times it, |d| <= 2^-24, d of the sign of a - 127 s.  So a factor
+// 127 / a made larger or smaller by 2^-20 in that direction puts every x on its
+// side: away from half-integers it changes nothing, on them it goes where d
+// does.  Where a = 127 s exactly, 127 / a is a power of two and the rounding
+// itself takes the half-integers to even.
+template <typename T>
 struct Q8Coder {
-    float s, inv;
     bool slow;  // zero, not finite, or so small or large that the fast path leaves the normal range
     Q8Bracket br;
-    __device__ __forceinline__ explicit Q8Coder(float scale)
-        : s(scale),
-          inv(scale >= 0x1p-100f && scale <= 0x1p100f ? fdiv(1.0f, scale) : 0.0f),
-          slow(!(scale >= 0x1p-100f && scale <= 0x1p100f)),
-          br(inv) {}
-    __device__ __forceinline__ int exact(float x) const {
-        return slow ? q8_exact((double)x, 1.0, (double)s) : q8_beside(x, 2.0f * fabsf(x), inv, s);
+    // amax: the largest |x| if the scale is RN(amax / 127), else negative.
+    __device__ __forceinline__ Q8Coder(float scale, float amax)
+        : slow(!(scale >= 0x1p-100f && scale <= 0x1p100f)), br(0.0f) {
+        if (slow) return;
+        if (sizeof(T) == 2) {
+            float a = amax;
+            if (amax < 0.0f) {  // an older scale: of some bf16 maximum, mostly
+                a = round_bf16(fmul(127.0f, scale));
+                if (fdiv(a, 127.0f) != scale) a = -1.0f;
+            }
+            if (a > 0.0f) {
+                const float r = __fmaf_rn(-127.0f, scale, a);  // its sign is exact
+                const float f = fdiv(127.0f, a);
+                br.lo = br.hi = r == 0.0f ? f : __fmaf_rn(f, r > 0.0f ? 0x1p-20f : -0x1p-20f, f);
+                return;
+            }
+        }
+        br = Q8Bracket(fdiv(1.0f, scale));
     }
 };
+// One code under a scale by the definition; 0 under a scale that is zero or not
+// finite.  Scales far from 1 are brought near it, with x, by a power of two
+// (exact for every x that reaches half a step).  A quotient passes 127 only
+// under a subnormal scale, whose own rounding is coarse: it is held to 127.
+__device__ __forceinline__ int q8_definition(float x, float scale) {
+    if (!(scale > 0.0f && scale < INFINITY)) return 0;
+    const float k = scale < 0x1p-60f ? 0x1p80f : (scale > 0x1p60f ? 0x1p-80f : 1.0f);
+    const float xs = fmul(x, k), s = fmul(scale, k);
+    const int c = q8_beside(xs, 2.0f * fabsf(xs), fdiv(1.0f, s), s);
+    return max(-127, min(127, c));
+}
+// The code nearest to i had / s (0 <= i <= 127, had <= s finite, s > 0): products
+// of a float and a small integer are exact in f64.
+__device__ __forceinline__ int q8_restated(int i, float had, float s) {
+    const double twice = 2.0 * i * (double)had;
+    int c = (int)rintf(fdiv(fmul((float)i, had), s));
+    const double up = (2 * c + 1) * (double)s, down = (2 * c - 1) * (double)s;
+    if (twice > up || (twice == up && (c & 1))) ++c;
+    else if (twice < down || (twice == down && (c & 1))) --c;
+    return c;
+}
 
 // The low bytes of four words, in order.
 __device__ __forceinline__ uint32_t q8_pack4(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
@@ -112,8 +155,7 @@ __device__ __forceinline__ uint32_t q8_pack4(uint32_t a, uint32_t b, uint32_t c,
 }
 
 // N codes of N values (N = 4 or 8) as N / 4 words; true if some of them have to
-// be decided by the definition (the caller does that from its packed vector, in
-// a call of its own: kept inline, the rare path's registers halved the CTAs).
+// be decided by the definition (the caller does that from its packed vector).
 template <int N, typename C>
 __device__ __forceinline__ bool q8_codes(const C& c, const float (&x)[N], uint32_t (&out)[N / 4]) {
     uint32_t diff = 0;
@@ -126,14 +168,13 @@ __device__ __forceinline__ bool q8_codes(const C& c, const float (&x)[N], uint32
 }
 // The codes of a packed vector by the definition.
 template <typename T>
-__device__ __noinline__ uint2 q8_decide(uint4 raw, float scale) {
+__device__ __forceinline__ uint2 q8_decide(uint4 raw, float scale) {
     constexpr int V = Vec<T>::N;
-    const Q8Coder c(scale);
     float x[V];
     uint32_t q[8] = {0, 0, 0, 0, 0, 0, 0, 0};
     Vec<T>::unpack(raw, x);
 #pragma unroll
-    for (int e = 0; e < V; ++e) q[e] = (uint32_t)c.exact(x[e]);
+    for (int e = 0; e < V; ++e) q[e] = (uint32_t)q8_definition(x[e], scale);
     return make_uint2(q8_pack4(q[0], q[1], q[2], q[3]), q8_pack4(q[4], q[5], q[6], q[7]));
 }
 __device__ __forceinline__ void q8_take(uint32_t (&c)[1], uint2 v) { c[0] = v.x; }
