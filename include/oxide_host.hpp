@@ -15,7 +15,8 @@
 //   oxide::KernelManager::launch_*       src/cuda_backend/kernels.rs:75-376
 //
 // plus the path's additions (silu_mul, add_rms_norm, scale_mask_softmax, rope
-// of q and k in one launch, argmax, sum / max / sum of squares, bf16 tensors).
+// of q and k in one launch, argmax, sum / max / sum of squares, bf16 tensors, the
+// int8 norms and the int8 KV cache).
 //
 // Semantics follow the Rust originals: every op borrows its inputs and returns
 // a newly allocated output tensor (Tensor::zeros) or an OxideError; shape
@@ -497,6 +498,76 @@ inline Result<std::pair<Tensor, Tensor>> add_rms_norm(const Tensor& x, const Ten
     return std::make_pair(std::move(h).value(), std::move(y).value());
 }
 
+// Rows of int8 codes with one f32 scale a row (scale: dims[:-1]); a code stands
+// for code * scale.  Codes are held apart from Tensor, whose ops know f32 and
+// bf16 only.
+struct Q8Rows {
+    Shape shape;
+    std::shared_ptr<DeviceBuffer> codes;
+    Tensor scale;
+    int8_t* data() const { return static_cast<int8_t*>(codes->ptr()); }
+    Result<std::vector<int8_t>> to_vec() const {
+        std::vector<int8_t> out(shape.elem_count());
+        if (!out.empty()) {
+            OXIDE_TRY(check_cuda(cudaMemcpyAsync(out.data(), data(), out.size(), cudaMemcpyDeviceToHost,
+                                                 current_stream()), "cudaMemcpyAsync"));
+            OXIDE_TRY(check_cuda(cudaStreamSynchronize(current_stream()), "cudaStreamSynchronize"));
+        }
+        return out;
+    }
+};
+
+namespace detail {
+inline Result<Q8Rows> q8_rows(const Tensor& x) {
+    auto codes = DeviceBuffer::allocate(x.elem_count(), x.device());
+    if (codes.is_err()) return codes.error();
+    auto scale = Tensor::empty(Shape(std::vector<size_t>(x.dims().begin(), x.dims().end() - 1)), DType::F32, x.device());
+    if (scale.is_err()) return scale.error();
+    return Q8Rows{x.shape(), std::move(codes).value(), std::move(scale).value()};
+}
+}  // namespace detail
+
+// rms_norm whose rows leave as int8 codes, scale = max|y| / 127.
+inline Result<Q8Rows> rms_norm_q8(const Tensor& x, const Tensor& w, float eps) {
+    auto cols = detail::norm_cols(x, w);
+    if (cols.is_err()) return cols.error();
+    auto q = detail::q8_rows(x);
+    if (q.is_err()) return q;
+    const Q8Rows& o = q.value();
+    const size_t c = cols.value(), rows = c ? x.elem_count() / c : 0;
+    const int rc = detail::bf16(x)
+        ? oxide_rms_norm_q8_bf16(x.as<oxide_bf16>(), w.as<oxide_bf16>(), o.data(), o.scale.as<float>(), rows, c, eps,
+                                 current_stream())
+        : oxide_rms_norm_q8_f32(x.as<float>(), w.as<float>(), o.data(), o.scale.as<float>(), rows, c, eps,
+                                current_stream());
+    OXIDE_TRY(check_status(rc));
+    return q;
+}
+
+// (h, codes): h = x + r, then rms_norm_q8(h).
+inline Result<std::pair<Tensor, Q8Rows>> add_rms_norm_q8(const Tensor& x, const Tensor& r, const Tensor& w, float eps) {
+    auto cols = detail::norm_cols(x, w);
+    if (cols.is_err()) return cols.error();
+    if (x.shape() != r.shape())
+        return OxideError{OxideError::Kind::ShapeMismatch,
+                          "add_rms_norm_q8: x " + x.shape().to_string() + ", residual " + r.shape().to_string()};
+    OXIDE_TRY(detail::same_dtype(x, r, "add_rms_norm_q8"));
+    auto h = Tensor::empty(x.shape(), x.dtype(), x.device());
+    if (h.is_err()) return h.error();
+    auto q = detail::q8_rows(x);
+    if (q.is_err()) return q.error();
+    const Tensor& ht = h.value();
+    const Q8Rows& o = q.value();
+    const size_t c = cols.value(), rows = c ? x.elem_count() / c : 0;
+    const int rc = detail::bf16(x)
+        ? oxide_add_rms_norm_q8_bf16(x.as<oxide_bf16>(), r.as<oxide_bf16>(), w.as<oxide_bf16>(), ht.as<oxide_bf16>(),
+                                     o.data(), o.scale.as<float>(), rows, c, eps, current_stream())
+        : oxide_add_rms_norm_q8_f32(x.as<float>(), r.as<float>(), w.as<float>(), ht.as<float>(), o.data(),
+                                    o.scale.as<float>(), rows, c, eps, current_stream());
+    OXIDE_TRY(check_status(rc));
+    return std::make_pair(std::move(h).value(), std::move(q).value());
+}
+
 // softmax along `dim` (src/ops/activation.rs:76-124).
 inline Result<Tensor> softmax(const Tensor& x, size_t dim) {
     if (dim >= x.rank())
@@ -835,6 +906,140 @@ class KvCache {
     std::vector<Tensor> k_, v_;
     std::vector<size_t> len_;
     size_t batch_ = 0, heads_ = 0, head_dim_ = 0, max_ = 0;
+};
+
+// KvCache held as int8 codes with one f32 scale per block of `block` positions
+// and head: update() quantises as it writes, read() gives values back, attend()
+// is one decode step of attention over a layer.
+class KvCacheQ8 {
+  public:
+    static Result<KvCacheQ8> create(size_t num_layers, size_t batch, size_t kv_heads, size_t head_dim,
+                                    size_t max_seq_len, size_t block = 64, int device = 0) {
+        if (block == 0 || block > 128 || (block & (block - 1)))
+            return OxideError::invalid("KvCacheQ8: block must be a power of two in [1, 128]");
+        KvCacheQ8 c;
+        c.batch_ = batch;
+        c.heads_ = kv_heads;
+        c.head_dim_ = head_dim;
+        c.max_ = max_seq_len;
+        c.block_ = block;
+        c.device_ = device;
+        c.len_.assign(num_layers, 0);
+        const size_t codes = batch * kv_heads * max_seq_len * head_dim, nblk = (max_seq_len + block - 1) / block;
+        for (size_t l = 0; l < 2 * num_layers; ++l) {
+            auto buf = DeviceBuffer::allocate(codes, device);
+            if (buf.is_err()) return buf.error();
+            if (codes)
+                OXIDE_TRY(check_cuda(cudaMemsetAsync(buf.value()->ptr(), 0, codes, current_stream()), "cudaMemsetAsync"));
+            auto sc = Tensor::zeros(Shape{batch, kv_heads, nblk}, DType::F32, device);
+            if (sc.is_err()) return sc.error();
+            c.codes_.push_back(std::move(buf).value());
+            c.scales_.push_back(std::move(sc).value());
+        }
+        return c;
+    }
+    Status update(size_t layer, const Tensor& key, const Tensor& value) {
+        OXIDE_TRY(check_layer(layer));
+        if (key.shape() != value.shape() || key.rank() != 4 || key.dims()[0] != batch_ || key.dims()[1] != heads_ ||
+            key.dims()[3] != head_dim_ || key.dtype() != value.dtype() || key.device() != device_ ||
+            value.device() != device_)
+            return OxideError::invalid("key/value " + key.shape().to_string() + " do not match the cache " +
+                                       Shape{batch_, heads_, max_, head_dim_}.to_string());
+        const size_t cur = len_[layer], add = key.dims()[2];
+        if (cur + add > max_)
+            return OxideError::invalid("KV cache overflow: " + std::to_string(cur + add) + " > " + std::to_string(max_));
+        const int rc = key.dtype() == DType::BF16
+            ? oxide_kv_cache_append_q8_bf16(k(layer), v(layer), k_scale(layer), v_scale(layer), key.as<oxide_bf16>(),
+                                            value.as<oxide_bf16>(), batch_, heads_, max_, head_dim_, block_, cur, nullptr,
+                                            add, nullptr, current_stream())
+            : oxide_kv_cache_append_q8_f32(k(layer), v(layer), k_scale(layer), v_scale(layer), key.as<float>(),
+                                           value.as<float>(), batch_, heads_, max_, head_dim_, block_, cur, nullptr, add,
+                                           nullptr, current_stream());
+        OXIDE_TRY(check_status(rc));
+        len_[layer] = cur + add;
+        return Unit{};
+    }
+    // (k, v) [batch, kv_heads, seq_len(layer), head_dim] as values.
+    Result<std::pair<Tensor, Tensor>> read(size_t layer, DType dtype = DType::F32) const {
+        OXIDE_TRY(check_layer(layer));
+        const Shape s{batch_, heads_, len_[layer], head_dim_};
+        auto kt = Tensor::empty(s, dtype, device_);
+        if (kt.is_err()) return kt.error();
+        auto vt = Tensor::empty(s, dtype, device_);
+        if (vt.is_err()) return vt.error();
+        const Tensor &ko = kt.value(), &vo = vt.value();
+        const int rc = dtype == DType::BF16
+            ? oxide_kv_cache_read_q8_bf16(k(layer), v(layer), k_scale(layer), v_scale(layer), ko.as<oxide_bf16>(),
+                                          vo.as<oxide_bf16>(), batch_, heads_, max_, head_dim_, block_, 0, len_[layer],
+                                          nullptr, current_stream())
+            : oxide_kv_cache_read_q8_f32(k(layer), v(layer), k_scale(layer), v_scale(layer), ko.as<float>(),
+                                         vo.as<float>(), batch_, heads_, max_, head_dim_, block_, 0, len_[layer], nullptr,
+                                         current_stream());
+        OXIDE_TRY(check_status(rc));
+        return std::make_pair(std::move(kt).value(), std::move(vt).value());
+    }
+    // q [batch, q_heads, head_dim] against the layer's positions (lens: device
+    // int32 [batch], fewer for some sequences; null: all of them).
+    Result<Tensor> attend(size_t layer, const Tensor& q, const int32_t* lens = nullptr) const {
+        OXIDE_TRY(check_layer(layer));
+        if (q.rank() != 3 || q.dims()[0] != batch_ || q.dims()[2] != head_dim_ || q.device() != device_)
+            return OxideError::invalid("attend: q " + q.shape().to_string() + " does not match the cache " +
+                                       Shape{batch_, heads_, max_, head_dim_}.to_string());
+        auto out = Tensor::empty(q.shape(), q.dtype(), device_);
+        if (out.is_err()) return out;
+        const size_t hq = q.dims()[1];
+        const uint64_t wb = oxide_decode_attention_q8_workspace_bytes(batch_, hq, heads_, head_dim_);
+        auto ws = DeviceBuffer::allocate(wb, device_);
+        if (ws.is_err()) return ws.error();
+        auto own = DeviceBuffer::allocate(batch_ * sizeof(int32_t), device_);
+        if (own.is_err()) return own.error();
+        if (!lens && batch_) {
+            const std::vector<int32_t> all(batch_, static_cast<int32_t>(len_[layer]));
+            OXIDE_TRY(check_cuda(cudaMemcpyAsync(own.value()->ptr(), all.data(), batch_ * sizeof(int32_t),
+                                                 cudaMemcpyHostToDevice, current_stream()), "cudaMemcpyAsync"));
+            lens = static_cast<const int32_t*>(own.value()->ptr());
+        }
+        const float scale = 1.0f / std::sqrt((float)head_dim_);
+        const int rc = q.dtype() == DType::BF16
+            ? oxide_decode_attention_q8_bf16(q.as<oxide_bf16>(), k(layer), v(layer), k_scale(layer), v_scale(layer), lens,
+                                             out.value().as<oxide_bf16>(), batch_, hq, heads_, max_, head_dim_, block_,
+                                             scale, ws.value()->ptr(), wb, current_stream())
+            : oxide_decode_attention_q8_f32(q.as<float>(), k(layer), v(layer), k_scale(layer), v_scale(layer), lens,
+                                            out.value().as<float>(), batch_, hq, heads_, max_, head_dim_, block_, scale,
+                                            ws.value()->ptr(), wb, current_stream());
+        OXIDE_TRY(check_status(rc));
+        OXIDE_TRY(check_cuda(cudaStreamSynchronize(current_stream()), "cudaStreamSynchronize"));  // ws lifetime
+        return out;
+    }
+    size_t seq_len(size_t layer) const { return len_[layer]; }
+    size_t current_seq_len() const { return len_.empty() ? 0 : len_[0]; }
+    size_t max_seq_len() const { return max_; }
+    size_t num_layers() const { return len_.size(); }
+    void clear() { std::fill(len_.begin(), len_.end(), 0); }
+    bool is_full() const { return current_seq_len() >= max_; }
+    size_t get_cache_size() const {
+        size_t n = 0;
+        for (const auto& b : codes_) n += b->bytes();
+        for (const auto& t : scales_) n += t.nbytes();
+        return n;
+    }
+
+  private:
+    KvCacheQ8() = default;
+    Status check_layer(size_t layer) const {
+        if (layer < len_.size()) return Unit{};
+        return OxideError::invalid("Layer index " + std::to_string(layer) + " out of range for " +
+                                   std::to_string(len_.size()) + " layers");
+    }
+    int8_t* k(size_t l) const { return static_cast<int8_t*>(codes_[2 * l]->ptr()); }
+    int8_t* v(size_t l) const { return static_cast<int8_t*>(codes_[2 * l + 1]->ptr()); }
+    float* k_scale(size_t l) const { return scales_[2 * l].as<float>(); }
+    float* v_scale(size_t l) const { return scales_[2 * l + 1].as<float>(); }
+    std::vector<std::shared_ptr<DeviceBuffer>> codes_;  // k, v of each layer
+    std::vector<Tensor> scales_;
+    std::vector<size_t> len_;
+    size_t batch_ = 0, heads_ = 0, head_dim_ = 0, max_ = 0, block_ = 64;
+    int device_ = 0;
 };
 
 // ---- launcher-level interface (src/cuda_backend) ------------------------------------------------

@@ -589,7 +589,7 @@ __global__ void __launch_bounds__(QT_THREADS, 1)
                     const uint64_t slot = part * NR + h;
                     if (L < p.head_dim)
                         p.part_o[slot * p.head_dim + L] =
-                            fmul(acc[h], qt_ex2(fsub(wm[h], m[h])));
+                            fmul(acc[h], ex2_approx(fsub(wm[h], m[h])));
                     if (L == 0) {
                         p.part_ml[slot * 2] = m[h];
                         p.part_ml[slot * 2 + 1] = fadd(fadd(lsum[h], lsum[8 + h]), fadd(lsum[16 + h], lsum[24 + h]));

@@ -65,7 +65,8 @@ __device__ __forceinline__ bool append_item(const AppendQ8Args& p, uint32_t i, A
     }
     if (n == 0 || n > p.max_seq - cur) return false;  // nothing to write, or it does not fit: the sequence is left as it is
     it.blk = (cur >> p.shift) + j;
-    it.start = it.blk << p.shift;  // an untouched block's may pass 2^31, not 2^32
+    if (it.blk >= p.nblk) return false;
+    it.start = it.blk << p.shift;
     const uint32_t end = cur + n;
     if (it.start >= end) return false;
     it.lo = max(it.start, cur);

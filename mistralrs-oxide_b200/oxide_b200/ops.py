@@ -11,9 +11,9 @@ op is one call into liboxide_b200.so.
 from __future__ import annotations
 
 import math
+from ctypes import c_float as _c_float
 from typing import Optional, Sequence
 
-import numpy as np
 import torch
 
 from . import _lib
@@ -67,20 +67,35 @@ def _stream() -> int:
     return torch.cuda.current_stream().cuda_stream
 
 
-def _one_device(op: str, ref: torch.Tensor, **named: Optional[torch.Tensor]) -> None:
-    """Every named tensor lives where ref does."""
-    for name, t in named.items():
-        if t is not None:
-            _need(t.device == ref.device, op, f"{name} is on {t.device}, not on {ref.device}")
+def _bad(op: str, msg: str) -> None:
+    """Refuse a call (the message is only made on this path)."""
+    raise OxideError(_lib.ERR_INVALID_ARG, op, msg)
+
+
+def _placed(op: str, ref: torch.Tensor, *ts: Optional[torch.Tensor]) -> None:
+    """Every tensor is contiguous and on ref's CUDA device."""
+    dev = ref.get_device()
+    if dev < 0 or not ref.is_contiguous():
+        _check(ref)
+    for t in ts:
+        if t is not None and (t.get_device() != dev or not t.is_contiguous()):
+            _check(t)
+            _bad(op, f"tensors are on {ref.device} and {t.device}: one device is needed")
+
+
+# The current stream's handle without making a Stream object (3 us a call).
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or \
+    (lambda dev: torch.cuda.current_stream(dev).cuda_stream)
 
 
 def _call_on(ref: torch.Tensor, name: str, *args) -> None:
     """Call an entry point on ref's device, on that device's current stream."""
-    if ref.device.index == torch.cuda.current_device():
-        call(name, *args, _stream())
+    dev = ref.get_device()
+    if dev == torch.cuda.current_device():
+        call(name, *args, _raw_stream(dev))
     else:
-        with torch.cuda.device(ref.device):
-            call(name, *args, _stream())
+        with torch.cuda.device(dev):
+            call(name, *args, _raw_stream(dev))
 
 
 def broadcast_shape(a: Sequence[int], b: Sequence[int]) -> list[int]:
@@ -322,11 +337,18 @@ def add_rms_norm(x: torch.Tensor, r: torch.Tensor, w: torch.Tensor, eps: float,
     return h, y
 
 
-def _norm_q8_out(op: str, x: torch.Tensor, out: Optional[torch.Tensor], scale: Optional[torch.Tensor]) -> None:
-    _need(out is None or (out.dtype == torch.int8 and out.numel() == x.numel()), op,
-          f"out must be int8 with {x.numel()} elements")
-    _need(scale is None or (scale.dtype == torch.float32 and scale.numel() == math.prod(x.shape[:-1])), op,
-          f"scale must be float32 with one value per row ({math.prod(x.shape[:-1])})")
+def _norm_q8_check(op: str, x: torch.Tensor, w: torch.Tensor, out, scale) -> int:
+    """Shapes and dtypes of the int8 norms; the row length."""
+    if x.dim() < 1 or w.dim() != 1 or w.shape[0] != x.shape[-1] or w.dtype != x.dtype:
+        _norm_check(x, w)
+    cols = x.shape[-1]
+    if cols < 1:
+        _bad(op, "rows must not be empty")
+    if out is not None and (out.dtype != torch.int8 or out.numel() != x.numel()):
+        _bad(op, f"out must be int8 with {x.numel()} elements")
+    if scale is not None and (scale.dtype != torch.float32 or scale.numel() * cols != x.numel()):
+        _bad(op, f"scale must be float32 with one value per row ({x.numel() // cols})")
+    return cols
 
 
 def rms_norm_q8(x: torch.Tensor, w: torch.Tensor, eps: float, out: Optional[torch.Tensor] = None,
@@ -334,14 +356,12 @@ def rms_norm_q8(x: torch.Tensor, w: torch.Tensor, eps: float, out: Optional[torc
     """(codes, scale): rms_norm (src/ops/norm.rs:4-51) whose rows leave as int8
     codes with one f32 scale a row, scale = max|y| / 127, code = the integer
     nearest to y / scale.  codes has x's shape, scale x.shape[:-1]."""
-    cols = _norm_check(x, w)
-    _need(cols >= 1, "rms_norm_q8", "rows must not be empty")
-    _norm_q8_out("rms_norm_q8", x, out, scale)
-    _check(x, w, out, scale)
-    _one_device("rms_norm_q8", x, weight=w, out=out, scale=scale)
+    cols = _norm_q8_check("rms_norm_q8", x, w, out, scale)
+    _placed("rms_norm_q8", x, w, out, scale)
     out = torch.empty_like(x, dtype=torch.int8) if out is None else out
-    scale = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device) if scale is None else scale
-    _call_on(x, f"oxide_rms_norm_q8_{_sfx(x)}", _p(x), _p(w), _p(out), _p(scale), x.numel() // cols, cols, float(eps))
+    scale = x.new_empty(x.shape[:-1], dtype=torch.float32) if scale is None else scale
+    _call_on(x, f"oxide_rms_norm_q8_{_sfx(x)}", x.data_ptr(), w.data_ptr(), out.data_ptr(), scale.data_ptr(),
+             x.numel() // cols, cols, float(eps))
     return out, scale
 
 
@@ -350,19 +370,17 @@ def add_rms_norm_q8(x: torch.Tensor, r: torch.Tensor, w: torch.Tensor, eps: floa
                     scale: Optional[torch.Tensor] = None):
     """(h, codes, scale): h = x + r (src/layers/transformer.rs:64-67), then
     rms_norm_q8(h).  h may be x or r (in place)."""
-    cols = _norm_check(x, w)
-    _need(cols >= 1, "add_rms_norm_q8", "rows must not be empty")
-    _need(r.shape == x.shape and r.dtype == x.dtype, "add_rms_norm_q8",
-          "residual must match the input's shape and dtype")
-    _out_like("add_rms_norm_q8", x, h=h)
-    _norm_q8_out("add_rms_norm_q8", x, out, scale)
-    _check(x, r, w, h, out, scale)
-    _one_device("add_rms_norm_q8", x, residual=r, weight=w, h=h, out=out, scale=scale)
+    cols = _norm_q8_check("add_rms_norm_q8", x, w, out, scale)
+    if r.shape != x.shape or r.dtype != x.dtype:
+        _bad("add_rms_norm_q8", "residual must match the input's shape and dtype")
+    if h is not None:
+        _out_like("add_rms_norm_q8", x, h=h)
+    _placed("add_rms_norm_q8", x, r, w, h, out, scale)
     h = torch.empty_like(x) if h is None else h
     out = torch.empty_like(x, dtype=torch.int8) if out is None else out
-    scale = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device) if scale is None else scale
-    _call_on(x, f"oxide_add_rms_norm_q8_{_sfx(x)}", _p(x), _p(r), _p(w), _p(h), _p(out), _p(scale),
-             x.numel() // cols, cols, float(eps))
+    scale = x.new_empty(x.shape[:-1], dtype=torch.float32) if scale is None else scale
+    _call_on(x, f"oxide_add_rms_norm_q8_{_sfx(x)}", x.data_ptr(), r.data_ptr(), w.data_ptr(), h.data_ptr(),
+             out.data_ptr(), scale.data_ptr(), x.numel() // cols, cols, float(eps))
     return h, out, scale
 
 
@@ -642,20 +660,27 @@ def decode_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
 
 
 # ---- the int8 KV cache ----
-def _q8_cache_check(op: str, k_cache, v_cache, k_scale, v_scale, block: int) -> None:
-    _need(k_cache.dim() == 4 and k_cache.dtype == torch.int8 and v_cache.dtype == torch.int8 and
-          v_cache.shape == k_cache.shape, op,
-          f"caches must be int8 [batch, kv_heads, max_seq, head_dim] alike, got {k_cache.dtype} "
-          f"{list(k_cache.shape)} and {v_cache.dtype} {list(v_cache.shape)}")
-    _need(block in (1, 2, 4, 8, 16, 32, 64, 128), op, "block must be a power of two in [1, 128]")
-    want = [k_cache.shape[0], k_cache.shape[1], -(-k_cache.shape[2] // block)]
+_Q8_BLOCKS = frozenset((1, 2, 4, 8, 16, 32, 64, 128))
+
+
+def _q8_cache_check(op: str, k_cache, v_cache, k_scale, v_scale, block: int):
+    """Shapes and dtypes of an int8 cache; its shape."""
+    shape = k_cache.shape
+    if len(shape) != 4 or k_cache.dtype != torch.int8 or v_cache.dtype != torch.int8 or v_cache.shape != shape:
+        _bad(op, f"caches must be int8 [batch, kv_heads, max_seq, head_dim] alike, got {k_cache.dtype} "
+                 f"{list(shape)} and {v_cache.dtype} {list(v_cache.shape)}")
+    if block not in _Q8_BLOCKS:
+        _bad(op, "block must be a power of two in [1, 128]")
+    want = (shape[0], shape[1], -(-shape[2] // block))
     for name, t in (("k_scale", k_scale), ("v_scale", v_scale)):
-        _need(t.dtype == torch.float32 and list(t.shape) == want, op,
-              f"{name} must be float32 {want}, got {t.dtype} {list(t.shape)}")
+        if t.dtype != torch.float32 or t.shape != want:
+            _bad(op, f"{name} must be float32 {list(want)}, got {t.dtype} {list(t.shape)}")
+    return shape
 
 
-def _q8_lens(op: str, name: str, t: Optional[torch.Tensor], batch: int) -> None:
-    _need(t is None or (t.dtype == torch.int32 and t.numel() == batch), op, f"{name} must be int32 with {batch} entries")
+def _q8_lens(op: str, name: str, t: torch.Tensor, batch: int) -> None:
+    if t.dtype != torch.int32 or t.numel() != batch:
+        _bad(op, f"{name} must be int32 with {batch} entries")
 
 
 def kv_cache_append_q8(k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor,
@@ -671,22 +696,26 @@ def kv_cache_append_q8(k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: to
     sequence whose length is negative or whose tokens do not fit is left as it
     is).  new_lens (int32 device tensor): tokens of a padded batch that count."""
     op = "kv_cache_append_q8"
-    _q8_cache_check(op, k_cache, v_cache, k_scale, v_scale, block)
-    b, hkv, m, d = k_cache.shape
-    _need(k.dim() == 4 and k.shape == v.shape and k.shape[0] == b and k.shape[1] == hkv and k.shape[3] == d and
-          k.dtype == v.dtype, op,
-          f"key/value {list(k.shape)}, {list(v.shape)} do not match the cache {list(k_cache.shape)}")
+    b, hkv, m, d = _q8_cache_check(op, k_cache, v_cache, k_scale, v_scale, block)
+    shape = k.shape
+    if len(shape) != 4 or shape != v.shape or shape[0] != b or shape[1] != hkv or shape[3] != d or k.dtype != v.dtype:
+        _bad(op, f"key/value {list(shape)}, {list(v.shape)} do not match the cache {list(k_cache.shape)}")
     each = cur_len if isinstance(cur_len, torch.Tensor) else None
-    _q8_lens(op, "cur_len", each, b)
-    _q8_lens(op, "new_lens", new_lens, b)
-    cur = 0 if each is not None else int(cur_len)
-    _need(cur >= 0, op, "cur_len must be >= 0")
-    _need(cur + k.shape[2] <= m, op, f"KV cache overflow: {cur + k.shape[2]} > {m}")
-    _check(k_cache, v_cache, k_scale, v_scale, k, v, each, new_lens)
-    _one_device(op, k_cache, v_cache=v_cache, k_scale=k_scale, v_scale=v_scale, key=k, value=v, cur_len=each,
-                new_lens=new_lens)
-    _call_on(k_cache, f"oxide_kv_cache_append_q8_{_sfx(k)}", _p(k_cache), _p(v_cache), _p(k_scale), _p(v_scale),
-             _p(k), _p(v), b, hkv, m, d, block, cur, _p(each), k.shape[2], _p(new_lens))
+    cur = 0
+    if each is not None:
+        _q8_lens(op, "cur_len", each, b)
+    else:
+        cur = int(cur_len)
+        if cur < 0:
+            _bad(op, "cur_len must be >= 0")
+    if new_lens is not None:
+        _q8_lens(op, "new_lens", new_lens, b)
+    if cur + shape[2] > m:
+        _bad(op, f"KV cache overflow: {cur + shape[2]} > {m}")
+    _placed(op, k_cache, v_cache, k_scale, v_scale, k, v, each, new_lens)
+    _call_on(k_cache, f"oxide_kv_cache_append_q8_{_sfx(k)}", k_cache.data_ptr(), v_cache.data_ptr(),
+             k_scale.data_ptr(), v_scale.data_ptr(), k.data_ptr(), v.data_ptr(), b, hkv, m, d, block, cur, _p(each),
+             shape[2], _p(new_lens))
 
 
 def kv_cache_read_q8(k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor,
@@ -696,23 +725,25 @@ def kv_cache_read_q8(k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torc
     int8 caches (default: to the end), code * scale in dtype (f32 or bf16);
     positions at or behind lens[b] (int32 device tensor) are zeros."""
     op = "kv_cache_read_q8"
-    _q8_cache_check(op, k_cache, v_cache, k_scale, v_scale, block)
-    b, hkv, m, d = k_cache.shape
-    start, n = int(start), m - int(start) if n is None else int(n)
-    _need(0 <= start and 0 <= n and start + n <= m, op, f"positions [{start}, {start + n}) out of range for {m}")
-    _q8_lens(op, "lens", lens, b)
+    b, hkv, m, d = _q8_cache_check(op, k_cache, v_cache, k_scale, v_scale, block)
+    start = int(start)
+    n = m - start if n is None else int(n)
+    if start < 0 or n < 0 or start + n > m:
+        _bad(op, f"positions [{start}, {start + n}) out of range for {m}")
+    if lens is not None:
+        _q8_lens(op, "lens", lens, b)
     dtype = k.dtype if k is not None else v.dtype if v is not None else dtype
     if dtype not in _SFX:
         raise OxideError(_lib.ERR_UNSUPPORTED, op, f"dtype {dtype} is not float32/bfloat16")
+    shape = (b, hkv, n, d)
     for name, t in (("k", k), ("v", v)):
-        _need(t is None or (t.dtype == dtype and list(t.shape) == [b, hkv, n, d]), op,
-              f"{name} must be {dtype} {[b, hkv, n, d]}")
-    _check(k_cache, v_cache, k_scale, v_scale, lens, k, v)
-    _one_device(op, k_cache, v_cache=v_cache, k_scale=k_scale, v_scale=v_scale, lens=lens, k=k, v=v)
-    k = torch.empty((b, hkv, n, d), dtype=dtype, device=k_cache.device) if k is None else k
-    v = torch.empty((b, hkv, n, d), dtype=dtype, device=k_cache.device) if v is None else v
-    _call_on(k_cache, f"oxide_kv_cache_read_q8_{_SFX[dtype]}", _p(k_cache), _p(v_cache), _p(k_scale), _p(v_scale),
-             _p(k), _p(v), b, hkv, m, d, block, start, n, _p(lens))
+        if t is not None and (t.dtype != dtype or t.shape != shape):
+            _bad(op, f"{name} must be {dtype} {list(shape)}")
+    _placed(op, k_cache, v_cache, k_scale, v_scale, lens, k, v)
+    k = k_cache.new_empty(shape, dtype=dtype) if k is None else k
+    v = k_cache.new_empty(shape, dtype=dtype) if v is None else v
+    _call_on(k_cache, f"oxide_kv_cache_read_q8_{_SFX[dtype]}", k_cache.data_ptr(), v_cache.data_ptr(),
+             k_scale.data_ptr(), v_scale.data_ptr(), k.data_ptr(), v.data_ptr(), b, hkv, m, d, block, start, n, _p(lens))
     return k, v
 
 
@@ -726,28 +757,32 @@ def decode_attention_q8(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.T
     every position).  An empty sequence gives zeros.  A workspace given must not
     be in use by another call that may run at the same time."""
     op = "decode_attention_q8"
-    _q8_cache_check(op, k_cache, v_cache, k_scale, v_scale, block)
-    _need(q.dim() == 3 and q.shape[0] == k_cache.shape[0] and q.shape[2] == k_cache.shape[3], op,
-          f"q {list(q.shape)} and caches {list(k_cache.shape)} do not match")
-    b, hq, d = q.shape
-    hkv, m = k_cache.shape[1], k_cache.shape[2]
-    _need(hkv >= 1 and hq % hkv == 0, op, f"{hq} query heads are not a multiple of {hkv} kv heads")
-    _q8_lens(op, "lens", lens, b)
-    _out_like(op, q, out=out)
-    need = int(_lib.lib().oxide_decode_attention_q8_workspace_bytes(b, hq, hkv, d))
-    _need(workspace is None or workspace.numel() * workspace.element_size() >= need, op,
-          f"workspace must hold {need} bytes")
-    _check(q, k_cache, v_cache, k_scale, v_scale, lens, workspace, out)
-    _one_device(op, q, k_cache=k_cache, v_cache=v_cache, k_scale=k_scale, v_scale=v_scale, lens=lens,
-                workspace=workspace, out=out)
-    if scale is None:
-        scale = float(np.float32(1) / np.sqrt(np.float32(d)))
+    b, hkv, m, d = _q8_cache_check(op, k_cache, v_cache, k_scale, v_scale, block)
+    if q.dim() != 3 or q.shape[0] != b or q.shape[2] != d:
+        _bad(op, f"q {list(q.shape)} and caches {list(k_cache.shape)} do not match")
+    hq = q.shape[1]
+    if hkv < 1 or hq % hkv != 0:
+        _bad(op, f"{hq} query heads are not a multiple of {hkv} kv heads")
+    if lens is not None:
+        _q8_lens(op, "lens", lens, b)
+    if out is not None:
+        _out_like(op, q, out=out)
+    need = _lib.lib().oxide_decode_attention_q8_workspace_bytes(b, hq, hkv, d)
     if workspace is None:
-        workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
+        size = need
+    else:
+        size = workspace.numel() * workspace.element_size()
+        if size < need:
+            _bad(op, f"workspace must hold {need} bytes")
+    _placed(op, q, k_cache, v_cache, k_scale, v_scale, lens, workspace, out)
+    if scale is None:  # 1 / sqrt(head_dim), each step rounded to f32
+        scale = 1.0 / _c_float(math.sqrt(d)).value if d else 1.0
+    if workspace is None:
+        workspace = q.new_empty(need, dtype=torch.uint8)
     out = torch.empty_like(q) if out is None else out
-    _call_on(q, f"oxide_decode_attention_q8_{_sfx(q)}", _p(q), _p(k_cache), _p(v_cache), _p(k_scale), _p(v_scale),
-             _p(lens), _p(out), b, hq, hkv, m, d, block, float(scale), _p(workspace),
-             workspace.numel() * workspace.element_size())
+    _call_on(q, f"oxide_decode_attention_q8_{_sfx(q)}", q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
+             k_scale.data_ptr(), v_scale.data_ptr(), _p(lens), out.data_ptr(), b, hq, hkv, m, d, block, float(scale),
+             workspace.data_ptr(), size)
     return out
 
 
@@ -761,7 +796,8 @@ class KvCacheQ8(KvCache):
     def __init__(self, num_layers: int, batch_size: int, num_kv_heads: int, head_dim: int,
                  max_seq_len: int, block: int = 64, dtype=torch.bfloat16, device="cuda"):
         super().__init__(0, batch_size, num_kv_heads, head_dim, max_seq_len, dtype, device)
-        _need(block in (1, 2, 4, 8, 16, 32, 64, 128), "KvCacheQ8", "block must be a power of two in [1, 128]")
+        if block not in _Q8_BLOCKS:
+            _bad("KvCacheQ8", "block must be a power of two in [1, 128]")
         shape = (batch_size, num_kv_heads, max_seq_len, head_dim)
         scales = (batch_size, num_kv_heads, -(-max_seq_len // block))
         self.block, self.dtype, self.num_layers = block, dtype, num_layers

@@ -100,6 +100,54 @@ def build(op: str, rows: int | None, dev):
         run = lambda s: ops.decode_attention(s[0], s[1], s[2], tl, workspace=ws, out=s[3])  # noqa: E731
         nb = int(np.sum(np.minimum(lens, c.keys))) * kvh * c.head_dim * es * 2 + 2 * c.batch * c.heads * c.head_dim * es
         return mk, run, nb, [c.batch, c.heads, kvh, c.keys, c.head_dim]
+    if op in ("add_rms_norm_q8_bf16_c5", "rms_norm_q8_f32_c1"):
+        # the norms with int8 rows, at the C5 hidden size and at C1
+        c = C1()
+        R = rows or (16384 if op == "add_rms_norm_q8_bf16_c5" else c.rows)
+        dt = BF16 if op == "add_rms_norm_q8_bf16_c5" else torch.float32
+        es = 2 if dt == BF16 else 4
+        w = (torch.rand(c.cols, generator=g, device=dev) + 0.5).to(dt)
+        out = lambda: (torch.empty(R, c.cols, dtype=torch.int8, device=dev), torch.empty(R, device=dev))  # noqa: E731
+        if dt == BF16:
+            mk = lambda: (rn(R, c.cols, dtype=dt), rn(R, c.cols, dtype=dt), torch.empty(R, c.cols, dtype=dt, device=dev),  # noqa: E731
+                          *out())
+            run = lambda s: ops.add_rms_norm_q8(s[0], s[1], w, c.eps, h=s[2], out=s[3], scale=s[4])  # noqa: E731
+            return mk, run, R * c.cols * (3 * es + 1) + R * 4 + c.cols * es, [R, c.cols]
+        mk = lambda: (rn(R, c.cols), *out())  # noqa: E731
+        run = lambda s: ops.rms_norm_q8(s[0], w, c.eps, out=s[1], scale=s[2])  # noqa: E731
+        return mk, run, R * c.cols * (es + 1) + R * 4 + c.cols * es, [R, c.cols]
+    if op in ("decode_attn_q8_bf16_c3", "decode_attn_q8_f32_c3", "kv_append_q8_bf16", "kv_read_q8_bf16"):
+        # the C3 decode step over an int8 cache with a scale per 64 positions and
+        # head; an append of 2048 tokens to 8 sequences; the cache of 8 x 8192 read back
+        c = C3()
+        kvh, d, block = NKV, c.head_dim, 64
+        dt = torch.float32 if op == "decode_attn_q8_f32_c3" else BF16
+        es = 4 if dt == torch.float32 else 2
+        m = c.keys if op.startswith("decode") else 8192
+
+        def cache():
+            codes = lambda: torch.randint(-127, 128, (c.batch, kvh, m, d), generator=g, device=dev, dtype=torch.int8)  # noqa: E731
+            scale = lambda: torch.rand(c.batch, kvh, m // block, generator=g, device=dev) * 0.02 + 0.01  # noqa: E731
+            return codes(), codes(), scale(), scale()
+
+        if op == "kv_append_q8_bf16":
+            n = rows or 2048
+            mk = lambda: (*cache(), rn(c.batch, kvh, n, d, dtype=dt), rn(c.batch, kvh, n, d, dtype=dt))  # noqa: E731
+            run = lambda s: ops.kv_cache_append_q8(*s, 0, block)  # noqa: E731
+            return mk, run, 2 * c.batch * kvh * n * d * (es + 1), [c.batch, kvh, n, d]
+        if op == "kv_read_q8_bf16":
+            out = lambda: torch.empty(c.batch, kvh, m, d, dtype=dt, device=dev)  # noqa: E731
+            mk = lambda: (*cache(), out(), out())  # noqa: E731
+            run = lambda s: ops.kv_cache_read_q8(*s[:4], block, k=s[4], v=s[5])  # noqa: E731
+            return mk, run, 2 * c.batch * kvh * m * d * (es + 1), [c.batch, kvh, m, d]
+        _, lens, _ = c.inputs()
+        tl = torch.from_numpy(lens).to(dev)
+        ws = torch.empty(int(_lib.lib().oxide_decode_attention_q8_workspace_bytes(c.batch, c.heads, kvh, d)),
+                         dtype=torch.uint8, device=dev)
+        mk = lambda: (rn(c.batch, c.heads, d, dtype=dt), *cache(), torch.empty(c.batch, c.heads, d, dtype=dt, device=dev))  # noqa: E731
+        run = lambda s: ops.decode_attention_q8(*s[:5], block, tl, workspace=ws, out=s[5])  # noqa: E731
+        total = int(np.sum(np.minimum(lens, c.keys)))
+        return mk, run, total * kvh * (2 * d + 8 // block) + 2 * c.batch * c.heads * d * es, [c.batch, c.heads, kvh, c.keys, d]
     if op in ("decode_weights_bf16_f32", "decode_weights_f16_f32"):
         # safetensors element decode of one Mistral MLP matrix [14336, 4096] to f32
         n = (rows or 14336) * 4096
@@ -298,7 +346,9 @@ OPS = ["rms_norm_f32_c1", "add_f32_c2", "mul_f32_c2", "add_mul_f32_c2", "silu_mu
        "repeat_kv_bf16_c5", "kv_append_bf16_c5", "decode_attn_bf16_c3", "decode_attn_f32_c3",
        "softmax_temperature_f32_c3", "sample_topk_f32_c3", "sample_topp_f32_c3",
        "decode_weights_bf16_f32", "decode_weights_f16_f32", "copy_like_c1", "copy_like_c3",
-       "copy_like_argmax_c3", "torch_copy_like_c1", "torch_copy_like_c3"]
+       "copy_like_argmax_c3", "torch_copy_like_c1", "torch_copy_like_c3",
+       "add_rms_norm_q8_bf16_c5", "rms_norm_q8_f32_c1", "kv_append_q8_bf16", "kv_read_q8_bf16",
+       "decode_attn_q8_bf16_c3", "decode_attn_q8_f32_c3"]
 
 
 def main(argv=None):

@@ -448,6 +448,78 @@ DEVICE_TEST(repeat_kv_and_kv_cache_match_oracle) {
            "Layer index 2 out of range for 2 layers");
 }
 
+// The code nearest to x / s, ties to even, in 64 bits.
+int8_t nearest_code(double x, double s) {
+    const double q = std::nearbyint(x / s);
+    return static_cast<int8_t>(s > 0 ? q : 0);
+}
+
+HOST_TEST(int8_cache_refuses_blocks) {
+    EXPECT(expect_err(KvCacheQ8::create(1, 1, 1, 8, 16, 48)).message.find("power of two") != std::string::npos);
+    EXPECT(expect_err(KvCacheQ8::create(1, 1, 1, 8, 16, 0)).kind == OxideError::Kind::InvalidArgument);
+}
+
+DEVICE_TEST(int8_norms_match_their_definition) {
+    const size_t rows = 5, cols = 256;
+    const auto x = randn(rows * cols, 50), r = randn(rows * cols, 51), w = uniform(cols, 52, 0.5f, 1.5f);
+    auto hq = unwrap(ops::add_rms_norm_q8(dev(x, {rows, cols}), dev(r, {rows, cols}), dev(w, {cols}), 1e-5f));
+    const auto h = host(hq.first);
+    const auto codes = unwrap(hq.second.to_vec());
+    const auto scale = host(hq.second.scale);
+    const auto alone = unwrap(unwrap(ops::rms_norm_q8(hq.first, dev(w, {cols}), 1e-5f)).to_vec());
+    EXPECT(alone == codes);
+    for (size_t i = 0; i < rows; ++i) {
+        double ss = 0, top = 0;
+        for (size_t j = 0; j < cols; ++j) {
+            const double v = h[i * cols + j];
+            EXPECT(h[i * cols + j] == x[i * cols + j] + r[i * cols + j]);
+            ss += v * v;
+            top = std::max(top, std::fabs(v * w[j]));
+        }
+        const double want = top / (127.0 * std::sqrt(ss / cols + 1e-5));
+        // an f32 sum of 256 squares over a warp and five more steps: under 32 roundings
+        EXPECT(std::fabs(scale[i] - want) <= 32 * std::ldexp(1.0, -24) * want);
+        for (size_t j = 0; j < cols; ++j)
+            EXPECT(codes[i * cols + j] == nearest_code((double)h[i * cols + j] * w[j] * 127.0, top));
+    }
+    EXPECT(expect_err(ops::rms_norm_q8(dev(x, {rows, cols}), dev(w, {cols / 2, 2}), 1e-5f)).kind ==
+           OxideError::Kind::InvalidArgument);
+}
+
+DEVICE_TEST(int8_cache_matches_its_definition) {
+    const size_t b = 2, hkv = 2, hq = 8, d = 64, n = 24, block = 16;
+    KvCacheQ8 cache = unwrap(KvCacheQ8::create(2, b, hkv, d, 40, block));
+    const auto k = randn(b * hkv * n * d, 60), v = randn(b * hkv * n * d, 61);
+    EXPECT(cache.update(1, dev(k, {b, hkv, n, d}), dev(v, {b, hkv, n, d})).is_ok());
+    EXPECT(cache.seq_len(1) == n && cache.seq_len(0) == 0);
+    auto kv = unwrap(cache.read(1));
+    const auto kr = host(kv.first), vr = host(kv.second);
+    for (size_t head = 0; head < b * hkv; ++head)
+        for (size_t j0 = 0; j0 < n; j0 += block) {
+            const size_t j1 = std::min(n, j0 + block);
+            for (const auto& [src, got] : {std::pair(&k, &kr), std::pair(&v, &vr)}) {
+                float top = 0;
+                for (size_t i = (head * n + j0) * d; i < (head * n + j1) * d; ++i) top = std::max(top, std::fabs((*src)[i]));
+                const float s = top / 127.0f;
+                for (size_t i = (head * n + j0) * d; i < (head * n + j1) * d; ++i)
+                    EXPECT((*got)[i] == (float)nearest_code((*src)[i], s) * s);
+            }
+        }
+    // attention over the cache is the oracle's over the values it stands for
+    const auto q = randn(b * hq * d, 62);
+    const auto got = host(unwrap(cache.attend(1, dev(q, {b, hq, d}))));
+    std::vector<float> ref(q.size());
+    orc_decode_attention_f32(q.data(), kr.data(), vr.data(), nullptr, ref.data(), b, hq, hkv, n, d,
+                             1.0f / std::sqrt((float)d), kThreads);
+    for (size_t i = 0; i < got.size(); ++i) EXPECT(std::fabs(got[i] - ref[i]) <= 1e-5f * (1.0f + std::fabs(ref[i])));
+    EXPECT(expect_err(cache.update(2, dev(k, {b, hkv, n, d}), dev(v, {b, hkv, n, d}))).message ==
+           "Layer index 2 out of range for 2 layers");
+    EXPECT(expect_err(cache.update(1, dev(k, {b, hkv, n, d}), dev(v, {b, hkv, n, d}))).message ==
+           "KV cache overflow: 48 > 40");
+    cache.clear();
+    EXPECT(cache.current_seq_len() == 0 && !cache.is_full());
+}
+
 DEVICE_TEST(decode_attention_and_sampling_match_oracle) {
     // one decode step over a cache of 40 positions, 8 query heads on 2 kv heads
     const size_t b = 2, hq = 8, hkv = 2, m = 40, d = 128;
