@@ -44,7 +44,7 @@ __global__ void __launch_bounds__(QW_WARPS * 32, 2) decode_attn_q8_warp_kernel(Q
     const uint32_t T = pre[p.batch] * heads, G = p.workers;
     const uint32_t c = blockIdx.x * QW_WARPS + warp;
     if (c >= G) return;
-    const uint32_t t0 = (uint32_t)((uint64_t)c * T / G), t1 = (uint32_t)((uint64_t)(c + 1) * T / G);
+    const uint32_t t0 = q8a_start(p, c, T), t1 = q8a_start(p, c + 1, T);
     if (t0 >= t1) return;
     TileWalk w{pre, p.batch, heads, 0, 0, 0, 0};
     w.seek(t0);
@@ -54,7 +54,7 @@ __global__ void __launch_bounds__(QW_WARPS * 32, 2) decode_attn_q8_warp_kernel(Q
     const float *ksh = nullptr, *vsh = nullptr;
     for (uint32_t t = t0; t < t1; ++t, w.next()) {
         if (t == t0 || w.lt == 0) {  // a new pair: its query heads and caches
-            const uint32_t kvh = w.kvh / p.chunks, h0 = (w.kvh % p.chunks) * NR;
+            const uint32_t kvh = p.by_chunks.div(w.kvh), h0 = (w.kvh - kvh * p.chunks) * NR;
             nh = min(p.rep - h0, (uint32_t)NR);
             len = q8a_len(p, w.b);
             const uint64_t bh = (uint64_t)w.b * p.kv_heads + kvh, row = (uint64_t)w.b * p.q_heads + kvh * p.rep + h0;
@@ -207,9 +207,9 @@ __global__ void __launch_bounds__(NW * 32) decode_attn_q8_combine_kernel(T* out,
     __shared__ float wm[NW], wl[NW];
     __shared__ float4 wo[NW][32 * DV];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const uint32_t bh = blockIdx.x, b = bh / p.q_heads, qh = bh - b * p.q_heads;
-    const uint32_t kvh = qh / p.rep, r = qh - kvh * p.rep, chunk = r / p.nr, h = r - chunk * p.nr;
-    const uint32_t heads = p.kv_heads * p.chunks, D = p.head_dim, DP = q8a_dims(D), W = p.workers;
+    const uint32_t bh = blockIdx.x, b = p.by_q_heads.div(bh), qh = bh - b * p.q_heads;
+    const uint32_t kvh = p.by_rep.div(qh), r = qh - kvh * p.rep, chunk = p.by_nr.div(r), h = r - chunk * p.nr;
+    const uint32_t heads = p.kv_heads * p.chunks, D = p.head_dim, DP = q8a_dims(D);
     const uint32_t before = p.pre_out[b], tb = p.pre_out[b + 1] - before, all = p.pre_out[p.batch] * heads;
     const uint32_t failed = *p.err;
     float M = -INFINITY, L = 0.0f;
@@ -219,20 +219,20 @@ __global__ void __launch_bounds__(NW * 32) decode_attn_q8_combine_kernel(T* out,
     if (tb) {
         const uint32_t pair = b * heads + kvh * p.chunks + chunk, tfirst = before * heads + (pair - b * heads) * tb,
                        tend = tfirst + tb;
-        const uint32_t c0 = tc_owner(tfirst, all, W), c1 = tc_owner(tend - 1, all, W);
+        const uint32_t c0 = q8a_owner(p, tfirst, all), c1 = q8a_owner(p, tend - 1, all);
         const uint32_t n = (c1 - c0 + 1) * p.halves;
         for (uint32_t i0 = warp; i0 < n; i0 += NW * QC_UNROLL) {
             float ms[QC_UNROLL], ls[QC_UNROLL];
             float4 o[QC_UNROLL][DV];
 #pragma unroll
             for (int u = 0; u < QC_UNROLL; ++u) {
-                const uint32_t i = i0 + u * NW, c = c0 + i / p.halves, half = i % p.halves;
+                const uint32_t i = i0 + u * NW, c = c0 + (i >> (p.halves - 1)), half = i & (p.halves - 1);
                 ms[u] = -INFINITY;
                 ls[u] = 0.0f;
 #pragma unroll
                 for (int k = 0; k < DV; ++k) o[u][k] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
                 if (i >= n) continue;
-                const uint32_t f0 = (uint32_t)((uint64_t)c * all / W), f1 = (uint32_t)((uint64_t)(c + 1) * all / W);
+                const uint32_t f0 = q8a_start(p, c, all), f1 = q8a_start(p, c + 1, all);
                 const uint32_t a = max(f0, tfirst), e = min(f1, tend);
                 if (a >= e || (e - a < p.halves && ((a - f0) ^ half) & 1)) continue;  // no tile, or the other half's one tile
                 const uint64_t slot = (((uint64_t)c + pair) * p.halves + half) * p.nr + h;
@@ -300,6 +300,7 @@ static cudaError_t launch_warp(Q8AttnArgs& a, cudaStream_t st) {
     const uint64_t tiles = (uint64_t)a.batch * a.kv_heads * a.chunks * ((a.max_seq + QW_TK - 1) / QW_TK);
     if (ctas > (tiles + QW_WARPS - 1) / QW_WARPS) ctas = (tiles + QW_WARPS - 1) / QW_WARPS;
     a.workers = (uint32_t)ctas * QW_WARPS;
+    a.inv_workers = 1.0 / a.workers;
     return launch_k(kern, (unsigned)ctas, QW_WARPS * 32, smem, st, a);
 }
 template <int NR>
@@ -371,6 +372,10 @@ static int attn_q8_entry(const char* name, const T* q, const int8_t* kc, const i
     a.shift = (uint32_t)q8_block_shift(block);
     a.nblk = (uint32_t)((max_seq + block - 1) / block);
     a.halves = 1;
+    a.by_q_heads = FastDiv(a.q_heads);
+    a.by_rep = FastDiv(a.rep);
+    a.by_nr = FastDiv(a.nr);
+    a.by_chunks = FastDiv(a.chunks);
     a.q_bf16 = sizeof(T) == 2;
     a.c1 = scale * 1.4426950408889634f;
     const int path = decode_path();

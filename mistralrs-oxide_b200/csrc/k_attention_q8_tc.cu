@@ -178,13 +178,13 @@ __global__ void __launch_bounds__(QT_THREADS, 1)
         tmem_relinquish();
     }
     pdl_wait();  // the previous kernel's writes (lengths, caches, queries) are visible
-    const uint32_t heads = p.kv_heads * p.chunks, G = p.workers;
+    const uint32_t heads = p.kv_heads * p.chunks;
     if (warp == 3) {  // the tile prefix and this CTA's first tile
         q8a_prefix(p, QT_TK, pre, blockIdx.x == 0);
         const uint32_t all = pre[p.batch] * heads;
         if (all) {
             TileWalk at{pre, p.batch, heads, 0, 0, 0, 0};
-            at.seek((uint32_t)((uint64_t)blockIdx.x * all / G));
+            at.seek(q8a_start(p, blockIdx.x, all));
             if (lane == 0) {
                 begin[0] = at.b;
                 begin[1] = at.kvh;
@@ -193,7 +193,7 @@ __global__ void __launch_bounds__(QT_THREADS, 1)
             }
             // The first pair's query heads and scales go ahead of the ring's 192 KB
             // a CTA: asked for behind them they came 3 us later.
-            const uint32_t kvh = at.kvh / p.chunks, h0 = (at.kvh % p.chunks) * NR;
+            const uint32_t kvh = p.by_chunks.div(at.kvh), h0 = (at.kvh - kvh * p.chunks) * NR;
             const uint32_t es = p.q_bf16 ? 2 : 4, bytes = min(p.rep - h0, (uint32_t)NR) * p.head_dim * es;
             if (lane * 128u < bytes)
                 prefetch_l2(static_cast<const char*>(p.q) +
@@ -208,8 +208,7 @@ __global__ void __launch_bounds__(QT_THREADS, 1)
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
     const uint32_t T = pre[p.batch] * heads;
-    const uint32_t t0 = (uint32_t)((uint64_t)blockIdx.x * T / G);
-    const uint32_t nt = (uint32_t)((uint64_t)(blockIdx.x + 1) * T / G) - t0;  // this CTA's tiles, n = 0 .. nt - 1
+    const uint32_t nt = q8a_start(p, blockIdx.x + 1, T) - q8a_start(p, blockIdx.x, T);  // this CTA's tiles, n = 0 .. nt - 1
     TileWalk w{pre, p.batch, heads, begin[0], begin[1], begin[2], begin[3]};  // (unset, and unused, without tiles)
 
     if (warp == 0) {
@@ -219,7 +218,7 @@ __global__ void __launch_bounds__(QT_THREADS, 1)
         if (!withhold) {
             for (; n < nt && !*abort; ++n) {
                 if (!warp_wait_all(bar(QB_EMPTY + s), ph, abort)) break;
-                const int z = (int)(w.b * p.kv_heads + (p.chunks == 1 ? w.kvh : w.kvh / p.chunks));
+                const int z = (int)(w.b * p.kv_heads + (p.by_chunks.div(w.kvh)));
                 const int y = (int)(w.lt * QT_TK);
                 const uint32_t sd = sbase + s * QT_STAGE_BYTES;
                 if (leader) {
@@ -309,8 +308,9 @@ __global__ void __launch_bounds__(QT_THREADS, 1)
     } else if (warp == 2) {
         // ---------------- digits of the query heads ----------------
         for (uint32_t n = 0, q = 0; n < nt; ++q) {
-            const uint32_t slot = q & 1u, h0 = (w.kvh % p.chunks) * NR, nh = min(p.rep - h0, (uint32_t)NR);
-            const uint64_t row = (uint64_t)w.b * p.q_heads + (w.kvh / p.chunks) * p.rep + h0;
+            const uint32_t slot = q & 1u, kvh = p.by_chunks.div(w.kvh), h0 = (w.kvh - kvh * p.chunks) * NR;
+            const uint32_t nh = min(p.rep - h0, (uint32_t)NR);
+            const uint64_t row = (uint64_t)w.b * p.q_heads + kvh * p.rep + h0;
             float x[NR][4];
 #pragma unroll
             for (int h = 0; h < NR; ++h) {
@@ -377,7 +377,7 @@ __global__ void __launch_bounds__(QT_THREADS, 1)
             if (ahead >= nt) return;
             if (ahead == 0 || w.lt == 0) {  // a new pair
                 len = q8a_len(p, w.b);
-                const uint64_t bh = (uint64_t)w.b * p.kv_heads + (p.chunks == 1 ? w.kvh : w.kvh / p.chunks);
+                const uint64_t bh = (uint64_t)w.b * p.kv_heads + (p.by_chunks.div(w.kvh));
                 ks = p.ks + bh * p.nblk;
                 vs = p.vs + bh * p.nblk;
             }
@@ -582,7 +582,7 @@ __global__ void __launch_bounds__(QT_THREADS, 1)
                     break;
                 }
                 const uint64_t part = ((uint64_t)blockIdx.x + (uint64_t)w.b * heads + w.kvh) * 2 + g;
-                const uint32_t nh = min(p.rep - (w.kvh % p.chunks) * NR, (uint32_t)NR);
+                const uint32_t nh = min(p.rep - (w.kvh - p.by_chunks.div(w.kvh) * p.chunks) * NR, (uint32_t)NR);
 #pragma unroll
                 for (int h = 0; h < NR; ++h) {
                     if ((uint32_t)h >= nh) continue;
@@ -657,6 +657,7 @@ cudaError_t decode_attention_q8_tc(Q8AttnArgs& a, bool withhold, cudaStream_t st
     if (!qt_map(&mk, a.kc, pairs, a.max_seq, a.head_dim) || !qt_map(&mv, a.vc, pairs, a.max_seq, a.head_dim))
         return cudaSuccess;
     a.workers = (uint32_t)G;
+    a.inv_workers = 1.0 / a.workers;
     a.halves = 2;
     *used = true;
     switch (a.nr) {

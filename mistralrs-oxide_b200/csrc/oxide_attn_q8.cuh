@@ -30,7 +30,9 @@ struct Q8AttnArgs {
     uint32_t batch, q_heads, kv_heads, head_dim;
     uint32_t rep, chunks, nr;  // query heads a kv head; pieces of at most nr of them
     uint32_t nblk, shift;      // scale blocks a head, log2 of their tokens
-    uint32_t workers, halves;  // halves: a worker's tiles go in turn to so many halves, each with a part of its own
+    uint32_t workers, halves;  // halves (1 or 2): a worker's tiles go in turn to so many, each with a part of its own
+    double inv_workers;        // 1 / workers
+    FastDiv by_q_heads, by_rep, by_nr, by_chunks;
     uint32_t q_bf16;
     float c1;                  // scale * log2(e)
 };
@@ -42,6 +44,29 @@ __device__ __forceinline__ uint32_t q8a_len(const Q8AttnArgs& p, uint32_t b) {
     if (!p.lens) return (uint32_t)p.max_seq;
     const int32_t l = p.lens[b];
     return l <= 0 ? 0u : ((uint64_t)l < p.max_seq ? (uint32_t)l : (uint32_t)p.max_seq);
+}
+
+// floor(c T / workers), where worker c's tiles begin (c <= workers, T < 2^31): the
+// f64 product is within one of it, the remainder says which.  (64-bit divisions
+// took most of the combine kernel's instructions.)
+__device__ __forceinline__ uint32_t q8a_start(const Q8AttnArgs& p, uint32_t c, uint32_t T) {
+    const uint64_t n = (uint64_t)c * T;
+    uint32_t q = (uint32_t)((double)n * p.inv_workers);
+    const int64_t r = (int64_t)(n - (uint64_t)q * p.workers);
+    if (r < 0) --q;
+    else if (r >= (int64_t)p.workers) ++q;
+    return q;
+}
+// The worker that has tile t: the largest c with q8a_start(c) <= t, that is
+// floor(((t + 1) workers - 1) / T) -- at most 12 bits, so an f32 quotient is
+// within one of it.
+__device__ __forceinline__ uint32_t q8a_owner(const Q8AttnArgs& p, uint32_t t, uint32_t T) {
+    const uint64_t n = ((uint64_t)t + 1) * p.workers - 1;
+    uint32_t q = (uint32_t)__fdividef((float)n, (float)T);
+    const int64_t r = (int64_t)(n - (uint64_t)q * T);
+    if (r < 0) --q;
+    else if (r >= (int64_t)T) ++q;
+    return q;
 }
 
 // One warp: the prefix of the batches' tile counts into shared memory, pre[0 .. batch].

@@ -162,3 +162,32 @@ def test_cache_class_refuses():
     raises("block must be", ops.KvCacheQ8, 1, 2, 2, 16, 40, block=48, device="cpu")
     assert c.get(0) is None and c.current_seq_len() == 0
     assert c.get_cache_size() == 2 * (2 * 2 * 40 * 16 + 2 * 2 * 3 * 4)
+
+
+def test_work_division_formulas():
+    """Host restatement of oxide_attn_q8.cuh's two divisions: worker c of W begins
+    at floor(c T / W), and tile t belongs to floor(((t + 1) W - 1) / T) -- from an
+    f64 product with 1 / W and from an f32 quotient off by up to two units in
+    the last place, each put right by its remainder."""
+    import random
+
+    import numpy as np
+
+    f = np.float32
+
+    def corrected(n, d, q):
+        r = n - q * d
+        return q - 1 if r < 0 else q + 1 if r >= d else q
+
+    rng = random.Random(5)
+    for _ in range(20000):
+        T = rng.choice([rng.randrange(1, 1 << 31), rng.randrange(1, 5000), (1 << 31) - 1])
+        W = rng.choice([1, 148, rng.randrange(1, 2561), 2560])
+        c = rng.choice([0, W, rng.randrange(0, W + 1)])
+        assert corrected(c * T, W, int(float(c * T) * (1.0 / W))) == c * T // W
+        t = rng.choice([0, T - 1, rng.randrange(0, T)])
+        n = (t + 1) * W - 1
+        for ulps in range(-2, 3):
+            q = f(f(n) / f(T)) * f(1 + ulps * 2.0 ** -23)
+            owner = corrected(n, T, int(q))
+            assert owner == n // T and owner * T // W <= t
