@@ -386,9 +386,9 @@ uint64_t oxide_decode_attention_workspace_bytes(uint64_t batch, uint64_t q_heads
                                                 uint64_t head_dim);
 /* Kernel choice of oxide_decode_attention_bf16 and, alike, of
  * oxide_decode_attention_q8_* (their other kernel is the warp-per-worker one;
- * the shapes their tcgen05 kernel takes: head_dim a multiple of 16 up to 128,
- * batch <= 1024, max_seq >= 128) (diagnostic; no reference counterpart): 0 (default) = the tcgen05 / TMA kernel wherever it applies
- * (sm_100, head_dim 128, q_heads / kv_heads in {1, 2, 4, 8}, batch <= 1024,
+ * the shapes their tcgen05 kernel takes: head_dim a multiple of 16, batch <=
+ * 1024, 16-byte aligned q and caches) (diagnostic; no reference counterpart):
+ * 0 (default) = the tcgen05 / TMA kernel wherever it applies (sm_100, head_dim 128, q_heads / kv_heads in {1, 2, 4, 8}, batch <= 1024,
  * max_seq >= 256), else the split-K mma.sync kernel; 1 = always the split-K
  * kernel; 2 = the tcgen05 kernel with its tile loads withheld, so that every
  * bounded wait in it runs out (about two seconds) and the launch ends with

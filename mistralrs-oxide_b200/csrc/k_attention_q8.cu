@@ -9,8 +9,7 @@
 //
 // Two kernels write partial results in one form (oxide_attn_q8.cuh) and
 // decode_attn_q8_combine_kernel merges them:
-//   k_attention_q8_tc.cu   head_dim a multiple of 16 up to 128, caches of at
-//                          least 128 positions: both products in int8 on
+//   k_attention_q8_tc.cu   head_dim a multiple of 16: both products in int8 on
 //                          tcgen05;
 //   here, any other shape  (head_dim up to 256, any group): a warp is a
 //                          worker and streams 32-key tiles.  Scores: lane =

@@ -4,11 +4,11 @@
 // Mathematics.  The cache's codes c, d are int8 as they lie in memory, so the
 // other operand of each product is written in int8 digits as well and the
 // products are exact integer sums:
-//   q of a head = (x) amax / Q_UNIT with |x| <= Q_UNIT = 8e6 integers, and
+//   q of a head = x u with integers |x| below 2^23 and u a power of two, and
 //   x = x0 + 256 x1 + 65536 x2 in balanced digits (-128 .. 127), so
-//   q . c = (x0 . c + 256 x1 . c + 65536 x2 . c) amax / Q_UNIT: the three digit
-//   rows are three columns of one product (each sum below 2^22, exact in f32),
-//   and q is held to 2^-23 of its largest element, as good as f32 sums;
+//   q . c = (x0 . c + 256 x1 . c + 65536 x2 . c) u: the three digit rows are
+//   three columns of one product (each sum at most 2^22, exact in f32), and q
+//   is held to 2^-23 of its largest element, as good as f32 sums;
 //   p_j vs_j (the softmax weight times the value block's scale) likewise, as
 //   integers against the largest of the tile, found in the log2 domain
 //   (t_j + log2 vs_j), so neither a far maximum in another tile nor blocks
@@ -18,13 +18,13 @@
 //
 // Work division as in k_attention_tc.cu (tiles of 128 keys laid end to end,
 // one CTA per SM, equal ranges); partials as in oxide_attn_q8.cuh, two halves
-// a CTA.  head_dim a multiple of 16 up to 128: the tile is 128 bytes wide and
-// TMA fills what lies past head_dim with zeros.
+// a CTA.  head_dim a multiple of 16: tiles are one or two halves of 128 bytes
+// wide (up to 128, up to 256), and TMA fills what lies past head_dim with zeros.
 //
 // CTA of 13 warps:
 //   warp 0      TMA producer: K and V tiles [128 keys x 128 bytes],
-//               128-byte swizzle, 6-stage ring (32 KB a stage: the bytes of
-//               half as many bf16 keys);
+//               128-byte swizzle, a ring of 192 KB: 6 stages of 32 KB, or 3 of
+//               64 KB with two halves;
 //   warp 1      TMEM owner and issuer of the scores' products,
 //                 S[128 keys x N] = K . X^T   (A = K, K-major; B = digits of q);
 //   warp 12     issuer of the outputs' products,
@@ -33,7 +33,10 @@
 //               N = 16 for up to 4 heads, 32 for 8 (M = 128 takes N in steps
 //               of 16).  One thread issuing both spent 2100 cycles a tile on
 //               waits and issue, twice what the loads allow;
-//   warp 2      the query heads' digits, one pair ahead;
+//   warp 2      the query heads' digits, one pair ahead, from raw bits loaded two
+//               pairs ahead.  (A second such warp gained nothing, nor did asking
+//               L2 for the queries four pairs early: 59.2 and 71.2 us where this
+//               takes 59.1, at 256 sequences of 200 keys, 32 heads.)
 //   warp 3      the tile prefix; then each tile's scales, ready for the softmax
 //               threads (the key scale, log2 of the value scale, masks), loaded
 //               two tiles ahead.  One scale for a lane's four keys wherever
@@ -42,7 +45,12 @@
 //   warps 4-7 and 8-11  two softmax groups that take the tiles in turn, each
 //               with its own S and O in TMEM, weights buffer and online state:
 //               one group's barriers and latencies hide behind the other's
-//               work.  Thread i = key i of S and dim i of O.
+//               work.  Thread i = key i of S and dim i of each half of O.
+// Measured (bf16 queries, 32 heads over 8, blocks of 64; time, and the codes'
+// rate of 6540 GB/s): 8 sequences of 1024 to 32768 keys 51.7 us (82 %), one of
+// 131072 keys 48.0 us (86 %); 8 of 8192 keys, head_dim 256, 49.5 us (83 %);
+// starting, joining the parts and the last tiles' way through the roles take 7
+// to 8 us whatever the lengths (one sequence of 100 keys: 7.6 us).
 // A group's buffers need few barriers: its O of tile k is read before its
 // weights of tile k + 1 are handed over, so that hand-over also says that O and
 // the weights buffer are free.
@@ -57,46 +65,51 @@
 
 namespace oxide {
 
-constexpr uint32_t QT_TK = 128, QT_DB = 128;  // keys a tile, bytes a row in shared memory
-constexpr int QT_STAGES = 6;
+constexpr uint32_t QT_TK = 128, QT_DB = 128;  // keys a tile, bytes a row of a tile half
 constexpr int QT_THREADS = 416;
 constexpr uint32_t QT_MAX_BATCH = 1024;
 // Maxima start here, not at -infinity: differences stay numbers, and a masked
 // score (-infinity) is a zero weight without being asked about.
 constexpr float QT_LOW = -3.0e38f;
 constexpr float Q_UNIT = 8.0e6f;  // below 0x7f7f7f = 8355711, the largest three balanced digits hold
-constexpr uint32_t QT_TMEM_COLS = 128, QT_TMEM_O = 64;  // S at 32 g, O at 64 + 32 g for group g
-constexpr uint32_t QT_TILE = QT_TK * QT_DB;       // 16 KB
-constexpr uint32_t QT_STAGE_BYTES = 2 * QT_TILE;  // K, V
-constexpr uint32_t QT_BBYTES = 32 * 128;          // a B operand: up to 32 rows of 128 bytes
-// shared memory map (offsets from a 1024-byte aligned base)
-constexpr uint32_t QT_OFF_Q = QT_STAGES * QT_STAGE_BYTES;                // 2 slots
-constexpr uint32_t QT_OFF_P = QT_OFF_Q + 2 * QT_BBYTES;                  // 2 groups
-constexpr uint32_t QT_OFF_PRE = QT_OFF_P + 2 * QT_BBYTES;
-constexpr uint32_t QT_OFF_SC = QT_OFF_PRE + (QT_MAX_BATCH + 8) * 4;      // a stage's keys: float2 [128]
-constexpr uint32_t QT_OFF_SQ = QT_OFF_SC + QT_STAGES * QT_TK * 8;        // [2][8] factors of the scores
-constexpr uint32_t QT_OFF_RED = QT_OFF_SQ + 2 * 8 * 4;                   // [2][4][16] each warp's tile maxima
-constexpr uint32_t QT_OFF_SUM = QT_OFF_RED + 2 * 4 * 16 * 4;             // [2][4][8] sums
-constexpr uint32_t QT_OFF_BAR = QT_OFF_SUM + 2 * 4 * 8 * 4;
-enum : int {
-    QB_FULL = 0,                      // [6] stage loaded (TMA bytes)
-    QB_EMPTY = QB_FULL + QT_STAGES,   // [6] stage consumed (MMA commit)
-    QB_CFULL = QB_EMPTY + QT_STAGES,  // [6] the stage's scales written (warp 3)
-    QB_QFULL = QB_CFULL + QT_STAGES,  // [2] digits of a pair's query heads written (warp 2)
-    QB_QEMPTY = QB_QFULL + 2,         // [2] read: MMA commit and the eight softmax warps
-    QB_SFULL = QB_QEMPTY + 2,         // [2] scores in TMEM (MMA commit)
-    QB_SEMPTY = QB_SFULL + 2,         // [2] scores read (4 warps)
-    QB_PFULL = QB_SEMPTY + 2,         // [2] weights written, O free (1 thread)
-    QB_OFULL = QB_PFULL + 2,          // [2] tile output in TMEM, weights read (MMA commit)
-    QB_DONE = QB_OFULL + 2,           // every product issued has completed
-    QB_COUNT = QB_DONE + 1
+constexpr uint32_t QT_TILE = QT_TK * QT_DB;  // 16 KB
+constexpr uint32_t QT_BBYTES = 32 * 128;     // a B operand: up to 32 rows of 128 bytes
+// Places of the kernel for DH halves of 128 bytes a row (head_dim up to 128, 256).
+template <int DH>
+struct QtMap {
+    static constexpr int STAGES = 6 / DH;
+    static constexpr uint32_t STAGE_BYTES = 2 * DH * QT_TILE;  // K, V
+    static constexpr uint32_t Q_BYTES = DH * QT_BBYTES;
+    // TMEM columns: S of group g at 32 g, its O (half x) at O + 32 (DH g + x)
+    static constexpr uint32_t TMEM_COLS = 128 * DH, O = 64;
+    // shared memory (offsets from a 1024-byte aligned base)
+    static constexpr uint32_t OFF_Q = STAGES * STAGE_BYTES;                  // 2 slots
+    static constexpr uint32_t OFF_P = OFF_Q + 2 * Q_BYTES;                   // 2 groups
+    static constexpr uint32_t OFF_PRE = OFF_P + 2 * QT_BBYTES;
+    static constexpr uint32_t OFF_SC = OFF_PRE + (QT_MAX_BATCH + 8) * 4;     // a stage's keys: float2 [128]
+    static constexpr uint32_t OFF_SQ = OFF_SC + STAGES * QT_TK * 8;          // [2][8] factors of the scores
+    static constexpr uint32_t OFF_RED = OFF_SQ + 2 * 8 * 4;                  // [2][4][16] each warp's tile maxima
+    static constexpr uint32_t OFF_SUM = OFF_RED + 2 * 4 * 16 * 4;            // [2][5][8] each warp's sums; the maxima
+    static constexpr uint32_t OFF_BAR = OFF_SUM + 2 * 5 * 8 * 4;
+    enum : int {
+        FULL = 0,                 // [stages] loaded (TMA bytes)
+        EMPTY = FULL + STAGES,    // [stages] consumed (MMA commit)
+        CFULL = EMPTY + STAGES,   // [stages] the tile's scales written (warp 3)
+        QFULL = CFULL + STAGES,   // [2] digits of a pair's query heads written (warp 2)
+        QEMPTY = QFULL + 2,       // [2] read: MMA commit and the eight softmax warps
+        SFULL = QEMPTY + 2,       // [2] scores in TMEM (MMA commit)
+        SEMPTY = SFULL + 2,       // [2] scores read (4 warps)
+        PFULL = SEMPTY + 2,       // [2] weights written, O free (1 thread)
+        OFULL = PFULL + 2,        // [2] tile output in TMEM, weights read (MMA commit)
+        DONE = OFULL + 2,         // every product issued has completed
+        COUNT = DONE + 1
+    };
+    static constexpr uint32_t OFF_MISC = OFF_BAR + ((COUNT + 1) & ~1) * 8;
+    static constexpr size_t SMEM = OFF_MISC + 48 + 1024;  // + alignment slack
 };
-constexpr uint32_t QT_OFF_MISC = QT_OFF_BAR + ((QB_COUNT + 1) & ~1) * 8;
-constexpr size_t QT_SMEM = QT_OFF_MISC + 48 + 1024;  // + alignment slack
-static_assert(QT_STAGES % 2 == 0, "a softmax group's stages repeat after half a ring");
-// Leaves room beside it for a CTA of the combine kernel (4.1 KB), which is
-// launched early and waits there.
-static_assert(QT_SMEM <= 221 * 1024, "shared memory of one CTA");
+// One half: room is left beside the CTA for one of the combine kernel (4.1 KB),
+// which is launched early and waits there.
+static_assert(QtMap<1>::SMEM <= 221 * 1024 && QtMap<2>::SMEM <= 227 * 1024, "shared memory of one CTA");
 static_assert(2 * 1024 <= Q8A_PARTS, "two parts a CTA fit the workspace");
 
 __device__ unsigned int g_device_status_q8;  // sticky failure flags, read by oxide_device_status
@@ -113,7 +126,7 @@ __device__ __forceinline__ void qt_load(uint32_t taddr, uint32_t (&v)[qt_cols<NR
     for (int i = 0; i < (int)qt_cols<NR>(); i += 8) tmem_ld8(taddr + i, v + i);
     tmem_wait_ld();
 }
-// Three digit sums as the number they spell (each sum is below 2^21 in
+// Three digit sums as the number they spell (each sum is at most 2^22 in
 // magnitude, so the lower two join in 32 bits).
 __device__ __forceinline__ float qt_spell(uint32_t d0, uint32_t d1, uint32_t d2) {
     return __fmaf_rn((float)(int)d2, 65536.0f, (float)((int)d1 * 256 + (int)d0));
@@ -134,47 +147,48 @@ __device__ __forceinline__ float qt_ex2(float t) {
     return y;
 }
 
-template <int NR>
+template <int NR, int DH>
 __global__ void __launch_bounds__(QT_THREADS, 1)
     decode_attn_q8_tc_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_constant__ CUtensorMap tmv,
                              Q8AttnArgs p, uint32_t withhold) {
     pdl_trigger();
+    typedef QtMap<DH> M;
     constexpr uint32_t N = qt_n<NR>();
     extern __shared__ __align__(1024) unsigned char smem_raw[];
     unsigned char* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
     const uint32_t sbase = smem_u32(smem);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    uint32_t* pre = reinterpret_cast<uint32_t*>(smem + QT_OFF_PRE);
-    float* sq = reinterpret_cast<float*>(smem + QT_OFF_SQ);
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + QT_OFF_MISC);
-    volatile int* abort = reinterpret_cast<volatile int*>(smem + QT_OFF_MISC + 4);
-    volatile int* consumed = reinterpret_cast<volatile int*>(smem + QT_OFF_MISC + 8);  // stages warp 1 waited for
-    uint32_t* begin = reinterpret_cast<uint32_t*>(smem + QT_OFF_MISC + 16);  // where this CTA's tiles begin: b, kvh, lt, tb
-    auto bar = [&](int i) { return sbase + QT_OFF_BAR + 8u * (uint32_t)i; };
+    uint32_t* pre = reinterpret_cast<uint32_t*>(smem + M::OFF_PRE);
+    float* sq = reinterpret_cast<float*>(smem + M::OFF_SQ);
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + M::OFF_MISC);
+    volatile int* abort = reinterpret_cast<volatile int*>(smem + M::OFF_MISC + 4);
+    volatile int* consumed = reinterpret_cast<volatile int*>(smem + M::OFF_MISC + 8);  // stages warp 1 waited for
+    uint32_t* begin = reinterpret_cast<uint32_t*>(smem + M::OFF_MISC + 16);  // where this CTA's tiles begin: b, kvh, lt, tb
+    auto bar = [&](int i) { return sbase + M::OFF_BAR + 8u * (uint32_t)i; };
 
     if (tid == 0) {
         *abort = 0;
         *consumed = 0;
-        for (int i = 0; i < QT_STAGES; ++i) {
-            mbar_init(bar(QB_FULL + i), 1);
-            mbar_init(bar(QB_EMPTY + i), 1);
-            mbar_init(bar(QB_CFULL + i), 1);
+        for (int i = 0; i < M::STAGES; ++i) {
+            mbar_init(bar(M::FULL + i), 1);
+            mbar_init(bar(M::EMPTY + i), 1);
+            mbar_init(bar(M::CFULL + i), 1);
         }
         for (int i = 0; i < 2; ++i) {
-            mbar_init(bar(QB_QFULL + i), 1);
-            mbar_init(bar(QB_QEMPTY + i), 9);
-            mbar_init(bar(QB_SFULL + i), 1);
-            mbar_init(bar(QB_SEMPTY + i), 4);
-            mbar_init(bar(QB_PFULL + i), 1);
-            mbar_init(bar(QB_OFULL + i), 1);
+            mbar_init(bar(M::QFULL + i), 1);
+            mbar_init(bar(M::QEMPTY + i), 9);
+            mbar_init(bar(M::SFULL + i), 1);
+            mbar_init(bar(M::SEMPTY + i), 4);
+            mbar_init(bar(M::PFULL + i), 1);
+            mbar_init(bar(M::OFULL + i), 1);
         }
-        mbar_init(bar(QB_DONE), 2);
+        mbar_init(bar(M::DONE), 2);
         mbar_init_fence();
         tma_prefetch_map(&tmk);
         tma_prefetch_map(&tmv);
     }
     if (warp == 1) {
-        tmem_alloc(smem_u32(tmem_slot), QT_TMEM_COLS);
+        tmem_alloc(smem_u32(tmem_slot), M::TMEM_COLS);
         tmem_relinquish();
     }
     pdl_wait();  // the previous kernel's writes (lengths, caches, queries) are visible
@@ -217,18 +231,21 @@ __global__ void __launch_bounds__(QT_THREADS, 1)
         uint32_t n = 0, s = 0, ph = 1;  // the stage and its phase
         if (!withhold) {
             for (; n < nt && !*abort; ++n) {
-                if (!warp_wait_all(bar(QB_EMPTY + s), ph, abort)) break;
+                if (!warp_wait_all(bar(M::EMPTY + s), ph, abort)) break;
                 const int z = (int)(w.b * p.kv_heads + (p.by_chunks.div(w.kvh)));
                 const int y = (int)(w.lt * QT_TK);
-                const uint32_t sd = sbase + s * QT_STAGE_BYTES;
+                const uint32_t sd = sbase + s * M::STAGE_BYTES;
                 if (leader) {
-                    mbar_arrive_expect_tx(bar(QB_FULL + s), QT_STAGE_BYTES);
-                    tma_load_3d(sd, &tmk, bar(QB_FULL + s), 0, y, z);
-                    tma_load_3d(sd + QT_TILE, &tmv, bar(QB_FULL + s), 0, y, z);
+                    mbar_arrive_expect_tx(bar(M::FULL + s), M::STAGE_BYTES);
+#pragma unroll
+                    for (int x = 0; x < DH; ++x) tma_load_3d(sd + x * QT_TILE, &tmk, bar(M::FULL + s), x * QT_DB, y, z);
+#pragma unroll
+                    for (int x = 0; x < DH; ++x)
+                        tma_load_3d(sd + (DH + x) * QT_TILE, &tmv, bar(M::FULL + s), x * QT_DB, y, z);
                 }
                 __syncwarp();
                 w.next();
-                if (++s == QT_STAGES) {
+                if (++s == M::STAGES) {
                     s = 0;
                     ph ^= 1u;
                 }
@@ -238,7 +255,7 @@ __global__ void __launch_bounds__(QT_THREADS, 1)
         // land before the CTA exits.
         if (leader && *abort) {
             for (uint32_t i = (uint32_t)*consumed; i < n; ++i)
-                tc_wait_drain(bar(QB_FULL + i % QT_STAGES), (i / QT_STAGES) & 1u);
+                tc_wait_drain(bar(M::FULL + i % M::STAGES), (i / M::STAGES) & 1u);
         }
         __syncwarp();
     } else if (warp == 1) {
@@ -246,7 +263,7 @@ __global__ void __launch_bounds__(QT_THREADS, 1)
         constexpr uint32_t IDESC_S = umma_idesc_s8(128, N, false, false);
         const bool leader = elect_one();
         const uint64_t kd = umma_desc(sbase, 16, 1024, UMMA_SWIZZLE_128B);
-        const uint64_t qd = umma_desc(sbase + QT_OFF_Q, 16, 1024, UMMA_SWIZZLE_128B);
+        const uint64_t qd = umma_desc(sbase + M::OFF_Q, 16, 1024, UMMA_SWIZZLE_128B);
         uint32_t left = 0, q = 0, s = 0, ph = 0;  // tiles left of the pair, its number, the stage and its phase
         for (uint32_t n = 0; n < nt; ++n) {
             const uint32_t g = n & 1u;
@@ -254,115 +271,148 @@ __global__ void __launch_bounds__(QT_THREADS, 1)
                 left = min(w.tb - w.lt, nt - n);
                 w.lt += left - 1;
                 w.next();
-                if (!warp_wait_all(bar(QB_QFULL + (q & 1u)), (q >> 1) & 1u, abort)) break;
+                if (!warp_wait_all(bar(M::QFULL + (q & 1u)), (q >> 1) & 1u, abort)) break;
             }
-            if (!warp_wait_all(bar(QB_FULL + s), ph, abort)) break;
+            if (!warp_wait_all(bar(M::FULL + s), ph, abort)) break;
             if (leader) *consumed = (int)n + 1;
-            if (!warp_wait_all(bar(QB_SEMPTY + g), ((n >> 1) & 1u) ^ 1u, abort)) break;
+            if (!warp_wait_all(bar(M::SEMPTY + g), ((n >> 1) & 1u) ^ 1u, abort)) break;
             tc_fence_after();
-            const uint64_t ka = kd + s * (QT_STAGE_BYTES >> 4), qa = qd + (q & 1u) * (QT_BBYTES >> 4);
+            const uint64_t ka = kd + s * (M::STAGE_BYTES >> 4), qa = qd + (q & 1u) * (M::Q_BYTES >> 4);
             --left;
             if (leader) {
 #pragma unroll
-                for (uint32_t kk = 0; kk < 4; ++kk)  // 32 dims (32 bytes) a product
-                    umma_s8(tmem + g * 32, ka + kk * 2, qa + kk * 2, IDESC_S, kk > 0);
-                umma_commit(bar(QB_SFULL + g));
-                if (left == 0) umma_commit(bar(QB_QEMPTY + (q & 1u)));  // the pair's last product that reads its digits
+                for (uint32_t kk = 0; kk < 4 * DH; ++kk)  // 32 dims (32 bytes) a product, four products a half
+                    umma_s8(tmem + g * 32, ka + (kk >> 2) * (QT_TILE >> 4) + (kk & 3) * 2,
+                            qa + (kk >> 2) * (QT_BBYTES >> 4) + (kk & 3) * 2, IDESC_S, kk > 0);
+                umma_commit(bar(M::SFULL + g));
+                if (left == 0) umma_commit(bar(M::QEMPTY + (q & 1u)));  // the pair's last product that reads its digits
             }
             __syncwarp();
             if (left == 0) ++q;
-            if (++s == QT_STAGES) {
+            if (++s == M::STAGES) {
                 s = 0;
                 ph ^= 1u;
             }
         }
-        if (leader) umma_commit(bar(QB_DONE));
+        if (leader) umma_commit(bar(M::DONE));
         __syncwarp();
     } else if (warp == 12) {
         // ---------------- issuer of the outputs ----------------
         constexpr uint32_t IDESC_O = umma_idesc_s8(128, N, true, false);
         const bool leader = elect_one();
-        const uint64_t vd = umma_desc(sbase + QT_TILE, 16, 1024, UMMA_SWIZZLE_128B);
-        const uint64_t pd = umma_desc(sbase + QT_OFF_P, 128, 1024, UMMA_SWIZZLE_NONE);
+        const uint64_t vd = umma_desc(sbase + DH * QT_TILE, 16, 1024, UMMA_SWIZZLE_128B);
+        const uint64_t pd = umma_desc(sbase + M::OFF_P, 128, 1024, UMMA_SWIZZLE_NONE);
         uint32_t s = 0;
         for (uint32_t n = 0; n < nt; ++n) {
             const uint32_t g = n & 1u;
-            if (!warp_wait_all(bar(QB_PFULL + g), (n >> 1) & 1u, abort)) break;
+            if (!warp_wait_all(bar(M::PFULL + g), (n >> 1) & 1u, abort)) break;
             tc_fence_after();
-            const uint64_t va = vd + s * (QT_STAGE_BYTES >> 4), pa = pd + g * (QT_BBYTES >> 4);
+            const uint64_t va = vd + s * (M::STAGE_BYTES >> 4), pa = pd + g * (QT_BBYTES >> 4);
             if (leader) {
 #pragma unroll
-                for (uint32_t kk = 0; kk < 4; ++kk)  // 32 keys a product: 4096 bytes of V, 256 of the weights
-                    umma_s8(tmem + QT_TMEM_O + g * 32, va + kk * 256, pa + kk * 16, IDESC_O, kk > 0);
-                umma_commit(bar(QB_OFULL + g));
-                umma_commit(bar(QB_EMPTY + s));
+                for (uint32_t kk = 0; kk < 4 * DH; ++kk)  // 32 keys a product: 4096 bytes of a V half, 256 of the weights
+                    umma_s8(tmem + M::O + (g * DH + (kk >> 2)) * 32, va + (kk >> 2) * (QT_TILE >> 4) + (kk & 3) * 256,
+                            pa + (kk & 3) * 16, IDESC_O, (kk & 3) > 0);
+                umma_commit(bar(M::OFULL + g));
+                umma_commit(bar(M::EMPTY + s));
             }
             __syncwarp();
-            if (++s == QT_STAGES) s = 0;
+            if (++s == M::STAGES) s = 0;
         }
         if (leader) {  // every product issued has completed before TMEM is freed
-            umma_commit(bar(QB_DONE));
-            if (!tc_wait_drain(bar(QB_DONE), 0)) *abort = 1;
+            umma_commit(bar(M::DONE));
+            if (!tc_wait_drain(bar(M::DONE), 0)) *abort = 1;
         }
         __syncwarp();
     } else if (warp == 2) {
         // ---------------- digits of the query heads ----------------
-        for (uint32_t n = 0, q = 0; n < nt; ++q) {
-            const uint32_t slot = q & 1u, kvh = p.by_chunks.div(w.kvh), h0 = (w.kvh - kvh * p.chunks) * NR;
-            const uint32_t nh = min(p.rep - h0, (uint32_t)NR);
-            const uint64_t row = (uint64_t)w.b * p.q_heads + kvh * p.rep + h0;
-            float x[NR][4];
+        // Dims 4 lane .. 4 lane + 3 (of each half); as a head is done, the next
+        // pair's is loaded, and stays as it lies in memory until its turn: a
+        // conversion beside the load made the warp wait for each head, some 5000
+        // cycles while HBM is busy (53.9 instead of 51.7 us at 8 sequences of 1024
+        // to 32768 keys, 72 instead of 59 at 256 of 200).
+        uint2 x[NR][2 * DH];
+        uint64_t row = 0;  // of the pair loaded next, and its heads (0: no more pairs)
+        uint32_t nh = 0;
+        auto place = [&](bool more) {
+            const uint32_t kvh = p.by_chunks.div(w.kvh), h0 = (w.kvh - kvh * p.chunks) * NR;
+            row = (uint64_t)w.b * p.q_heads + kvh * p.rep + h0;
+            nh = more ? p.rep - h0 : 0;
+        };
+        auto load = [&](uint32_t h, uint2 (&v)[2 * DH]) {
 #pragma unroll
-            for (int h = 0; h < NR; ++h) {
-#pragma unroll
-                for (int e = 0; e < 4; ++e) x[h][e] = 0.0f;
-                if ((uint32_t)h < nh && 4u * lane < p.head_dim) {
-                    const uint64_t at = (row + h) * p.head_dim + 4u * lane;
-                    if (p.q_bf16) {
-                        const uint2 v = __ldg(reinterpret_cast<const uint2*>(static_cast<const bf16_t*>(p.q) + at));
-                        x[h][0] = bf16_lo(v.x);
-                        x[h][1] = bf16_hi(v.x);
-                        x[h][2] = bf16_lo(v.y);
-                        x[h][3] = bf16_hi(v.y);
-                    } else {
-                        const float4 v = __ldg(reinterpret_cast<const float4*>(static_cast<const float*>(p.q) + at));
-                        x[h][0] = v.x;
-                        x[h][1] = v.y;
-                        x[h][2] = v.z;
-                        x[h][3] = v.w;
-                    }
-                }
+            for (int half = 0; half < DH; ++half) {
+                const uint32_t d = 4u * lane + 128u * half;
+                const bool there = h < nh && d < p.head_dim;
+                const uint2* at = reinterpret_cast<const uint2*>(static_cast<const char*>(p.q) +
+                                                                 ((row + h) * p.head_dim + d) * (p.q_bf16 ? 2 : 4));
+                v[2 * half] = v[2 * half + 1] = make_uint2(0, 0);
+                if (there) v[2 * half] = __ldg(at);
+                if (there && !p.q_bf16) v[2 * half + 1] = __ldg(at + 1);
             }
-            if (!warp_wait(bar(QB_QEMPTY + slot), ((q >> 1) & 1u) ^ 1u, abort)) break;
-#pragma unroll
-            for (int h = 0; h < NR; ++h) {
-                uint32_t a = 0;
-#pragma unroll
-                for (int e = 0; e < 4; ++e) a = max(a, q8_abs_bits(x[h][e]));
-                a = q8_warp_max(a);
-                const bool bad = a >= Q8_INF, tiny = a < 0x21800000u;  // not finite; below 2^-60
-                const float up = tiny ? 0x1p80f : 1.0f, amax = fmul(__uint_as_float(a), up);
-                const float inv = bad || a == 0 ? 0.0f : fdiv(Q_UNIT, amax);
-                uint32_t d[4];
-#pragma unroll
-                for (int e = 0; e < 4; ++e) d[e] = qt_digits(bad ? 0.0f : fmul(fmul(x[h][e], up), inv));
-#pragma unroll
-                for (int g = 0; g < 3; ++g) {
-                    const uint32_t r = g * NR + h;
-                    *reinterpret_cast<uint32_t*>(smem + QT_OFF_Q + slot * QT_BBYTES + r * 128 +
-                                                 (((lane >> 2) ^ (r & 7)) << 4) + ((lane & 3) << 2)) =
-                        q8_pack4(d[0] >> (8 * g), d[1] >> (8 * g), d[2] >> (8 * g), d[3] >> (8 * g));
-                }
-                if (lane == 0)
-                    sq[slot * 8 + h] = bad ? q8_nan() : fmul(fmul(fdiv(amax, Q_UNIT), p.c1), tiny ? 0x1p-80f : 1.0f);
-            }
-            fence_async_smem();  // the digits are visible to the tensor core
-            __syncwarp();
-            if (lane == 0) mbar_arrive(bar(QB_QFULL + slot));
+        };
+        auto value = [&](const uint2 (&v)[2 * DH], int i) {  // element i of the lane's four (of each half)
+            const uint2 lo = v[i >> 2 << 1], hi = v[(i >> 2 << 1) + 1];
+            const uint32_t b = (i & 2) ? lo.y : lo.x, f = (i & 2) ? ((i & 1) ? hi.y : hi.x) : ((i & 1) ? lo.y : lo.x);
+            return p.q_bf16 ? ((i & 1) ? bf16_hi(b) : bf16_lo(b)) : __uint_as_float(f);
+        };
+        uint32_t slot = 0;
+        uint32_t n = 0;
+        auto step = [&]() {
+            if (n >= nt) return;
             const uint32_t cnt = min(w.tb - w.lt, nt - n);
             n += cnt;
             w.lt += cnt - 1;
             w.next();
+        };
+        place(n < nt);
+#pragma unroll
+        for (int h = 0; h < NR; ++h) load(h, x[h]);
+        for (uint32_t ph = 1; n < nt; ph ^= slot, slot ^= 1u) {
+            step();
+            if (!warp_wait_all(bar(M::QEMPTY + slot), ph, abort)) break;
+            unsigned char* out = smem + M::OFF_Q + slot * M::Q_BYTES;
+            place(n < nt);
+#pragma unroll
+            for (int h = 0; h < NR; ++h) {
+                uint32_t a = 0;
+                float u[4 * DH];
+#pragma unroll
+                for (int e = 0; e < 4 * DH; ++e) {
+                    u[e] = value(x[h], e);
+                    a = max(a, q8_abs_bits(u[e]));
+                }
+                a = q8_warp_max(a);
+                // The unit is a power of two: 2^22 of them (2^21 where the
+                // largest element would pass three digits) reach from 2^e to
+                // the largest element, 2^e <= amax < 2^(e + 1).  Elements below
+                // 2^-60 are brought up first.
+                const bool bad = a >= Q8_INF, tiny = a < 0x21800000u;  // not finite; below 2^-60
+                const float up = tiny ? 0x1p80f : 1.0f, amax = fmul(__uint_as_float(a), up);
+                const uint32_t e = __float_as_uint(amax) & 0x7f800000u;
+                const uint32_t k = amax <= fmul(__uint_as_float(e), 1.992f) ? 22u : 21u;
+                const float inv = bad || a == 0 ? 0.0f : __uint_as_float(((254u + k) << 23) - e);
+                if (lane == 0)
+                    sq[slot * 8 + h] = bad ? q8_nan()
+                                           : (a == 0 ? 0.0f : fmul(fmul(__uint_as_float(e - (k << 23)), p.c1), tiny ? 0x1p-80f : 1.0f));
+#pragma unroll
+                for (int half = 0; half < DH; ++half) {
+                    uint32_t d[4];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) d[i] = qt_digits(bad ? 0.0f : fmul(fmul(u[4 * half + i], up), inv));
+#pragma unroll
+                    for (int g = 0; g < 3; ++g) {
+                        const uint32_t r = g * NR + h;
+                        *reinterpret_cast<uint32_t*>(out + half * QT_BBYTES + r * 128 + (((lane >> 2) ^ (r & 7)) << 4) +
+                                                     ((lane & 3) << 2)) =
+                            q8_pack4(d[0] >> (8 * g), d[1] >> (8 * g), d[2] >> (8 * g), d[3] >> (8 * g));
+                    }
+                }
+                load(h, x[h]);
+            }
+            fence_async_smem();  // the digits are visible to the tensor core
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bar(M::QFULL + slot));
         }
     } else if (warp == 3) {
         // ---------------- scales of the tiles: keys 4 lane .. 4 lane + 3 ----------------
@@ -424,13 +474,13 @@ __global__ void __launch_bounds__(QT_THREADS, 1)
                     if (4 * lane + i >= x.live) r[i] = make_float2(0.0f, INFINITY);
             }
             // the output product of the stage's last tile came after its scales were read
-            if (!warp_wait_all(bar(QB_EMPTY + s), ph, abort)) return false;
-            float4* out = reinterpret_cast<float4*>(smem + QT_OFF_SC) + (s * QT_TK + 4 * lane) / 2;
+            if (!warp_wait_all(bar(M::EMPTY + s), ph, abort)) return false;
+            float4* out = reinterpret_cast<float4*>(smem + M::OFF_SC) + (s * QT_TK + 4 * lane) / 2;
             out[0] = make_float4(r[0].x, r[0].y, r[1].x, r[1].y);
             out[1] = make_float4(r[2].x, r[2].y, r[3].x, r[3].y);
             __syncwarp();
-            if (lane == 0) mbar_arrive(bar(QB_CFULL + s));
-            if (++s == QT_STAGES) {
+            if (lane == 0) mbar_arrive(bar(M::CFULL + s));
+            if (++s == M::STAGES) {
                 s = 0;
                 ph ^= 1u;
             }
@@ -445,57 +495,62 @@ __global__ void __launch_bounds__(QT_THREADS, 1)
             if (n + 1 >= nt || !put(b)) break;
             load(b);
         }
-    } else if (warp >= 4) {
+    } else if (warp < 12) {
         // ---------------- softmax and epilogue: group g takes tiles n = g mod 2 ----------------
         const uint32_t g = (uint32_t)(warp >> 2) - 1, q4 = (uint32_t)(warp & 3);
         const uint32_t L = q4 * 32 + (uint32_t)lane;  // key of the S tile, dim of the O tile
-        const uint32_t s_tmem = tmem + ((q4 * 32u) << 16) + g * 32, o_tmem = s_tmem + QT_TMEM_O;
+        const uint32_t s_tmem = tmem + ((q4 * 32u) << 16) + g * 32, o_tmem = tmem + ((q4 * 32u) << 16) + M::O + g * DH * 32;
         const int nbar = 1 + (int)g;
-        float* red = reinterpret_cast<float*>(smem + QT_OFF_RED) + g * 64;   // [4][16]
-        float* lsum = reinterpret_cast<float*>(smem + QT_OFF_SUM) + g * 32;  // [4][8]
-        unsigned char* pt = smem + QT_OFF_P + g * QT_BBYTES;
+        float* red = reinterpret_cast<float*>(smem + M::OFF_RED) + g * 64;   // [4][16]
+        float* lsum = reinterpret_cast<float*>(smem + M::OFF_SUM) + g * 40;  // [4][8] sums of a finished pair, [8] its maxima
+        unsigned char* pt = smem + M::OFF_P + g * QT_BBYTES;
         // m, l: online softmax of the scores; wm, acc: the same for the
         // weights times scales; corr, tf: factors of the output not yet read
-        float m[NR], l[NR], wm[NR], acc[NR], corr[NR], tf[NR];
-        bool fail = false, pending = false;
+        float m[NR], l[NR], wm[NR], acc[DH][NR], corr[NR], tf[NR];
+        bool fail = false;
+#pragma unroll
+        for (int h = 0; h < NR; ++h) corr[h] = tf[h] = 0.0f;
 
-        const float2* scales = reinterpret_cast<const float2*>(smem + QT_OFF_SC) + L;
+        const float2* scales = reinterpret_cast<const float2*>(smem + M::OFF_SC) + L;
         uint32_t st = g, ph = 0, k = 0;  // the stage and its phase, and the number, of this group's next tile
         auto epilogue = [&](uint32_t k) {  // add the output of this group's tile k
-            const bool ok = warp_wait_all(bar(QB_OFULL + g), k & 1u, abort);
+            const bool ok = warp_wait_all(bar(M::OFULL + g), k & 1u, abort);
             fail |= !ok;
             if (!ok) return;
             tc_fence_after();
-            uint32_t o[qt_cols<NR>()];
-            qt_load<NR>(o_tmem, o);
-            tc_fence_before();
 #pragma unroll
-            for (int h = 0; h < NR; ++h)
-                acc[h] = __fmaf_rn(acc[h], corr[h], fmul(qt_spell(o[h], o[NR + h], o[2 * NR + h]), tf[h]));
+            for (int x = 0; x < DH; ++x) {
+                uint32_t o[qt_cols<NR>()];
+                qt_load<NR>(o_tmem + 32 * x, o);
+#pragma unroll
+                for (int h = 0; h < NR; ++h)
+                    acc[x][h] = __fmaf_rn(acc[x][h], corr[h], fmul(qt_spell(o[h], o[NR + h], o[2 * NR + h]), tf[h]));
+            }
+            tc_fence_before();
         };
-
         bool dead = false;
         for (uint32_t n = 0, q = 0; n < nt && !dead; ++q) {
             const uint32_t cnt = min(w.tb - w.lt, nt - n), j0 = (n ^ g) & 1u;
             // every warp waits for the digits, also of a pair without a tile
             // for it: its arrival below then belongs to this use of the slot
-            fail |= !warp_wait_all(bar(QB_QFULL + (q & 1u)), (q >> 1) & 1u, abort);
+            fail |= !warp_wait_all(bar(M::QFULL + (q & 1u)), (q >> 1) & 1u, abort);
             float f[NR];
 #pragma unroll
             for (int h = 0; h < NR; ++h) {
                 f[h] = sq[(q & 1u) * 8 + h];
                 m[h] = wm[h] = QT_LOW;
-                l[h] = acc[h] = 0.0f;
+                l[h] = 0.0f;
+#pragma unroll
+                for (int x = 0; x < DH; ++x) acc[x][h] = 0.0f;
             }
             __syncwarp();
-            if (lane == 0) mbar_arrive(bar(QB_QEMPTY + (q & 1u)));
-            pending = false;
+            if (lane == 0) mbar_arrive(bar(M::QEMPTY + (q & 1u)));
             for (uint32_t j = j0; j < cnt; j += 2) {
                 float t[NR], tv[NR];
-                bool ok = warp_wait_all(bar(QB_CFULL + st), ph, abort);
+                bool ok = warp_wait_all(bar(M::CFULL + st), ph, abort);
                 const float2 sc = scales[st * QT_TK];  // key scale; log2 of the value scale, or the mark of a masked key
                 const float mask = sc.y == INFINITY ? -INFINITY : 0.0f, lv = sc.y == INFINITY ? 0.0f : sc.y;
-                ok = warp_wait_all(bar(QB_SFULL + g), k & 1u, abort) && ok;
+                ok = warp_wait_all(bar(M::SFULL + g), k & 1u, abort) && ok;
                 fail |= !ok;
                 if (ok) {
                     tc_fence_after();
@@ -503,7 +558,7 @@ __global__ void __launch_bounds__(QT_THREADS, 1)
                     qt_load<NR>(s_tmem, v);
                     tc_fence_before();
                     __syncwarp();
-                    if (lane == 0) mbar_arrive(bar(QB_SEMPTY + g));
+                    if (lane == 0) mbar_arrive(bar(M::SEMPTY + g));
 #pragma unroll
                     for (int h = 0; h < NR; ++h) {
                         t[h] = __fmaf_rn(qt_spell(v[h], v[NR + h], v[2 * NR + h]), fmul(sc.x, f[h]), mask);
@@ -521,7 +576,7 @@ __global__ void __launch_bounds__(QT_THREADS, 1)
                         red[q4 * 16 + 8 + h] = b;
                     }
                 }
-                if (pending) epilogue(k - 1);  // its product has run meanwhile; the weights buffer and O are free after it
+                if (j != j0) epilogue(k - 1);  // its product has run meanwhile; the weights buffer and O are free after it
                 nbar_sync128(nbar);            // the four warps' maxima are in red
                 float mn[NR], wt[NR], wn[NR];
                 bool moved = false;
@@ -560,12 +615,11 @@ __global__ void __launch_bounds__(QT_THREADS, 1)
                     dead = true;
                     break;
                 }
-                if ((tid & 127) == 0) mbar_arrive(bar(QB_PFULL + g));  // every thread has written its weights and read O
-                pending = true;
+                if ((tid & 127) == 0) mbar_arrive(bar(M::PFULL + g));  // every thread has written its weights and read O
                 ++k;
                 st += 2;
-                if (st >= QT_STAGES) {
-                    st -= QT_STAGES;
+                if (st >= M::STAGES) {
+                    st -= M::STAGES;
                     ph ^= 1u;
                 }
             }
@@ -576,24 +630,25 @@ __global__ void __launch_bounds__(QT_THREADS, 1)
                 for (int h = 0; h < NR; ++h) {
                     const float x = warp_sum(l[h]);
                     if (lane == 0) lsum[q4 * 8 + h] = x;
-                }
-                if (nbar_or128(fail, nbar)) {
-                    dead = true;
-                    break;
+                    if (L == 0) lsum[32 + h] = m[h];
                 }
                 const uint64_t part = ((uint64_t)blockIdx.x + (uint64_t)w.b * heads + w.kvh) * 2 + g;
                 const uint32_t nh = min(p.rep - (w.kvh - p.by_chunks.div(w.kvh) * p.chunks) * NR, (uint32_t)NR);
 #pragma unroll
                 for (int h = 0; h < NR; ++h) {
-                    if ((uint32_t)h >= nh) continue;
-                    const uint64_t slot = part * NR + h;
-                    if (L < p.head_dim)
-                        p.part_o[slot * p.head_dim + L] =
-                            fmul(acc[h], ex2_approx(fsub(wm[h], m[h])));
-                    if (L == 0) {
-                        p.part_ml[slot * 2] = m[h];
-                        p.part_ml[slot * 2 + 1] = fadd(fadd(lsum[h], lsum[8 + h]), fadd(lsum[16 + h], lsum[24 + h]));
-                    }
+                    const float f = ex2_approx(fsub(wm[h], m[h]));
+#pragma unroll
+                    for (int x = 0; x < DH; ++x)
+                        if ((uint32_t)h < nh && L + 128 * x < p.head_dim)
+                            p.part_o[(part * NR + h) * p.head_dim + L + 128 * x] = fmul(acc[x][h], f);
+                }
+                if (nbar_or128(fail, nbar)) {
+                    dead = true;
+                    break;
+                }
+                if (L < nh) {
+                    p.part_ml[(part * NR + L) * 2] = lsum[32 + L];
+                    p.part_ml[(part * NR + L) * 2 + 1] = fadd(fadd(lsum[L], lsum[8 + L]), fadd(lsum[16 + L], lsum[24 + L]));
                 }
                 // lsum is written again behind the next tile's barriers
             }
@@ -607,7 +662,7 @@ __global__ void __launch_bounds__(QT_THREADS, 1)
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    if (warp == 1) tmem_dealloc(tmem, QT_TMEM_COLS);
+    if (warp == 1) tmem_dealloc(tmem, M::TMEM_COLS);
     if (tid == 0 && *abort) {
         atomicOr(p.err, 1u);
         atomicOr(&g_device_status_q8, OXIDE_DEVICE_WAIT_TIMEOUT);
@@ -635,18 +690,30 @@ static bool qt_map(CUtensorMap* m, const void* base, uint64_t heads, uint64_t ma
 
 bool tc_enabled();  // an sm_100 device, and not switched off (k_attention_tc.cu)
 
-template <int NR>
+template <int NR, int DH>
 static cudaError_t qt_launch(const CUtensorMap& mk, const CUtensorMap& mv, const Q8AttnArgs& a, bool withhold,
                              cudaStream_t st) {
-    auto kern = decode_attn_q8_tc_kernel<NR>;
-    if (!ensure_dyn_smem(reinterpret_cast<const void*>(kern), QT_SMEM)) return cudaErrorInvalidConfiguration;
-    return launch_k(kern, a.workers, QT_THREADS, QT_SMEM, st, mk, mv, a, withhold ? 1u : 0u);
+    auto kern = decode_attn_q8_tc_kernel<NR, DH>;
+    constexpr size_t smem = QtMap<DH>::SMEM;
+    if (!ensure_dyn_smem(reinterpret_cast<const void*>(kern), smem)) return cudaErrorInvalidConfiguration;
+    return launch_k(kern, a.workers, QT_THREADS, smem, st, mk, mv, a, withhold ? 1u : 0u);
+}
+
+template <int DH>
+static cudaError_t qt_launch_nr(const CUtensorMap& mk, const CUtensorMap& mv, const Q8AttnArgs& a, bool withhold,
+                                cudaStream_t st) {
+    switch (a.nr) {
+        case 1: return qt_launch<1, DH>(mk, mv, a, withhold, st);
+        case 2: return qt_launch<2, DH>(mk, mv, a, withhold, st);
+        case 4: return qt_launch<4, DH>(mk, mv, a, withhold, st);
+        default: return qt_launch<8, DH>(mk, mv, a, withhold, st);
+    }
 }
 
 cudaError_t decode_attention_q8_tc(Q8AttnArgs& a, bool withhold, cudaStream_t st, bool* used) {
     *used = false;
-    // head_dim: rows of whole 16-byte units (TMA strides), at most one 128-byte row.
-    if (!tc_enabled() || a.head_dim % 16 != 0 || a.head_dim > QT_DB || a.batch > QT_MAX_BATCH || a.max_seq < QT_TK ||
+    // head_dim: rows of whole 16-byte units (TMA strides), at most two 128-byte halves.
+    if (!tc_enabled() || a.head_dim % 16 != 0 || a.head_dim > 2 * QT_DB || a.batch > QT_MAX_BATCH ||
         !aligned16(a.kc) || !aligned16(a.vc) || !aligned16(a.q))
         return cudaSuccess;
     const uint64_t pairs = (uint64_t)a.batch * a.kv_heads, tiles = pairs * a.chunks * ((a.max_seq + QT_TK - 1) / QT_TK);
@@ -660,12 +727,7 @@ cudaError_t decode_attention_q8_tc(Q8AttnArgs& a, bool withhold, cudaStream_t st
     a.inv_workers = 1.0 / a.workers;
     a.halves = 2;
     *used = true;
-    switch (a.nr) {
-        case 1: return qt_launch<1>(mk, mv, a, withhold, st);
-        case 2: return qt_launch<2>(mk, mv, a, withhold, st);
-        case 4: return qt_launch<4>(mk, mv, a, withhold, st);
-        default: return qt_launch<8>(mk, mv, a, withhold, st);
-    }
+    return a.head_dim <= QT_DB ? qt_launch_nr<1>(mk, mv, a, withhold, st) : qt_launch_nr<2>(mk, mv, a, withhold, st);
 }
 
 int device_status_q8(int reset, uint32_t* flags) {

@@ -68,7 +68,11 @@ def values(codes, scales, block):
     return codes.to(F64) * per
 
 
-GRID = 0.5 / 8.0e6  # half a step of the tensor-core kernel's integers
+# Half a step of the tensor-core kernel's integers: of the weights (1 / 8e6 of the
+# largest), and of the queries.  Those count units 2^(e - 22) where the head's
+# largest element lies in [2^e, 1.992 2^e], else 2^(e - 21): half a unit is at
+# most 2^-23 of it either way (2^(e - 22) / (1.992 2^e) < 2^-22.99).
+GRID, GRID_Q = 0.5 / 8.0e6, 2.0 ** -22.99
 
 
 def attend(q, kc, vc, ks, vs, lens, block, scale):
@@ -77,9 +81,8 @@ def attend(q, kc, vc, ks, vs, lens, block, scale):
     u = 2^-24 a rounding.
     Scores sum head_dim products and take eight more roundings (the factors, the
     log2(e) factor, the difference from the maximum), each at most u of
-    sum |q k| scale.  The tensor-core kernel writes q in integers of 1 / 8e6 of
-    the head's largest element, so a score is off by GRID max|q| sum |k| scale
-    more.  Both act on numerator and denominator: twice, relative to sum p |v|.
+    sum |q k| scale.  The tensor-core kernel writes q in integers, so a score is
+    off by GRID_Q max|q| sum |k| scale more.  Both act on numerator and denominator: twice, relative to sum p |v|.
     Weights: three base-2 functions (2^-22 each) and 16 roundings in the sums of
     the parts and the quotient, again twice.  And the kernel writes p vs of a
     tile of 128 keys in integers of 1 / 8e6 of the tile's largest: an output is
@@ -102,7 +105,7 @@ def attend(q, kc, vc, ks, vs, lens, block, scale):
         one = p @ v.abs()
         size = (qi.abs() @ k.abs().transpose(1, 2)).amax(-1, keepdim=True) * abs(scale)
         wide = qi.abs().amax(-1, keepdim=True) * k.abs().sum(-1).amax(-1)[:, None, None] * abs(scale)
-        t = one * (2 * ((d + 8) * u * size + GRID * wide) + 2 * (3 * 2.0 ** -22 + 16 * u))
+        t = one * (2 * ((d + 8) * u * size + GRID_Q * wide) + 2 * (3 * 2.0 ** -22 + 16 * u))
         pv = p * vs[i, :, :nb].to(F64).repeat_interleave(block, 1)[:, None, :n]
         for j in range(0, n, 128):
             top = pv[:, :, j:j + 128].amax(-1, keepdim=True)

@@ -83,7 +83,18 @@ def test_work_division(cuda, hq, hkv, d, b, m):
     _run(case, 32, _lens(cuda, lens))
 
 
-@pytest.mark.parametrize("hq,hkv,d", [(8, 2, 128), (2, 2, 128), (16, 2, 128), (6, 2, 80), (3, 3, 33)])
+@pytest.mark.parametrize("hq,hkv,d", [(12, 3, 128), (20, 2, 128), (8, 2, 256), (2, 2, 176)])
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_many_short_sequences(cuda, hq, hkv, d, dtype):
+    """Several sequences to a worker, none, one and two tiles long, in a cache of
+    less than two tiles; the query heads change with every one of them."""
+    case = _case(cuda, 500, hq, hkv, d, 200, 16, dtype)
+    _run(case, 16, _lens(cuda, [(i * 83) % 201 for i in range(500)]))
+    case = _case(cuda, 400, hq, hkv, d, 7, 4, dtype)
+    _run(case, 4, _lens(cuda, [i % 8 for i in range(400)]))
+
+
+@pytest.mark.parametrize("hq,hkv,d", [(8, 2, 128), (2, 2, 128), (16, 2, 128), (6, 2, 80), (3, 3, 33), (8, 2, 256)])
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
 def test_anything_behind_the_length(cuda, hq, hkv, d, dtype):
     """Codes and scales behind a sequence's end may hold anything, -128 and NaN
@@ -99,7 +110,7 @@ def test_anything_behind_the_length(cuda, hq, hkv, d, dtype):
     _run([*case[:3], *[torch.nan_to_num(s, nan=0.0, posinf=0.0) for s in case[3:]]], block, _lens(cuda, lens))
 
 
-@pytest.mark.parametrize("hq,hkv,d", [(8, 2, 128), (2, 2, 128), (6, 2, 80)])
+@pytest.mark.parametrize("hq,hkv,d", [(8, 2, 128), (2, 2, 128), (6, 2, 80), (8, 2, 256)])
 def test_not_finite_inside(cuda, hq, hkv, d):
     """A block with the scale NaN among a sequence's keys, in k or in v, and a
     query head with a NaN or an infinity make exactly their heads NaN."""
@@ -280,7 +291,7 @@ def _on_path(path, case, block, lens):
 
 
 @pytest.mark.parametrize("hq,hkv,d", [(1, 1, 128), (4, 2, 128), (8, 2, 128), (16, 2, 128), (6, 2, 128), (24, 2, 128),
-                                      (8, 2, 64), (8, 2, 16), (4, 4, 112)])
+                                      (8, 2, 64), (8, 2, 16), (4, 4, 112), (8, 2, 256), (3, 1, 144), (16, 1, 208)])
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
 def test_both_kernels(cuda, hq, hkv, d, dtype):
     """Shapes that the tensor-core kernel takes, on it and on the other one."""
