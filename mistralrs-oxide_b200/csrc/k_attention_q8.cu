@@ -11,14 +11,16 @@
 // decode_attn_q8_combine_kernel merges them:
 //   k_attention_q8_tc.cu   head_dim a multiple of 16: both products in int8 on
 //                          tcgen05;
-//   here, any other shape  (head_dim up to 256, any group): a warp is a
-//                          worker and streams 32-key tiles.  Scores: lane =
-//                          key, its row read in 16-byte (4-byte, 1-byte)
-//                          pieces against the group's query heads in shared
-//                          memory; P V: lane = four dims (one, for odd
-//                          sizes), each key's weights broadcast by shuffles.
-//                          f32 throughout.
-// Bound by HBM bytes, 2 head_dim a key and kv head.
+//   here, any other shape  (head_dim up to 256, any group, more than 1024
+//                          sequences): a warp is a worker and streams 32-key
+//                          tiles.  Scores: lane = key, its row read in words of
+//                          16 or 4 bytes against the group's query heads in
+//                          shared memory; P V: lane = four dims, each key's
+//                          weights broadcast by shuffles.  f32 throughout.
+// Bound by HBM bytes, 2 head_dim a key and kv head; the kernel here by its
+// instructions, some 1200 for 32 keys and four heads: 8 sequences of 16384 keys,
+// 32 heads over 8, head_dim 37, take 139 us (214 with a load a byte and a dim a
+// lane), 0.56 TB/s; 32 of 4096 keys, head_dim 20, 60 us (96 with one key at a time).
 #include "oxide_attn_q8.cuh"
 
 namespace oxide {
@@ -26,13 +28,27 @@ namespace oxide {
 constexpr int QW_WARPS = 8;
 constexpr uint32_t QW_TK = 32;  // keys a tile
 
-// Dims a lane owns: D4: four of every 128 (NG groups); else one of every 32.
-template <int NR, int NG, bool D4>
+// The four bytes at `a`, which need not lie on a word: from the aligned words
+// around them, neither of them behind `last`, the word of the array's last byte
+// (bytes behind it are anything: they are nobody's dims).
+__device__ __forceinline__ uint32_t qw_word(const int8_t* a, const uint32_t* last) {
+    const uintptr_t u = reinterpret_cast<uintptr_t>(a);
+    const uint32_t* w = reinterpret_cast<const uint32_t*>(u & ~(uintptr_t)3);
+    const uint32_t lo = __ldg(w), hi = __ldg(w < last ? w + 1 : last);
+    return __funnelshift_r(lo, hi, 8u * (uint32_t)(u & 3));
+}
+
+// A lane owns four dims of every 128 (NG of them) in P V; head_dim up to 64 and
+// 32 leaves half of the lanes and more without dims, so KG = 2 and 4 keys are
+// taken at once.  WORDS: rows start on words (head_dim a multiple of 4, aligned
+// caches); else words are put together from two.
+template <int NR, int NG, int KG, bool WORDS>
 __global__ void __launch_bounds__(QW_WARPS * 32, 2) decode_attn_q8_warp_kernel(Q8AttnArgs p) {
     pdl_begin();
     extern __shared__ __align__(16) unsigned char smem[];
-    constexpr int W = D4 ? 4 : 1;
+    constexpr int W = 4, LANES = 32 / KG;  // dims a lane and group; lanes a key
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const uint32_t kg = lane / LANES, dl = lane % LANES;
     const uint32_t D = p.head_dim, DP = (D + 3) & ~3u;
     float* qs = reinterpret_cast<float*>(smem) + (size_t)warp * NR * DP;  // this warp's query heads [NR][DP]
     uint32_t* pre = reinterpret_cast<uint32_t*>(smem + (size_t)QW_WARPS * NR * DP * 4);
@@ -51,6 +67,11 @@ __global__ void __launch_bounds__(QW_WARPS * 32, 2) decode_attn_q8_warp_kernel(Q
     uint32_t nh = 0, len = 0;
     const int8_t *kh = nullptr, *vh = nullptr;
     const float *ksh = nullptr, *vsh = nullptr;
+    const uint64_t bytes = (uint64_t)p.batch * p.kv_heads * p.max_seq * D;
+    auto last_word = [&](const int8_t* c) {
+        return reinterpret_cast<const uint32_t*>(reinterpret_cast<uintptr_t>(c + bytes - 1) & ~(uintptr_t)3);
+    };
+    const uint32_t *klast = last_word(p.kc), *vlast = last_word(p.vc);
     for (uint32_t t = t0; t < t1; ++t, w.next()) {
         if (t == t0 || w.lt == 0) {  // a new pair: its query heads and caches
             const uint32_t kvh = p.by_chunks.div(w.kvh), h0 = (w.kvh - kvh * p.chunks) * NR;
@@ -91,7 +112,7 @@ __global__ void __launch_bounds__(QW_WARPS * 32, 2) decode_attn_q8_warp_kernel(Q
             ks = __ldg(ksh + (key >> p.shift));
             vs = __ldg(vsh + (key >> p.shift));
             const int8_t* row = kh + (uint64_t)key * D;
-            if (D4 && D % 16 == 0) {
+            if (WORDS && D % 16 == 0) {
 #pragma unroll 4
                 for (uint32_t i = 0; i < D; i += 16) {
                     const uint4 v = __ldg(reinterpret_cast<const uint4*>(row + i));
@@ -110,22 +131,19 @@ __global__ void __launch_bounds__(QW_WARPS * 32, 2) decode_attn_q8_warp_kernel(Q
                         }
                     }
                 }
-            } else if (D4) {
-#pragma unroll 4
-                for (uint32_t i = 0; i < D; i += 4) {
-                    float f[4];
-                    q8_unpack4(__ldg(reinterpret_cast<const unsigned int*>(row + i)), f);
-#pragma unroll
-                    for (int h = 0; h < NR; ++h)
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) dot[h] = __fmaf_rn(f[e], qs[h * DP + i + e], dot[h]);
-                }
             } else {
 #pragma unroll 4
-                for (uint32_t i = 0; i < D; ++i) {
-                    const float f = (float)__ldg(reinterpret_cast<const signed char*>(row + i));
+                for (uint32_t i = 0; i < D; i += 4) {  // (qs is zero past head_dim)
+                    float f[4];
+                    q8_unpack4(WORDS ? __ldg(reinterpret_cast<const unsigned int*>(row + i)) : qw_word(row + i, klast), f);
 #pragma unroll
-                    for (int h = 0; h < NR; ++h) dot[h] = __fmaf_rn(f, qs[h * DP + i], dot[h]);
+                    for (int h = 0; h < NR; ++h) {
+                        const float4 qv = *reinterpret_cast<const float4*>(qs + h * DP + i);
+                        dot[h] = __fmaf_rn(f[0], qv.x, dot[h]);
+                        dot[h] = __fmaf_rn(f[1], qv.y, dot[h]);
+                        dot[h] = __fmaf_rn(f[2], qv.z, dot[h]);
+                        dot[h] = __fmaf_rn(f[3], qv.w, dot[h]);
+                    }
                 }
             }
         }
@@ -145,17 +163,17 @@ __global__ void __launch_bounds__(QW_WARPS * 32, 2) decode_attn_q8_warp_kernel(Q
         }
         const int8_t* vrow = vh + (uint64_t)key0 * D;
 #pragma unroll 8
-        for (uint32_t j = 0; j < nk; ++j) {
+        for (uint32_t j0 = 0; j0 < nk; j0 += KG) {
+            const uint32_t j = j0 + kg;  // (keys past nk: their weight is zero)
             float f[NG][W];
 #pragma unroll
             for (int g = 0; g < NG; ++g) {
-                const uint32_t d = W * (lane + 32 * g);
-                if constexpr (D4) {
-                    const uint32_t x = d < D ? __ldg(reinterpret_cast<const unsigned int*>(vrow + (uint64_t)j * D + d)) : 0u;
-                    q8_unpack4(x, f[g]);
-                } else {
-                    f[g][0] = d < D ? (float)__ldg(reinterpret_cast<const signed char*>(vrow + (uint64_t)j * D + d)) : 0.0f;
-                }
+                const uint32_t d = W * (dl + 32 * g);
+                const int8_t* at = vrow + (uint64_t)j * D + d;
+                uint32_t x = 0u;
+                if (d < D && (KG == 1 || j < nk))
+                    x = WORDS ? __ldg(reinterpret_cast<const unsigned int*>(at)) : qw_word(at, vlast);
+                q8_unpack4(x, f[g]);
             }
 #pragma unroll
             for (int h = 0; h < NR; ++h) {
@@ -171,6 +189,10 @@ __global__ void __launch_bounds__(QW_WARPS * 32, 2) decode_attn_q8_warp_kernel(Q
 #pragma unroll
             for (int h = 0; h < NR; ++h) {
                 const float ls = warp_sum(l[h]);
+#pragma unroll
+                for (int o = LANES; o < 32; o *= 2)  // the keys taken at once
+#pragma unroll
+                    for (int e = 0; e < W; ++e) acc[h][e] = fadd(acc[h][e], __shfl_xor_sync(0xffffffffu, acc[h][e], o));
                 if ((uint32_t)h >= nh) continue;
                 const uint64_t slot = part * NR + h;
                 if (lane == 0) {
@@ -181,8 +203,8 @@ __global__ void __launch_bounds__(QW_WARPS * 32, 2) decode_attn_q8_warp_kernel(Q
                 for (int g = 0; g < NG; ++g)
 #pragma unroll
                     for (int e = 0; e < W; ++e) {
-                        const uint32_t d = W * (lane + 32 * g) + e;
-                        if (d < D) p.part_o[slot * DP + d] = acc[h][g * W + e];
+                        const uint32_t d = W * (dl + 32 * g) + e;
+                        if (kg == 0 && d < D) p.part_o[slot * DP + d] = acc[h][g * W + e];
                     }
             }
         }
@@ -288,9 +310,9 @@ int q8_block_shift(uint64_t block);
 int q8_cache_check(const char* name, uint64_t batch, uint64_t kv_heads, uint64_t max_seq, uint64_t head_dim,
                    uint64_t block);
 
-template <int NR, int NG, bool D4>
+template <int NR, int NG, int KG, bool WORDS>
 static cudaError_t launch_warp(Q8AttnArgs& a, cudaStream_t st) {
-    auto kern = decode_attn_q8_warp_kernel<NR, NG, D4>;
+    auto kern = decode_attn_q8_warp_kernel<NR, NG, KG, WORDS>;
     const size_t smem = (size_t)QW_WARPS * NR * ((a.head_dim + 3) & ~3u) * 4 + (a.batch + 1) * 4;
     if (!ensure_dyn_smem(reinterpret_cast<const void*>(kern), smem)) return cudaErrorInvalidConfiguration;
     // one worker a resident warp, as many as the workspace has parts for
@@ -302,10 +324,20 @@ static cudaError_t launch_warp(Q8AttnArgs& a, cudaStream_t st) {
     a.inv_workers = 1.0 / a.workers;
     return launch_k(kern, (unsigned)ctas, QW_WARPS * 32, smem, st, a);
 }
-template <int NR>
-static cudaError_t launch_warp_d(Q8AttnArgs& a, bool d4, cudaStream_t st) {
-    if (!d4) return launch_warp<NR, 8, false>(a, st);
-    return a.head_dim <= 128 ? launch_warp<NR, 1, true>(a, st) : launch_warp<NR, 2, true>(a, st);
+template <int NR, bool WORDS>
+static cudaError_t launch_warp_d(Q8AttnArgs& a, cudaStream_t st) {
+    if (a.head_dim > 128) return launch_warp<NR, 2, 1, WORDS>(a, st);
+    if (a.head_dim > 64) return launch_warp<NR, 1, 1, WORDS>(a, st);
+    return a.head_dim > 32 ? launch_warp<NR, 1, 2, WORDS>(a, st) : launch_warp<NR, 1, 4, WORDS>(a, st);
+}
+template <bool WORDS>
+static cudaError_t launch_warp_nr(Q8AttnArgs& a, cudaStream_t st) {
+    switch (a.nr) {
+        case 1: return launch_warp_d<1, WORDS>(a, st);
+        case 2: return launch_warp_d<2, WORDS>(a, st);
+        case 4: return launch_warp_d<4, WORDS>(a, st);
+        default: return launch_warp_d<8, WORDS>(a, st);
+    }
 }
 
 template <typename T, int DV>
@@ -381,14 +413,9 @@ static int attn_q8_entry(const char* name, const T* q, const int8_t* kc, const i
     bool done = false;  // the tcgen05 kernel ran
     cudaError_t e = path == 1 ? cudaSuccess : decode_attention_q8_tc(a, path == 2, st, &done);
     const uint64_t word = head_dim % 16 == 0 ? 16 : 4;
-    const bool d4 = head_dim % 4 == 0 && (reinterpret_cast<uintptr_t>(kc) & (word - 1)) == 0 &&
-                    (reinterpret_cast<uintptr_t>(vc) & 3) == 0;
-    if (e == cudaSuccess && !done) switch (nr) {
-        case 1: e = launch_warp_d<1>(a, d4, st); break;
-        case 2: e = launch_warp_d<2>(a, d4, st); break;
-        case 4: e = launch_warp_d<4>(a, d4, st); break;
-        default: e = launch_warp_d<8>(a, d4, st); break;
-    }
+    const bool words = head_dim % 4 == 0 && (reinterpret_cast<uintptr_t>(kc) & (word - 1)) == 0 &&
+                       (reinterpret_cast<uintptr_t>(vc) & 3) == 0;
+    if (e == cudaSuccess && !done) e = words ? launch_warp_nr<true>(a, st) : launch_warp_nr<false>(a, st);
     if (e == cudaSuccess) e = head_dim <= 128 ? launch_combine<T, 1>(out, a, st) : launch_combine<T, 2>(out, a, st);
     if (e != cudaSuccess) {
         cudaGetLastError();
