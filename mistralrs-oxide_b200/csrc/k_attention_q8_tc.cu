@@ -18,8 +18,12 @@
 //
 // Work division as in k_attention_tc.cu (tiles of 128 keys laid end to end,
 // one CTA per SM, equal ranges); partials as in oxide_attn_q8.cuh, two halves
-// a CTA.  head_dim a multiple of 16: tiles are one or two halves of 128 bytes
-// wide (up to 128, up to 256), and TMA fills what lies past head_dim with zeros.
+// a CTA.  head_dim a multiple of 16, in one piece up to 128 and in two halves
+// above (half_dims each, rounded up to 16): a box is as wide as its piece and its
+// rows are 128 bytes apart in shared memory, whose rest is anything -- it meets
+// digits that are zero, or dims that nobody reads.  (Boxes of 128 bytes, filled
+// with zeros past head_dim, took 63.6 us instead of 38.8 at 8 sequences of 16384
+// keys, head_dim 80, and 47.2 instead of 37.6 at 8192 keys, head_dim 144.)
 //
 // CTA of 13 warps:
 //   warp 0      TMA producer: K and V tiles [128 keys x 128 bytes],
@@ -220,7 +224,7 @@ __global__ void __launch_bounds__(QT_THREADS, 1)
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    const uint32_t tmem = *tmem_slot;
+    const uint32_t tmem = *tmem_slot, hd = p.half_dims;
     const uint32_t T = pre[p.batch] * heads;
     const uint32_t nt = q8a_start(p, blockIdx.x + 1, T) - q8a_start(p, blockIdx.x, T);  // this CTA's tiles, n = 0 .. nt - 1
     TileWalk w{pre, p.batch, heads, begin[0], begin[1], begin[2], begin[3]};  // (unset, and unused, without tiles)
@@ -236,12 +240,12 @@ __global__ void __launch_bounds__(QT_THREADS, 1)
                 const int y = (int)(w.lt * QT_TK);
                 const uint32_t sd = sbase + s * M::STAGE_BYTES;
                 if (leader) {
-                    mbar_arrive_expect_tx(bar(M::FULL + s), M::STAGE_BYTES);
+                    mbar_arrive_expect_tx(bar(M::FULL + s), 2 * DH * QT_TK * hd);
 #pragma unroll
-                    for (int x = 0; x < DH; ++x) tma_load_3d(sd + x * QT_TILE, &tmk, bar(M::FULL + s), x * QT_DB, y, z);
+                    for (int x = 0; x < DH; ++x) tma_load_3d(sd + x * QT_TILE, &tmk, bar(M::FULL + s), x * (int)hd, y, z);
 #pragma unroll
                     for (int x = 0; x < DH; ++x)
-                        tma_load_3d(sd + (DH + x) * QT_TILE, &tmv, bar(M::FULL + s), x * QT_DB, y, z);
+                        tma_load_3d(sd + (DH + x) * QT_TILE, &tmv, bar(M::FULL + s), x * (int)hd, y, z);
                 }
                 __syncwarp();
                 w.next();
@@ -342,8 +346,8 @@ __global__ void __launch_bounds__(QT_THREADS, 1)
         auto load = [&](uint32_t h, uint2 (&v)[2 * DH]) {
 #pragma unroll
             for (int half = 0; half < DH; ++half) {
-                const uint32_t d = 4u * lane + 128u * half;
-                const bool there = h < nh && d < p.head_dim;
+                const uint32_t d = 4u * lane + hd * half;
+                const bool there = h < nh && 4u * lane < hd && d < p.head_dim;
                 const uint2* at = reinterpret_cast<const uint2*>(static_cast<const char*>(p.q) +
                                                                  ((row + h) * p.head_dim + d) * (p.q_bf16 ? 2 : 4));
                 v[2 * half] = v[2 * half + 1] = make_uint2(0, 0);
@@ -639,8 +643,8 @@ __global__ void __launch_bounds__(QT_THREADS, 1)
                     const float f = ex2_approx(fsub(wm[h], m[h]));
 #pragma unroll
                     for (int x = 0; x < DH; ++x)
-                        if ((uint32_t)h < nh && L + 128 * x < p.head_dim)
-                            p.part_o[(part * NR + h) * p.head_dim + L + 128 * x] = fmul(acc[x][h], f);
+                        if ((uint32_t)h < nh && L < hd && L + hd * x < p.head_dim)
+                            p.part_o[(part * NR + h) * p.head_dim + L + hd * x] = fmul(acc[x][h], f);
                 }
                 if (nbar_or128(fail, nbar)) {
                     dead = true;
@@ -674,14 +678,15 @@ typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t,
                                   CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
 
 // A cache [heads, max_seq, head_dim] of bytes as a TMA map with boxes of 128
-// positions by 128 bytes, 128-byte swizzle; bytes past head_dim and positions
+// positions by `width` bytes, 128-byte swizzle; bytes past head_dim and positions
 // past max_seq are filled with zeros.  False if the driver refuses it.
-static bool qt_map(CUtensorMap* m, const void* base, uint64_t heads, uint64_t max_seq, uint64_t head_dim) {
+static bool qt_map(CUtensorMap* m, const void* base, uint64_t heads, uint64_t max_seq, uint64_t head_dim,
+                   uint32_t width) {
     static EncodeTiledFn enc = reinterpret_cast<EncodeTiledFn>(driver_fn("cuTensorMapEncodeTiled"));
     if (!enc) return false;
     const cuuint64_t dims[3] = {head_dim, max_seq, heads};
     const cuuint64_t strides[2] = {head_dim, max_seq * head_dim};
-    const cuuint32_t box[3] = {QT_DB, QT_TK, 1};
+    const cuuint32_t box[3] = {width, QT_TK, 1};
     const cuuint32_t es[3] = {1, 1, 1};
     return enc(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<void*>(base), dims, strides, box, es,
                CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
@@ -720,8 +725,10 @@ cudaError_t decode_attention_q8_tc(Q8AttnArgs& a, bool withhold, cudaStream_t st
     uint64_t G = (uint64_t)sm_count();
     if (G > tiles) G = tiles;
     if (2 * G > Q8A_PARTS) return cudaSuccess;
+    a.half_dims = a.head_dim <= QT_DB ? a.head_dim : (a.head_dim / 2 + 15) / 16 * 16;
     CUtensorMap mk, mv;
-    if (!qt_map(&mk, a.kc, pairs, a.max_seq, a.head_dim) || !qt_map(&mv, a.vc, pairs, a.max_seq, a.head_dim))
+    if (!qt_map(&mk, a.kc, pairs, a.max_seq, a.head_dim, a.half_dims) ||
+        !qt_map(&mv, a.vc, pairs, a.max_seq, a.head_dim, a.half_dims))
         return cudaSuccess;
     a.workers = (uint32_t)G;
     a.inv_workers = 1.0 / a.workers;

@@ -31,6 +31,7 @@ struct Q8AttnArgs {
     uint32_t rep, chunks, nr;  // query heads a kv head; pieces of at most nr of them
     uint32_t nblk, shift;      // scale blocks a head, log2 of their tokens
     uint32_t workers, halves;  // halves (1 or 2): a worker's tiles go in turn to so many, each with a part of its own
+    uint32_t half_dims;        // dims of a tile's half (k_attention_q8_tc.cu)
     double inv_workers;        // 1 / workers
     FastDiv by_q_heads, by_rep, by_nr, by_chunks;
     uint32_t q_bf16;
