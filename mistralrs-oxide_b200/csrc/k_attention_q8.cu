@@ -220,15 +220,21 @@ __global__ void __launch_bounds__(QW_WARPS * 32, 2) decode_attn_q8_warp_kernel(Q
 // NW: 8 warps while there are fewer CTAs than SMs -- a CTA then merges many
 // parts (one sequence of 131072 keys, 37 parts a head: the whole call 51.0 us
 // against 53.0 with 4) -- else 4, so that more CTAs are resident at once (8
-// sequences of 1024 to 32768, 256 CTAs: 54.7 us against 55.9 with 8).
+// sequences of 1024 to 32768, 256 CTAs: 54.7 us against 55.9 with 8).  With two
+// pairs and more to a worker a head has four parts at most, which one warp loads
+// at once: NW = 1, a head to each of a CTA's four warps (2048 pairs 51.2 us
+// against 57.5 with NW = 4, 512 pairs 22.4 against 22.7; but 150 pairs 43.1
+// against 41.7).
 constexpr int QC_UNROLL = 5;
 template <typename T, int DV, int NW>
-__global__ void __launch_bounds__(NW * 32) decode_attn_q8_combine_kernel(T* out, Q8AttnArgs p) {
+__global__ void __launch_bounds__(NW == 1 ? 128 : NW * 32) decode_attn_q8_combine_kernel(T* out, Q8AttnArgs p) {
     pdl_begin();
     __shared__ float wm[NW], wl[NW];
     __shared__ float4 wo[NW][32 * DV];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const uint32_t bh = blockIdx.x, b = p.by_q_heads.div(bh), qh = bh - b * p.q_heads;
+    const uint32_t bh = NW == 1 ? blockIdx.x * 4 + warp : blockIdx.x, first = NW == 1 ? 0 : warp;
+    if (NW == 1 && bh >= p.batch * p.q_heads) return;
+    const uint32_t b = p.by_q_heads.div(bh), qh = bh - b * p.q_heads;
     const uint32_t kvh = p.by_rep.div(qh), r = qh - kvh * p.rep, chunk = p.by_nr.div(r), h = r - chunk * p.nr;
     const uint32_t heads = p.kv_heads * p.chunks, D = p.head_dim, DP = q8a_dims(D);
     const uint32_t before = p.pre_out[b], tb = p.pre_out[b + 1] - before, all = p.pre_out[p.batch] * heads;
@@ -242,7 +248,7 @@ __global__ void __launch_bounds__(NW * 32) decode_attn_q8_combine_kernel(T* out,
                        tend = tfirst + tb;
         const uint32_t c0 = q8a_owner(p, tfirst, all), c1 = q8a_owner(p, tend - 1, all);
         const uint32_t n = (c1 - c0 + 1) * p.halves;
-        for (uint32_t i0 = warp; i0 < n; i0 += NW * QC_UNROLL) {
+        for (uint32_t i0 = first; i0 < n; i0 += NW * QC_UNROLL) {
             float ms[QC_UNROLL], ls[QC_UNROLL];
             float4 o[QC_UNROLL][DV];
 #pragma unroll
@@ -281,6 +287,18 @@ __global__ void __launch_bounds__(NW * 32) decode_attn_q8_combine_kernel(T* out,
                 M = mn;
             }
         }
+    }
+    if constexpr (NW == 1) {
+#pragma unroll
+        for (int k = 0; k < DV; ++k) {
+            const float o[4] = {acc[k].x, acc[k].y, acc[k].z, acc[k].w};
+#pragma unroll
+            for (uint32_t e = 0; e < 4; ++e) {
+                const uint32_t d = 4 * (lane + 32 * k) + e;
+                if (d < D) Vec<T>::store1(out + (uint64_t)bh * D + d, failed ? q8_nan() : (L == 0.0f ? 0.0f : fdiv(o[e], L)));
+            }
+        }
+        return;
     }
     if (lane == 0) {
         wm[warp] = M;
@@ -343,6 +361,8 @@ static cudaError_t launch_warp_nr(Q8AttnArgs& a, cudaStream_t st) {
 template <typename T, int DV>
 static cudaError_t launch_combine(T* out, const Q8AttnArgs& a, cudaStream_t st) {
     const unsigned grid = a.batch * a.q_heads;
+    if ((uint64_t)a.batch * a.kv_heads * a.chunks >= 2ull * a.workers)
+        return launch_k(decode_attn_q8_combine_kernel<T, DV, 1>, (grid + 3) / 4, 128, 0, st, out, a);
     return grid < (unsigned)sm_count() ? launch_k(decode_attn_q8_combine_kernel<T, DV, 8>, grid, 256, 0, st, out, a)
                                        : launch_k(decode_attn_q8_combine_kernel<T, DV, 4>, grid, 128, 0, st, out, a);
 }

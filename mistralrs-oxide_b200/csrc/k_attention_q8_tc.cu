@@ -40,7 +40,7 @@
 //   warp 2      the query heads' digits, one pair ahead, from raw bits loaded two
 //               pairs ahead.  (A second such warp gained nothing, nor did asking
 //               L2 for the queries four pairs early: 59.2 and 71.2 us where this
-//               takes 59.1, at 256 sequences of 200 keys, 32 heads.)
+//               took 59.1, at 256 sequences of 200 keys, 32 heads.)
 //   warp 3      the tile prefix; then each tile's scales, ready for the softmax
 //               threads (the key scale, log2 of the value scale, masks), loaded
 //               two tiles ahead.  One scale for a lane's four keys wherever
@@ -628,37 +628,37 @@ __global__ void __launch_bounds__(QT_THREADS, 1)
                 }
             }
             if (dead) break;
-            if (j0 < cnt) {  // the pair is complete here: its partial
-                epilogue(k - 1);
-#pragma unroll
-                for (int h = 0; h < NR; ++h) {
-                    const float x = warp_sum(l[h]);
-                    if (lane == 0) lsum[q4 * 8 + h] = x;
-                    if (L == 0) lsum[32 + h] = m[h];
-                }
-                const uint64_t part = ((uint64_t)blockIdx.x + (uint64_t)w.b * heads + w.kvh) * 2 + g;
-                const uint32_t nh = min(p.rep - (w.kvh - p.by_chunks.div(w.kvh) * p.chunks) * NR, (uint32_t)NR);
-#pragma unroll
-                for (int h = 0; h < NR; ++h) {
-                    const float f = ex2_approx(fsub(wm[h], m[h]));
-#pragma unroll
-                    for (int x = 0; x < DH; ++x)
-                        if ((uint32_t)h < nh && L < hd && L + hd * x < p.head_dim)
-                            p.part_o[(part * NR + h) * p.head_dim + L + hd * x] = fmul(acc[x][h], f);
-                }
-                if (nbar_or128(fail, nbar)) {
-                    dead = true;
-                    break;
-                }
-                if (L < nh) {
-                    p.part_ml[(part * NR + L) * 2] = lsum[32 + L];
-                    p.part_ml[(part * NR + L) * 2 + 1] = fadd(fadd(lsum[L], lsum[8 + L]), fadd(lsum[16 + L], lsum[24 + L]));
-                }
-                // lsum is written again behind the next tile's barriers
-            }
+            // the pair is complete here; what its partial does not wait for comes
+            // while its last output product runs
+            const uint64_t part = ((uint64_t)blockIdx.x + (uint64_t)w.b * heads + w.kvh) * 2 + g;
+            const uint32_t nh = min(p.rep - (w.kvh - p.by_chunks.div(w.kvh) * p.chunks) * NR, (uint32_t)NR);
             n += cnt;
             w.lt += cnt - 1;
             w.next();
+            if (j0 >= cnt) continue;
+#pragma unroll
+            for (int h = 0; h < NR; ++h) {
+                const float x = warp_sum(l[h]);
+                if (lane == 0) lsum[q4 * 8 + h] = x;
+                if (L == 0) lsum[32 + h] = m[h];
+                f[h] = ex2_approx(fsub(wm[h], m[h]));
+            }
+            epilogue(k - 1);
+#pragma unroll
+            for (int h = 0; h < NR; ++h)
+#pragma unroll
+                for (int x = 0; x < DH; ++x)
+                    if ((uint32_t)h < nh && L < hd && L + hd * x < p.head_dim)
+                        p.part_o[(part * NR + h) * p.head_dim + L + hd * x] = fmul(acc[x][h], f[h]);
+            if (nbar_or128(fail, nbar)) {
+                dead = true;
+                break;
+            }
+            if (L < nh) {
+                p.part_ml[(part * NR + L) * 2] = lsum[32 + L];
+                p.part_ml[(part * NR + L) * 2 + 1] = fadd(fadd(lsum[L], lsum[8 + L]), fadd(lsum[16 + L], lsum[24 + L]));
+            }
+            // lsum is written again behind the next tile's barriers
         }
         if (fail || dead) *abort = 1;
     }
