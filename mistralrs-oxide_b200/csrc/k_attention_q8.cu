@@ -211,8 +211,8 @@ __global__ void __launch_bounds__(QW_WARPS * 32, 2) decode_attn_q8_warp_kernel(Q
     }
 }
 
-// Merge the parts of one (batch, query head): warp w of NW takes every NW-th
-// part of the pair, the loads of QC_UNROLL of them in flight at once (the
+// Merge the parts of one (batch, query head): with NW warps, warp w takes every
+// NW-th part of the pair, the loads of QC_UNROLL of them in flight at once (the
 // parts' places follow from the tile division alone), lane = four dims (DV of
 // them 128 apart), and the NW states are joined through shared memory.  A part
 // without keys has sum 0; a pair without keys gives zeros; NaN if a wait of the
@@ -220,107 +220,132 @@ __global__ void __launch_bounds__(QW_WARPS * 32, 2) decode_attn_q8_warp_kernel(Q
 // NW: 8 warps while there are fewer CTAs than SMs -- a CTA then merges many
 // parts (one sequence of 131072 keys, 37 parts a head: the whole call 51.0 us
 // against 53.0 with 4) -- else 4, so that more CTAs are resident at once (8
-// sequences of 1024 to 32768, 256 CTAs: 54.7 us against 55.9 with 8).  With two
-// pairs and more to a worker a head has four parts at most, which one warp loads
-// at once: NW = 1, a head to each of a CTA's four warps (2048 pairs 51.2 us
-// against 57.5 with NW = 4, 512 pairs 22.4 against 22.7; but 150 pairs 43.1
-// against 41.7).
+// sequences of 1024 to 32768, 256 CTAs: 54.7 us against 55.9 with 8).  With as
+// many pairs as workers have parts, a head has four parts or fewer on average,
+// which one warp loads at once: EACH gives a head to each of a CTA's four warps
+// (2048 pairs 51.2 us against 57.5 without, 512 pairs 22.4 against 22.7; but 150
+// pairs 43.1 against 41.7).  A long sequence among short ones, whose heads then have
+// hundreds of parts, gains nothing from four warps that take a CTA's heads in turn
+// (65536 keys beside 399 sequences of 60, 296 parts: 87 us against 82).
 constexpr int QC_UNROLL = 5;
-template <typename T, int DV, int NW>
-__global__ void __launch_bounds__(NW == 1 ? 128 : NW * 32) decode_attn_q8_combine_kernel(T* out, Q8AttnArgs p) {
+struct Q8Parts {  // the parts of a head: workers c0 .. that had tiles tfirst .. tend - 1 of its pair
+    uint32_t pair, h, tfirst, tend, c0, n;
+};
+__device__ __forceinline__ Q8Parts q8_parts(const Q8AttnArgs& p, uint32_t bh, uint32_t heads, uint32_t all) {
+    const uint32_t b = p.by_q_heads.div(bh), qh = bh - b * p.q_heads;
+    const uint32_t kvh = p.by_rep.div(qh), r = qh - kvh * p.rep, chunk = p.by_nr.div(r);
+    const uint32_t before = p.pre_out[b], tb = p.pre_out[b + 1] - before;
+    Q8Parts x{b * heads + kvh * p.chunks + chunk, r - chunk * p.nr, 0, 0, 0, 0};
+    if (tb) {
+        x.tfirst = before * heads + (x.pair - b * heads) * tb;
+        x.tend = x.tfirst + tb;
+        x.c0 = q8a_owner(p, x.tfirst, all);
+        x.n = (q8a_owner(p, x.tend - 1, all) - x.c0 + 1) * p.halves;
+    }
+    return x;
+}
+template <int DV>
+struct Q8State {
+    float M, L;
+    float4 acc[DV];
+};
+// The parts first, first + step, ... of a head.
+template <int DV>
+__device__ __forceinline__ Q8State<DV> q8_merge(const Q8AttnArgs& p, const Q8Parts& x, uint32_t all, uint32_t first,
+                                                uint32_t step, uint32_t lane) {
+    const uint32_t DP = q8a_dims(p.head_dim);
+    Q8State<DV> s;
+    s.M = -INFINITY;
+    s.L = 0.0f;
+#pragma unroll
+    for (int k = 0; k < DV; ++k) s.acc[k] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    for (uint32_t i0 = first; i0 < x.n; i0 += step * QC_UNROLL) {
+        float ms[QC_UNROLL], ls[QC_UNROLL];
+        float4 o[QC_UNROLL][DV];
+#pragma unroll
+        for (int u = 0; u < QC_UNROLL; ++u) {
+            const uint32_t i = i0 + u * step, c = x.c0 + (i >> (p.halves - 1)), half = i & (p.halves - 1);
+            ms[u] = -INFINITY;
+            ls[u] = 0.0f;
+#pragma unroll
+            for (int k = 0; k < DV; ++k) o[u][k] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            if (i >= x.n) continue;
+            const uint32_t f0 = q8a_start(p, c, all), f1 = q8a_start(p, c + 1, all);
+            const uint32_t a = max(f0, x.tfirst), e = min(f1, x.tend);
+            if (a >= e || (e - a < p.halves && ((a - f0) ^ half) & 1)) continue;  // no tile, or the other half's one tile
+            const uint64_t slot = (((uint64_t)c + x.pair) * p.halves + half) * p.nr + x.h;
+            ms[u] = p.part_ml[slot * 2];
+            ls[u] = p.part_ml[slot * 2 + 1];
+#pragma unroll
+            for (int k = 0; k < DV; ++k) {
+                const uint32_t d = 4 * (lane + 32 * k);
+                if (d < DP) o[u][k] = *reinterpret_cast<const float4*>(p.part_o + slot * DP + d);
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < QC_UNROLL; ++u) {
+            if (ls[u] == 0.0f) continue;
+            const float mn = fmaxf(s.M, ms[u]);
+            const float cr = s.M == -INFINITY ? 0.0f : ex2_approx(fsub(s.M, mn)), w = ex2_approx(fsub(ms[u], mn));
+            s.L = __fmaf_rn(ls[u], w, fmul(s.L, cr));
+#pragma unroll
+            for (int k = 0; k < DV; ++k) {
+                s.acc[k].x = __fmaf_rn(o[u][k].x, w, fmul(s.acc[k].x, cr));
+                s.acc[k].y = __fmaf_rn(o[u][k].y, w, fmul(s.acc[k].y, cr));
+                s.acc[k].z = __fmaf_rn(o[u][k].z, w, fmul(s.acc[k].z, cr));
+                s.acc[k].w = __fmaf_rn(o[u][k].w, w, fmul(s.acc[k].w, cr));
+            }
+            s.M = mn;
+        }
+    }
+    return s;
+}
+
+template <typename T, int DV, int NW, bool EACH>
+__global__ void __launch_bounds__(NW * 32) decode_attn_q8_combine_kernel(T* out, Q8AttnArgs p) {
     pdl_begin();
     __shared__ float wm[NW], wl[NW];
     __shared__ float4 wo[NW][32 * DV];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const uint32_t bh = NW == 1 ? blockIdx.x * 4 + warp : blockIdx.x, first = NW == 1 ? 0 : warp;
-    if (NW == 1 && bh >= p.batch * p.q_heads) return;
-    const uint32_t b = p.by_q_heads.div(bh), qh = bh - b * p.q_heads;
-    const uint32_t kvh = p.by_rep.div(qh), r = qh - kvh * p.rep, chunk = p.by_nr.div(r), h = r - chunk * p.nr;
-    const uint32_t heads = p.kv_heads * p.chunks, D = p.head_dim, DP = q8a_dims(D);
-    const uint32_t before = p.pre_out[b], tb = p.pre_out[b + 1] - before, all = p.pre_out[p.batch] * heads;
-    const uint32_t failed = *p.err;
-    float M = -INFINITY, L = 0.0f;
-    float4 acc[DV];
-#pragma unroll
-    for (int k = 0; k < DV; ++k) acc[k] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    if (tb) {
-        const uint32_t pair = b * heads + kvh * p.chunks + chunk, tfirst = before * heads + (pair - b * heads) * tb,
-                       tend = tfirst + tb;
-        const uint32_t c0 = q8a_owner(p, tfirst, all), c1 = q8a_owner(p, tend - 1, all);
-        const uint32_t n = (c1 - c0 + 1) * p.halves;
-        for (uint32_t i0 = first; i0 < n; i0 += NW * QC_UNROLL) {
-            float ms[QC_UNROLL], ls[QC_UNROLL];
-            float4 o[QC_UNROLL][DV];
-#pragma unroll
-            for (int u = 0; u < QC_UNROLL; ++u) {
-                const uint32_t i = i0 + u * NW, c = c0 + (i >> (p.halves - 1)), half = i & (p.halves - 1);
-                ms[u] = -INFINITY;
-                ls[u] = 0.0f;
-#pragma unroll
-                for (int k = 0; k < DV; ++k) o[u][k] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                if (i >= n) continue;
-                const uint32_t f0 = q8a_start(p, c, all), f1 = q8a_start(p, c + 1, all);
-                const uint32_t a = max(f0, tfirst), e = min(f1, tend);
-                if (a >= e || (e - a < p.halves && ((a - f0) ^ half) & 1)) continue;  // no tile, or the other half's one tile
-                const uint64_t slot = (((uint64_t)c + pair) * p.halves + half) * p.nr + h;
-                ms[u] = p.part_ml[slot * 2];
-                ls[u] = p.part_ml[slot * 2 + 1];
-#pragma unroll
-                for (int k = 0; k < DV; ++k) {
-                    const uint32_t d = 4 * (lane + 32 * k);
-                    if (d < DP) o[u][k] = *reinterpret_cast<const float4*>(p.part_o + slot * DP + d);
-                }
-            }
-#pragma unroll
-            for (int u = 0; u < QC_UNROLL; ++u) {
-                if (ls[u] == 0.0f) continue;
-                const float mn = fmaxf(M, ms[u]);
-                const float cr = M == -INFINITY ? 0.0f : ex2_approx(fsub(M, mn)), x = ex2_approx(fsub(ms[u], mn));
-                L = __fmaf_rn(ls[u], x, fmul(L, cr));
-#pragma unroll
-                for (int k = 0; k < DV; ++k) {
-                    acc[k].x = __fmaf_rn(o[u][k].x, x, fmul(acc[k].x, cr));
-                    acc[k].y = __fmaf_rn(o[u][k].y, x, fmul(acc[k].y, cr));
-                    acc[k].z = __fmaf_rn(o[u][k].z, x, fmul(acc[k].z, cr));
-                    acc[k].w = __fmaf_rn(o[u][k].w, x, fmul(acc[k].w, cr));
-                }
-                M = mn;
-            }
-        }
-    }
-    if constexpr (NW == 1) {
+    const uint32_t heads = p.kv_heads * p.chunks, D = p.head_dim, all = p.pre_out[p.batch] * heads;
+    const uint32_t failed = *p.err, bh = EACH ? blockIdx.x * NW + warp : blockIdx.x;
+    if (EACH && bh >= p.batch * p.q_heads) return;
+    const Q8State<DV> s =
+        q8_merge<DV>(p, q8_parts(p, bh, heads, all), all, EACH ? 0 : warp, EACH ? 1 : NW, lane);
+    if constexpr (EACH) {
 #pragma unroll
         for (int k = 0; k < DV; ++k) {
-            const float o[4] = {acc[k].x, acc[k].y, acc[k].z, acc[k].w};
+            const float o[4] = {s.acc[k].x, s.acc[k].y, s.acc[k].z, s.acc[k].w};
 #pragma unroll
             for (uint32_t e = 0; e < 4; ++e) {
                 const uint32_t d = 4 * (lane + 32 * k) + e;
-                if (d < D) Vec<T>::store1(out + (uint64_t)bh * D + d, failed ? q8_nan() : (L == 0.0f ? 0.0f : fdiv(o[e], L)));
+                const float y = failed ? q8_nan() : (s.L == 0.0f ? 0.0f : fdiv(o[e], s.L));
+                if (d < D) Vec<T>::store1(out + (uint64_t)bh * D + d, y);
             }
         }
-        return;
-    }
-    if (lane == 0) {
-        wm[warp] = M;
-        wl[warp] = L;
-    }
-#pragma unroll
-    for (int k = 0; k < DV; ++k) wo[warp][lane + 32 * k] = acc[k];
-    __syncthreads();
-    for (uint32_t d = threadIdx.x; d < D; d += NW * 32) {
-        float mx = -INFINITY, ls = 0.0f, o = 0.0f;
-#pragma unroll
-        for (int i = 0; i < NW; ++i) mx = fmaxf(mx, wm[i]);
-#pragma unroll
-        for (int i = 0; i < NW; ++i) {
-            if (wl[i] == 0.0f) continue;
-            const float x = ex2_approx(fsub(wm[i], mx));
-            ls = __fmaf_rn(wl[i], x, ls);
-            o = __fmaf_rn(reinterpret_cast<const float*>(wo[i])[d], x, o);
+    } else {
+        if (lane == 0) {
+            wm[warp] = s.M;
+            wl[warp] = s.L;
         }
-        float y = ls == 0.0f ? 0.0f : fdiv(o, ls);
-        if (failed) y = q8_nan();
-        Vec<T>::store1(out + (uint64_t)bh * D + d, y);
+#pragma unroll
+        for (int k = 0; k < DV; ++k) wo[warp][lane + 32 * k] = s.acc[k];
+        __syncthreads();
+        for (uint32_t d = threadIdx.x; d < D; d += NW * 32) {
+            float mx = -INFINITY, ls = 0.0f, o = 0.0f;
+#pragma unroll
+            for (int i = 0; i < NW; ++i) mx = fmaxf(mx, wm[i]);
+#pragma unroll
+            for (int i = 0; i < NW; ++i) {
+                if (wl[i] == 0.0f) continue;
+                const float x = ex2_approx(fsub(wm[i], mx));
+                ls = __fmaf_rn(wl[i], x, ls);
+                o = __fmaf_rn(reinterpret_cast<const float*>(wo[i])[d], x, o);
+            }
+            float y = ls == 0.0f ? 0.0f : fdiv(o, ls);
+            if (failed) y = q8_nan();
+            Vec<T>::store1(out + (uint64_t)bh * D + d, y);
+        }
     }
 }
 
@@ -361,10 +386,10 @@ static cudaError_t launch_warp_nr(Q8AttnArgs& a, cudaStream_t st) {
 template <typename T, int DV>
 static cudaError_t launch_combine(T* out, const Q8AttnArgs& a, cudaStream_t st) {
     const unsigned grid = a.batch * a.q_heads;
-    if ((uint64_t)a.batch * a.kv_heads * a.chunks >= 2ull * a.workers)
-        return launch_k(decode_attn_q8_combine_kernel<T, DV, 1>, (grid + 3) / 4, 128, 0, st, out, a);
-    return grid < (unsigned)sm_count() ? launch_k(decode_attn_q8_combine_kernel<T, DV, 8>, grid, 256, 0, st, out, a)
-                                       : launch_k(decode_attn_q8_combine_kernel<T, DV, 4>, grid, 128, 0, st, out, a);
+    if ((uint64_t)a.batch * a.kv_heads * a.chunks >= (uint64_t)a.halves * a.workers)
+        return launch_k(decode_attn_q8_combine_kernel<T, DV, 4, true>, (grid + 3) / 4, 128, 0, st, out, a);
+    return grid < (unsigned)sm_count() ? launch_k(decode_attn_q8_combine_kernel<T, DV, 8, false>, grid, 256, 0, st, out, a)
+                                       : launch_k(decode_attn_q8_combine_kernel<T, DV, 4, false>, grid, 128, 0, st, out, a);
 }
 
 static uint64_t attn_q8_parts(uint64_t batch, uint64_t q_heads, uint64_t kv_heads) {

@@ -94,6 +94,20 @@ def test_many_short_sequences(cuda, hq, hkv, d, dtype):
     _run(case, 4, _lens(cuda, [i % 8 for i in range(400)]))
 
 
+@pytest.mark.parametrize("hq,hkv,d", [(2, 2, 128), (12, 3, 64), (8, 2, 37), (3, 1, 256)])
+def test_a_long_sequence_among_short_ones(cuda, hq, hkv, d):
+    """Its parts are many, the others' few, in the same launch; the batch does not
+    fill the last group of heads, and most sequences are empty in the end."""
+    b, m = 381, 5000 if d > 64 else 20000
+    case = _case(cuda, b, hq, hkv, d, m, 128, "bf16")
+    lens = [(i * 7) % 40 for i in range(b)]
+    lens[b // 2], lens[b - 1] = m, m - 77
+    _run(case, 128, _lens(cuda, lens))
+    lens = [0] * b
+    lens[3] = m
+    _run(case, 128, _lens(cuda, lens))
+
+
 @pytest.mark.parametrize("hq,hkv,d", [(8, 2, 128), (2, 2, 128), (16, 2, 128), (6, 2, 80), (3, 3, 33), (8, 2, 256)])
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
 def test_anything_behind_the_length(cuda, hq, hkv, d, dtype):
