@@ -16,7 +16,8 @@
 // almost every code; the products of two floats are exact in f64, max|p| there
 // is the largest of the elements whose f32 product is the f32 maximum (rounding
 // is monotonic), and a code next to a half-integer is decided from the f64
-// product (oxide_q8.cuh).
+// product (oxide_q8.cuh).  Rows of vectors look for max|p| in f64 only where they
+// have such a code, one in ten at 4096 columns.
 //
 // Layout.  A warp (rows of at most 128 vectors of 16 bytes) or a CTA owns a
 // row and keeps it packed in registers, four vectors a thread, so each row
@@ -24,9 +25,10 @@
 // w stays in registers too, and CTAs take rows in turn (reading w twice a row
 // through L1 instead left L1 the bound: 118 us at [16384, 4096] bf16 against
 // 72 us of bytes).  Bound by HBM bytes: x, r and h in their type, one byte out.
-// Measured: add + norm bf16 [16384, 4096] 78 us, 6.0 TB/s; f32 [2048, 4096] 16.5
-// us, 2.6 TB/s -- a row's chain of load, two reductions and codes takes 3 us, five
-// rows in turn to a CTA; eight rows 2.6 us, launch latency.
+// Measured: add + norm bf16 [16384, 4096] 78 us, 6.0 TB/s; f32 [2048, 4096] 14.0
+// us, 3.0 TB/s -- a row's chain of load, reduction and codes takes 3 us, four rows
+// in turn to a CTA -- and [16384, 4096] 77 us, 4.4 TB/s; eight rows 2.6 us, launch
+// latency.
 // Rows that do not divide into aligned vectors are held element by element in
 // the same way (up to 16 a thread); longer ones are read twice, the second
 // time through L1 / L2.
@@ -136,12 +138,15 @@ __device__ __forceinline__ double norm_q8_refine(float top, int turn, VISIT visi
 struct NormRow {
     double top;   // max|p|
     float scale;
+    bool rounded;  // top is the f32 maximum of products that f32 rounds
 };
 template <typename T, bool WARP, typename VISIT>
-__device__ __forceinline__ NormRow norm_q8_row(float ss, float top, int turn, const NormQ8Args& p, VISIT visit) {
+__device__ __forceinline__ NormRow norm_q8_row(float ss, float top, const NormQ8Args& p, VISIT visit) {
     NormRow r;
+    r.rounded = false;
     if (norm_sure(top) && ss >= 0x1p-80f && ss <= 0x1p100f) {
-        r.top = sizeof(T) == 4 ? norm_q8_refine<WARP>(top, turn, visit) : (double)top;
+        r.top = (double)top;
+        r.rounded = sizeof(T) == 4;
         const float rms = fsqrt(fadd(fdiv(ss, (float)p.cols), p.eps));
         r.scale = fdiv(top, fmul(127.0f, rms));
         return r;
@@ -162,6 +167,25 @@ __device__ __forceinline__ NormRow norm_q8_row(float ss, float top, int turn, co
         r.top = 0.0;
     }
     return r;
+}
+
+// f32 rows: the exact max|p| (all threads of the row).
+template <typename T, bool WARP, typename VISIT>
+__device__ __forceinline__ void norm_q8_exact(NormRow& r, int turn, VISIT visit) {
+    if (sizeof(T) == 4 && r.rounded) {
+        r.top = norm_q8_refine<WARP>((float)r.top, turn, visit);
+        r.rounded = false;
+    }
+}
+// The same behind the row's codes, if one of its threads has codes to decide.
+// In every row and before the codes it took 16.0 us instead of 14.6 at f32
+// [2048, 4096], 98 instead of 85 at [16384, 4096]; rows held element by element
+// are the faster for it, 20.9 instead of 22.6 us at [2047, 4097].
+template <typename T, bool WARP, typename VISIT>
+__device__ __forceinline__ void norm_q8_settle(NormRow& r, bool open, int turn, VISIT visit) {
+    if constexpr (sizeof(T) == 4) {
+        if (WARP ? __any_sync(0xffffffffu, open) : __syncthreads_or(open)) norm_q8_exact<T, WARP>(r, turn, visit);
+    }
 }
 
 // Codes nearest(127 p / top).
@@ -200,9 +224,11 @@ __device__ __noinline__ uint2 norm_decide(uint4 h, uint4 w, double top) {
 constexpr int NQ_VPT = 4;  // 16-byte vectors a thread holds
 
 // WARP: eight rows per 256-thread CTA; else one row per CTA of up to MAXT threads.
-// The register budget of 85 (three CTAs of 256) holds x, r and w of a thread.
+// The register budget of 85 (three CTAs of 256) holds x, r and w of a thread; f32
+// without r has room for a fourth CTA (14.0 us against 14.6, 77 against 85; with r
+// it spills, 27.8 against 22.0).
 template <typename T, bool ADD, bool WARP, int MAXT>
-__global__ void __launch_bounds__(MAXT, MAXT == 256 ? 3 : 1)
+__global__ void __launch_bounds__(MAXT, MAXT == 256 ? (sizeof(T) == 4 && !ADD ? 4 : 3) : 1)
     rmsnorm_q8_vec_kernel(const T* x, const T* r, const T* w, T* h, int8_t* y, float* scale, NormQ8Args p) {
     pdl_begin();
     constexpr int V = Vec<T>::N;
@@ -267,7 +293,7 @@ __global__ void __launch_bounds__(MAXT, MAXT == 256 ? 3 : 1)
         }
         float ss = fadd(acc.x, acc.y);
         norm_q8_reduce<WARP>(ss, top, turn);
-        const NormRow nr = norm_q8_row<T, WARP>(ss, top, turn, p, [&](auto f) {
+        auto visit = [&](auto f) {
 #pragma unroll
             for (int k = 0; k < NQ_VPT; ++k) {
                 if (t + k * tpr < nvec) {
@@ -278,7 +304,8 @@ __global__ void __launch_bounds__(MAXT, MAXT == 256 ? 3 : 1)
                     for (int e = 0; e < V; ++e) f(v[e], wv[e]);
                 }
             }
-        });
+        };
+        NormRow nr = norm_q8_row<T, WARP>(ss, top, p, visit);
         const NormCoder<T> coder(nr.top);
         uint32_t open = 0;  // vectors with codes that the definition has to decide
 #pragma unroll
@@ -299,6 +326,7 @@ __global__ void __launch_bounds__(MAXT, MAXT == 256 ? 3 : 1)
                 q8_store(y + off + (uint64_t)j * V, c);
             }
         }
+        norm_q8_settle<T, WARP>(nr, open != 0, turn, visit);
         if (open) {  // once more, behind the other stores
 #pragma unroll
             for (int k = 0; k < NQ_VPT; ++k)
@@ -349,10 +377,12 @@ __global__ void __launch_bounds__(MAXT, MAXT == 320 ? 3 : 1)
             top = norm_larger(top, fabsf(fmul(v[k], wv[k])));
         }
         norm_q8_reduce<false>(ss, top, turn);
-        const NormRow nr = norm_q8_row<T, false>(ss, top, turn, p, [&](auto f) {
+        auto visit = [&](auto f) {
 #pragma unroll
             for (int k = 0; k < EPT; ++k) f(v[k], wv[k]);
-        });
+        };
+        NormRow nr = norm_q8_row<T, false>(ss, top, p, visit);
+        norm_q8_exact<T, false>(nr, turn, visit);
         const NormCoder<T> coder(nr.top);
         uint32_t c[EPT], diff = 0;
 #pragma unroll
@@ -401,9 +431,11 @@ __global__ void __launch_bounds__(1024)
             top = norm_larger(top, fabsf(fmul(v, Vec<T>::load1(w + i))));
         }
         norm_q8_reduce<false>(ss, top, turn);
-        const NormRow nr = norm_q8_row<T, false>(ss, top, turn, p, [&](auto f) {
+        auto visit = [&](auto f) {
             for (uint32_t i = threadIdx.x; i < p.cols; i += blockDim.x) f(held(i), Vec<T>::load1(w + i));
-        });
+        };
+        NormRow nr = norm_q8_row<T, false>(ss, top, p, visit);
+        norm_q8_exact<T, false>(nr, turn, visit);
         const NormCoder<T> coder(nr.top);
 #pragma unroll 4
         for (uint32_t i = threadIdx.x; i < p.cols; i += blockDim.x) {
