@@ -86,6 +86,20 @@ def test_extreme_rows(cuda, dtype, cols):
 
 
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("residual", [False, True])
+@pytest.mark.parametrize("rows,cols", [(9000, 512), (5000, 515), (4000, 1024), (3000, 4096), (900, 5121), (700, 8191),
+                                       (500, 9001), (300, 8192)])
+def test_many_rows(cuda, dtype, residual, rows, cols):
+    """Several rows in turn to a warp and a CTA, some with codes that the
+    definition has to decide (every tenth f32 row at 4096 columns) and some not."""
+    x, r, w = _inputs(cuda, rows, cols, dtype, seed=11)
+    if residual:
+        _check(x, r, w, ops.add_rms_norm_q8(x, r, w, EPS))
+    else:
+        _check(x, None, w, ops.rms_norm_q8(x, w, EPS))
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
 @pytest.mark.parametrize("cols", [1024, 4096, 99])
 def test_in_place_sum_and_given_outputs(cuda, dtype, cols):
     x, r, w = _inputs(cuda, 33, cols, dtype, seed=5)
