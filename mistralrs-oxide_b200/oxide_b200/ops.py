@@ -10,6 +10,7 @@ op is one call into liboxide_b200.so.
 """
 from __future__ import annotations
 
+import functools
 import math
 from ctypes import c_float as _c_float
 from typing import Optional, Sequence
@@ -747,6 +748,14 @@ def kv_cache_read_q8(k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torc
     return k, v
 
 
+@functools.lru_cache(maxsize=1024)
+def _q8_attend_plan(b: int, hq: int, hkv: int, d: int):
+    """Workspace bytes of decode_attention_q8, and its default scale
+    1 / sqrt(head_dim) with each step rounded to f32."""
+    return (_lib.lib().oxide_decode_attention_q8_workspace_bytes(b, hq, hkv, d),
+            1.0 / _c_float(math.sqrt(d)).value if d else 1.0)
+
+
 def decode_attention_q8(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor,
                         v_scale: torch.Tensor, block: int, lens: Optional[torch.Tensor] = None,
                         scale: Optional[float] = None, workspace: Optional[torch.Tensor] = None,
@@ -767,7 +776,7 @@ def decode_attention_q8(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.T
         _q8_lens(op, "lens", lens, b)
     if out is not None:
         _out_like(op, q, out=out)
-    need = _lib.lib().oxide_decode_attention_q8_workspace_bytes(b, hq, hkv, d)
+    need, plain_scale = _q8_attend_plan(b, hq, hkv, d)
     if workspace is None:
         size = need
     else:
@@ -775,10 +784,10 @@ def decode_attention_q8(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.T
         if size < need:
             _bad(op, f"workspace must hold {need} bytes")
     _placed(op, q, k_cache, v_cache, k_scale, v_scale, lens, workspace, out)
-    if scale is None:  # 1 / sqrt(head_dim), each step rounded to f32
-        scale = 1.0 / _c_float(math.sqrt(d)).value if d else 1.0
+    if scale is None:
+        scale = plain_scale
     if workspace is None:
-        workspace = q.new_empty(need, dtype=torch.uint8)
+        workspace = torch.empty_strided((need,), (1,), dtype=torch.uint8, device=q.device)
     out = torch.empty_like(q) if out is None else out
     _call_on(q, f"oxide_decode_attention_q8_{_sfx(q)}", q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
              k_scale.data_ptr(), v_scale.data_ptr(), _p(lens), out.data_ptr(), b, hq, hkv, m, d, block, float(scale),

@@ -247,6 +247,41 @@ def test_graph_replay_with_growing_lengths(cuda):
         assert torch.equal(out, ops.decode_attention_q8(*case, 64, lens))
 
 
+@pytest.mark.parametrize("b,hq,hkv,d", [(3, 8, 2, 128), (299, 3, 1, 128), (301, 1, 1, 37), (151, 6, 2, 256),
+                                        (1201, 2, 2, 20), (1, 1, 1, 16)])
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_nothing_around_output_and_workspace(cuda, b, hq, hkv, d, dtype):
+    """Guards around both, whichever way the heads are merged."""
+    case = _case(cuda, b, hq, hkv, d, 150, 16, dtype)
+    lens = _lens(cuda, [(i * 47) % 151 for i in range(b)])
+    n = int(_lib.lib().oxide_decode_attention_q8_workspace_bytes(b, hq, hkv, d))
+    ws = torch.full((n + 4096,), 171, dtype=torch.uint8, device=cuda)
+    out = torch.full((b * hq * d + 64,), 7.0, dtype=case[0].dtype, device=cuda)
+    _run(case, 16, lens, workspace=ws[2048:2048 + n], out=out[32:32 + b * hq * d].view(b, hq, d))
+    assert bool((ws[:2048] == 171).all()) and bool((ws[2048 + n:] == 171).all())
+    assert bool((out[:32] == 7).all()) and bool((out[32 + b * hq * d:] == 7).all())
+
+
+def test_two_graphs_at_once(cuda):
+    """Two captured steps, replayed on two streams."""
+    cases = [_case(cuda, b, 8, 2, 128, 3000, 64, "bf16", seed=b) for b in (2, 5)]
+    want = [ops.decode_attention_q8(*c, 64) for c in cases]
+    torch.cuda.synchronize()
+    graphs, outs = [], []
+    for c in cases:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(ops.decode_attention_q8(*c, 64))
+        graphs.append(g)
+    streams = [torch.cuda.Stream() for _ in cases]
+    for _ in range(20):
+        for s, g in zip(streams, graphs):
+            with torch.cuda.stream(s):
+                g.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(outs, want))
+
+
 def test_matches_bf16_attention_of_the_values(cuda):
     """Against the unquantised operator over the values read back (exact in bf16
     when the scales are powers of two)."""
