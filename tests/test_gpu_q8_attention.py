@@ -365,10 +365,11 @@ def test_query_magnitudes(cuda):
     _close(got, want, tol)
 
 
-def test_a_wait_that_runs_out(cuda):
+@pytest.mark.parametrize("b,hq,hkv,d,m", [(2, 8, 2, 128, 1024), (3, 16, 2, 256, 700), (300, 4, 2, 64, 200)])
+def test_a_wait_that_runs_out(cuda, b, hq, hkv, d, m):
     """With its copies withheld every wait of the tensor-core kernel runs out:
     NaN outputs and the sticky flag, then the context works on."""
-    case = _case(cuda, 2, 8, 2, 128, 1024, 64, "bf16")
+    case = _case(cuda, b, hq, hkv, d, m, 64, "bf16")
     flags = _lib.C.c_uint32()
     _lib.call("oxide_device_status", 1, _lib.C.byref(flags))
     out = _on_path(2, case, 64, None)
