@@ -75,7 +75,8 @@ def test_lengths_out_of_range_and_all_positions(cuda, d):
 
 
 @pytest.mark.parametrize("hq,hkv,d,b,m", [(8, 2, 128, 1, 1), (8, 2, 128, 1, 40000), (32, 8, 128, 2, 9000),
-                                          (4, 4, 128, 300, 130), (4, 1, 64, 1, 30000), (2, 2, 48, 700, 40)])
+                                          (4, 4, 128, 300, 130), (4, 1, 64, 1, 30000), (2, 2, 48, 700, 40),
+                                          (67, 1, 128, 1, 5000), (67, 1, 37, 2, 900)])
 def test_work_division(cuda, hq, hkv, d, b, m):
     """One sequence over every worker, and many sequences to a worker."""
     case = _case(cuda, b, hq, hkv, d, m, 32, "bf16")
@@ -248,7 +249,7 @@ def test_graph_replay_with_growing_lengths(cuda):
 
 
 @pytest.mark.parametrize("b,hq,hkv,d", [(3, 8, 2, 128), (299, 3, 1, 128), (301, 1, 1, 37), (151, 6, 2, 256),
-                                        (1201, 2, 2, 20), (1, 1, 1, 16)])
+                                        (1201, 2, 2, 20), (1, 1, 1, 16), (4096, 2, 1, 16)])
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
 def test_nothing_around_output_and_workspace(cuda, b, hq, hkv, d, dtype):
     """Guards around both, whichever way the heads are merged."""
@@ -260,6 +261,22 @@ def test_nothing_around_output_and_workspace(cuda, b, hq, hkv, d, dtype):
     _run(case, 16, lens, workspace=ws[2048:2048 + n], out=out[32:32 + b * hq * d].view(b, hq, d))
     assert bool((ws[:2048] == 171).all()) and bool((ws[2048 + n:] == 171).all())
     assert bool((out[:32] == 7).all()) and bool((out[32 + b * hq * d:] == 7).all())
+
+
+@pytest.mark.parametrize("d", [128, 36, 37, 256, 1])
+@pytest.mark.parametrize("k_off,v_off,q_off", [(1, 0, 0), (0, 2, 0), (3, 5, 1), (4, 8, 0), (0, 0, 1), (16, 16, 8)])
+def test_unaligned(cuda, d, k_off, v_off, q_off):
+    """Tensors that start anywhere give the same values."""
+    case = _case(cuda, 3, 4, 2, d, 333, 8, "bf16")
+
+    def moved(t, off):
+        buf = torch.full((t.numel() + off + 16,), 99, dtype=t.dtype, device=cuda)
+        buf[off:off + t.numel()] = t.reshape(-1)
+        return buf[off:off + t.numel()].view(t.shape)
+
+    lens = _lens(cuda, [333, 64, 100])
+    out = moved(torch.zeros_like(case[0]), q_off)
+    _run((moved(case[0], q_off), moved(case[1], k_off), moved(case[2], v_off), *case[3:]), 8, lens, out=out)
 
 
 def test_two_graphs_at_once(cuda):
