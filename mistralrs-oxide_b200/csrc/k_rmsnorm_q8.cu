@@ -15,9 +15,10 @@
 // bf16: p is exact in f32 (two 8-bit significands).  f32: p in f32 decides
 // almost every code; the products of two floats are exact in f64, max|p| there
 // is the largest of the elements whose f32 product is the f32 maximum (rounding
-// is monotonic), and a code next to a half-integer is decided from the f64
-// product (oxide_q8.cuh).  Rows of vectors look for max|p| in f64 only where they
-// have such a code, one in ten at 4096 columns.
+// is monotonic), and a code next to a half-integer is decided by the sign of
+// 254 p - (2 n + 1) max|p|, taken without rounding (norm_nearest; the f64 quotient
+// 127 p / max|p| is off by 2^-46 and missed half-integers).  Rows of vectors look
+// for max|p| in f64 only where they have such a code, one in ten at 4096 columns.
 //
 // Layout.  A warp (rows of at most 128 vectors of 16 bytes) or a CTA owns a
 // row and keeps it packed in registers, four vectors a thread, so each row
@@ -188,6 +189,24 @@ __device__ __forceinline__ void norm_q8_settle(NormRow& r, bool open, int turn, 
     }
 }
 
+// nearest(127 p / top) for |p| <= top of at most 48 bits each, ties to even; 0
+// where top is zero.  The f64 quotient, off by 2^-46, decides all but those next
+// to a half-integer.  There 254 |p| = hi + lo exactly, and hi - (2 n + 1) top
+// from one fused step is less than 2^16 units of the last place of either, so
+// exact: the sum of the two has the sign of 254 |p| - (2 n + 1) top. 
+static __device__ __noinline__ int norm_nearest(double p, double top) {
+    if (!(top > 0.0)) return 0;
+    const double a = fabs(p), q = 127.0 * a / top, n = rint(q);
+    int c = (int)n;
+    if (fabs(q - n) > 0.5 - 0x1p-40) {
+        const double hi = 254.0 * a, lo = __fma_rn(254.0, a, -hi);
+        const double up = __fma_rn(-(2.0 * n + 1.0), top, hi) + lo, down = __fma_rn(-(2.0 * n - 1.0), top, hi) + lo;
+        if (up > 0.0 || (up == 0.0 && (c & 1))) ++c;
+        else if (down < 0.0 || (down == 0.0 && (c & 1))) --c;
+    }
+    return p < 0.0 ? -c : c;
+}
+
 // Codes nearest(127 p / top).
 template <typename T>
 struct NormCoder {
@@ -202,7 +221,7 @@ struct NormCoder {
           slow(!norm_sure(ftop)),
           br(inv) {}
     __device__ __forceinline__ int exact(float h, float w) const {
-        if (sizeof(T) == 4 || slow) return q8_exact((double)h * (double)w, 127.0, top);
+        if (sizeof(T) == 4 || slow) return norm_nearest((double)h * (double)w, top);
         const float p = fmul(h, w);  // 16 bits; 254 |p| and (2 n + 1) top are exact
         return q8_beside(p, 254.0f * fabsf(p), inv, ftop);
     }
@@ -342,8 +361,9 @@ __global__ void __launch_bounds__(MAXT, MAXT == 256 ? (sizeof(T) == 4 && !ADD ? 
 
 // Rows that are no whole aligned vectors, element by element in registers:
 // thread t holds columns t + k blockDim.x, EPT of them, and its part of w.
-// [2047, 4097] f32 20.3 us, 2.1 TB/s: loads of one element a thread.  (Aligned
-// vectors shifted into place between neighbours took 24.6 us.)
+// [2047, 4097] f32 19.3 us, 2.2 TB/s: loads of one element a thread.  (Aligned
+// vectors shifted into place between neighbours took 24.6 us; all of a thread's
+// codes decided by the definition where one of them has to be, 21.6.)
 template <typename T, bool ADD, int EPT, int MAXT>
 __global__ void __launch_bounds__(MAXT, MAXT == 320 ? 3 : (MAXT == 640 ? 2 : 1))
     rmsnorm_q8_odd_kernel(const T* x, const T* r, const T* w, T* h, int8_t* y, float* scale, NormQ8Args p) {
@@ -384,16 +404,19 @@ __global__ void __launch_bounds__(MAXT, MAXT == 320 ? 3 : (MAXT == 640 ? 2 : 1))
         NormRow nr = norm_q8_row<T, false>(ss, top, p, visit);
         norm_q8_exact<T, false>(nr, turn, visit);
         const NormCoder<T> coder(nr.top);
-        uint32_t c[EPT], diff = 0;
+        uint32_t c[EPT], open = 0;  // pairs with codes that the definition has to decide
 #pragma unroll
         for (int k = 0; k < EPT; k += 2) {
+            uint32_t diff = 0;
             const uint2 q = coder.br.two(fmul2(f2(v[k], v[k + 1]), f2(wv[k], wv[k + 1])), diff);
             c[k] = q.x;
             c[k + 1] = q.y;
+            open |= (coder.slow || diff != 0 ? 1u : 0u) << k;
         }
-        if (coder.slow || diff != 0) {
+        if (open) {
 #pragma unroll
-            for (int k = 0; k < EPT; ++k) c[k] = (uint32_t)coder.exact(v[k], wv[k]);
+            for (int k = 0; k < EPT; ++k)
+                if (open >> (k & ~1) & 1u) c[k] = (uint32_t)coder.exact(v[k], wv[k]);
         }
 #pragma unroll
         for (int k = 0; k < EPT; ++k) {

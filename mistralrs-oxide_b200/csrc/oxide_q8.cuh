@@ -11,7 +11,8 @@
 // the order of any sum or on the rounding of a reciprocal, and a 64-bit
 // evaluation of the definition gives the same ones (near a half-integer
 // x - (n + 1/2) s is a multiple of ulp(s) / 4, so another quotient is at least
-// 2^-26 away from it, far above f64's 2^-47).
+// 2^-26 away from it, far above f64's 2^-47).  The norms' quotients are of
+// 48-bit products: theirs take another decision (k_rmsnorm_q8.cu).
 #pragma once
 
 #include "oxide_common.cuh"
@@ -54,15 +55,6 @@ __device__ __forceinline__ uint32_t q8_vec_amax(uint4 v, uint32_t a, bf16_t) {
 }
 __device__ __forceinline__ uint32_t q8_amax_join(uint32_t a, float) { return a; }
 __device__ __forceinline__ uint32_t q8_amax_join(uint32_t a, bf16_t) { return max(a << 16, a & 0xffff0000u); }
-
-// The definition in f64 for every divisor: nearest(x num / den), 0 where the
-// divisor is zero or not finite.  The quotient passes 127 only against a
-// subnormal scale, whose own rounding is coarse: it is held to 127.
-static __device__ __noinline__ int q8_exact(double x, double num, double den) {
-    if (!(den > 0.0 && den <= 1.7976931348623157e308)) return 0;
-    const double q = rint(x * num / den);
-    return (int)(q > 127.0 ? 127.0 : (q < -127.0 ? -127.0 : q));
-}
 
 // The bracket of x times a factor.
 struct Q8Bracket {

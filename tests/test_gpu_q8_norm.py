@@ -160,3 +160,41 @@ def test_other_stream_and_graph(cuda):
     graph.replay()
     torch.cuda.synchronize()
     _check(x, r, w, (h, codes, scale))
+
+
+def _integer_codes(h, w):
+    """nearest(127 p / max|p|), ties to even, of one row of f32 values, in whole
+    numbers: products of two significands have 48 bits and do not fit f64's 127 p."""
+    from fractions import Fraction
+    p = [Fraction(a) * Fraction(b) for a, b in zip(h.tolist(), w.tolist())]
+    top = max(abs(v) for v in p)
+    return [round(127 * v / top) for v in p]  # round() of a Fraction takes ties to even
+
+
+@pytest.mark.parametrize("cols", [64, 1024, 8192, 77, 4097, 17000])
+@pytest.mark.parametrize("residual", [False, True])
+def test_exact_ties_of_full_products(cuda, cols, residual):
+    """f32 rows whose products fill 48 bits and whose quotients are half-integers:
+    w the same everywhere, the largest h 254 a units and the others (2 n + 1) a,
+    with an a of 16 bits, so 127 p / max|p| is n + 1/2.  Some elements stand a
+    unit beside their tie.  Rows above and below the range of f32 products too."""
+    g = torch.Generator().manual_seed(cols)
+    scales = [1.0, 2.0 ** 60, 2.0 ** -70, 2.0 ** 40] * 3
+    x = torch.zeros(len(scales), cols, dtype=torch.float64)
+    w = (2 ** 23 + int(torch.randint(0, 2 ** 22, (1,), generator=g)) * 2 + 1) / 2.0 ** 23
+    for i, s in enumerate(scales):
+        a = int(torch.randint(2 ** 15, 2 ** 16, (1,), generator=g)) | 1
+        n = torch.randint(-127, 127, (cols,), generator=g)
+        u = (2 * n + 1) * a
+        u[::7] += (n[::7] % 3) - 1
+        u.clamp_(-254 * a, 254 * a)
+        u[int(torch.randint(0, cols, (1,), generator=g))] = 254 * a
+        x[i] = u.double() * s / 2.0 ** 22
+    x, w = x.float(), torch.full((cols,), w, dtype=torch.float32)
+    r = torch.zeros_like(x)
+    if residual:
+        codes = ops.add_rms_norm_q8(x.to(cuda), r.to(cuda), w.to(cuda), EPS)[1]
+    else:
+        codes = ops.rms_norm_q8(x.to(cuda), w.to(cuda), EPS)[0]
+    for i in range(len(scales)):
+        assert codes[i].tolist() == _integer_codes(x[i], w), i
