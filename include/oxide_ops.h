@@ -328,7 +328,9 @@ int oxide_kv_cache_append_bf16(oxide_bf16* k_cache, oxide_bf16* v_cache, const o
  * Caches [batch, kv_heads, max_seq, head_dim] of int8 codes with f32 scales
  * [batch, kv_heads, nblk], nblk = ceil(max_seq / block): one scale for each
  * `block` consecutive positions of a head (block a power of two in [1, 128]);
- * a code c stands for c * scale.  API addition: the reference's cache is f32.
+ * a code c stands for c * scale.  Scales are finite and not negative, or NaN (an
+ * append leaves no others; a cache made elsewhere must not hold others where
+ * tokens are appended).  API addition: the reference's cache is f32.
  *
  * Append: k, v [batch, kv_heads, new_len, head_dim] are quantised into
  * positions [cur, cur + n) of each sequence, both in one launch.  cur is
@@ -422,13 +424,13 @@ int oxide_decode_attention_bf16(const oxide_bf16* q, const oxide_bf16* k_cache, 
  * h / (q_heads / kv_heads).  q, out [batch, q_heads, head_dim], f32 or bf16,
  * head_dim <= 256, batch <= 4096.  Sums, scores and softmax statistics are
  * f32 (the tensor-core products are exact integer sums of q and p written in
- * 23 bits).  A sequence of length 0 gives zeros; a key whose block has the
- * scale NaN, or a query head that holds a NaN or an infinity, gives NaN;
- * positions at or behind lens[b] and their scales may hold anything.  out must
- * not alias q.  `workspace` is device memory of at least
- * oxide_decode_attention_q8_workspace_bytes(...) bytes, 16-byte aligned, that
- * no other call which may run at the same time uses; it needs no
- * initialisation. */
+ * 23 bits).  A sequence of length 0 gives zeros; a key whose block has a
+ * scale, in k or in v, that is NaN, infinite or negative, or a query head that
+ * holds a NaN or an infinity, gives NaN; positions at or behind lens[b] and
+ * their scales may hold anything.  out must not alias q.  `workspace` is
+ * device memory of at least oxide_decode_attention_q8_workspace_bytes(...)
+ * bytes, 16-byte aligned, that no other call which may run at the same time
+ * uses; it needs no initialisation. */
 uint64_t oxide_decode_attention_q8_workspace_bytes(uint64_t batch, uint64_t q_heads, uint64_t kv_heads,
                                                    uint64_t head_dim);
 int oxide_decode_attention_q8_f32(const float* q, const int8_t* k_cache, const int8_t* v_cache,

@@ -109,8 +109,8 @@ __global__ void __launch_bounds__(QW_WARPS * 32, 2) decode_attn_q8_warp_kernel(Q
         for (int h = 0; h < NR; ++h) dot[h] = 0.0f;
         if (on) {
             const uint32_t key = key0 + lane;
-            ks = __ldg(ksh + (key >> p.shift));
             vs = __ldg(vsh + (key >> p.shift));
+            ks = q8a_key_scale(__ldg(ksh + (key >> p.shift)), vs);
             const int8_t* row = kh + (uint64_t)key * D;
             if (WORDS && D % 16 == 0) {
 #pragma unroll 4

@@ -456,12 +456,11 @@ __global__ void __launch_bounds__(QT_THREADS, 1)
             ++ahead;
             w.next();
         };
-        // What a softmax thread needs of its key: the key scale and log2 of the
-        // value scale.  A value scale that is NaN, infinite or negative makes
-        // the key's scores NaN; +infinity as the log2 marks a masked key.
+        // What a softmax thread needs of its key: the key scale (NaN where the scales
+        // are not sound) and log2 of the value scale; +infinity as the log2 marks a
+        // masked key.
         auto ready = [&](float k, float v) -> float2 {
-            const bool sound = v >= 0.0f && v < INFINITY;
-            return make_float2(sound ? k : q8_nan(), sound ? lg2_approx(v) : 0.0f);
+            return make_float2(q8a_key_scale(k, v), v >= 0.0f && v < INFINITY ? lg2_approx(v) : 0.0f);
         };
         auto put = [&](const Keys& x) -> bool {
             float2 r[4];

@@ -70,6 +70,12 @@ __device__ __forceinline__ uint32_t q8a_owner(const Q8AttnArgs& p, uint32_t t, u
     return q;
 }
 
+// The key scale to use: a key whose block has a scale that is NaN, infinite or
+// negative, in k or in v, has the score NaN, in both kernels alike.
+__device__ __forceinline__ float q8a_key_scale(float k, float v) {
+    return k >= 0.0f && k < INFINITY && v >= 0.0f && v < INFINITY ? k : q8_nan();
+}
+
 // One warp: the prefix of the batches' tile counts into shared memory, pre[0 .. batch].
 __device__ __forceinline__ void q8a_prefix(const Q8AttnArgs& p, uint32_t tile, uint32_t* pre, bool store) {
     const uint32_t lane = threadIdx.x & 31;

@@ -396,3 +396,23 @@ def test_a_wait_that_runs_out(cuda, b, hq, hkv, d, m):
     _run(case, 64, None)
     _lib.call("oxide_device_status", 0, _lib.C.byref(flags))
     assert flags.value == 0
+
+
+@pytest.mark.parametrize("hq,hkv,d", [(8, 2, 128), (2, 2, 128), (6, 2, 80), (8, 2, 256), (4, 2, 37), (6, 3, 20)])
+@pytest.mark.parametrize("block", [1, 16])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), float("-inf"), -0.01])
+def test_scales_that_are_not_sound(cuda, hq, hkv, d, block, bad):
+    """A key or value scale that is NaN, infinite or negative makes exactly the
+    heads NaN that read its block, on either kernel."""
+    lens, rep = _lens(cuda, [200, 200, 200]), hq // hkv
+    case = _case(cuda, 3, hq, hkv, d, 256, block, "f32")
+    clean = [_on_path(path, case, block, lens) for path in (0, 1)]
+    case[3][0, 0, 77 // block] = bad
+    case[4][1, hkv - 1, 199 // block] = bad
+    case[3][2, 0, 255 // block] = case[4][2, 0, 240 // block] = bad  # behind the length
+    want = torch.zeros(3, hq, dtype=torch.bool, device=cuda)
+    want[0, :rep] = want[1, -rep:] = True
+    for path in (0, 1):
+        got = _on_path(path, case, block, lens)
+        assert torch.equal(torch.isnan(got).all(-1), want) and torch.equal(torch.isnan(got).any(-1), want)
+        assert torch.equal(got[~want], clean[path][~want])
