@@ -426,8 +426,8 @@ int oxide_decode_attention_bf16(const oxide_bf16* q, const oxide_bf16* k_cache, 
  * f32 (the tensor-core products are exact integer sums of q and p written in
  * 23 bits).  A sequence of length 0 gives zeros; a key whose block has a
  * scale, in k or in v, that is NaN, infinite or negative, or a query head that
- * holds a NaN or an infinity, gives NaN; positions at or behind lens[b] and
- * their scales may hold anything.  out must not alias q.  `workspace` is
+ * holds a NaN or an infinity, or whose every score is -infinity, gives NaN;
+ * positions at or behind lens[b] and their scales may hold anything.  out must not alias q.  `workspace` is
  * device memory of at least oxide_decode_attention_q8_workspace_bytes(...)
  * bytes, 16-byte aligned, that no other call which may run at the same time
  * uses; it needs no initialisation. */

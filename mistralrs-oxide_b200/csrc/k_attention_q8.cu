@@ -215,8 +215,9 @@ __global__ void __launch_bounds__(QW_WARPS * 32, 2) decode_attn_q8_warp_kernel(Q
 // NW-th part of the pair, the loads of QC_UNROLL of them in flight at once (the
 // parts' places follow from the tile division alone), lane = four dims (DV of
 // them 128 apart), and the NW states are joined through shared memory.  A part
-// without keys has sum 0; a pair without keys gives zeros; NaN if a wait of the
-// main kernel ran out.
+// whose scores are all -infinity has sum 0.  A pair without keys gives zeros; one
+// with keys and no weight (every score -infinity) gives NaN, as 0 / 0 in the
+// definition, and so does everything if a wait of the main kernel ran out.
 // NW: 8 warps while there are fewer CTAs than SMs -- a CTA then merges many
 // parts (one sequence of 131072 keys, 37 parts a head: the whole call 51.0 us
 // against 53.0 with 4) -- else 4, so that more CTAs are resident at once (8
@@ -310,8 +311,9 @@ __global__ void __launch_bounds__(NW * 32) decode_attn_q8_combine_kernel(T* out,
     const uint32_t heads = p.kv_heads * p.chunks, D = p.head_dim, all = p.pre_out[p.batch] * heads;
     const uint32_t failed = *p.err, bh = EACH ? blockIdx.x * NW + warp : blockIdx.x;
     if (EACH && bh >= p.batch * p.q_heads) return;
-    const Q8State<DV> s =
-        q8_merge<DV>(p, q8_parts(p, bh, heads, all), all, EACH ? 0 : warp, EACH ? 1 : NW, lane);
+    const Q8Parts x = q8_parts(p, bh, heads, all);
+    const Q8State<DV> s = q8_merge<DV>(p, x, all, EACH ? 0 : warp, EACH ? 1 : NW, lane);
+    const float none = x.n == 0 ? 0.0f : q8_nan();
     if constexpr (EACH) {
 #pragma unroll
         for (int k = 0; k < DV; ++k) {
@@ -319,7 +321,7 @@ __global__ void __launch_bounds__(NW * 32) decode_attn_q8_combine_kernel(T* out,
 #pragma unroll
             for (uint32_t e = 0; e < 4; ++e) {
                 const uint32_t d = 4 * (lane + 32 * k) + e;
-                const float y = failed ? q8_nan() : (s.L == 0.0f ? 0.0f : fdiv(o[e], s.L));
+                const float y = failed ? q8_nan() : (s.L == 0.0f ? none : fdiv(o[e], s.L));
                 if (d < D) Vec<T>::store1(out + (uint64_t)bh * D + d, y);
             }
         }
@@ -338,11 +340,11 @@ __global__ void __launch_bounds__(NW * 32) decode_attn_q8_combine_kernel(T* out,
 #pragma unroll
             for (int i = 0; i < NW; ++i) {
                 if (wl[i] == 0.0f) continue;
-                const float x = ex2_approx(fsub(wm[i], mx));
-                ls = __fmaf_rn(wl[i], x, ls);
-                o = __fmaf_rn(reinterpret_cast<const float*>(wo[i])[d], x, o);
+                const float f = ex2_approx(fsub(wm[i], mx));
+                ls = __fmaf_rn(wl[i], f, ls);
+                o = __fmaf_rn(reinterpret_cast<const float*>(wo[i])[d], f, o);
             }
-            float y = ls == 0.0f ? 0.0f : fdiv(o, ls);
+            float y = ls == 0.0f ? none : fdiv(o, ls);
             if (failed) y = q8_nan();
             Vec<T>::store1(out + (uint64_t)bh * D + d, y);
         }

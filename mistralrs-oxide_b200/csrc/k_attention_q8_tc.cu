@@ -73,8 +73,9 @@ constexpr uint32_t QT_TK = 128, QT_DB = 128;  // keys a tile, bytes a row of a t
 constexpr int QT_THREADS = 416;
 constexpr uint32_t QT_MAX_BATCH = 1024;
 // Maxima start here, not at -infinity: differences stay numbers, and a masked
-// score (-infinity) is a zero weight without being asked about.
-constexpr float QT_LOW = -3.0e38f;
+// score (-infinity) is a zero weight without being asked about.  No finite
+// score is lower.
+constexpr float QT_LOW = -3.402823466e38f;
 constexpr float Q_UNIT = 8.0e6f;  // below 0x7f7f7f = 8355711, the largest three balanced digits hold
 constexpr uint32_t QT_TILE = QT_TK * QT_DB;  // 16 KB
 constexpr uint32_t QT_BBYTES = 32 * 128;     // a B operand: up to 32 rows of 128 bytes

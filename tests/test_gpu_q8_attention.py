@@ -416,3 +416,32 @@ def test_scales_that_are_not_sound(cuda, hq, hkv, d, block, bad):
         got = _on_path(path, case, block, lens)
         assert torch.equal(torch.isnan(got).all(-1), want) and torch.equal(torch.isnan(got).any(-1), want)
         assert torch.equal(got[~want], clean[path][~want])
+
+
+@pytest.mark.parametrize("hq,hkv,d", [(8, 2, 128), (2, 2, 128), (6, 2, 80), (8, 2, 256), (4, 2, 37), (6, 3, 20)])
+@pytest.mark.parametrize("m", [1, 40, 300])
+def test_scores_of_minus_infinity(cuda, hq, hkv, d, m):
+    """A head whose every score is -infinity (an infinite query element over codes
+    of the other sign; products beyond f32) has no softmax: NaN, not the zeros of
+    an empty sequence.  Where one key has a finite score, it takes all."""
+    case = _case(cuda, 4, hq, hkv, d, m, 16, "f32")
+    q, kc, vc, ks, vs = case
+    q[0, 0, 3] = float("inf")
+    q[1, hq - 1, 3] = float("-inf")
+    kc[0, :, :, 3] = -7
+    kc[1, :, :, 3] = 7
+    q[2] = 3e38
+    kc[2] = -100
+    q[3] = 3e38
+    kc[3] = -100
+    kc[3, :, m // 2] = 0
+    lens = _lens(cuda, [m, m, m, m])
+    bad = torch.zeros(4, hq, dtype=torch.bool, device=cuda)
+    bad[0, 0] = bad[1, hq - 1] = bad[2] = True
+    only = (vc[3, :, m // 2].double() * vs[3, :, m // 2 // 16, None]).repeat_interleave(hq // hkv, 0)
+    for path in (0, 1):
+        got = _on_path(path, case, 16, lens)
+        assert torch.equal(torch.isnan(got).all(-1), bad) and torch.equal(torch.isnan(got).any(-1), bad)
+        # one weight of 1: the product code * scale, and at most four roundings and two base-2 functions
+        assert bool(((got[3] - only).abs() <= (4 * 2.0 ** -24 + 2 * 2.0 ** -22) * only.abs()).all())
+        assert bool((_on_path(path, case, 16, _lens(cuda, [0, 0, 0, 0])) == 0).all())
