@@ -423,8 +423,9 @@ int oxide_decode_attention_bf16(const oxide_bf16* q, const oxide_bf16* k_cache, 
  * to [0, max_seq]), out = sum_j p_j v_j; query head h reads kv head
  * h / (q_heads / kv_heads).  q, out [batch, q_heads, head_dim], f32 or bf16,
  * head_dim <= 256, batch <= 4096.  Sums, scores and softmax statistics are
- * f32 (the tensor-core products are exact integer sums of q and p written in
- * 23 bits).  A sequence of length 0 gives zeros; a key whose block has a
+ * f32.  On the tensor cores both products are exact integer sums: of q held to
+ * 2^-23 of its head's largest element, and of the weights (p times the value
+ * scale) held to 2^-61 of the largest of each tile of 128 keys.  A sequence of length 0 gives zeros; a key whose block has a
  * scale, in k or in v, that is NaN, infinite or negative, or a query head that
  * holds a NaN or an infinity, or whose every score is -infinity, gives NaN;
  * positions at or behind lens[b] and their scales may hold anything.  out must not alias q.  `workspace` is

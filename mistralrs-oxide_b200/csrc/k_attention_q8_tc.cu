@@ -9,12 +9,16 @@
 //   q . c = (x0 . c + 256 x1 . c + 65536 x2 . c) u: the three digit rows are
 //   three columns of one product (each sum at most 2^22, exact in f32), and q
 //   is held to 2^-23 of its largest element, as good as f32 sums;
-//   p_j vs_j (the softmax weight times the value block's scale) likewise, as
-//   integers against the largest of the tile, found in the log2 domain
+//   p_j vs_j (the softmax weight times the value block's scale) likewise, in
+//   eight digits: an integer in units of 2^-30 of the largest of the tile, and
+//   what that leaves in units of 2^-61.  The largest is found in the log2 domain
 //   (t_j + log2 vs_j), so neither a far maximum in another tile nor blocks
-//   with very different scales cost a weight its digits.
-// The padding of the N side, which a group of at most eight query heads leaves
-// anyway, carries the digits: the tensor cores read the cache once.
+//   with very different scales cost a weight its digits.  A weight down to 2^-37 of
+//   its tile's largest keeps f32's 24 bits: where one key holds the weight and its
+//   values are zero or cancel, the others make up the output (with three digits
+//   it was off by 1 % where that key's score was 12 to 14 above theirs).
+// The N side of a product, which is 16 wide at least, carries the digits: the
+// tensor cores read the cache once for up to eight query heads of a kv head.
 //
 // Work division as in k_attention_tc.cu (tiles of 128 keys laid end to end,
 // one CTA per SM, equal ranges); partials as in oxide_attn_q8.cuh, two halves
@@ -27,15 +31,18 @@
 //
 // CTA of 13 warps:
 //   warp 0      TMA producer: K and V tiles [128 keys x 128 bytes],
-//               128-byte swizzle, a ring of 192 KB: 6 stages of 32 KB, or 3 of
-//               64 KB with two halves;
+//               128-byte swizzle, a ring of up to 192 KB: 6 stages of 32 KB, or
+//               3 of 64 KB with two halves (5 and 2 with eight heads, whose
+//               operands take the room);
 //   warp 1      TMEM owner and issuer of the scores' products,
 //                 S[128 keys x N] = K . X^T   (A = K, K-major; B = digits of q);
 //   warp 12     issuer of the outputs' products,
 //                 O[128 dims x N] = V^T . Y^T (A = V read MN-major; B = digits
-//                                              of the weights),
-//               N = 16 for up to 4 heads, 32 for 8 (M = 128 takes N in steps
-//               of 16).  One thread issuing both spent 2100 cycles a tile on
+//                                              of the weights, N-major: a
+//                                              key's digits are 8 to 64 bytes
+//                                              in a row, one to four stores of
+//                                              its thread),
+//               N = digits times heads, in steps of 16.  One thread issuing both spent 2100 cycles a tile on
 //               waits and issue, twice what the loads allow;
 //   warp 2      the query heads' digits, one pair ahead, from raw bits loaded two
 //               pairs ahead.  (A second such warp gained nothing, nor did asking
@@ -76,21 +83,33 @@ constexpr uint32_t QT_MAX_BATCH = 1024;
 // score (-infinity) is a zero weight without being asked about.  No finite
 // score is lower.
 constexpr float QT_LOW = -3.402823466e38f;
-constexpr float Q_UNIT = 8.0e6f;  // below 0x7f7f7f = 8355711, the largest three balanced digits hold
 constexpr uint32_t QT_TILE = QT_TK * QT_DB;  // 16 KB
-constexpr uint32_t QT_BBYTES = 32 * 128;     // a B operand: up to 32 rows of 128 bytes
-// Places of the kernel for DH halves of 128 bytes a row (head_dim up to 128, 256).
-template <int DH>
+constexpr uint32_t QT_SMEM = 227 * 1024;     // what a CTA can have
+constexpr int QT_QD = 3, QT_PD = 8;           // digits of a query element, of a weight
+
+// Rows of a B operand, and columns of its product: `digits` of NR query heads
+// (M = 128 takes N in steps of 16).
+constexpr uint32_t qt_n(int nr, int digits) { return (uint32_t)(nr * digits + 15) / 16 * 16; }
+
+// Places of the kernel for NR query heads and DH halves of 128 bytes a
+// row (head_dim up to 128, 256).
+template <int NR, int DH>
 struct QtMap {
-    static constexpr int STAGES = 6 / DH;
-    static constexpr uint32_t STAGE_BYTES = 2 * DH * QT_TILE;  // K, V
-    static constexpr uint32_t Q_BYTES = DH * QT_BBYTES;
-    // TMEM columns: S of group g at 32 g, its O (half x) at O + 32 (DH g + x)
-    static constexpr uint32_t TMEM_COLS = 128 * DH, O = 64;
+    static constexpr uint32_t NS = qt_n(NR, QT_QD), NO = qt_n(NR, QT_PD);  // columns of S, of O
+    static constexpr uint32_t STAGE_BYTES = 2 * DH * QT_TILE;           // K, V
+    static constexpr uint32_t Q_HALF = NS * QT_DB, Q_BYTES = DH * Q_HALF, P_BYTES = NO * QT_DB;
+    // as many stages as fit, at most 192 KB
+    static constexpr uint32_t FIXED = 2 * Q_BYTES + 2 * P_BYTES + (QT_MAX_BATCH + 8) * 4 + 2048 + 1024;
+    static constexpr int FIT = (int)((QT_SMEM - FIXED) / (STAGE_BYTES + QT_TK * 8));
+    static constexpr int STAGES = FIT < 6 / DH ? FIT : 6 / DH;
+    // TMEM columns: S of group g at SW g, its O (half x) at O + OW (DH g + x)
+    static constexpr uint32_t SW = NS < 32 ? 32 : NS, OW = NO < 32 ? 32 : NO, O = 2 * SW;
+    static constexpr uint32_t TMEM_USED = O + 2 * DH * OW;
+    static constexpr uint32_t TMEM_COLS = TMEM_USED <= 128 ? 128 : (TMEM_USED <= 256 ? 256 : 512);
     // shared memory (offsets from a 1024-byte aligned base)
     static constexpr uint32_t OFF_Q = STAGES * STAGE_BYTES;                  // 2 slots
     static constexpr uint32_t OFF_P = OFF_Q + 2 * Q_BYTES;                   // 2 groups
-    static constexpr uint32_t OFF_PRE = OFF_P + 2 * QT_BBYTES;
+    static constexpr uint32_t OFF_PRE = OFF_P + 2 * P_BYTES;
     static constexpr uint32_t OFF_SC = OFF_PRE + (QT_MAX_BATCH + 8) * 4;     // a stage's keys: float2 [128]
     static constexpr uint32_t OFF_SQ = OFF_SC + STAGES * QT_TK * 8;          // [2][8] factors of the scores
     static constexpr uint32_t OFF_RED = OFF_SQ + 2 * 8 * 4;                  // [2][4][16] each warp's tile maxima
@@ -112,33 +131,53 @@ struct QtMap {
     static constexpr uint32_t OFF_MISC = OFF_BAR + ((COUNT + 1) & ~1) * 8;
     static constexpr size_t SMEM = OFF_MISC + 48 + 1024;  // + alignment slack
 };
-// One half: room is left beside the CTA for one of the combine kernel (4.1 KB),
-// which is launched early and waits there.
-static_assert(QtMap<1>::SMEM <= 221 * 1024 && QtMap<2>::SMEM <= 227 * 1024, "shared memory of one CTA");
 static_assert(2 * 1024 <= Q8A_PARTS, "two parts a CTA fit the workspace");
 
 __device__ unsigned int g_device_status_q8;  // sticky failure flags, read by oxide_device_status
 
-// Columns of a product, and how many of them are read back (three digits a head).
-template <int NR>
-constexpr uint32_t qt_n() { return (3 * NR + 15) / 16 * 16; }
-template <int NR>
-constexpr uint32_t qt_cols() { return (3 * NR + 7) / 8 * 8; }
-
-template <int NR>
-__device__ __forceinline__ void qt_load(uint32_t taddr, uint32_t (&v)[qt_cols<NR>()]) {
+// C columns of TMEM (a multiple of 8).
+template <int C>
+__device__ __forceinline__ void qt_load(uint32_t taddr, uint32_t (&v)[C]) {
+    if constexpr (C == 16) tmem_ld16(taddr, v);
+    else
 #pragma unroll
-    for (int i = 0; i < (int)qt_cols<NR>(); i += 8) tmem_ld8(taddr + i, v + i);
+        for (int i = 0; i < C; i += 8) tmem_ld8(taddr + i, v + i);
     tmem_wait_ld();
 }
-// Three digit sums as the number they spell (each sum is at most 2^22 in
-// magnitude, so the lower two join in 32 bits).
+// The number that the sums of four digits spell.  Each sum is at most 2^22 in
+// magnitude, so two of them join in 32 bits; the upper two are a whole number
+// that f32 holds, or else far above the lower ones.
+__device__ __forceinline__ float qt_spell(uint32_t d0, uint32_t d1, uint32_t d2, uint32_t d3) {
+    return __fmaf_rn((float)((int)d3 * 256 + (int)d2), 65536.0f, (float)((int)d1 * 256 + (int)d0));
+}
 __device__ __forceinline__ float qt_spell(uint32_t d0, uint32_t d1, uint32_t d2) {
     return __fmaf_rn((float)(int)d2, 65536.0f, (float)((int)d1 * 256 + (int)d0));
 }
-// Balanced digits of |x| <= Q_UNIT in bytes 0, 1, 2.
-__device__ __forceinline__ uint32_t qt_digits(float x) {
-    return ((uint32_t)__float2int_rn(x) + 0x808080u) ^ 0x808080u;
+// Balanced digits of an integer in bytes 0 .. 3 (|x| <= 0x7f7f7f7f, or 0x7f7f7f for
+// the first three alone).
+__device__ __forceinline__ uint32_t qt_digits(int x) { return ((uint32_t)x + 0x80808080u) ^ 0x80808080u; }
+// Scores: digit i of head h is column i NR + h.
+template <int NR>
+__device__ __forceinline__ void qt_scores(uint32_t taddr, float (&x)[NR]) {
+    uint32_t v[(3 * NR + 7) / 8 * 8];
+    qt_load(taddr, v);
+#pragma unroll
+    for (int h = 0; h < NR; ++h) x[h] = qt_spell(v[h], v[NR + h], v[2 * NR + h]);
+}
+// Outputs: digit i of head h is column 8 h + i, the upper four first.
+template <int NR>
+__device__ __forceinline__ void qt_outputs(uint32_t taddr, float (&x)[NR]) {
+    constexpr int H = NR < 2 ? NR : 2;  // heads at once
+#pragma unroll
+    for (int h0 = 0; h0 < NR; h0 += H) {
+        uint32_t v[8 * H];
+        qt_load(taddr + 8 * h0, v);
+#pragma unroll
+        for (int h = 0; h < H; ++h) {
+            const uint32_t* d = v + 8 * h;
+            x[h0 + h] = __fmaf_rn(qt_spell(d[4], d[5], d[6], d[7]), 0x1p-31f, qt_spell(d[0], d[1], d[2], d[3]));
+        }
+    }
 }
 
 __device__ __forceinline__ void prefetch_l2(const void* p) {
@@ -152,13 +191,15 @@ __device__ __forceinline__ float qt_ex2(float t) {
     return y;
 }
 
+// 96 registers: CTAs of the combine kernel, which is launched early, then fit beside
+// this one and wait there (with 104, one quarter of the register file is short of
+// two of their warps: 1.5 us a call).  Eight heads or two halves need more.
 template <int NR, int DH>
-__global__ void __launch_bounds__(QT_THREADS, 1)
+__global__ void __launch_bounds__(QT_THREADS, 1) __maxnreg__(NR < 8 && DH == 1 ? 96 : 128)
     decode_attn_q8_tc_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_constant__ CUtensorMap tmv,
                              Q8AttnArgs p, uint32_t withhold) {
     pdl_trigger();
-    typedef QtMap<DH> M;
-    constexpr uint32_t N = qt_n<NR>();
+    typedef QtMap<NR, DH> M;
     extern __shared__ __align__(1024) unsigned char smem_raw[];
     unsigned char* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
     const uint32_t sbase = smem_u32(smem);
@@ -265,7 +306,7 @@ __global__ void __launch_bounds__(QT_THREADS, 1)
         __syncwarp();
     } else if (warp == 1) {
         // ---------------- issuer of the scores ----------------
-        constexpr uint32_t IDESC_S = umma_idesc_s8(128, N, false, false);
+        constexpr uint32_t IDESC_S = umma_idesc_s8(128, M::NS, false, false);
         const bool leader = elect_one();
         const uint64_t kd = umma_desc(sbase, 16, 1024, UMMA_SWIZZLE_128B);
         const uint64_t qd = umma_desc(sbase + M::OFF_Q, 16, 1024, UMMA_SWIZZLE_128B);
@@ -287,8 +328,8 @@ __global__ void __launch_bounds__(QT_THREADS, 1)
             if (leader) {
 #pragma unroll
                 for (uint32_t kk = 0; kk < 4 * DH; ++kk)  // 32 dims (32 bytes) a product, four products a half
-                    umma_s8(tmem + g * 32, ka + (kk >> 2) * (QT_TILE >> 4) + (kk & 3) * 2,
-                            qa + (kk >> 2) * (QT_BBYTES >> 4) + (kk & 3) * 2, IDESC_S, kk > 0);
+                    umma_s8(tmem + g * M::SW, ka + (kk >> 2) * (QT_TILE >> 4) + (kk & 3) * 2,
+                            qa + (kk >> 2) * (M::Q_HALF >> 4) + (kk & 3) * 2, IDESC_S, kk > 0);
                 umma_commit(bar(M::SFULL + g));
                 if (left == 0) umma_commit(bar(M::QEMPTY + (q & 1u)));  // the pair's last product that reads its digits
             }
@@ -303,21 +344,21 @@ __global__ void __launch_bounds__(QT_THREADS, 1)
         __syncwarp();
     } else if (warp == 12) {
         // ---------------- issuer of the outputs ----------------
-        constexpr uint32_t IDESC_O = umma_idesc_s8(128, N, true, false);
+        constexpr uint32_t IDESC_O = umma_idesc_s8(128, M::NO, true, true);
         const bool leader = elect_one();
         const uint64_t vd = umma_desc(sbase + DH * QT_TILE, 16, 1024, UMMA_SWIZZLE_128B);
-        const uint64_t pd = umma_desc(sbase + M::OFF_P, 128, 1024, UMMA_SWIZZLE_NONE);
+        const uint64_t pd = umma_desc(sbase + M::OFF_P, 128, QT_TK * 16, UMMA_SWIZZLE_NONE);
         uint32_t s = 0;
         for (uint32_t n = 0; n < nt; ++n) {
             const uint32_t g = n & 1u;
             if (!warp_wait_all(bar(M::PFULL + g), (n >> 1) & 1u, abort)) break;
             tc_fence_after();
-            const uint64_t va = vd + s * (M::STAGE_BYTES >> 4), pa = pd + g * (QT_BBYTES >> 4);
+            const uint64_t va = vd + s * (M::STAGE_BYTES >> 4), pa = pd + g * (M::P_BYTES >> 4);
             if (leader) {
 #pragma unroll
-                for (uint32_t kk = 0; kk < 4 * DH; ++kk)  // 32 keys a product: 4096 bytes of a V half, 256 of the weights
-                    umma_s8(tmem + M::O + (g * DH + (kk >> 2)) * 32, va + (kk >> 2) * (QT_TILE >> 4) + (kk & 3) * 256,
-                            pa + (kk & 3) * 16, IDESC_O, (kk & 3) > 0);
+                for (uint32_t kk = 0; kk < 4 * DH; ++kk)  // 32 keys a product: 4096 bytes of a V half, 512 of the weights
+                    umma_s8(tmem + M::O + (g * DH + (kk >> 2)) * M::OW, va + (kk >> 2) * (QT_TILE >> 4) + (kk & 3) * 256,
+                            pa + (kk & 3) * 32, IDESC_O, (kk & 3) > 0);
                 umma_commit(bar(M::OFULL + g));
                 umma_commit(bar(M::EMPTY + s));
             }
@@ -361,7 +402,6 @@ __global__ void __launch_bounds__(QT_THREADS, 1)
             const uint32_t b = (i & 2) ? lo.y : lo.x, f = (i & 2) ? ((i & 1) ? hi.y : hi.x) : ((i & 1) ? lo.y : lo.x);
             return p.q_bf16 ? ((i & 1) ? bf16_hi(b) : bf16_lo(b)) : __uint_as_float(f);
         };
-        uint32_t slot = 0;
         uint32_t n = 0;
         auto step = [&]() {
             if (n >= nt) return;
@@ -373,9 +413,10 @@ __global__ void __launch_bounds__(QT_THREADS, 1)
         place(n < nt);
 #pragma unroll
         for (int h = 0; h < NR; ++h) load(h, x[h]);
-        for (uint32_t ph = 1; n < nt; ph ^= slot, slot ^= 1u) {
+        for (uint32_t q = 0; n < nt; ++q) {
+            const uint32_t slot = q & 1u;
             step();
-            if (!warp_wait_all(bar(M::QEMPTY + slot), ph, abort)) break;
+            if (!warp_wait_all(bar(M::QEMPTY + slot), (~q >> 1) & 1u, abort)) break;
             unsigned char* out = smem + M::OFF_Q + slot * M::Q_BYTES;
             place(n < nt);
 #pragma unroll
@@ -388,14 +429,15 @@ __global__ void __launch_bounds__(QT_THREADS, 1)
                     a = max(a, q8_abs_bits(u[e]));
                 }
                 a = q8_warp_max(a);
-                // The unit is a power of two: 2^22 of them (2^21 where the
-                // largest element would pass three digits) reach from 2^e to
-                // the largest element, 2^e <= amax < 2^(e + 1).  Elements below
+                // The unit is a power of two: 2^K of them (half as many where the
+                // largest element would pass the digits) reach from 2^e to the
+                // largest element, 2^e <= amax < 2^(e + 1).  Elements below
                 // 2^-60 are brought up first.
+                constexpr uint32_t K = 22;
                 const bool bad = a >= Q8_INF, tiny = a < 0x21800000u;  // not finite; below 2^-60
                 const float up = tiny ? 0x1p80f : 1.0f, amax = fmul(__uint_as_float(a), up);
                 const uint32_t e = __float_as_uint(amax) & 0x7f800000u;
-                const uint32_t k = amax <= fmul(__uint_as_float(e), 1.992f) ? 22u : 21u;
+                const uint32_t k = amax <= fmul(__uint_as_float(e), 1.992f) ? K : K - 1;
                 const float inv = bad || a == 0 ? 0.0f : __uint_as_float(((254u + k) << 23) - e);
                 if (lane == 0)
                     sq[slot * 8 + h] = bad ? q8_nan()
@@ -404,11 +446,11 @@ __global__ void __launch_bounds__(QT_THREADS, 1)
                 for (int half = 0; half < DH; ++half) {
                     uint32_t d[4];
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) d[i] = qt_digits(bad ? 0.0f : fmul(fmul(u[4 * half + i], up), inv));
+                    for (int i = 0; i < 4; ++i) d[i] = qt_digits(__float2int_rn(bad ? 0.0f : fmul(fmul(u[4 * half + i], up), inv)));
 #pragma unroll
-                    for (int g = 0; g < 3; ++g) {
+                    for (int g = 0; g < QT_QD; ++g) {
                         const uint32_t r = g * NR + h;
-                        *reinterpret_cast<uint32_t*>(out + half * QT_BBYTES + r * 128 + (((lane >> 2) ^ (r & 7)) << 4) +
+                        *reinterpret_cast<uint32_t*>(out + half * M::Q_HALF + r * 128 + (((lane >> 2) ^ (r & 7)) << 4) +
                                                      ((lane & 3) << 2)) =
                             q8_pack4(d[0] >> (8 * g), d[1] >> (8 * g), d[2] >> (8 * g), d[3] >> (8 * g));
                     }
@@ -503,13 +545,14 @@ __global__ void __launch_bounds__(QT_THREADS, 1)
         // ---------------- softmax and epilogue: group g takes tiles n = g mod 2 ----------------
         const uint32_t g = (uint32_t)(warp >> 2) - 1, q4 = (uint32_t)(warp & 3);
         const uint32_t L = q4 * 32 + (uint32_t)lane;  // key of the S tile, dim of the O tile
-        const uint32_t s_tmem = tmem + ((q4 * 32u) << 16) + g * 32, o_tmem = tmem + ((q4 * 32u) << 16) + M::O + g * DH * 32;
+        const uint32_t s_tmem = tmem + ((q4 * 32u) << 16) + g * M::SW, o_tmem = tmem + ((q4 * 32u) << 16) + M::O + g * DH * M::OW;
         const int nbar = 1 + (int)g;
         float* red = reinterpret_cast<float*>(smem + M::OFF_RED) + g * 64;   // [4][16]
         float* lsum = reinterpret_cast<float*>(smem + M::OFF_SUM) + g * 40;  // [4][8] sums of a finished pair, [8] its maxima
-        unsigned char* pt = smem + M::OFF_P + g * QT_BBYTES;
+        unsigned char* pt = smem + M::OFF_P + g * M::P_BYTES;
         // m, l: online softmax of the scores; wm, acc: the same for the
-        // weights times scales; corr, tf: factors of the output not yet read
+        // weights times scales (acc in units of 2^-30); corr, tf: factors of the
+        // output not yet read
         float m[NR], l[NR], wm[NR], acc[DH][NR], corr[NR], tf[NR];
         bool fail = false;
 #pragma unroll
@@ -524,11 +567,10 @@ __global__ void __launch_bounds__(QT_THREADS, 1)
             tc_fence_after();
 #pragma unroll
             for (int x = 0; x < DH; ++x) {
-                uint32_t o[qt_cols<NR>()];
-                qt_load<NR>(o_tmem + 32 * x, o);
+                float o[NR];
+                qt_outputs<NR>(o_tmem + M::OW * x, o);
 #pragma unroll
-                for (int h = 0; h < NR; ++h)
-                    acc[x][h] = __fmaf_rn(acc[x][h], corr[h], fmul(qt_spell(o[h], o[NR + h], o[2 * NR + h]), tf[h]));
+                for (int h = 0; h < NR; ++h) acc[x][h] = __fmaf_rn(acc[x][h], corr[h], fmul(o[h], tf[h]));
             }
             tc_fence_before();
         };
@@ -558,14 +600,14 @@ __global__ void __launch_bounds__(QT_THREADS, 1)
                 fail |= !ok;
                 if (ok) {
                     tc_fence_after();
-                    uint32_t v[qt_cols<NR>()];
-                    qt_load<NR>(s_tmem, v);
+                    float v[NR];
+                    qt_scores<NR>(s_tmem, v);
                     tc_fence_before();
                     __syncwarp();
                     if (lane == 0) mbar_arrive(bar(M::SEMPTY + g));
 #pragma unroll
                     for (int h = 0; h < NR; ++h) {
-                        t[h] = __fmaf_rn(qt_spell(v[h], v[NR + h], v[2 * NR + h]), fmul(sc.x, f[h]), mask);
+                        t[h] = __fmaf_rn(v[h], fmul(sc.x, f[h]), mask);
                         tv[h] = fadd(t[h], lv);
                     }
                 } else {
@@ -602,17 +644,25 @@ __global__ void __launch_bounds__(QT_THREADS, 1)
                         wm[h] = wn[h];
                     }
                 }
+                uint32_t d[2 * NR];
 #pragma unroll
                 for (int h = 0; h < NR; ++h) {
                     l[h] = fadd(l[h], qt_ex2(fsub(t[h], m[h])));
-                    tf[h] = fmul(qt_ex2(fsub(wt[h], wm[h])), 1.0f / Q_UNIT);
-                    const uint32_t d = qt_digits(fmul(qt_ex2(fsub(tv[h], wt[h])), Q_UNIT));
-#pragma unroll
-                    for (int i = 0; i < 3; ++i) {  // row r of the B operand, byte L: K-major cores of 8 rows x 16 bytes
-                        const uint32_t r8 = i * NR + h;
-                        pt[(r8 >> 3) * 1024 + (L >> 4) * 128 + (r8 & 7) * 16 + (L & 15)] = (unsigned char)(d >> (8 * i));
-                    }
+                    tf[h] = qt_ex2(fsub(wt[h], wm[h]));
+                    // the weight in units of 2^-30 of the tile's largest, and what that
+                    // leaves in units of 2^-61
+                    const float y = fmul(qt_ex2(fsub(tv[h], wt[h])), 0x1p30f);
+                    const int n = __float2int_rn(y);
+                    d[2 * h] = qt_digits(n);
+                    d[2 * h + 1] = qt_digits(__float2int_rn(fmul(fsub(y, (float)n), 0x1p31f)));
                 }
+                // the B operand, N-major: 16 columns (two heads) of every key, key by key
+                if constexpr (NR == 1) *reinterpret_cast<uint2*>(pt + L * 16) = make_uint2(d[0], d[1]);
+                else
+#pragma unroll
+                    for (int c = 0; c < NR / 2; ++c)
+                        *reinterpret_cast<uint4*>(pt + c * QT_TK * 16 + L * 16) =
+                            make_uint4(d[4 * c], d[4 * c + 1], d[4 * c + 2], d[4 * c + 3]);
                 fence_async_smem();  // the weights are visible to the tensor core
                 tc_fence_before();
                 if (nbar_or128(fail, nbar)) {
@@ -649,7 +699,7 @@ __global__ void __launch_bounds__(QT_THREADS, 1)
 #pragma unroll
                 for (int x = 0; x < DH; ++x)
                     if ((uint32_t)h < nh && L < hd && L + hd * x < p.head_dim)
-                        p.part_o[(part * NR + h) * p.head_dim + L + hd * x] = fmul(acc[x][h], f[h]);
+                        p.part_o[(part * NR + h) * p.head_dim + L + hd * x] = fmul(fmul(acc[x][h], 0x1p-30f), f[h]);
             if (nbar_or128(fail, nbar)) {
                 dead = true;
                 break;
@@ -699,7 +749,10 @@ template <int NR, int DH>
 static cudaError_t qt_launch(const CUtensorMap& mk, const CUtensorMap& mv, const Q8AttnArgs& a, bool withhold,
                              cudaStream_t st) {
     auto kern = decode_attn_q8_tc_kernel<NR, DH>;
-    constexpr size_t smem = QtMap<DH>::SMEM;
+    constexpr size_t smem = QtMap<NR, DH>::SMEM;
+    static_assert(smem <= QT_SMEM && QtMap<NR, DH>::STAGES >= 2 && QtMap<NR, DH>::TMEM_USED <= 512, "fits an SM");
+    // one half: room is left beside the CTA for one of the combine kernel (4.1 KB)
+    static_assert(DH == 2 || smem <= 221 * 1024, "the combine kernel waits beside the CTA");
     if (!ensure_dyn_smem(reinterpret_cast<const void*>(kern), smem)) return cudaErrorInvalidConfiguration;
     return launch_k(kern, a.workers, QT_THREADS, smem, st, mk, mv, a, withhold ? 1u : 0u);
 }

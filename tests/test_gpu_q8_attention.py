@@ -445,3 +445,46 @@ def test_scores_of_minus_infinity(cuda, hq, hkv, d, m):
         # one weight of 1: the product code * scale, and at most four roundings and two base-2 functions
         assert bool(((got[3] - only).abs() <= (4 * 2.0 ** -24 + 2 * 2.0 ** -22) * only.abs()).all())
         assert bool((_on_path(path, case, 16, _lens(cuda, [0, 0, 0, 0])) == 0).all())
+
+
+def _sink_case(dev, hq, hkv, d, m, dtype, gap):
+    """One key (position 5) whose score is about `gap` above the others' and whose
+    values are zero, so that the others make up the output.  Queries are whole
+    numbers of a few bits, which every form of the kernels holds exactly."""
+    g = torch.Generator(device=dev).manual_seed(hq * 31 + d * 1009 + m)
+    q = torch.randint(1, 8, (2, hq, d), generator=g, device=dev).to(DT[dtype])
+    kc = torch.randint(-6, 7, (2, hkv, m, d), generator=g, device=dev).to(torch.int8)
+    vc = torch.randint(-127, 128, (2, hkv, m, d), generator=g, device=dev).to(torch.int8)
+    kc[:, :, 5] = 100
+    vc[:, :, 5] = 0
+    ks = torch.full((2, hkv, -(-m // 16)), 1.0, device=dev)
+    scale = gap / (4.0 * d * 100)  # q . k of the strong key: about 4 d 100
+    vs = torch.rand((2, hkv, -(-m // 16)), generator=g, device=dev) + 0.5
+    return (q, kc, vc, ks, vs), scale
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("hq,hkv,d,m", [(2, 2, 128, 100), (4, 2, 128, 300), (8, 2, 128, 100), (16, 2, 128, 1000), (6, 2, 64, 100),
+                                        (8, 2, 256, 129), (16, 2, 256, 100), (2, 2, 37, 100), (3, 1, 144, 700)])
+@pytest.mark.parametrize("gap", [4, 8, 12, 16, 20, 24, 30])
+def test_a_sink_without_values(cuda, hq, hkv, d, m, dtype, gap):
+    """The weights of the other keys keep their bits however far the strongest key
+    is above them: f32's tolerance relative to sum p |v|, on either kernel.  u =
+    2^-24 a rounding: scores of at most d products and eight roundings more, three
+    base-2 functions of 2^-22 and 16 roundings in the sums and the quotient, twice
+    (numerator and denominator).  The tensor-core kernel holds a weight to 2^-61 of
+    the largest p vs of its tile beside that."""
+    (q, kc, vc, ks, vs), scale = _sink_case(cuda, hq, hkv, d, m, dtype, gap)
+    want, mag, _ = _q8.attend(q, kc, vc, ks, vs, None, 16, scale)
+    u, rep = 2.0 ** -24, hq // hkv
+    k = _q8.values(kc, ks, 16)
+    size = (q.double().view(2, hkv, rep, d).abs() @ k.abs().transpose(2, 3)).amax(-1).view(2, hq, 1) * scale
+    held = 2.0 ** -61 * vs.double().amax(-1) * vc.double().abs().sum(2).amax(-1)
+    tol = mag * (2 * (d + 8) * u * size + 2 * (3 * 2.0 ** -22 + 16 * u)) + held.repeat_interleave(rep, 1)[..., None]
+    for path in (0, 1):
+        _lib.lib().oxide_debug_decode_attention_path(path)
+        try:
+            got = ops.decode_attention_q8(q, kc, vc, ks, vs, 16, scale=scale)
+        finally:
+            _lib.lib().oxide_debug_decode_attention_path(0)
+        _close(got, want, tol)
