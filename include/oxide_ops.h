@@ -424,7 +424,7 @@ int oxide_decode_attention_bf16(const oxide_bf16* q, const oxide_bf16* k_cache, 
  * h / (q_heads / kv_heads).  q, out [batch, q_heads, head_dim], f32 or bf16,
  * head_dim <= 256, batch <= 4096.  Sums, scores and softmax statistics are
  * f32.  On the tensor cores both products are exact integer sums: of q held to
- * 2^-23 of its head's largest element, and of the weights (p times the value
+ * 2^-61 (bf16: 2^-31) of its head's largest element, and of the weights (p times the value
  * scale) held to 2^-61 of the largest of each tile of 128 keys.  A sequence of length 0 gives zeros; a key whose block has a
  * scale, in k or in v, that is NaN, infinite or negative, or a query head that
  * holds a NaN or an infinity, or whose every score is -infinity, gives NaN;

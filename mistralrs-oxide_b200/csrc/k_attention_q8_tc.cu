@@ -4,11 +4,14 @@
 // Mathematics.  The cache's codes c, d are int8 as they lie in memory, so the
 // other operand of each product is written in int8 digits as well and the
 // products are exact integer sums:
-//   q of a head = x u with integers |x| below 2^23 and u a power of two, and
-//   x = x0 + 256 x1 + 65536 x2 in balanced digits (-128 .. 127), so
-//   q . c = (x0 . c + 256 x1 . c + 65536 x2 . c) u: the three digit rows are
-//   three columns of one product (each sum at most 2^22, exact in f32), and q
-//   is held to 2^-23 of its largest element, as good as f32 sums;
+//   q of a head = x u with integers |x| below 2^31 and u a power of two, and
+//   x = x0 + 256 x1 + 65536 x2 + 2^24 x3 in balanced digits (-128 .. 127), so
+//   q . c = (x0 . c + 256 x1 . c + ...) u: the four digit rows are four columns
+//   of one product, each sum at most 2^22 and exact.  bf16 elements are exact so
+//   far, those below 2^-23 of the head's largest rounded to 2^-31 of it; f32
+//   elements take four digits more, for what the first ones leave (2^-61).  So
+//   a strong channel over small codes costs the others nothing (with three
+//   digits, an element of 1e4 beside others of 1 left scores off by 1e-3);
 //   p_j vs_j (the softmax weight times the value block's scale) likewise, in
 //   eight digits: an integer in units of 2^-30 of the largest of the tile, and
 //   what that leaves in units of 2^-61.  The largest is found in the log2 domain
@@ -85,17 +88,17 @@ constexpr uint32_t QT_MAX_BATCH = 1024;
 constexpr float QT_LOW = -3.402823466e38f;
 constexpr uint32_t QT_TILE = QT_TK * QT_DB;  // 16 KB
 constexpr uint32_t QT_SMEM = 227 * 1024;     // what a CTA can have
-constexpr int QT_QD = 3, QT_PD = 8;           // digits of a query element, of a weight
+constexpr int QT_PD = 8;                     // digits of a weight
 
 // Rows of a B operand, and columns of its product: `digits` of NR query heads
 // (M = 128 takes N in steps of 16).
 constexpr uint32_t qt_n(int nr, int digits) { return (uint32_t)(nr * digits + 15) / 16 * 16; }
 
-// Places of the kernel for NR query heads and DH halves of 128 bytes a
+// Places of the kernel for NR query heads of QD digits and DH halves of 128 bytes a
 // row (head_dim up to 128, 256).
-template <int NR, int DH>
+template <int NR, int DH, int QD>
 struct QtMap {
-    static constexpr uint32_t NS = qt_n(NR, QT_QD), NO = qt_n(NR, QT_PD);  // columns of S, of O
+    static constexpr uint32_t NS = qt_n(NR, QD), NO = qt_n(NR, QT_PD);  // columns of S, of O
     static constexpr uint32_t STAGE_BYTES = 2 * DH * QT_TILE;           // K, V
     static constexpr uint32_t Q_HALF = NS * QT_DB, Q_BYTES = DH * Q_HALF, P_BYTES = NO * QT_DB;
     // as many stages as fit, at most 192 KB
@@ -135,13 +138,12 @@ static_assert(2 * 1024 <= Q8A_PARTS, "two parts a CTA fit the workspace");
 
 __device__ unsigned int g_device_status_q8;  // sticky failure flags, read by oxide_device_status
 
-// C columns of TMEM (a multiple of 8).
+// C columns of TMEM (8, 16 or 32).
 template <int C>
 __device__ __forceinline__ void qt_load(uint32_t taddr, uint32_t (&v)[C]) {
-    if constexpr (C == 16) tmem_ld16(taddr, v);
-    else
-#pragma unroll
-        for (int i = 0; i < C; i += 8) tmem_ld8(taddr + i, v + i);
+    if constexpr (C == 32) tmem_ld32(taddr, v);
+    else if constexpr (C == 16) tmem_ld16(taddr, v);
+    else tmem_ld8(taddr, v);
     tmem_wait_ld();
 }
 // The number that the sums of four digits spell.  Each sum is at most 2^22 in
@@ -150,19 +152,22 @@ __device__ __forceinline__ void qt_load(uint32_t taddr, uint32_t (&v)[C]) {
 __device__ __forceinline__ float qt_spell(uint32_t d0, uint32_t d1, uint32_t d2, uint32_t d3) {
     return __fmaf_rn((float)((int)d3 * 256 + (int)d2), 65536.0f, (float)((int)d1 * 256 + (int)d0));
 }
-__device__ __forceinline__ float qt_spell(uint32_t d0, uint32_t d1, uint32_t d2) {
-    return __fmaf_rn((float)(int)d2, 65536.0f, (float)((int)d1 * 256 + (int)d0));
-}
-// Balanced digits of an integer in bytes 0 .. 3 (|x| <= 0x7f7f7f7f, or 0x7f7f7f for
-// the first three alone).
+// Balanced digits of an integer, |x| <= 0x7f7f7f7f, in bytes 0 .. 3.
 __device__ __forceinline__ uint32_t qt_digits(int x) { return ((uint32_t)x + 0x80808080u) ^ 0x80808080u; }
-// Scores: digit i of head h is column i NR + h.
-template <int NR>
+// Scores: digit i of head h is column i NR + h.  Of eight digits the upper four
+// come first; the lower ones count units of 2^-31 of theirs.
+template <int NR, int QD>
 __device__ __forceinline__ void qt_scores(uint32_t taddr, float (&x)[NR]) {
-    uint32_t v[(3 * NR + 7) / 8 * 8];
+    uint32_t v[(4 * NR + 7) / 8 * 8];
     qt_load(taddr, v);
 #pragma unroll
-    for (int h = 0; h < NR; ++h) x[h] = qt_spell(v[h], v[NR + h], v[2 * NR + h]);
+    for (int h = 0; h < NR; ++h) x[h] = qt_spell(v[h], v[NR + h], v[2 * NR + h], v[3 * NR + h]);
+    if constexpr (QD == 8) {
+        qt_load(taddr + 4 * NR, v);
+#pragma unroll
+        for (int h = 0; h < NR; ++h)
+            x[h] = __fmaf_rn(qt_spell(v[h], v[NR + h], v[2 * NR + h], v[3 * NR + h]), 0x1p-31f, x[h]);
+    }
 }
 // Outputs: digit i of head h is column 8 h + i, the upper four first.
 template <int NR>
@@ -194,12 +199,14 @@ __device__ __forceinline__ float qt_ex2(float t) {
 // 96 registers: CTAs of the combine kernel, which is launched early, then fit beside
 // this one and wait there (with 104, one quarter of the register file is short of
 // two of their warps: 1.5 us a call).  Eight heads or two halves need more.
-template <int NR, int DH>
+// QD: digits of a query element, 4 for bf16 and 8 for f32.
+template <int NR, int DH, int QD>
 __global__ void __launch_bounds__(QT_THREADS, 1) __maxnreg__(NR < 8 && DH == 1 ? 96 : 128)
     decode_attn_q8_tc_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_constant__ CUtensorMap tmv,
                              Q8AttnArgs p, uint32_t withhold) {
     pdl_trigger();
-    typedef QtMap<NR, DH> M;
+    typedef QtMap<NR, DH, QD> M;
+    constexpr bool BF16 = QD == 4;
     extern __shared__ __align__(1024) unsigned char smem_raw[];
     unsigned char* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
     const uint32_t sbase = smem_u32(smem);
@@ -254,7 +261,7 @@ __global__ void __launch_bounds__(QT_THREADS, 1) __maxnreg__(NR < 8 && DH == 1 ?
             // The first pair's query heads and scales go ahead of the ring's 192 KB
             // a CTA: asked for behind them they came 3 us later.
             const uint32_t kvh = p.by_chunks.div(at.kvh), h0 = (at.kvh - kvh * p.chunks) * NR;
-            const uint32_t es = p.q_bf16 ? 2 : 4, bytes = min(p.rep - h0, (uint32_t)NR) * p.head_dim * es;
+            const uint32_t es = BF16 ? 2 : 4, bytes = min(p.rep - h0, (uint32_t)NR) * p.head_dim * es;
             if (lane * 128u < bytes)
                 prefetch_l2(static_cast<const char*>(p.q) +
                             ((uint64_t)at.b * p.q_heads + kvh * p.rep + h0) * p.head_dim * es + lane * 128u);
@@ -391,16 +398,16 @@ __global__ void __launch_bounds__(QT_THREADS, 1) __maxnreg__(NR < 8 && DH == 1 ?
                 const uint32_t d = 4u * lane + hd * half;
                 const bool there = h < nh && 4u * lane < hd && d < p.head_dim;
                 const uint2* at = reinterpret_cast<const uint2*>(static_cast<const char*>(p.q) +
-                                                                 ((row + h) * p.head_dim + d) * (p.q_bf16 ? 2 : 4));
+                                                                 ((row + h) * p.head_dim + d) * (BF16 ? 2 : 4));
                 v[2 * half] = v[2 * half + 1] = make_uint2(0, 0);
                 if (there) v[2 * half] = __ldg(at);
-                if (there && !p.q_bf16) v[2 * half + 1] = __ldg(at + 1);
+                if (there && !BF16) v[2 * half + 1] = __ldg(at + 1);
             }
         };
         auto value = [&](const uint2 (&v)[2 * DH], int i) {  // element i of the lane's four (of each half)
             const uint2 lo = v[i >> 2 << 1], hi = v[(i >> 2 << 1) + 1];
             const uint32_t b = (i & 2) ? lo.y : lo.x, f = (i & 2) ? ((i & 1) ? hi.y : hi.x) : ((i & 1) ? lo.y : lo.x);
-            return p.q_bf16 ? ((i & 1) ? bf16_hi(b) : bf16_lo(b)) : __uint_as_float(f);
+            return BF16 ? ((i & 1) ? bf16_hi(b) : bf16_lo(b)) : __uint_as_float(f);
         };
         uint32_t n = 0;
         auto step = [&]() {
@@ -429,30 +436,39 @@ __global__ void __launch_bounds__(QT_THREADS, 1) __maxnreg__(NR < 8 && DH == 1 ?
                     a = max(a, q8_abs_bits(u[e]));
                 }
                 a = q8_warp_max(a);
-                // The unit is a power of two: 2^K of them (half as many where the
-                // largest element would pass the digits) reach from 2^e to the
-                // largest element, 2^e <= amax < 2^(e + 1).  Elements below
+                // The unit is a power of two: 2^30 of them (2^29 where the
+                // largest element would pass four digits) reach from 2^e to
+                // the largest element, 2^e <= amax < 2^(e + 1).  Elements below
                 // 2^-60 are brought up first.
-                constexpr uint32_t K = 22;
                 const bool bad = a >= Q8_INF, tiny = a < 0x21800000u;  // not finite; below 2^-60
                 const float up = tiny ? 0x1p80f : 1.0f, amax = fmul(__uint_as_float(a), up);
                 const uint32_t e = __float_as_uint(amax) & 0x7f800000u;
-                const uint32_t k = amax <= fmul(__uint_as_float(e), 1.992f) ? K : K - 1;
+                const uint32_t k = amax <= fmul(__uint_as_float(e), 1.992f) ? 30u : 29u;
                 const float inv = bad || a == 0 ? 0.0f : __uint_as_float(((254u + k) << 23) - e);
                 if (lane == 0)
                     sq[slot * 8 + h] = bad ? q8_nan()
                                            : (a == 0 ? 0.0f : fmul(fmul(__uint_as_float(e - (k << 23)), p.c1), tiny ? 0x1p-80f : 1.0f));
 #pragma unroll
                 for (int half = 0; half < DH; ++half) {
-                    uint32_t d[4];
+                    float y[4];  // in units
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) d[i] = qt_digits(__float2int_rn(bad ? 0.0f : fmul(fmul(u[4 * half + i], up), inv)));
+                    for (int i = 0; i < 4; ++i) y[i] = bad ? 0.0f : fmul(fmul(u[4 * half + i], up), inv);
 #pragma unroll
-                    for (int g = 0; g < QT_QD; ++g) {
-                        const uint32_t r = g * NR + h;
-                        *reinterpret_cast<uint32_t*>(out + half * M::Q_HALF + r * 128 + (((lane >> 2) ^ (r & 7)) << 4) +
-                                                     ((lane & 3) << 2)) =
-                            q8_pack4(d[0] >> (8 * g), d[1] >> (8 * g), d[2] >> (8 * g), d[3] >> (8 * g));
+                    for (int g0 = 0; g0 < QD; g0 += 4) {  // the upper four digits, then those of the rest
+                        uint32_t d[4];
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const int n = __float2int_rn(y[i]);
+                            d[i] = qt_digits(n);
+                            y[i] = fmul(fsub(y[i], (float)n), 0x1p31f);  // exact
+                        }
+#pragma unroll
+                        for (int g = 0; g < 4; ++g) {
+                            const uint32_t r = (g0 + g) * NR + h;
+                            *reinterpret_cast<uint32_t*>(out + half * M::Q_HALF + r * 128 + (((lane >> 2) ^ (r & 7)) << 4) +
+                                                         ((lane & 3) << 2)) =
+                                q8_pack4(d[0] >> (8 * g), d[1] >> (8 * g), d[2] >> (8 * g), d[3] >> (8 * g));
+                        }
                     }
                 }
                 load(h, x[h]);
@@ -601,7 +617,7 @@ __global__ void __launch_bounds__(QT_THREADS, 1) __maxnreg__(NR < 8 && DH == 1 ?
                 if (ok) {
                     tc_fence_after();
                     float v[NR];
-                    qt_scores<NR>(s_tmem, v);
+                    qt_scores<NR, QD>(s_tmem, v);
                     tc_fence_before();
                     __syncwarp();
                     if (lane == 0) mbar_arrive(bar(M::SEMPTY + g));
@@ -745,26 +761,26 @@ static bool qt_map(CUtensorMap* m, const void* base, uint64_t heads, uint64_t ma
 
 bool tc_enabled();  // an sm_100 device, and not switched off (k_attention_tc.cu)
 
-template <int NR, int DH>
+template <int NR, int DH, int QD>
 static cudaError_t qt_launch(const CUtensorMap& mk, const CUtensorMap& mv, const Q8AttnArgs& a, bool withhold,
                              cudaStream_t st) {
-    auto kern = decode_attn_q8_tc_kernel<NR, DH>;
-    constexpr size_t smem = QtMap<NR, DH>::SMEM;
-    static_assert(smem <= QT_SMEM && QtMap<NR, DH>::STAGES >= 2 && QtMap<NR, DH>::TMEM_USED <= 512, "fits an SM");
+    auto kern = decode_attn_q8_tc_kernel<NR, DH, QD>;
+    constexpr size_t smem = QtMap<NR, DH, QD>::SMEM;
+    static_assert(smem <= QT_SMEM && QtMap<NR, DH, QD>::STAGES >= 2 && QtMap<NR, DH, QD>::TMEM_USED <= 512, "fits an SM");
     // one half: room is left beside the CTA for one of the combine kernel (4.1 KB)
     static_assert(DH == 2 || smem <= 221 * 1024, "the combine kernel waits beside the CTA");
     if (!ensure_dyn_smem(reinterpret_cast<const void*>(kern), smem)) return cudaErrorInvalidConfiguration;
     return launch_k(kern, a.workers, QT_THREADS, smem, st, mk, mv, a, withhold ? 1u : 0u);
 }
 
-template <int DH>
+template <int DH, int QD>
 static cudaError_t qt_launch_nr(const CUtensorMap& mk, const CUtensorMap& mv, const Q8AttnArgs& a, bool withhold,
                                 cudaStream_t st) {
     switch (a.nr) {
-        case 1: return qt_launch<1, DH>(mk, mv, a, withhold, st);
-        case 2: return qt_launch<2, DH>(mk, mv, a, withhold, st);
-        case 4: return qt_launch<4, DH>(mk, mv, a, withhold, st);
-        default: return qt_launch<8, DH>(mk, mv, a, withhold, st);
+        case 1: return qt_launch<1, DH, QD>(mk, mv, a, withhold, st);
+        case 2: return qt_launch<2, DH, QD>(mk, mv, a, withhold, st);
+        case 4: return qt_launch<4, DH, QD>(mk, mv, a, withhold, st);
+        default: return qt_launch<8, DH, QD>(mk, mv, a, withhold, st);
     }
 }
 
@@ -787,7 +803,9 @@ cudaError_t decode_attention_q8_tc(Q8AttnArgs& a, bool withhold, cudaStream_t st
     a.inv_workers = 1.0 / a.workers;
     a.halves = 2;
     *used = true;
-    return a.head_dim <= QT_DB ? qt_launch_nr<1>(mk, mv, a, withhold, st) : qt_launch_nr<2>(mk, mv, a, withhold, st);
+    if (a.q_bf16)
+        return a.head_dim <= QT_DB ? qt_launch_nr<1, 4>(mk, mv, a, withhold, st) : qt_launch_nr<2, 4>(mk, mv, a, withhold, st);
+    return a.head_dim <= QT_DB ? qt_launch_nr<1, 8>(mk, mv, a, withhold, st) : qt_launch_nr<2, 8>(mk, mv, a, withhold, st);
 }
 
 int device_status_q8(int reset, uint32_t* flags) {

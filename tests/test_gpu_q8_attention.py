@@ -488,3 +488,31 @@ def test_a_sink_without_values(cuda, hq, hkv, d, m, dtype, gap):
         finally:
             _lib.lib().oxide_debug_decode_attention_path(0)
         _close(got, want, tol)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("hq,hkv,d", [(2, 2, 128), (4, 2, 128), (8, 2, 128), (16, 2, 128), (6, 2, 64), (8, 2, 256), (16, 2, 256),
+                                      (2, 2, 37), (3, 1, 144)])
+@pytest.mark.parametrize("strong", [100.0, 1e4, 1e6])
+def test_a_strong_channel_over_zero_codes(cuda, hq, hkv, d, dtype, strong):
+    """One query element far above the others, and keys that are zero there: the
+    scores come from the small elements, which keep their bits.  u = 2^-24 a
+    rounding: scores of d products and eight roundings more, relative to sum |q k|;
+    three base-2 functions of 2^-22 and 16 roundings in sums and quotient; twice.
+    (bf16 elements are whole units of 2^-30 of the largest down to 2^-23 of it, f32
+    ones of 2^-61 down to 2^-37: nothing is left out.)"""
+    block = 16
+    q, kc, vc, ks, vs = _case(cuda, 2, hq, hkv, d, 300, block, dtype, seed=int(strong))
+    q[:, :, 7] = strong
+    kc[..., 7] = 0
+    # elements of at least 2^-10, so that bf16's and f32's lie in whole units
+    q.copy_(torch.where(q.abs() < 2.0 ** -10, torch.full_like(q, 2.0 ** -10), q))
+    lens = _lens(cuda, [300, 77])
+    want, mag, _ = _q8.attend(q, kc, vc, ks, vs, lens, block, d ** -0.5)
+    u, rep = 2.0 ** -24, hq // hkv
+    size = (q.double().view(2, hkv, rep, d).abs() @ _q8.values(kc, ks, block).abs().transpose(2, 3)).amax(-1)
+    size = size.view(2, hq, 1) * d ** -0.5
+    held = 2.0 ** -61 * vs.double().amax(-1) * vc.double().abs().sum(2).amax(-1)
+    tol = mag * (2 * (d + 8) * u * size + 2 * (3 * 2.0 ** -22 + 16 * u)) + held.repeat_interleave(rep, 1)[..., None]
+    for path in (0, 1):
+        _close(_on_path(path, (q, kc, vc, ks, vs), block, lens), want, tol)
