@@ -147,7 +147,7 @@ def build(op: str, rows: int | None, dev):
         mk = lambda: (rn(c.batch, c.heads, d, dtype=dt), *cache(), torch.empty(c.batch, c.heads, d, dtype=dt, device=dev))  # noqa: E731
         run = lambda s: ops.decode_attention_q8(*s[:5], block, tl, workspace=ws, out=s[5])  # noqa: E731
         total = int(np.sum(np.minimum(lens, c.keys)))
-        return mk, run, total * kvh * (2 * d + 8 // block) + 2 * c.batch * c.heads * d * es, [c.batch, c.heads, kvh, c.keys, d]
+        return mk, run, total * kvh * 2 * d + total * kvh * 8 // block + 2 * c.batch * c.heads * d * es, [c.batch, c.heads, kvh, c.keys, d]
     if op in ("decode_weights_bf16_f32", "decode_weights_f16_f32"):
         # safetensors element decode of one Mistral MLP matrix [14336, 4096] to f32
         n = (rows or 14336) * 4096
