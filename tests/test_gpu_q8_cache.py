@@ -275,3 +275,23 @@ def test_graph_of_decode_steps(cuda):
         graph.replay()
     torch.cuda.synchronize()
     _same(cache, want)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("d,block", [(128, 1), (128, 16), (128, 64), (128, 128), (256, 128), (37, 1), (37, 16), (20, 64)])
+def test_scales_of_fresh_blocks_hold_anything(cuda, dtype, d, block):
+    """NaN, infinities and anything else among the scales of blocks at or behind
+    each sequence's length: blocks that receive tokens get their own scale, the
+    others keep what they hold."""
+    b, h, m, cur = 3, 2, 300, [0, 77, 169]
+    cache, g = _cache(cuda, b, h, m, d, block, d * 1000 + block)
+    for scales in cache[2:]:
+        for i, n in enumerate(cur):
+            fresh = scales[i, :, -(-n // block):]
+            fresh[:, 0::3] = float("nan")
+            fresh[:, 1::3] = float("inf")
+    _append(cache, _tokens(g, cuda, b, h, 131, d, dtype), cur, [131, 100, 120], block)
+    for scales in cache[2:]:
+        for i, n in enumerate((131, 177, 289)):
+            assert bool(torch.isfinite(scales[i, :, :-(-n // block)]).all())
+    _append(cache, _tokens(g, cuda, b, h, 9, d, dtype), [131, 177, 289], [9, 0, 5], block)
