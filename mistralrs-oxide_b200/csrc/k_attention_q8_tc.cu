@@ -45,8 +45,9 @@
 //                                              key's digits are 8 to 64 bytes
 //                                              in a row, one to four stores of
 //                                              its thread),
-//               N = digits times heads, in steps of 16.  One thread issuing both spent 2100 cycles a tile on
-//               waits and issue, twice what the loads allow;
+//               N = digits times heads, in steps of 16.  One thread issuing
+//               both spent 2100 cycles a tile on waits and issue, twice what
+//               the loads allow;
 //   warp 2      the query heads' digits, one pair ahead, from raw bits loaded two
 //               pairs ahead.  (A second such warp gained nothing, nor did asking
 //               L2 for the queries four pairs early: 59.2 and 71.2 us where this
@@ -189,7 +190,8 @@ __device__ __forceinline__ void prefetch_l2(const void* p) {
     asm volatile("prefetch.global.L2 [%0];" ::"l"(p) : "memory");
 }
 
-// Weights and rescaling factors: results below 2^-126 are zero.
+// Weights and rescaling factors: off by at most 2^-22 of the result, as ex2_approx
+// everywhere in these kernels; results below 2^-126 are zero.
 __device__ __forceinline__ float qt_ex2(float t) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(t));
@@ -566,9 +568,9 @@ __global__ void __launch_bounds__(QT_THREADS, 1) __maxnreg__(NR < 8 && DH == 1 ?
         float* red = reinterpret_cast<float*>(smem + M::OFF_RED) + g * 64;   // [4][16]
         float* lsum = reinterpret_cast<float*>(smem + M::OFF_SUM) + g * 40;  // [4][8] sums of a finished pair, [8] its maxima
         unsigned char* pt = smem + M::OFF_P + g * M::P_BYTES;
-        // m, l: online softmax of the scores; wm, acc: the same for the
-        // weights times scales (acc in units of 2^-30); corr, tf: factors of the
-        // output not yet read
+        // m, l: online softmax of the scores; wm (relative to m), acc: the same for
+        // the weights times scales (acc in units of 2^-30); corr, tf: factors of
+        // the output not yet read
         float m[NR], l[NR], wm[NR], acc[DH][NR], corr[NR], tf[NR];
         bool fail = false;
 #pragma unroll
@@ -608,7 +610,7 @@ __global__ void __launch_bounds__(QT_THREADS, 1) __maxnreg__(NR < 8 && DH == 1 ?
             __syncwarp();
             if (lane == 0) mbar_arrive(bar(M::QEMPTY + (q & 1u)));
             for (uint32_t j = j0; j < cnt; j += 2) {
-                float t[NR], tv[NR];
+                float t[NR];
                 bool ok = warp_wait_all(bar(M::CFULL + st), ph, abort);
                 const float2 sc = scales[st * QT_TK];  // key scale; log2 of the value scale, or the mark of a masked key
                 const float mask = sc.y == INFINITY ? -INFINITY : 0.0f, lv = sc.y == INFINITY ? 0.0f : sc.y;
@@ -624,15 +626,14 @@ __global__ void __launch_bounds__(QT_THREADS, 1) __maxnreg__(NR < 8 && DH == 1 ?
 #pragma unroll
                     for (int h = 0; h < NR; ++h) {
                         t[h] = __fmaf_rn(v[h], fmul(sc.x, f[h]), mask);
-                        tv[h] = fadd(t[h], lv);
                     }
                 } else {
 #pragma unroll
-                    for (int h = 0; h < NR; ++h) t[h] = tv[h] = -INFINITY;
+                    for (int h = 0; h < NR; ++h) t[h] = -INFINITY;
                 }
 #pragma unroll
                 for (int h = 0; h < NR; ++h) {
-                    const float a = warp_fmax(t[h]), b = warp_fmax(tv[h]);
+                    const float a = warp_fmax(t[h]), b = warp_fmax(fadd(t[h], lv));
                     if (lane == 0) {
                         red[q4 * 16 + h] = a;
                         red[q4 * 16 + 8 + h] = b;
@@ -640,22 +641,27 @@ __global__ void __launch_bounds__(QT_THREADS, 1) __maxnreg__(NR < 8 && DH == 1 ?
                 }
                 if (j != j0) epilogue(k - 1);  // its product has run meanwhile; the weights buffer and O are free after it
                 nbar_sync128(nbar);            // the four warps' maxima are in red
+                // The largest weight of the tile, wt, and of the tiles so far, wm, are
+                // log2 of it relative to the largest score: differences of near
+                // numbers, so scores of some hundred (whose sum with log2 of a
+                // scale is off by 1e-5) cost the outputs nothing.
                 float mn[NR], wt[NR], wn[NR];
                 bool moved = false;
 #pragma unroll
                 for (int h = 0; h < NR; ++h) {
                     const float* r = red + h;
                     mn[h] = fmaxf(fmaxf(fmaxf(r[0], r[16]), fmaxf(r[32], r[48])), m[h]);
-                    wt[h] = fmaxf(fmaxf(fmaxf(r[8], r[24]), fmaxf(r[40], r[56])), QT_LOW);
-                    wn[h] = fmaxf(wt[h], wm[h]);
+                    wt[h] = fmaxf(fsub(fmaxf(fmaxf(r[8], r[24]), fmaxf(r[40], r[56])), mn[h]), QT_LOW);
+                    wn[h] = fmaxf(wt[h], fadd(wm[h], fsub(m[h], mn[h])));
                     moved |= mn[h] != m[h] || wn[h] != wm[h];
                     corr[h] = 1.0f;
                 }
                 if (moved) {  // the same for every thread of the group
 #pragma unroll
                     for (int h = 0; h < NR; ++h) {
-                        l[h] = fmul(l[h], qt_ex2(fsub(m[h], mn[h])));
-                        corr[h] = qt_ex2(fsub(wm[h], wn[h]));
+                        const float dm = fsub(m[h], mn[h]);
+                        l[h] = fmul(l[h], qt_ex2(dm));
+                        corr[h] = qt_ex2(fsub(fadd(wm[h], dm), wn[h]));
                         m[h] = mn[h];
                         wm[h] = wn[h];
                     }
@@ -663,11 +669,12 @@ __global__ void __launch_bounds__(QT_THREADS, 1) __maxnreg__(NR < 8 && DH == 1 ?
                 uint32_t d[2 * NR];
 #pragma unroll
                 for (int h = 0; h < NR; ++h) {
-                    l[h] = fadd(l[h], qt_ex2(fsub(t[h], m[h])));
+                    const float dt = fsub(t[h], m[h]);
+                    l[h] = fadd(l[h], qt_ex2(dt));
                     tf[h] = qt_ex2(fsub(wt[h], wm[h]));
                     // the weight in units of 2^-30 of the tile's largest, and what that
                     // leaves in units of 2^-61
-                    const float y = fmul(qt_ex2(fsub(tv[h], wt[h])), 0x1p30f);
+                    const float y = fmul(qt_ex2(fsub(fadd(dt, lv), wt[h])), 0x1p30f);
                     const int n = __float2int_rn(y);
                     d[2 * h] = qt_digits(n);
                     d[2 * h + 1] = qt_digits(__float2int_rn(fmul(fsub(y, (float)n), 0x1p31f)));
@@ -707,7 +714,7 @@ __global__ void __launch_bounds__(QT_THREADS, 1) __maxnreg__(NR < 8 && DH == 1 ?
                 const float x = warp_sum(l[h]);
                 if (lane == 0) lsum[q4 * 8 + h] = x;
                 if (L == 0) lsum[32 + h] = m[h];
-                f[h] = ex2_approx(fsub(wm[h], m[h]));
+                f[h] = ex2_approx(wm[h]);
             }
             epilogue(k - 1);
 #pragma unroll

@@ -516,3 +516,32 @@ def test_a_strong_channel_over_zero_codes(cuda, hq, hkv, d, dtype, strong):
     tol = mag * (2 * (d + 8) * u * size + 2 * (3 * 2.0 ** -22 + 16 * u)) + held.repeat_interleave(rep, 1)[..., None]
     for path in (0, 1):
         _close(_on_path(path, (q, kc, vc, ks, vs), block, lens), want, tol)
+
+
+@pytest.mark.parametrize("hq,hkv,d", [(2, 2, 128), (4, 2, 128), (8, 2, 128), (16, 2, 128), (8, 2, 256), (2, 2, 37), (6, 2, 64)])
+@pytest.mark.parametrize("n", [1, 100, 400])
+@pytest.mark.parametrize("score", [-3000.0, -70.0, 40.0, 300.0, 5000.0])
+def test_scores_far_from_zero(cuda, hq, hkv, d, n, score):
+    """Keys that are alike have weights of exactly 1 / n however large their score
+    is, so its rounding is nobody's excuse: the output is the mean of the values
+    within three base-2 functions (2^-22), 16 roundings in the sums and the
+    quotient and a sum of n values, twice, and 2^-61 of the tile's largest."""
+    g = torch.Generator(device=cuda).manual_seed(n + d)
+    q = torch.full((2, hq, d), 0.7, device=cuda)
+    kc = torch.full((2, hkv, n, d), 91, dtype=torch.int8, device=cuda)
+    vc = torch.randint(-127, 128, (2, hkv, n, d), generator=g, device=cuda).to(torch.int8)
+    blocks = -(-n // 16)
+    ks = torch.full((2, hkv, blocks), 0.013, device=cuda)
+    vs = (torch.rand((2, hkv, blocks), generator=g, device=cuda) + 0.1) * 0.02
+    scale = score / (0.7 * 91 * 0.013 * d)
+    v = _q8.values(vc, vs, 16)
+    want, mag = (t.mean(2).repeat_interleave(hq // hkv, 1) for t in (v, v.abs()))
+    held = 2.0 ** -61 * vs.double().amax(-1) * vc.double().abs().sum(2).amax(-1)
+    tol = mag * 2 * (3 * 2.0 ** -22 + (16 + n / 32) * 2.0 ** -24) + held.repeat_interleave(hq // hkv, 1)[..., None]
+    for path in (0, 1):
+        _lib.lib().oxide_debug_decode_attention_path(path)
+        try:
+            got = ops.decode_attention_q8(q, kc, vc, ks, vs, 16, scale=scale)
+        finally:
+            _lib.lib().oxide_debug_decode_attention_path(0)
+        _close(got, want, tol)
