@@ -194,7 +194,7 @@ __device__ __forceinline__ void norm_q8_settle(NormRow& r, bool open, int turn, 
 // to a half-integer.  There 254 |p| = hi + lo exactly, and hi - (2 n + 1) top
 // from one fused step is less than 2^16 units of the last place of either, so
 // exact: the sum of the two has the sign of 254 |p| - (2 n + 1) top. 
-static __device__ __noinline__ int norm_nearest(double p, double top) {
+static __device__ __forceinline__ int norm_nearest_here(double p, double top) {
     if (!(top > 0.0)) return 0;
     const double a = fabs(p), q = 127.0 * a / top, n = rint(q);
     int c = (int)n;
@@ -206,6 +206,9 @@ static __device__ __noinline__ int norm_nearest(double p, double top) {
     }
     return p < 0.0 ? -c : c;
 }
+
+// The same as a call, for kernels with many places of it.
+static __device__ __noinline__ int norm_nearest(double p, double top) { return norm_nearest_here(p, top); }
 
 // Codes nearest(127 p / top).
 template <typename T>
@@ -226,7 +229,9 @@ struct NormCoder {
         return q8_beside(p, 254.0f * fabsf(p), inv, ftop);
     }
 };
-// The codes of a packed vector by the definition.
+// The codes of a packed vector by the definition.  (Without a call of norm_nearest
+// inside, which cost the kernels 50 bytes of spills: f32 [16384, 4096] with r 140.6
+// us against 144.1.)
 template <typename T>
 __device__ __noinline__ uint2 norm_decide(uint4 h, uint4 w, double top) {
     constexpr int V = Vec<T>::N;
@@ -236,16 +241,19 @@ __device__ __noinline__ uint2 norm_decide(uint4 h, uint4 w, double top) {
     Vec<T>::unpack(h, hv);
     Vec<T>::unpack(w, wv);
 #pragma unroll
-    for (int e = 0; e < V; ++e) q[e] = (uint32_t)c.exact(hv[e], wv[e]);
+    for (int e = 0; e < V; ++e)
+        q[e] = (uint32_t)(sizeof(T) == 4 ? norm_nearest_here((double)hv[e] * (double)wv[e], top) : c.exact(hv[e], wv[e]));
     return make_uint2(q8_pack4(q[0], q[1], q[2], q[3]), q8_pack4(q[4], q[5], q[6], q[7]));
 }
 
 constexpr int NQ_VPT = 4;  // 16-byte vectors a thread holds
 
 // WARP: eight rows per 256-thread CTA; else one row per CTA of up to MAXT threads.
-// The register budget of 85 (three CTAs of 256) holds x, r and w of a thread; f32
-// without r has room for a fourth CTA (14.0 us against 14.6, 77 against 85; with r
-// it spills, 27.8 against 22.0).
+// Three CTAs of 256 an SM at 80 registers, four for f32 without r at 64 (14.0 us
+// against 14.6 with three, 77 against 85; with r four were slower, 27.8 against
+// 22.0).  All of these spill some: f32 about 100 bytes a thread, bf16 with r 40.
+// Two CTAs, which spill nothing, were slower everywhere: bf16 [16384, 4096] with r
+// 87.9 us against 82.0, f32 with r 158 against 141, f32 116 against 78.
 template <typename T, bool ADD, bool WARP, int MAXT>
 __global__ void __launch_bounds__(MAXT, MAXT == 256 ? (sizeof(T) == 4 && !ADD ? 4 : 3) : 1)
     rmsnorm_q8_vec_kernel(const T* x, const T* r, const T* w, T* h, int8_t* y, float* scale, NormQ8Args p) {
