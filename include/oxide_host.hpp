@@ -910,7 +910,10 @@ class KvCache {
 
 // KvCache held as int8 codes with one f32 scale per block of `block` positions
 // and head: update() quantises as it writes, read() gives values back, attend()
-// is one decode step of attention over a layer.
+// is one decode step of attention over a layer.  Lengths are counted on the host,
+// one for all sequences of a layer; attend() allocates its workspace and waits for
+// the stream.  A step that is captured, ragged or must not wait calls the oxide_*
+// functions with lengths on the device and a workspace of its own.
 class KvCacheQ8 {
   public:
     static Result<KvCacheQ8> create(size_t num_layers, size_t batch, size_t kv_heads, size_t head_dim,

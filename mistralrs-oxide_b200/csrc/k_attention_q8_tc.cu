@@ -62,10 +62,11 @@
 //               one group's barriers and latencies hide behind the other's
 //               work.  Thread i = key i of S and dim i of each half of O.
 // Measured (bf16 queries, 32 heads over 8, blocks of 64; time, and the codes'
-// rate of 6540 GB/s): 8 sequences of 1024 to 32768 keys 51.2 us (83 %), one of
-// 131072 keys 47.6 us (86 %); 8 of 8192 keys, head_dim 256, 49.5 us (83 %);
-// starting, joining the parts and the last tiles' way through the roles take 7
-// to 8 us whatever the lengths (one sequence of 100 keys: 7.4 us).
+// rate of 6540 GB/s): 8 sequences of 1024 to 32768 keys 51.5 us (82 %), one of
+// 131072 keys 48.3 us (85 %); 8 of 8192 keys, head_dim 256, 49.5 us (83 %); 64
+// heads over 8 at 8 of 8192 keys 36.0 us (57 %), f32 queries 40.5; starting,
+// joining the parts and the last tiles' way through the roles take 7 to 8 us
+// whatever the lengths (one sequence of 100 keys: 7.3 us).
 // A group's buffers need few barriers: its O of tile k is read before its
 // weights of tile k + 1 are handed over, so that hand-over also says that O and
 // the weights buffer are free.

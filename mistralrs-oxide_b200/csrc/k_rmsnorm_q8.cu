@@ -26,10 +26,10 @@
 // w stays in registers too, and CTAs take rows in turn (reading w twice a row
 // through L1 instead left L1 the bound: 118 us at [16384, 4096] bf16 against
 // 72 us of bytes).  Bound by HBM bytes: x, r and h in their type, one byte out.
-// Measured: add + norm bf16 [16384, 4096] 78 us, 6.0 TB/s; f32 [2048, 4096] 14.0
-// us, 3.0 TB/s -- a row's chain of load, reduction and codes takes 3 us, four rows
-// in turn to a CTA -- and [16384, 4096] 77 us, 4.4 TB/s; eight rows 2.6 us, launch
-// latency.
+// Measured: add + norm bf16 [16384, 4096] 78 us, 6.0 TB/s, without r 57 us; f32
+// [2048, 4096] 14.3 us, 2.9 TB/s -- a row's chain of load, reduction and codes
+// takes 3 us, four rows in turn to a CTA -- and [16384, 4096] 78 us, 4.3 TB/s;
+// eight rows 2.5 us, launch latency.
 // Rows that do not divide into aligned vectors are held element by element in
 // the same way (up to 16 a thread); longer ones are read twice, the second
 // time through L1 / L2.
@@ -250,7 +250,7 @@ constexpr int NQ_VPT = 4;  // 16-byte vectors a thread holds
 
 // WARP: eight rows per 256-thread CTA; else one row per CTA of up to MAXT threads.
 // Three CTAs of 256 an SM at 80 registers, four for f32 without r at 64 (14.0 us
-// against 14.6 with three, 77 against 85; with r four were slower, 27.8 against
+// against 14.6 with three, 77 against 85 when it was chosen; with r four were slower, 27.8 against
 // 22.0).  All of these spill some: f32 about 100 bytes a thread, bf16 with r 40.
 // Two CTAs, which spill nothing, were slower everywhere: bf16 [16384, 4096] with r
 // 87.9 us against 82.0, f32 with r 158 against 141, f32 116 against 78.

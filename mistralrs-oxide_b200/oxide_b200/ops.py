@@ -809,7 +809,11 @@ class KvCacheQ8(KvCache):
     positions and head: about half the memory of bf16 caches and, in a decode
     step, half the bytes read.  update() quantises as it writes
     (kv_cache_append_q8), get() reads values back (kv_cache_read_q8, in
-    `dtype`), attend() is one decode step of attention over a layer."""
+    `dtype`), attend() is one decode step of attention over a layer.
+    Lengths are counted on the host, one for all sequences of a layer, as in
+    KvCache: a captured graph replays update() and attend() at the lengths it
+    was captured with.  Ragged batches, padded prompts and captured steps call
+    the functions on the caches with int32 lengths on the device."""
 
     def __init__(self, num_layers: int, batch_size: int, num_kv_heads: int, head_dim: int,
                  max_seq_len: int, block: int = 64, dtype=torch.bfloat16, device="cuda"):
