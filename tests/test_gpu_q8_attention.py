@@ -545,3 +545,20 @@ def test_scores_far_from_zero(cuda, hq, hkv, d, n, score):
         finally:
             _lib.lib().oxide_debug_decode_attention_path(0)
         _close(got, want, tol)
+
+
+@pytest.mark.parametrize("hq,hkv,d", [(8, 2, 128), (2, 2, 128), (6, 2, 80), (16, 2, 256), (4, 2, 37), (6, 3, 20)])
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_queries_that_are_not_finite(cuda, hq, hkv, d, dtype):
+    """A NaN or an infinity in a query head makes that head NaN and no other, on
+    either kernel."""
+    case = _case(cuda, 3, hq, hkv, d, 300, 16, dtype)
+    lens = _lens(cuda, [300, 1, 129])
+    clean = [_on_path(path, case, 16, lens) for path in (0, 1)]
+    for b, h, i, v in ((0, 0, d - 1, "nan"), (1, hq - 1, 0, "inf"), (2, 1, d // 2, "-inf")):
+        case[0][b, h, i] = float(v)
+    bad = ~torch.isfinite(case[0]).all(-1)
+    for path in (0, 1):
+        got = _on_path(path, case, 16, lens)
+        assert torch.equal(torch.isnan(got).all(-1), bad) and torch.equal(torch.isnan(got).any(-1), bad)
+        assert torch.equal(got[~bad], clean[path][~bad])
