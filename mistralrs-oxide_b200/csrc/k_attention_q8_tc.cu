@@ -156,6 +156,15 @@ __device__ __forceinline__ float qt_spell(uint32_t d0, uint32_t d1, uint32_t d2,
 }
 // Balanced digits of an integer, |x| <= 0x7f7f7f7f, in bytes 0 .. 3.
 __device__ __forceinline__ uint32_t qt_digits(int x) { return ((uint32_t)x + 0x80808080u) ^ 0x80808080u; }
+// Byte j of word i becomes byte i of word j: digit rows from the digits of four dims.
+__device__ __forceinline__ void qt_transpose(uint32_t (&d)[4]) {
+    const uint32_t a = __byte_perm(d[0], d[1], 0x5140), b = __byte_perm(d[2], d[3], 0x5140);
+    const uint32_t c = __byte_perm(d[0], d[1], 0x7362), e = __byte_perm(d[2], d[3], 0x7362);
+    d[0] = __byte_perm(a, b, 0x5410);
+    d[1] = __byte_perm(a, b, 0x7632);
+    d[2] = __byte_perm(c, e, 0x5410);
+    d[3] = __byte_perm(c, e, 0x7632);
+}
 // Scores: digit i of head h is column i NR + h.  Of eight digits the upper four
 // come first; the lower ones count units of 2^-31 of theirs.
 template <int NR, int QD>
@@ -465,12 +474,12 @@ __global__ void __launch_bounds__(QT_THREADS, 1) __maxnreg__(NR < 8 && DH == 1 ?
                             d[i] = qt_digits(n);
                             y[i] = fmul(fsub(y[i], (float)n), 0x1p31f);  // exact
                         }
+                        qt_transpose(d);
 #pragma unroll
                         for (int g = 0; g < 4; ++g) {
                             const uint32_t r = (g0 + g) * NR + h;
                             *reinterpret_cast<uint32_t*>(out + half * M::Q_HALF + r * 128 + (((lane >> 2) ^ (r & 7)) << 4) +
-                                                         ((lane & 3) << 2)) =
-                                q8_pack4(d[0] >> (8 * g), d[1] >> (8 * g), d[2] >> (8 * g), d[3] >> (8 * g));
+                                                         ((lane & 3) << 2)) = d[g];
                         }
                     }
                 }
