@@ -50,8 +50,8 @@
 //               the loads allow;
 //   warp 2      the query heads' digits, one pair ahead, from raw bits loaded two
 //               pairs ahead.  (A second such warp gained nothing, nor did asking
-//               L2 for the queries four pairs early: 59.2 and 71.2 us where this
-//               took 59.1, at 256 sequences of 200 keys, 32 heads.)
+//               L2 for the queries four pairs early, when it was tried: 59.2 and
+//               71.2 us where this took 59.1, at 256 sequences of 200 keys.)
 //   warp 3      the tile prefix; then each tile's scales, ready for the softmax
 //               threads (the key scale, log2 of the value scale, masks), loaded
 //               two tiles ahead.  One scale for a lane's four keys wherever
@@ -62,11 +62,11 @@
 //               one group's barriers and latencies hide behind the other's
 //               work.  Thread i = key i of S and dim i of each half of O.
 // Measured (bf16 queries, 32 heads over 8, blocks of 64; time, and the codes'
-// rate of 6540 GB/s): 8 sequences of 1024 to 32768 keys 51.5 us (82 %), one of
-// 131072 keys 48.3 us (85 %); 8 of 8192 keys, head_dim 256, 49.5 us (83 %); 64
-// heads over 8 at 8 of 8192 keys 36.0 us (57 %), f32 queries 40.5; starting,
-// joining the parts and the last tiles' way through the roles take 7 to 8 us
-// whatever the lengths (one sequence of 100 keys: 7.3 us).
+// rate of 6540 GB/s): 8 sequences of 1024 to 32768 keys 52 us (81 %), one of
+// 131072 keys 48.4 us (85 %); 8 of 8192 keys, head_dim 256, 48.7 us (84 %); 64
+// heads over 8 at 8 of 8192 keys 35.4 us (58 %), f32 queries 38.8; 256 of 200 keys
+// 48.5 us; starting, joining the parts and the last tiles' way through the roles
+// take 7 to 8 us whatever the lengths (one sequence of 100 keys: 7.2 us).
 // A group's buffers need few barriers: its O of tile k is read before its
 // weights of tile k + 1 are handed over, so that hand-over also says that O and
 // the weights buffer are free.
@@ -156,7 +156,9 @@ __device__ __forceinline__ float qt_spell(uint32_t d0, uint32_t d1, uint32_t d2,
 }
 // Balanced digits of an integer, |x| <= 0x7f7f7f7f, in bytes 0 .. 3.
 __device__ __forceinline__ uint32_t qt_digits(int x) { return ((uint32_t)x + 0x80808080u) ^ 0x80808080u; }
-// Byte j of word i becomes byte i of word j: digit rows from the digits of four dims.
+// Byte j of word i becomes byte i of word j: digit rows from the digits of four
+// dims.  (A shift and a pack a byte made this warp the bound of short sequences:
+// 256 of 200 keys 51.4 us instead of 48.5, f32 queries 58.3 instead of 55.0.)
 __device__ __forceinline__ void qt_transpose(uint32_t (&d)[4]) {
     const uint32_t a = __byte_perm(d[0], d[1], 0x5140), b = __byte_perm(d[2], d[3], 0x5140);
     const uint32_t c = __byte_perm(d[0], d[1], 0x7362), e = __byte_perm(d[2], d[3], 0x7362);
